@@ -1,0 +1,532 @@
+"""The operators of serving a model from kept histories, and of scoring its logits, as timed cases.
+
+A case's `kind` says what it calls:
+
+  attend  recml_amd.cached_attention: attention of new events over keys and values kept in 4 or 8 bits
+  store   recml_amd.kv_write and recml_amd.kv_read: events' keys and values quantised into the pages, and read back
+  score   recml_amd.token_log_probs: log probabilities of given items from logits, entropy, top alternatives, gradients
+
+Kept keys and values are blocks of 32 values along the head dim (the last block may be shorter) that share a power of
+two: codes in e2m1 (4 bits, two to a byte, the even index in the low half) or e4m3 (8 bits), [pages, heads, page_size,
+bytes], and exponents [pages, heads, blocks, page_size] (uint8, biased by 127).  The power is the smallest under which
+the block's largest magnitude rounds to a code.
+
+Sizes are those of recml_amd.workloads, bench.py and the example model; `draw` spreads the same kinds over their range.
+The lengths of a batch come from the case alone (`len_seed`), which sequence has which, and every value, from the seed.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+_DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
+_BYTES = {"fp32": 4, "bf16": 2}
+_BUCKETS = 128
+
+
+def _attend(name, B, L, H, d, bits, *, new=1, ragged=False, lens="full", pos=False, ts=False, dtype="bf16", page=64, len_seed=1):
+  return dict(name=name, kind="attend", B=B, L=L, H=H, d=d, bits=bits, new=new, ragged=ragged, lens=lens, pos=pos, ts=ts, dtype=dtype,
+              page=page, len_seed=len_seed)
+
+
+def _store(name, B, L, H, d, bits, *, new=1, ragged=False, lens="full", dtype="bf16", page=64, len_seed=1):
+  return dict(name=name, kind="store", B=B, L=L, H=H, d=d, bits=bits, new=new, ragged=ragged, lens=lens, dtype=dtype, page=page,
+              len_seed=len_seed)
+
+
+def _score(name, rows, vocab, *, tokens=1, top=0, entropy=False, grad=False, masked=0.0, dtype="bf16"):
+  return dict(name=name, kind="score", rows=rows, vocab=vocab, tokens=tokens, top=top, entropy=entropy, grad=grad, masked=masked,
+              dtype=dtype)
+
+
+def listed():
+  return [
+      # one user's next event: a single step of a single history, where nothing but latency counts
+      _attend("one event, one history, 4 bits", 1, 2048, 8, 128, 4, lens="uniform", pos=True, ts=True, len_seed=2),
+      # the headline batch in serving: an event each, histories of power-law length, both bias tables
+      _attend("an event each, jagged, 4 bits", 64, 2048, 8, 128, 4, lens="power", pos=True, ts=True, len_seed=3),
+      # long histories, many of them: the largest read of a cache
+      _attend("long histories, 4 bits", 192, 4096, 8, 128, 4, pos=True),
+      # a session's events at once on the ranking model's heads, a few more for some users than for others
+      _attend("sessions of events, 8 bits", 128, 1024, 8, 64, 8, new=24, ragged=True, lens="uniform", pos=True, len_seed=4),
+      # the example model's narrow heads in Keras' default type, an odd length
+      _attend("narrow heads, fp32, 8 bits", 32, 50, 4, 16, 8, new=2, lens="uniform", dtype="fp32", page=32, len_seed=9),
+      # a batch's newest events written and read back
+      _store("an event each stored, 4 bits", 64, 2048, 8, 128, 4, lens="power", len_seed=3),
+      # whole histories taken into the cache and read back
+      _store("histories stored, 4 bits", 64, 2048, 8, 128, 4, new=2048, ragged=True, len_seed=5),
+      # one request over the whole vocabulary, items already seen masked out
+      _score("one request, a million items", 1, 1000000, tokens=8, top=10, entropy=True, masked=0.01),
+      # a batch of requests with candidate items
+      _score("requests with candidates", 64, 20000, tokens=100, top=20, masked=0.01),
+      # fp32 logits of an odd vocabulary
+      _score("odd vocabulary, fp32", 4096, 20011, top=5, entropy=True, dtype="fp32"),
+      # the example model's training step: every position's next item, with the gradient of the logits
+      _score("example model's loss", 1600, 20000, grad=True),
+      # training over the largest vocabulary whose logits are worth keeping, entropy as a regulariser
+      _score("large loss with entropy", 8192, 100000, entropy=True, grad=True),
+  ]
+
+
+def _log_int(rng, lo, hi):
+  return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.99)))))))
+
+
+def _cost(case):
+  w = work(case)
+  return max(w["bytes"], w["flops"] / 50)
+
+
+def draw(rng):
+  """One more case of the listed kinds, that costs no more than the largest listed one of its kind."""
+  while True:
+    kind = rng.choice(("attend", "attend", "store", "score", "score"))
+    dtype = rng.choice(("bf16", "bf16", "bf16", "fp32"))
+    if kind == "score":
+      grad = rng.random() < 0.5
+      vocab = _log_int(rng, 2, 1000000)
+      case = _score("", _log_int(rng, 1, 16384), vocab, tokens=rng.choice((1, 1, 2, 5, 33, 100)), top=min(vocab, rng.choice((0, 0, 1, 5, 10, 50))),
+                    entropy=rng.random() < 0.5, grad=grad, masked=0.0 if vocab < 100 else rng.choice((0.0, 0.0, 0.05, 0.5)), dtype=dtype)
+      cap = "large loss with entropy"
+    else:
+      B, L, H, d = _log_int(rng, 1, 256), _log_int(rng, 24, 4096), rng.choice((1, 2, 3, 4, 8, 8, 12, 16)), rng.choice((16, 32, 64, 64, 96, 128, 128, 256))
+      bits, lens, page, len_seed = rng.choice((4, 4, 8)), rng.choice(("uniform", "power", "full")), rng.choice((32, 64, 64, 128)), rng.randrange(1 << 16)
+      if kind == "attend":
+        pos = rng.random() < 0.7
+        case = _attend("", B, L, H, d, bits, new=min(L, rng.choice((1, 1, 1, 2, 5, 16, 33, 64))), ragged=rng.random() < 0.4, lens=lens, pos=pos,
+                       ts=pos and rng.random() < 0.5, dtype=dtype, page=page, len_seed=len_seed)
+        cap = "long histories, 4 bits"
+      else:
+        case = _store("", B, L, H, d, bits, new=_log_int(rng, 1, L), ragged=rng.random() < 0.5, lens=lens, dtype=dtype, page=page,
+                      len_seed=len_seed)
+        cap = "histories stored, 4 bits"
+    del case["name"]
+    if _cost(case) <= next(_cost(c) for c in listed() if c["name"] == cap):
+      return case
+
+
+# ---------------------------------------------------------------------------
+# lengths and work
+# ---------------------------------------------------------------------------
+
+
+def _lengths(case):
+  """(how many events each history keeps, how many of them are this call's), before they are dealt to the sequences."""
+  B, L = case["B"], case["L"]
+  rng = np.random.default_rng(case["len_seed"])
+  if case["lens"] == "uniform":
+    n = rng.integers(max(1, L // 8), L + 1, B).astype(np.int64)
+  elif case["lens"] == "power":
+    lo, e = min(16, L), -0.2
+    x = (lo**e + rng.random(B) * (L**e - lo**e)) ** (1.0 / e)
+    n = np.clip(np.floor(x), lo, L).astype(np.int64)
+  else:
+    n = np.full(B, L, dtype=np.int64)
+  new = rng.integers(1, case["new"] + 1, B) if case["ragged"] else np.full(B, case["new"])
+  return np.maximum(n, new), new.astype(np.int64)
+
+
+def _row_bytes(case):
+  """Bytes of one (event, head) row of codes with its exponents."""
+  return case["d"] * case["bits"] // 8 + -(-case["d"] // 32)
+
+
+def work(case):
+  if case["kind"] == "score":
+    n, e = case["rows"] * case["vocab"], _BYTES[case["dtype"]]
+    return {"bytes": n * e * (2 if case["grad"] else 1) + case["rows"] * (case["tokens"] * 12 + case["top"] * 12 + 4),
+            "flops": n * (8 if case["grad"] else 4)}
+  H, d, e = case["H"], case["d"], _BYTES[case["dtype"]]
+  n, new = _lengths(case)
+  rows = int(new.sum()) * H
+  if case["kind"] == "store":
+    return {"bytes": 2 * rows * (d * e + _row_bytes(case) + d * 2), "flops": 2 * rows * d * 4}
+  pairs = int((new * n - new * (new - 1) // 2).sum())
+  nbytes = 2 * int(n.sum()) * H * _row_bytes(case) + 2 * rows * d * e
+  if case["pos"]:
+    nbytes += H * (int(n.max()) + case["new"]) * 4
+  if case["ts"]:
+    nbytes += int(n.sum()) * 8 + H * (_BUCKETS + 1) * 4
+  return {"bytes": nbytes, "flops": 4 * d * pairs * H}
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+
+
+class _Draws:
+  """Device-side random values of one seed."""
+
+  def __init__(self, seed):
+    self.dev = torch.device("cuda")
+    self.gen = torch.Generator(device=self.dev).manual_seed(seed)
+    self.host = np.random.default_rng(seed)
+
+  def normal(self, shape, std, dtype=torch.float32):
+    return torch.randn(shape, device=self.dev, generator=self.gen).mul_(std).to(dtype)
+
+  def uniform(self, shape):
+    return torch.rand(shape, device=self.dev, generator=self.gen)
+
+  def put(self, a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(self.dev)
+
+
+def _prepare_score(case, r):
+  R, V = case["rows"], case["vocab"]
+  x = r.normal((R, V), 2.5)
+  if case["masked"]:
+    x.masked_fill_(r.uniform((R, V)) < case["masked"], -math.inf)
+    x[:, 0] = 0.5                            # (an item that nobody has seen: no row is masked out as a whole)
+  tokens = torch.randint(0, V, (R, case["tokens"]), device=r.dev, generator=r.gen)
+  state = dict(kind="score", top=case["top"], entropy=case["entropy"], grad=case["grad"], logits=x.to(_DTYPES[case["dtype"]]), tokens=tokens)
+  if case["grad"]:
+    if case["masked"]:                       # (a loss takes items that can occur)
+      state["tokens"] = torch.where(torch.isfinite(x.gather(1, tokens)), tokens, 0)
+    state["g_tokens"] = r.normal((R, case["tokens"]), 1.0)
+    state["g_entropy"] = r.normal((R,), 0.1) if case["entropy"] else None
+    state["g_top"] = r.normal((R, case["top"]), 0.1) if case["top"] else None
+  return state
+
+
+def _prepare_pages(case, r):
+  B, L, H, d, bits, page = case["B"], case["L"], case["H"], case["d"], case["bits"], case["page"]
+  dt, blocks = _DTYPES[case["dtype"]], -(-d // 32)
+  n, new = _lengths(case)
+  order = r.host.permutation(B)
+  n, new = n[order], new[order]
+  held, most = -(-n // page), -(-L // page)
+  # pages in no order, as they come back from histories that ended; entries past a history's end name none
+  free = r.host.permutation(int(held.sum()) + 8)
+  table = np.full((B, most), -1, dtype=np.int32)
+  at = np.arange(most)[None, :] < held[:, None]
+  table[at] = free[: int(held.sum())]
+  state = dict(kind=case["kind"], bits=bits, d=d, page=page, max_len=L, new=case["new"], dtype=dt, ragged=case["ragged"],
+               page_table=r.put(table), lengths=r.put(n.astype(np.int32)), starts=r.put((n - new).astype(np.int32)))
+  if case["ragged"]:
+    state["offsets"] = r.put(np.concatenate([[0], np.cumsum(new)]).astype(np.int32))
+  shape = (int(new.sum()), H, d) if case["ragged"] else (B, case["new"], H, d)
+  if case["kind"] == "store":
+    state["new_k"], state["new_v"] = (r.normal(shape, 0.3, dt) for _ in range(2))
+    for name in ("k", "v"):
+      state[name] = torch.zeros((len(free), H, page, d * bits // 8), dtype=torch.uint8, device=r.dev)
+      state[name + "_scales"] = torch.ones((len(free), H, blocks, page), dtype=torch.uint8, device=r.dev)
+    return state
+  state["q"] = r.normal(shape, 0.3, dt)
+  for name in ("k", "v"):
+    codes, scales = _quantised(r.normal((len(free), H, page, d), 0.3), bits)
+    state[name], state[name + "_scales"] = codes, scales.transpose(2, 3).contiguous()
+  if case["pos"]:
+    state["pos_bias"] = r.normal((H, 2 * L - 1), 0.05)
+  if case["ts"]:
+    gaps = torch.ceil(-torch.log1p(-r.uniform((B, L)).double()) * 3600.0).to(torch.int64)
+    state["timestamps"] = 1_600_000_000 + torch.cumsum(gaps, 1)
+    state["ts_bias"] = r.normal((H, _BUCKETS + 1), 0.1)
+  return state
+
+
+def prepare(case, seed):
+  r = _Draws(seed)
+  return _prepare_score(case, r) if case["kind"] == "score" else _prepare_pages(case, r)
+
+
+# ---------------------------------------------------------------------------
+# the plain forms
+# ---------------------------------------------------------------------------
+
+
+def _power(e):
+  """2^e in fp32 for whole e in [-126, 127], by its bits: a device's pow is not exact."""
+  return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _quantised(x, bits):
+  """fp32 rows [..., d] as codes [..., bytes] and block exponents [..., blocks].  Every step is exact: the powers of two
+  scale without rounding, so the borders between codes are where the definition has them."""
+  d = x.shape[-1]
+  blocks = -(-d // 32)
+  x = torch.nn.functional.pad(x, (0, 32 * blocks - d)).unflatten(-1, (blocks, 32))
+  top = x.abs().amax(-1)
+  mantissa, exponent = torch.frexp(top)
+  e = exponent - (3 if bits == 4 else 9) + (mantissa > (0.875 if bits == 4 else 0.90625)).to(exponent.dtype)
+  e = torch.where(top > 0, e, -126).clamp(-126, 126)
+  bad = ~torch.isfinite(top).all(-1, keepdim=True)
+  scales = torch.where(bad, 255, e + 127).to(torch.uint8)
+  y = torch.where(bad[..., None], 0.0, x * _power(-e)[..., None])
+  y = y.flatten(-2)[..., :d]
+  if bits == 8:
+    return y.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8), scales
+  m = y.abs()
+  code = torch.where(m < 2, torch.round(2 * m), torch.where(m < 4, torch.round(m) + 2, torch.round(m / 2) + 4)).clamp(max=7)
+  code = code.to(torch.uint8) | (torch.signbit(y).to(torch.uint8) << 3)
+  return code[..., 0::2] | (code[..., 1::2] << 4), scales
+
+
+def _values(codes, scales, bits, d):
+  """fp32 rows [..., d] of codes [..., bytes] and exponents [..., blocks]."""
+  if bits == 8:
+    y = codes.view(torch.float8_e4m3fn).float()
+  else:
+    grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=codes.device)
+    grid = torch.cat([grid, -grid])
+    i = torch.arange(256, device=codes.device)
+    y = torch.stack([grid[i & 15], grid[i >> 4]], 1)[codes.long()].flatten(-2)
+  power = torch.where(scales == 255, math.nan, _power(scales.to(torch.int32) - 127))
+  return y * power.repeat_interleave(32, -1)[..., :d]
+
+
+def _places(s):
+  """Sequence and place in it of each of this call's events, shaped like the events' leading axes."""
+  dev = s["lengths"].device
+  if s["ragged"]:
+    o = s["offsets"].long()
+    b = torch.repeat_interleave(torch.arange(len(o) - 1, device=dev), o[1:] - o[:-1], output_size=(s["q"] if "q" in s else s["new_k"]).shape[0])
+    return b, torch.arange(len(b), device=dev) - o[b]
+  B, n = (s["q"] if "q" in s else s["new_k"]).shape[:2]
+  return torch.arange(B, device=dev)[:, None].expand(B, n), torch.arange(n, device=dev)[None, :].expand(B, n)
+
+
+def _store_plain(s):
+  b, t = _places(s)
+  at = s["starts"].long()[b] + t
+  pages, slots = s["page_table"].long()[b, at // s["page"]], at % s["page"]
+  back = []
+  for name in ("k", "v"):
+    codes, scales = _quantised(s["new_" + name].float(), s["bits"])
+    s[name][pages, :, slots] = codes
+    s[name + "_scales"][pages, :, :, slots] = scales
+    back.append(_values(s[name][pages, :, slots], s[name + "_scales"][pages, :, :, slots], s["bits"], s["d"]).to(torch.bfloat16))
+  return back
+
+
+def _gathered(s, name):
+  """All histories' rows, [B, H, places, d] in fp32; places that no page holds are rows of page 0, which the mask leaves out."""
+  pages = s["page_table"].long().clamp(min=0)
+  rows = _values(s[name][pages], s[name + "_scales"][pages].transpose(-1, -2), s["bits"], s["d"])
+  return rows.transpose(1, 2).flatten(2, 3)
+
+
+def _attend_plain(s):
+  q, lengths = s["q"].float(), s["lengths"].long()
+  b, t = _places(s)
+  k, v = _gathered(s, "k"), _gathered(s, "v")
+  if s["ragged"]:
+    rows = torch.zeros((len(lengths), s["new"], *q.shape[1:]), device=q.device)
+    rows[b, t] = q
+    count = (s["offsets"][1:] - s["offsets"][:-1]).long()
+  else:
+    rows, count = q, torch.full_like(lengths, s["new"])
+  logits = rows.transpose(1, 2) @ k.transpose(-1, -2)                                      # [B, H, new, places]
+  i = (lengths - count)[:, None] + torch.arange(s["new"], device=q.device)                 # [B, new]
+  j = torch.arange(k.shape[2], device=q.device)
+  last = s["max_len"] - 1
+  if "pos_bias" in s:
+    logits = logits + s["pos_bias"][:, (last + j - i[..., None]).clamp(0, 2 * last)].transpose(0, 1)
+  if "timestamps" in s:
+    ts = s["timestamps"]
+    nxt = torch.minimum(i + 1, lengths[:, None] - 1).clamp(0, last)
+    gap = ts.gather(1, nxt)[..., None] - ts[:, j.clamp(max=last)][:, None, :]
+    gap = gap.abs().clamp(1, 10**9).float().double()
+    bucket = torch.floor(torch.log(gap) / float(np.float32(0.301))).long().clamp(max=_BUCKETS)
+    logits = logits + s["ts_bias"][:, bucket].transpose(0, 1)
+  keep = (j <= i[..., None]) & (j < lengths[:, None, None])
+  weights = torch.where(keep[:, None], logits / (1 + torch.exp(-logits)) / s["max_len"], 0.0)
+  out = (weights @ v).transpose(1, 2)
+  return (out[b, t] if s["ragged"] else out).to(s["dtype"])
+
+
+def _score_plain(s):
+  x, tokens, k = s["logits"].float(), s["tokens"], s["top"]
+  top = x.amax(-1, keepdim=True)
+  lse = top + torch.log(torch.exp(x - top).sum(-1, keepdim=True))
+  out = {"log_probs": x.gather(1, tokens) - lse}
+  p = torch.exp(x - lse) if s["entropy"] or s["grad"] else None
+  entropy = None
+  if s["entropy"]:
+    entropy = -torch.where(p > 0, p * (x - lse), 0.0).sum(-1, keepdim=True)
+    out["entropy"] = entropy[:, 0]
+  first = None
+  if k:
+    # by value, then by index: ordered integers of the values above the indices counted down
+    n = x.view(torch.int32).long()
+    n = torch.where(n < 0, -1 - (n & 0x7FFFFFFF), n)
+    n = torch.where(x == 0, 0, n)
+    key = (n << 32) + (0xFFFFFFFF - torch.arange(x.shape[1], device=x.device))
+    first = 0xFFFFFFFF - (torch.topk(key, k, dim=-1).values & 0xFFFFFFFF)
+    out["top_tokens"], out["top_log_probs"] = first, x.gather(1, first) - lse
+  if s["grad"]:
+    total = s["g_tokens"].sum(-1, keepdim=True)
+    if k:
+      total = total + s["g_top"].sum(-1, keepdim=True)
+    inner = total
+    if s["entropy"]:
+      inner = inner + s["g_entropy"][:, None] * torch.where(p > 0, x - lse + entropy, 0.0)
+    g = -p * inner
+    g = g.scatter_add(1, tokens, s["g_tokens"])
+    if k:
+      g = g.scatter_add(1, first, s["g_top"])
+    out["d_logits"] = g.to(s["logits"].dtype)
+  return out
+
+
+# ---------------------------------------------------------------------------
+# the framework's calls
+# ---------------------------------------------------------------------------
+
+
+def _own_run(s):
+  import recml_amd
+  if s["kind"] == "score":
+    if not s["grad"]:
+      with torch.no_grad():
+        got = recml_amd.token_log_probs(s["logits"], s["tokens"], top=s["top"], entropy=s["entropy"])
+    else:
+      x = s["logits"].detach().requires_grad_(True)
+      got = recml_amd.token_log_probs(x, s["tokens"], top=s["top"], entropy=s["entropy"])
+    out = {"log_probs": got.log_probs.detach()}
+    if s["entropy"]:
+      out["entropy"] = got.entropy.detach()
+    if s["top"]:
+      out["top_tokens"], out["top_log_probs"] = got.top_tokens, got.top_log_probs.detach()
+    if s["grad"]:
+      pairs = [(got.log_probs, s["g_tokens"]), (got.entropy, s["g_entropy"]), (got.top_log_probs, s["g_top"])]
+      pairs = [(y, g) for y, g in pairs if g is not None]
+      out["d_logits"] = torch.autograd.grad([y for y, _ in pairs], x, [g for _, g in pairs])[0]
+    return out
+  pages = recml_amd.KVPages(s["k"], s["k_scales"], s["v"], s["v_scales"], head_dim=s["d"])
+  if s["kind"] == "store":
+    if s["ragged"]:
+      recml_amd.kv_write(pages, s["new_k"], s["new_v"], s["page_table"], s["starts"], offsets=s["offsets"], max_new=s["new"])
+      return recml_amd.kv_read(pages, s["page_table"], s["starts"], offsets=s["offsets"], max_new=s["new"], total=s["new_k"].shape[0])
+    recml_amd.kv_write(pages, s["new_k"], s["new_v"], s["page_table"], s["starts"])
+    return recml_amd.kv_read(pages, s["page_table"], s["starts"], count=s["new"])
+  how = dict(offsets=s["offsets"], max_new=s["new"]) if s["ragged"] else {}
+  return recml_amd.cached_attention(s["q"], pages, s["page_table"], s["lengths"], max_len=s["max_len"], pos_bias=s.get("pos_bias"),
+                                    timestamps=s.get("timestamps"), ts_bias=s.get("ts_bias"), **how)
+
+
+def run(state):
+  if own:
+    return _own_run(state)
+  return {"attend": _attend_plain, "store": _store_plain, "score": _score_plain}[state["kind"]](state)
+
+
+# ---------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------
+
+
+def _exact_power(e):
+  """2^e in 64 bits for whole e."""
+  return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def _exact_levels(bits, dev):
+  """The magnitudes of the codes in rising order."""
+  if bits == 4:
+    return torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64, device=dev)
+  e4m3 = [f / 512 for f in range(8)] + [(1 + f / 8) * 2.0 ** (e - 7) for e in range(1, 16) for f in range(8)]
+  return torch.tensor(e4m3[:127], dtype=torch.float64, device=dev)     # (the last code is no number)
+
+
+def _exact_stored(x, bits):
+  """What values become in the cache: the nearest level (ties to the even code) times the block's power."""
+  x = x.double()
+  levels = _exact_levels(bits, x.device)
+  most = levels[-1] + (1.0 if bits == 4 else 16.0)       # half a step past the largest code rounds to it
+  parts = []
+  for block in x.split(32, -1):
+    top = block.abs().amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2(top / most)).clamp(-200, 200)
+    e = torch.where(top > most * _exact_power(e), e + 1, torch.where(top <= most * _exact_power(e - 1), e - 1, e)).clamp(min=-126)
+    power = torch.where(top > 0, _exact_power(e), 1.0)
+    m = block.abs() / power
+    hi = torch.searchsorted(levels, m.contiguous()).clamp(1, len(levels) - 1)
+    lo = hi - 1
+    below, above = m - levels[lo], levels[hi] - m
+    code = torch.where((below < above) | ((below == above) & (lo % 2 == 0)), lo, hi)
+    parts.append(levels[code] * power * torch.sign(block))
+  return torch.cat(parts, -1)
+
+
+def _exact_kept(s, name, b, length):
+  """One history's rows in 64 bits: [length, H, d]."""
+  page = s["page"]
+  ids = s["page_table"][b, : -(-length // page)].long()
+  codes = s[name][ids].transpose(1, 2).flatten(0, 1)[:length]                  # [length, H, bytes]
+  e = s[name + "_scales"][ids].permute(0, 3, 1, 2).flatten(0, 1)[:length].double() - 127.0
+  if s["bits"] == 4:
+    codes = torch.stack([codes % 16, torch.div(codes, 16, rounding_mode="floor")], -1).flatten(-2).long()
+    magnitude, negative = codes % 8, codes >= 8
+  else:
+    magnitude, negative = codes.long() % 128, codes >= 128
+  y = _exact_levels(s["bits"], codes.device)[magnitude]
+  return torch.where(negative, -y, y) * _exact_power(e).repeat_interleave(32, -1)[..., : s["d"]]
+
+
+def _exact_attend(s):
+  L, out = s["max_len"], torch.zeros(s["q"].shape, dtype=torch.float64, device=s["q"].device)
+  lengths = s["lengths"].tolist()
+  offsets = s["offsets"].tolist() if s["ragged"] else None
+  for b, length in enumerate(lengths):
+    q = (s["q"][offsets[b] : offsets[b + 1]] if s["ragged"] else s["q"][b]).double()
+    k, v = _exact_kept(s, "k", b, length), _exact_kept(s, "v", b, length)
+    x = torch.matmul(q.transpose(0, 1), k.permute(1, 2, 0).contiguous())      # [H, new, length]
+    i = torch.arange(length - len(q), length, device=q.device)[:, None]
+    j = torch.arange(length, device=q.device)[None, :]
+    if "pos_bias" in s:
+      x = x + s["pos_bias"].double()[:, L - 1 + j - i]
+    if "timestamps" in s:
+      ts = s["timestamps"][b]
+      gap = (ts[(i + 1).clamp(max=length - 1)] - ts[j]).abs().clamp(1, 10**9).to(torch.float32).double()
+      x = x + s["ts_bias"].double()[:, (torch.log(gap) / float(np.float32(0.301))).floor().long().clamp(max=_BUCKETS)]
+    w = torch.where(j <= i, x * torch.sigmoid(x) / L, 0.0)
+    got = torch.matmul(w, v.transpose(0, 1).contiguous()).transpose(0, 1)
+    if s["ragged"]:
+      out[offsets[b] : offsets[b + 1]] = got
+    else:
+      out[b] = got
+  return out
+
+
+def _exact_score(s):
+  R, V = s["logits"].shape
+  step = max(1, (1 << 27) // V)
+  parts = []
+  for r in range(0, R, step):
+    x, tokens = s["logits"][r : r + step].double(), s["tokens"][r : r + step]
+    lp = torch.log_softmax(x, -1)
+    p = lp.exp()
+    out = {"log_probs": lp.gather(1, tokens)}
+    h = -torch.where(p > 0, p * lp, 0.0).sum(-1, keepdim=True)
+    if s["entropy"]:
+      out["entropy"] = h[:, 0]
+    first = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, : s["top"]] if s["top"] else None
+    if s["top"]:
+      out["top_log_probs"] = lp.gather(1, first)
+    if s["grad"]:
+      g = torch.zeros_like(x).scatter_add(1, tokens, s["g_tokens"][r : r + step].double())
+      if s["top"]:
+        g = g.scatter_add(1, first, s["g_top"][r : r + step].double())
+      g = g - p * g.sum(-1, keepdim=True)
+      if s["entropy"]:
+        g = g - s["g_entropy"][r : r + step].double()[:, None] * torch.where(p > 0, p * (lp + h), 0.0)
+      out["d_logits"] = g
+    parts.append(out)
+  got = {name: torch.cat([part[name] for part in parts]) for name in parts[0]}
+  if s["top"]:
+    got["top_tokens"] = None
+  return got
+
+
+def exact(case, seed):
+  s = prepare(case, seed)
+  if s["kind"] == "store":
+    return [_exact_stored(s["new_" + name], s["bits"]) for name in ("k", "v")]
+  return _exact_attend(s) if s["kind"] == "attend" else _exact_score(s)
