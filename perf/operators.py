@@ -255,7 +255,7 @@ def _quantised(x, bits):
   top = x.abs().amax(-1)
   mantissa, exponent = torch.frexp(top)
   e = exponent - (3 if bits == 4 else 9) + (mantissa > (0.875 if bits == 4 else 0.90625)).to(exponent.dtype)
-  e = torch.where(top > 0, e, -126).clamp(-126, 126)
+  e = torch.where(top > 0, e, -126).clamp(-126, 125 if bits == 4 else 119)     # (no code stands for more than fp32 holds)
   bad = ~torch.isfinite(top).all(-1, keepdim=True)
   scales = torch.where(bad, 255, e + 127).to(torch.uint8)
   y = torch.where(bad[..., None], 0.0, x * _power(-e)[..., None])
@@ -444,7 +444,8 @@ def _exact_stored(x, bits):
   for block in x.split(32, -1):
     top = block.abs().amax(-1, keepdim=True)
     e = torch.ceil(torch.log2(top / most)).clamp(-200, 200)
-    e = torch.where(top > most * _exact_power(e), e + 1, torch.where(top <= most * _exact_power(e - 1), e - 1, e)).clamp(min=-126)
+    e = torch.where(top > most * _exact_power(e), e + 1, torch.where(top <= most * _exact_power(e - 1), e - 1, e))
+    e = e.clamp(-126, 125 if bits == 4 else 119)
     power = torch.where(top > 0, _exact_power(e), 1.0)
     m = block.abs() / power
     hi = torch.searchsorted(levels, m.contiguous()).clamp(1, len(levels) - 1)
