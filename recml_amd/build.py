@@ -15,6 +15,9 @@ SOURCES = [os.path.join(_HERE, "csrc", "hstu_attn.hip"), os.path.join(_HERE, "cs
 BLOCK_LIB_PATH = os.path.join(LIB_DIR, "libhstu_block.so")
 BLOCK_SOURCES = [os.path.join(_HERE, "csrc", "hstu_block.hip"), os.path.join(_HERE, "csrc", "hstu_gemm.hip"),
                  os.path.join(_HERE, "csrc", "hstu_block_small.hip")]
+# serving from kept histories and scoring of logits
+SERVE_LIB_PATH = os.path.join(LIB_DIR, "libhstu_serve.so")
+SERVE_SOURCES = [os.path.join(_HERE, "csrc", name) for name in ("hstu_cache.hip", "hstu_cached_attn.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 # the block's microbenchmark: a stand-alone program (its own main), evidence for what bounds the kernel
 MICRO_PATH = os.path.join(LIB_DIR, "micro_fwd_stream")
@@ -63,6 +66,11 @@ def build_block_library(verbose: bool = False) -> str:
   return _compile(BLOCK_SOURCES, BLOCK_LIB_PATH, verbose=verbose)
 
 
+def build_serve_library(verbose: bool = False) -> str:
+  """Compiles the serving operators into recml_amd/lib/libhstu_serve.so."""
+  return _compile(SERVE_SOURCES, SERVE_LIB_PATH, verbose=verbose)
+
+
 def build_native(verbose: bool = False) -> str:
   """Compiles the native host side into recml_amd/lib/_native.so (host code only; links the two libraries above)."""
   import sysconfig
@@ -101,5 +109,6 @@ def build_microbench(verbose: bool = False) -> str:
 if __name__ == "__main__":
   print(build_library(verbose=True))
   print(build_block_library(verbose=True))
+  print(build_serve_library(verbose=True))
   print(build_native(verbose=True))
   print(build_microbench(verbose=True))

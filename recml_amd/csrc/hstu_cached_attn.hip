@@ -1,0 +1,595 @@
+// Attention of new events over kept keys and values in 4 or 8 bits, for gfx950 (MI355X): see include/hstu_serve.h.
+//
+//   out_i = 1/n sum_{j <= i} silu(alpha q_i . k_j + pos[L - 1 + j - i] + ts_w[bucket(ts_{i + 1} - ts_j)]) v_j
+//
+// There is no softmax, so parts of the keys are independent sums: a workgroup takes `chunk` keys of one (sequence, head,
+// block of queries), its four waves every fourth 32 of them, and where a sequence has several parts a second kernel adds
+// them in order.
+//
+// A wave's step is 32 keys on the 16x16x32 bf16 matrix instruction.  Both formats are exact in bf16 (2 or 4 significant
+// bits times a power of two), so codes become operands by the hardware's scaled conversions without rounding:
+//   S^T = K Q^T   rows are keys.  Row r of tile t is key 8 (r / 4) + 4 t + r % 4, so that the lanes that get a query's
+//                 logits hold eight consecutive keys of it: exactly the eight that the second product's operand wants
+//                 of them, and the activated weights go from registers to registers.
+//   O^T = V^T P^T rows are the head's dims.  A lane reads its own run of d / 16 dims of its eight keys, scales each key's
+//                 run by that key's exponent on conversion, and pairs the keys up with byte permutes: nothing goes
+//                 through LDS, and the cache keeps rows as they are written.
+// The contraction order along d and along the keys is free as long as both operands agree: K's lane takes a run of d / 4
+// dims (one block of exponents at d = 128), and Q is read the same way.
+// fp32 queries run as three bf16 parts (24 bits: all of them), activated weights as three as well.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "hstu_serve_common.h"
+
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int THREADS = 64 * WAVES;
+constexpr int STEP = 32;             // keys of a wave's step
+constexpr int MAX_BUCKETS = 128;
+
+struct Params {
+  HstuKvPages g;
+  const int32_t* lengths;
+  const int32_t* offsets;
+  const void* q;
+  void* out;
+  int64_t total;
+  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;
+  const float* pos;
+  const int64_t* ts;
+  const float* ts_tab;
+  float* partial;                    // [row][head][part][d], null with one part
+  int32_t per_seq, max_len, pos_heads, ts_heads, ts_buckets;
+  int32_t chunk, parts, qblocks;
+  float alpha, inv_n, buckets_per_log2;
+  int32_t thr[MAX_BUCKETS + 2];      // thr[b]: smallest time difference of bucket b or a later one
+};
+
+// What a sequence's geometry says of the call: its first row, its rows, the place of row 0, and how many places are there.
+struct Seq {
+  int64_t first, place0;
+  int count, limit, last_ts;
+};
+
+__device__ __forceinline__ Seq seq_of(const Params& p, int b) {
+  Seq s;
+  if (p.offsets) {
+    int64_t o0 = p.offsets[b], o1 = p.offsets[b + 1];
+    o0 = o0 < 0 ? 0 : o0 > p.total ? p.total : o0;
+    o1 = o1 < o0 ? o0 : o1 > p.total ? p.total : o1;
+    s.first = o0;
+    s.count = (int)(o1 - o0 < p.per_seq ? o1 - o0 : p.per_seq);
+  } else {
+    s.first = (int64_t)b * p.per_seq;
+    s.count = p.per_seq;
+  }
+  const int n = p.lengths[b];
+  s.place0 = (int64_t)n - s.count;
+  const int64_t held = (int64_t)p.g.table_pages * p.g.page_size;
+  int limit = n < p.max_len ? n : p.max_len;
+  limit = limit < held ? limit : (int)held;
+  s.limit = limit < 0 ? 0 : limit;
+  s.last_ts = (n < p.max_len ? n : p.max_len) - 1;
+  return s;
+}
+
+// One past the last key that row t attends to (0: none, its output is zeros).
+__device__ __forceinline__ int keys_of(const Seq& s, int t) {
+  const int64_t i = s.place0 + t;
+  return t < s.count && i >= 0 && i < s.limit ? (int)i + 1 : 0;
+}
+
+template <int N>
+struct Bytes { uint32_t w[N < 4 ? 1 : N / 4]; };
+
+template <int N>
+__device__ __forceinline__ Bytes<N> load_bytes(const uint8_t* at) {
+  Bytes<N> r;
+  if constexpr (N == 1) r.w[0] = *at;
+  else if constexpr (N == 2) r.w[0] = *(const uint16_t*)at;
+  else if constexpr (N == 4) r.w[0] = *(const uint32_t*)at;
+  else if constexpr (N == 8) { const uint2 v = *(const uint2*)at; r.w[0] = v.x; r.w[1] = v.y; }
+  else {
+#pragma unroll
+    for (int i = 0; i < N / 16; ++i) {
+      const uint4 v = ((const uint4*)at)[i];
+      r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
+    }
+  }
+  return r;
+}
+
+// Values 2 I and 2 I + 1 of a run of codes, times `power`, as a pair of bf16.
+template <int BITS, int I, int N>
+__device__ __forceinline__ uint32_t pair_at(const Bytes<N>& c, float power) {
+  if constexpr (BITS == 4) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.w[I / 4], power, I % 4));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.w[I / 2], power, I % 2 == 1));
+}
+
+template <int BITS, int N, int COUNT, int I = 0>
+__device__ __forceinline__ void pairs_of(const Bytes<N>& c, float power, uint32_t* out) {
+  if constexpr (I < COUNT) {
+    out[I] = pair_at<BITS, I>(c, power);
+    pairs_of<BITS, N, COUNT, I + 1>(c, power, out);
+  }
+}
+
+__device__ __forceinline__ bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(bf16x8, uint4{a, b, c, d});
+}
+
+__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
+
+// x as bf16 parts whose sum it is (the third one takes what is left to its last bit)
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+  for (int n = 0; n < PARTS; ++n) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack2(rest[2 * i], rest[2 * i + 1]);
+      if (n + 1 < PARTS) {
+        // (what is left of an infinity is nothing)
+        const float lo = __builtin_bit_cast(float, w[i] << 16), hi = __builtin_bit_cast(float, w[i] & 0xffff0000u);
+        rest[2 * i] = __builtin_isinf(lo) ? 0.f : rest[2 * i] - lo;
+        rest[2 * i + 1] = __builtin_isinf(hi) ? 0.f : rest[2 * i + 1] - hi;
+      }
+    }
+    out[n] = operand(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <int DP, int BITS, bool F32, int NQ>
+__global__ __launch_bounds__(THREADS) void hstu_cached_attn_kernel(const Params p) {
+  constexpr int QP = F32 ? 3 : 1;             // bf16 parts of queries and weights
+  constexpr int KS = DP / 32;                 // matrix steps along d
+  constexpr int KB = DP / 4 * BITS / 8;       // bytes of a lane's run of a key
+  constexpr int KBLK = DP > 128 ? 2 : 1;      // blocks of exponents in it
+  constexpr int VN = DP / 16;                 // dims of a lane's run of a value
+  constexpr int VB = VN * BITS / 8;
+  constexpr int ACC = VN * 4 * NQ;            // accumulators of a lane
+  extern __shared__ float lds[];              // sums of two waves [2][ACC][64]; before that the timestamp tables
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int H = p.g.H, d = p.g.d, page = p.g.page_size;
+  int idx = blockIdx.x;
+  const int h = idx % H; idx /= H;
+  const int part = idx % p.parts; idx /= p.parts;
+  const int qb = idx % p.qblocks, b = idx / p.qblocks;
+  const Seq s = seq_of(p, b);
+  const int t0 = qb * 16 * NQ;
+  if (t0 >= s.count) return;
+  const int t1 = t0 + 16 * NQ < s.count ? t0 + 16 * NQ : s.count;
+  // the block's keys: those of its last row that is there
+  int end = 0;
+  {
+    const int64_t last = s.place0 + t1 - 1;
+    end = last < 0 ? 0 : last < s.limit ? (int)last + 1 : s.limit;
+    if (s.place0 + t0 >= s.limit) end = 0;
+  }
+  const int k0 = part * p.chunk;
+  if (part > 0 && k0 >= end) return;
+  const int k1 = end - k0 < p.chunk ? end : k0 + p.chunk;
+
+  if (p.ts) {
+    int32_t* const thr = (int32_t*)lds;
+    float* const tab = lds + MAX_BUCKETS + 2;
+    for (int i = threadIdx.x; i < MAX_BUCKETS + 2; i += THREADS) thr[i] = p.thr[i];
+    for (int i = threadIdx.x; i <= p.ts_buckets; i += THREADS) tab[i] = p.ts_tab[(int64_t)(p.ts_heads > 1 ? h : 0) * (p.ts_buckets + 1) + i];
+    __syncthreads();
+  }
+
+  // queries: lane (r, g) has row r's dims g d/4 ... of each tile
+  bf16x8 q[NQ][KS][QP];
+  int keys[NQ];
+  int64_t tq[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int t = t0 + 16 * n + r;
+    keys[n] = keys_of(s, t);
+    const int64_t row = (p.offsets ? s.first * p.q_st : (int64_t)b * p.q_sb) + (int64_t)t * p.q_st + (int64_t)h * p.q_sh;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int e = g * (DP / 4) + 8 * k;
+      float x[8] = {};
+      if (keys[n] > 0 && e < d) {
+        if constexpr (F32) {
+          const floatx4* at = (const floatx4*)((const float*)p.q + row + e);
+          const floatx4 a = at[0], c = at[1];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = c[i]; }
+        } else {
+          unpack8(*(const uint4*)((const bf16_t*)p.q + row + e), x);
+        }
+      }
+      split8<QP>(x, q[n][k]);
+    }
+    tq[n] = 0;
+    if (p.ts && keys[n] > 0) tq[n] = p.ts[(int64_t)b * p.max_len + (keys[n] < s.last_ts ? keys[n] : s.last_ts)];
+  }
+
+  floatx4 acc[NQ][VN];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int j = 0; j < VN; ++j) acc[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  const int row_bytes = d * BITS / 8, blocks = (d + 31) / 32;
+  const uint8_t* const kc = (const uint8_t*)p.g.k_codes;
+  const uint8_t* const vc = (const uint8_t*)p.g.v_codes;
+  const uint8_t* const ks = (const uint8_t*)p.g.k_scales;
+  const uint8_t* const vs = (const uint8_t*)p.g.v_scales;
+  const bool k_there = g * (DP / 4) < d, v_there = r * VN < d;
+  const float* const pos = p.pos ? p.pos + (int64_t)(p.pos_heads > 1 ? h : 0) * (2 * (int64_t)p.max_len - 1) : nullptr;
+
+  for (int key0 = k0 + STEP * wave; key0 < k1; key0 += STEP * WAVES) {
+    const int at = key0 / page, slot0 = key0 - at * page;
+    const int id = __builtin_amdgcn_readfirstlane(p.g.page_table[(int64_t)b * p.g.table_pages + at]);
+    if (id < 0 || id >= p.g.n_pages) continue;
+    const int64_t head = (int64_t)id * H + h;
+    const uint8_t* const kr = kc + (head * page + slot0) * row_bytes;
+    const uint8_t* const vr = vc + (head * page + slot0) * row_bytes + r * VB;
+    const uint8_t* const kx = ks + head * blocks * page + slot0;
+    const uint8_t* const vx = vs + head * blocks * page + slot0 + 8 * g;
+
+    Bytes<KB> kraw[2] = {};
+    uint32_t ke[2][KBLK] = {};
+    if (k_there) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int key = 8 * (r >> 2) + 4 * t + (r & 3);
+        kraw[t] = load_bytes<KB>(kr + key * row_bytes + g * KB);
+#pragma unroll
+        for (int m = 0; m < KBLK; ++m) ke[t][m] = kx[(g * (DP / 4) / 32 + m) * page + key];
+      }
+    }
+    Bytes<VB> vraw[8] = {};
+    uint32_t ve[2];
+    if (v_there) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vraw[i] = load_bytes<VB>(vr + (8 * g + i) * row_bytes);
+    }
+    {
+      const uint2 e = *(const uint2*)(vx + (r * VN / 32 < blocks ? r * VN / 32 : blocks - 1) * page);
+      ve[0] = e.x; ve[1] = e.y;
+    }
+    // rows past the block's last key hold anything: zeros in their place
+    if (key0 + STEP > k1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (key0 + 8 * g + i >= k1) {
+#pragma unroll
+          for (uint32_t& w : vraw[i].w) w = 0;
+          ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
+        }
+    }
+    // a value row that is not finite makes the kept weights of its key NaN instead (0 times it would be NaN for the others)
+    uint32_t nan_keys = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nan_keys |= ((ve[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu ? 1u << i : 0u;
+
+    floatx4 st[2][NQ];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t w[DP / 8];
+#pragma unroll
+      for (int m = 0; m < KBLK; ++m) {
+        const float power = ke[t][m] == 255u ? __builtin_nanf("") : power_of(ke[t][m]);
+        // (a run of two blocks: half of its bytes each)
+        constexpr int HALF = KB / KBLK;
+        Bytes<HALF> half;
+#pragma unroll
+        for (int i = 0; i < (HALF < 4 ? 1 : HALF / 4); ++i) half.w[i] = kraw[t].w[m * (HALF / 4) + i];
+        pairs_of<BITS, HALF, DP / 8 / KBLK>(half, power, w + m * (DP / 8 / KBLK));
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) st[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const bf16x8 a = operand(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int c = 0; c < QP; ++c) st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[n][k][c], st[t][n], 0, 0, 0);
+      }
+    }
+
+    bf16x8 w8[NQ][QP];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p.alpha * st[i / 4][n][i % 4];
+      const int j0 = key0 + 8 * g;                       // the lane's keys: j0 .. j0 + 7
+      if (pos) {
+        // (kept pairs lie inside the table; the others read its ends)
+        const int64_t top = 2 * ((int64_t)p.max_len - 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          int64_t e = (int64_t)p.max_len + j0 + i - keys[n];
+          e = e < 0 ? 0 : e > top ? top : e;
+          x[i] += pos[e];
+        }
+      }
+      if (p.ts) {
+        const int32_t* const thr = (const int32_t*)lds;
+        const float* const tab = lds + MAX_BUCKETS + 2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = j0 + i < p.max_len ? j0 + i : p.max_len - 1;
+          int64_t gap = tq[n] - p.ts[(int64_t)b * p.max_len + j];
+          gap = gap < 0 ? -gap : gap;
+          const int dt = gap < 1 ? 1 : gap > 1000000000 ? 1000000000 : (int)gap;
+          int bk = (int)(__builtin_amdgcn_logf((float)dt) * p.buckets_per_log2);
+          bk = bk < 0 ? 0 : bk > p.ts_buckets ? p.ts_buckets : bk;
+          bk = dt < thr[bk] ? bk - 1 : dt >= thr[bk + 1] ? bk + 1 : bk;
+          x[i] += tab[bk];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float y = silu(x[i]);
+        if (nan_keys >> i & 1u) y = __builtin_nanf("");
+        x[i] = j0 + i < keys[n] ? y : 0.f;
+      }
+      split8<QP>(x, w8[n]);
+    }
+
+    uint32_t pairs[8][VN / 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t e = (ve[i / 4] >> (8 * (i % 4))) & 0xffu;
+      pairs_of<BITS, VB, VN / 2>(vraw[i], power_of(e == 255u ? 127u : e), pairs[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        w[m] = __builtin_amdgcn_perm(pairs[2 * m + 1][j / 2], pairs[2 * m][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+      const bf16x8 a = operand(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int c = 0; c < QP; ++c) acc[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w8[n][c], acc[n][j], 0, 0, 0);
+    }
+  }
+
+  // the four waves' sums, in a fixed order: 2 and 3 onto 0 and 1, then 1 onto 0
+  __syncthreads();
+  auto put = [&](float* to) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int j = 0; j < VN; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[((n * VN + j) * 4 + i) * 64 + lane] = acc[n][j][i];
+  };
+  auto add = [&](const float* from) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int j = 0; j < VN; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][j][i] += from[((n * VN + j) * 4 + i) * 64 + lane];
+  };
+  if (wave >= 2) put(lds + (wave - 2) * ACC * 64);
+  __syncthreads();
+  if (wave < 2) add(lds + wave * ACC * 64);
+  __syncthreads();
+  if (wave == 1) put(lds);
+  __syncthreads();
+  if (wave != 0) return;
+  add(lds);
+
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int t = t0 + 16 * n + r;
+    if (t >= s.count) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = (4 * g + i) * VN;        // dims e .. e + VN - 1
+      if (e >= d) continue;
+      if (p.partial) {
+        float* to = p.partial + (((s.first + t) * H + h) * p.parts + part) * d + e;
+#pragma unroll
+        for (int j = 0; j < VN; j += 2) *(floatx2*)(to + j) = floatx2{acc[n][j][i], acc[n][j + 1][i]};
+      } else {
+        const int64_t to = (p.offsets ? s.first * p.o_st : (int64_t)b * p.o_sb) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + e;
+#pragma unroll
+        for (int j = 0; j < VN; j += 2) {
+          const float y0 = acc[n][j][i] * p.inv_n, y1 = acc[n][j + 1][i] * p.inv_n;
+          if constexpr (F32) *(floatx2*)((float*)p.out + to + j) = floatx2{y0, y1};
+          else *(uint32_t*)((bf16_t*)p.out + to + j) = pack2(y0, y1);
+        }
+      }
+    }
+  }
+}
+
+// The parts of a row, added in order: a thread has four dims of one (row, head).
+template <bool F32>
+__global__ __launch_bounds__(THREADS) void hstu_cached_attn_join(const Params p) {
+  const int H = p.g.H, d4 = p.g.d / 4;
+  const int64_t per = (int64_t)p.per_seq * H * d4;
+  const int64_t groups = (per + THREADS - 1) / THREADS;
+  const int b = (int)(blockIdx.x / groups);
+  int64_t e = (blockIdx.x % groups) * THREADS + threadIdx.x;
+  if (e >= per) return;
+  const int c = (int)(e % d4); e /= d4;
+  const int h = (int)(e % H), t = (int)(e / H);
+  const Seq s = seq_of(p, b);
+  if (t >= s.count) return;
+  const int n = (keys_of(s, t) + p.chunk - 1) / p.chunk;
+  const floatx4* from = (const floatx4*)(p.partial + ((s.first + t) * H + h) * p.parts * (int64_t)p.g.d) + c;
+  floatx4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int m = 0; m < n; ++m) y += from[(int64_t)m * d4];
+  const int64_t to = (p.offsets ? s.first * p.o_st : (int64_t)b * p.o_sb) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 4 * c;
+  y *= p.inv_n;
+  if constexpr (F32) *(floatx4*)((float*)p.out + to) = y;
+  else *(uint2*)((bf16_t*)p.out + to) = uint2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+}
+
+// The bucket law's integer thresholds up to bucket `count`: thr[b] is the smallest time difference in [1, 1e9] whose bucket
+// floor(ln(fl32(dt)) / size) is b or more (INT32_MAX: none).
+void thresholds(float size, int count, int32_t* out) {
+  static std::mutex lock;
+  static float known = -1.f;
+  static int32_t table[MAX_BUCKETS + 2];
+  std::lock_guard<std::mutex> hold(lock);
+  if (known != size) {
+    auto bucket = [size](int32_t dt) { return floor(log((double)(float)dt) / (double)size); };
+    int32_t lo = 1;
+    for (int b = 0; b < MAX_BUCKETS + 2; ++b) {
+      if (bucket(1000000000) < b) { table[b] = 0x7fffffff; continue; }
+      int32_t x = lo, y = 1000000000;              // the answer lies in [x, y]
+      while (x < y) {
+        const int32_t m = x + (y - x) / 2;
+        if (bucket(m) >= b) y = m; else x = m + 1;
+      }
+      table[b] = lo = x;
+    }
+    known = size;
+  }
+  for (int b = 0; b < MAX_BUCKETS + 2; ++b) out[b] = b <= count ? table[b] : 0x7fffffff;
+}
+
+struct Split { int nq, qblocks, parts, chunk; };
+
+// How a call is cut up, by its sizes alone (the lengths are on the device).
+Split split_of(const HstuCachedAttnArgs& a) {
+  Split s;
+  const bool f32 = a.dtype == HSTU_SERVE_FP32;
+  const int most = a.pages.d > 128 ? (f32 ? 1 : 2) : f32 ? 2 : 4;
+  s.nq = a.rows_per_seq > 32 ? 4 : a.rows_per_seq > 16 ? 2 : 1;
+  s.nq = std::min(s.nq, most);
+  s.qblocks = (a.rows_per_seq + 16 * s.nq - 1) / (16 * s.nq);
+  const int64_t cap = std::min<int64_t>(a.max_len, (int64_t)a.pages.table_pages * a.pages.page_size);
+  const int64_t base = (int64_t)a.pages.B * a.pages.H * s.qblocks;
+  int64_t parts = (2048 + base - 1) / base;
+  parts = std::max<int64_t>(1, std::min(parts, (cap + 255) / 256));
+  const int64_t chunk = std::max<int64_t>(128, ((cap + parts - 1) / parts + 127) / 128 * 128);
+  s.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
+  s.parts = (int)std::max<int64_t>(1, (cap + s.chunk - 1) / s.chunk);
+  return s;
+}
+
+int check(const HstuCachedAttnArgs* a) {
+  if (!a) return serve_fail(HSTU_SERVE_ERR_NULL, "args is null");
+  if (a->struct_size != sizeof(HstuCachedAttnArgs) || a->version != HSTU_SERVE_ABI_VERSION)
+    return serve_fail(HSTU_SERVE_ERR_VERSION, "struct_size %u version %u, expected %zu and %d", a->struct_size, a->version, sizeof(HstuCachedAttnArgs), HSTU_SERVE_ABI_VERSION);
+  if (const int rc = serve_check_pages(a->pages)) return rc;
+  if (a->dtype != HSTU_SERVE_BF16 && a->dtype != HSTU_SERVE_FP32) return serve_fail(HSTU_SERVE_ERR_SHAPE, "dtype %d", a->dtype);
+  if (a->rows_per_seq < 0 || a->total_rows < 0 || a->max_len < 1) return serve_fail(HSTU_SERVE_ERR_SHAPE, "rows_per_seq=%d total_rows=%lld max_len=%d", a->rows_per_seq, (long long)a->total_rows, a->max_len);
+  if (a->max_len > 1 << 30 || a->rows_per_seq > 1 << 30) return serve_fail(HSTU_SERVE_ERR_SHAPE, "rows_per_seq=%d max_len=%d: at most 2^30", a->rows_per_seq, a->max_len);
+  if (a->pos_tab && a->pos_heads != 1 && a->pos_heads != a->pages.H) return serve_fail(HSTU_SERVE_ERR_SHAPE, "pos_heads=%d: 1 or %d", a->pos_heads, a->pages.H);
+  if (a->timestamps) {
+    if (!a->ts_tab) return serve_fail(HSTU_SERVE_ERR_NULL, "ts_tab is null");
+    if (a->ts_heads != 1 && a->ts_heads != a->pages.H) return serve_fail(HSTU_SERVE_ERR_SHAPE, "ts_heads=%d: 1 or %d", a->ts_heads, a->pages.H);
+    if (a->ts_buckets < 0 || a->ts_buckets > MAX_BUCKETS) return serve_fail(HSTU_SERVE_ERR_SHAPE, "ts_buckets=%d: at most %d", a->ts_buckets, MAX_BUCKETS);
+    if (!(a->ts_bucket_size > 0.f)) return serve_fail(HSTU_SERVE_ERR_SHAPE, "ts_bucket_size must be positive");
+  }
+  return HSTU_SERVE_OK;
+}
+
+bool nothing(const HstuCachedAttnArgs& a) { return a.pages.B == 0 || a.rows_per_seq == 0 || (a.offsets && a.total_rows == 0); }
+
+size_t workspace_of(const HstuCachedAttnArgs& a, const Split& s) {
+  if (s.parts == 1) return 0;
+  const int64_t rows = a.offsets ? a.total_rows : (int64_t)a.pages.B * a.rows_per_seq;
+  return (size_t)rows * a.pages.H * s.parts * a.pages.d * sizeof(float);
+}
+
+template <int DP, int BITS, bool F32, int NQ>
+void launch(const Params& p, uint32_t grid, hipStream_t st) {
+  constexpr int ACC = DP / 16 * 4 * NQ;
+  const size_t lds = std::max<size_t>((size_t)2 * ACC * 64 * sizeof(float), (2 * MAX_BUCKETS + 4) * sizeof(float));
+  hstu_cached_attn_kernel<DP, BITS, F32, NQ><<<grid, THREADS, lds, st>>>(p);
+}
+
+template <int DP, int BITS>
+void launch_nq(const Params& p, bool f32, int nq, uint32_t grid, hipStream_t st) {
+  if (f32) {
+    if constexpr (DP <= 128) { if (nq == 2) return launch<DP, BITS, true, 2>(p, grid, st); }
+    return launch<DP, BITS, true, 1>(p, grid, st);
+  }
+  if constexpr (DP <= 128) { if (nq == 4) return launch<DP, BITS, false, 4>(p, grid, st); }
+  if (nq == 2) return launch<DP, BITS, false, 2>(p, grid, st);
+  launch<DP, BITS, false, 1>(p, grid, st);
+}
+
+template <int BITS>
+void launch_width(const Params& p, bool f32, int nq, uint32_t grid, hipStream_t st) {
+  if (p.g.d <= 32) launch_nq<32, BITS>(p, f32, nq, grid, st);
+  else if (p.g.d <= 64) launch_nq<64, BITS>(p, f32, nq, grid, st);
+  else if (p.g.d <= 128) launch_nq<128, BITS>(p, f32, nq, grid, st);
+  else launch_nq<256, BITS>(p, f32, nq, grid, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t hstu_cached_attn_workspace_bytes(const HstuCachedAttnArgs* a) {
+  serve_clear_error();
+  if (check(a) || nothing(*a)) return 0;
+  return workspace_of(*a, split_of(*a));
+}
+
+int hstu_cached_attn(const HstuCachedAttnArgs* a, void* stream) {
+  serve_clear_error();
+  if (const int rc = check(a)) return rc;
+  if (nothing(*a)) return HSTU_SERVE_OK;
+  if (!a->lengths || !a->q || !a->out) return serve_fail(HSTU_SERVE_ERR_NULL, "lengths, q or out is null");
+  const int64_t unit = a->dtype == HSTU_SERVE_FP32 ? 4 : 8;
+  for (const void* t : {a->q, (const void*)a->out})
+    if (!serve_aligned16(t)) return serve_fail(HSTU_SERVE_ERR_SHAPE, "q and out start on 16-byte boundaries");
+  for (const int64_t st : {a->q_stride_t, a->q_stride_h, a->o_stride_t, a->o_stride_h, a->offsets ? (int64_t)0 : a->q_stride_b, a->offsets ? (int64_t)0 : a->o_stride_b})
+    if (st % unit) return serve_fail(HSTU_SERVE_ERR_SHAPE, "a stride of %lld elements: rows start on 16-byte boundaries", (long long)st);
+  const Split s = split_of(*a);
+  const size_t need = workspace_of(*a, s);
+  if (need && (!a->workspace || a->workspace_bytes < need || !serve_aligned16(a->workspace)))
+    return serve_fail(HSTU_SERVE_ERR_WORKSPACE, "workspace of %zu bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
+  const int64_t grid = (int64_t)a->pages.B * a->pages.H * s.qblocks, most = 0x7fffffff;
+  const int64_t per = (int64_t)a->rows_per_seq * a->pages.H * (a->pages.d / 4), join = (per + THREADS - 1) / THREADS * a->pages.B;
+  if (grid > most / s.parts || join > most) return serve_fail(HSTU_SERVE_ERR_SHAPE, "too many workgroups for one call");
+  Params p;
+  p.g = a->pages;
+  p.lengths = a->lengths; p.offsets = a->offsets;
+  p.q = a->q; p.out = a->out;
+  p.total = a->total_rows;
+  p.q_sb = a->q_stride_b; p.q_st = a->q_stride_t; p.q_sh = a->q_stride_h;
+  p.o_sb = a->o_stride_b; p.o_st = a->o_stride_t; p.o_sh = a->o_stride_h;
+  p.pos = a->pos_tab; p.ts = a->timestamps; p.ts_tab = a->ts_tab;
+  p.partial = s.parts > 1 ? (float*)a->workspace : nullptr;
+  p.per_seq = a->rows_per_seq; p.max_len = a->max_len; p.pos_heads = a->pos_heads; p.ts_heads = a->ts_heads; p.ts_buckets = a->ts_buckets;
+  p.chunk = s.chunk; p.parts = s.parts; p.qblocks = s.qblocks;
+  p.alpha = a->alpha; p.inv_n = a->inv_n; p.buckets_per_log2 = 0.f;
+  if (a->timestamps) {
+    thresholds(a->ts_bucket_size, a->ts_buckets, p.thr);
+    p.buckets_per_log2 = (float)(0.69314718055994530942 / (double)a->ts_bucket_size);
+  }
+  hipStream_t st = (hipStream_t)stream;
+  const bool f32 = a->dtype == HSTU_SERVE_FP32;
+  if (a->pages.bits == 4) launch_width<4>(p, f32, s.nq, (uint32_t)(grid * s.parts), st);
+  else launch_width<8>(p, f32, s.nq, (uint32_t)(grid * s.parts), st);
+  if (const int rc = serve_launched("hstu_cached_attn")) return rc;
+  if (s.parts > 1) {
+    if (f32) hstu_cached_attn_join<true><<<(uint32_t)join, THREADS, 0, st>>>(p);
+    else hstu_cached_attn_join<false><<<(uint32_t)join, THREADS, 0, st>>>(p);
+    return serve_launched("hstu_cached_attn_join");
+  }
+  return HSTU_SERVE_OK;
+}
+
+}

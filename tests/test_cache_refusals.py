@@ -1,0 +1,103 @@
+"""What the cache's entry points refuse, before any work (no GPU)."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import recml_amd
+from recml_amd import _lib_serve
+
+
+def _rows_args(**kw):
+  a = _lib_serve.HstuKvRowsArgs()
+  a.struct_size, a.version = C.sizeof(a), _lib_serve.ABI_VERSION
+  _pages(a.pages)
+  a.starts, a.rows_per_seq, a.dtype, a.k, a.v = 0x1000, 3, _lib_serve.BF16, 0x2000, 0x3000
+  a.k_stride_b = a.v_stride_b = 3 * 128
+  a.k_stride_t = a.v_stride_t = 128
+  a.k_stride_h = a.v_stride_h = 64
+  return _set(a, kw)
+
+
+def _attn_args(**kw):
+  a = _lib_serve.HstuCachedAttnArgs()
+  a.struct_size, a.version = C.sizeof(a), _lib_serve.ABI_VERSION
+  _pages(a.pages)
+  a.lengths, a.rows_per_seq, a.dtype, a.q, a.out, a.max_len, a.alpha, a.inv_n = 0x1000, 1, _lib_serve.BF16, 0x2000, 0x3000, 4096, 1.0, 1.0
+  a.q_stride_b = a.o_stride_b = 128
+  a.q_stride_t = a.o_stride_t = 128
+  a.q_stride_h = a.o_stride_h = 64
+  return _set(a, kw)
+
+
+def _pages(g):
+  g.k_codes, g.k_scales, g.v_codes, g.v_scales, g.page_table = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000
+  g.n_pages, g.page_size, g.table_pages, g.B, g.H, g.d, g.bits = 128, 64, 64, 2, 2, 64, 4
+
+
+def _set(a, kw):
+  for name, value in kw.items():
+    setattr(a.pages if hasattr(a.pages, name) else a, name, value)
+  return a
+
+
+PAGES = [(dict(bits=6), -4, "bits"), (dict(d=40), -4, "d=40"), (dict(d=512), -4, "d=512"), (dict(page_size=48), -4, "page_size"), (dict(page_size=0), -4, "page_size"),
+         (dict(H=0), -4, "H=0"), (dict(k_codes=None), -1, "null"), (dict(v_scales=0x40008), -4, "16-byte"), (dict(page_table=None), -1, "page_table"),
+         (dict(struct_size=8), -2, "struct_size"), (dict(version=99), -2, "version"), (dict(dtype=7), -4, "dtype"), (dict(rows_per_seq=-1), -4, "rows_per_seq")]
+
+
+@pytest.mark.parametrize("change,status,word", PAGES + [(dict(starts=None), -1, "starts"), (dict(k=0x2004), -4, "16-byte"), (dict(v_stride_t=100), -4, "stride")])
+def test_rows_refused(change, status, word):
+  lib = _lib_serve.load()
+  for fn in (lib.hstu_kv_write, lib.hstu_kv_read):
+    assert fn(C.byref(_rows_args(**change)), None) == status
+    assert word in lib.hstu_serve_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,word", PAGES + [
+    (dict(lengths=None), -1, "lengths"), (dict(q=0x2002), -4, "16-byte"), (dict(o_stride_h=4), -4, "stride"), (dict(max_len=0), -4, "max_len"),
+    (dict(pos_tab=0x6000, pos_heads=3), -4, "pos_heads"), (dict(timestamps=0x6000), -1, "ts_tab"),
+    (dict(timestamps=0x6000, ts_tab=0x7000, ts_heads=1, ts_buckets=129, ts_bucket_size=0.3), -4, "ts_buckets"),
+    (dict(timestamps=0x6000, ts_tab=0x7000, ts_heads=1, ts_buckets=128, ts_bucket_size=0.0), -4, "ts_bucket_size"),
+    (dict(), -5, "workspace"), (dict(workspace=0x9000, workspace_bytes=64), -5, "workspace")])
+def test_attention_refused(change, status, word):
+  lib = _lib_serve.load()
+  assert lib.hstu_cached_attn(C.byref(_attn_args(**change)), None) == status
+  assert word in lib.hstu_serve_last_error().decode()
+
+
+def test_null_and_nothing_to_do():
+  lib = _lib_serve.load()
+  assert lib.hstu_kv_write(None, None) == -1 and lib.hstu_kv_read(None, None) == -1 and lib.hstu_cached_attn(None, None) == -1
+  for change in (dict(B=0), dict(rows_per_seq=0), dict(offsets=0x9000, total_rows=0)):
+    assert lib.hstu_kv_write(C.byref(_rows_args(**change)), None) == 0
+    assert lib.hstu_cached_attn(C.byref(_attn_args(**change)), None) == 0
+    assert lib.hstu_cached_attn_workspace_bytes(C.byref(_attn_args(**change))) == 0
+
+
+def test_workspace_grows_with_what_is_split():
+  lib = _lib_serve.load()
+  one = lib.hstu_cached_attn_workspace_bytes(C.byref(_attn_args()))
+  assert one > 0 and one % (2 * 2 * 64 * 4) == 0
+  assert lib.hstu_cached_attn_workspace_bytes(C.byref(_attn_args(max_len=64))) == 0
+  assert lib.hstu_cached_attn_workspace_bytes(C.byref(_attn_args(bits=3))) == 0
+
+
+def test_python_refuses_cpu_tensors_and_odd_pages():
+  with pytest.raises(ValueError, match="GPU"):
+    recml_amd.KVPages(*(torch.zeros((2, 2, 32, 32), dtype=torch.uint8) for _ in range(4)), head_dim=64)
+  with pytest.raises(ValueError, match="head_dim"):
+    recml_amd.KVPages(*(torch.zeros((2, 2, 32, 32), dtype=torch.uint8) for _ in range(4)), head_dim=40)
+  with pytest.raises(TypeError, match="KVPages"):
+    recml_amd.kv_write(None, None, None, None, None)
+  with pytest.raises(ValueError, match="bits"):
+    recml_amd.KVPages.empty(1, 32, 1, 32, bits=2)
+
+
+def test_header_and_binding_agree():
+  import os
+  import re
+  header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "hstu_serve.h")).read()
+  assert int(re.search(r"HSTU_SERVE_ABI_VERSION (\d+)", header).group(1)) == _lib_serve.ABI_VERSION
+  assert set(re.findall(r"^(?:int|size_t|const char\*) (hstu_\w+)\(", header, re.M)) == set(_lib_serve.EXPORTS)
