@@ -5,6 +5,9 @@
  *   hstu_cached_attn   the pointwise-SiLU attention (recml/layers/keras/hstu.py:356-390) of each
  *                      sequence's newest events over its kept keys and values
  *
+ *   hstu_log_probs_fwd log probabilities of given tokens, the entropy and the largest entries of rows of logits
+ *   hstu_log_probs_bwd the gradient of those for the logits
+ *
  * A cache's codes are [n_pages, H, page_size, d * bits / 8] bytes, its exponents
  * [n_pages, H, (d + 31) / 32, page_size] bytes, one pair for the keys and one for the values.  A block
  * of 32 values of one (event, head) row (the row's last block may be shorter) shares the power 2^(e - 127)
@@ -113,6 +116,43 @@ typedef struct HstuCachedAttnArgs {
 
 size_t hstu_cached_attn_workspace_bytes(const HstuCachedAttnArgs* args);
 int hstu_cached_attn(const HstuCachedAttnArgs* args, void* stream);
+
+/* Of each of `rows` rows of `vocab` logits (bf16 or fp32, row stride in elements, any alignment of the type):
+ *   log_probs[row][c] = x[tokens[row][c]] - ln sum_j exp x_j; 0 where the token is negative (nothing asked), NaN where it
+ *                  is past the vocabulary
+ *   entropy[row]   = -sum_j p_j ln p_j (or null)
+ *   top_log_probs, top_tokens: the `top` largest entries (at most 256) in falling order, ties by the lower token; NaN
+ *                  comes before all others
+ * A row whose sum of exponentials is not finite and positive (a NaN, +inf, nothing but -inf) has NaN for all of them.
+ * stats: [rows][3], what the backward needs (or null).
+ * The backward writes d_logits (typed like the logits) = sum over the outputs of their gradients times theirs by the
+ * logits: g_tokens [rows][count], g_entropy [rows], g_top [rows][top], each or null; tokens, top_tokens and stats as the
+ * forward had and left them.  The same token twice gets both gradients; negative tokens none; one past the vocabulary
+ * makes its row NaN.  The forward's workspace: hstu_log_probs_workspace_bytes(args) bytes; the backward has none. */
+typedef struct HstuLogProbsArgs {
+  uint32_t struct_size;   /* sizeof(HstuLogProbsArgs) */
+  uint32_t version;       /* HSTU_SERVE_ABI_VERSION   */
+  const void* logits;
+  int64_t rows, stride;
+  int32_t vocab, dtype, count, top;
+  const int64_t* tokens;  /* [rows][count] */
+  float* log_probs;
+  float* entropy;
+  float* stats;
+  float* top_log_probs;
+  int64_t* top_tokens;
+  const float* g_tokens;
+  const float* g_entropy;
+  const float* g_top;
+  void* d_logits;
+  int64_t d_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} HstuLogProbsArgs;
+
+size_t hstu_log_probs_workspace_bytes(const HstuLogProbsArgs* args);
+int hstu_log_probs_fwd(const HstuLogProbsArgs* args, void* stream);
+int hstu_log_probs_bwd(const HstuLogProbsArgs* args, void* stream);
 
 int hstu_serve_abi_version(void);
 const char* hstu_serve_last_error(void);

@@ -19,6 +19,9 @@ EXPORTS = (
     "hstu_kv_read",
     "hstu_cached_attn",
     "hstu_cached_attn_workspace_bytes",
+    "hstu_log_probs_fwd",
+    "hstu_log_probs_bwd",
+    "hstu_log_probs_workspace_bytes",
 )
 
 
@@ -63,6 +66,21 @@ class HstuCachedAttnArgs(C.Structure):
   ]
 
 
+class HstuLogProbsArgs(C.Structure):
+  """Field-for-field image of `struct HstuLogProbsArgs`."""
+
+  _fields_ = [
+      ("struct_size", C.c_uint32), ("version", C.c_uint32),
+      ("logits", C.c_void_p), ("rows", C.c_int64), ("stride", C.c_int64),
+      ("vocab", C.c_int32), ("dtype", C.c_int32), ("count", C.c_int32), ("top", C.c_int32),
+      ("tokens", C.c_void_p), ("log_probs", C.c_void_p), ("entropy", C.c_void_p), ("stats", C.c_void_p),
+      ("top_log_probs", C.c_void_p), ("top_tokens", C.c_void_p),
+      ("g_tokens", C.c_void_p), ("g_entropy", C.c_void_p), ("g_top", C.c_void_p),
+      ("d_logits", C.c_void_p), ("d_stride", C.c_int64),
+      ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+  ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -83,12 +101,15 @@ def load():
     lib.hstu_serve_abi_version.argtypes = []
     lib.hstu_serve_last_error.restype = C.c_char_p
     lib.hstu_serve_last_error.argtypes = []
-    for name, args in (("hstu_kv_write", HstuKvRowsArgs), ("hstu_kv_read", HstuKvRowsArgs), ("hstu_cached_attn", HstuCachedAttnArgs)):
+    for name, args in (("hstu_kv_write", HstuKvRowsArgs), ("hstu_kv_read", HstuKvRowsArgs), ("hstu_cached_attn", HstuCachedAttnArgs),
+                       ("hstu_log_probs_fwd", HstuLogProbsArgs), ("hstu_log_probs_bwd", HstuLogProbsArgs)):
       fn = getattr(lib, name)
       fn.restype = C.c_int
       fn.argtypes = [C.POINTER(args), C.c_void_p]
-    lib.hstu_cached_attn_workspace_bytes.restype = C.c_size_t
-    lib.hstu_cached_attn_workspace_bytes.argtypes = [C.POINTER(HstuCachedAttnArgs)]
+    for name, args in (("hstu_cached_attn_workspace_bytes", HstuCachedAttnArgs), ("hstu_log_probs_workspace_bytes", HstuLogProbsArgs)):
+      fn = getattr(lib, name)
+      fn.restype = C.c_size_t
+      fn.argtypes = [C.POINTER(args)]
     ver = lib.hstu_serve_abi_version()
     if ver != ABI_VERSION:
       raise RuntimeError(f"libhstu_serve.so has ABI {ver}, expected {ABI_VERSION}")

@@ -17,7 +17,7 @@ BLOCK_SOURCES = [os.path.join(_HERE, "csrc", "hstu_block.hip"), os.path.join(_HE
                  os.path.join(_HERE, "csrc", "hstu_block_small.hip")]
 # serving from kept histories and scoring of logits
 SERVE_LIB_PATH = os.path.join(LIB_DIR, "libhstu_serve.so")
-SERVE_SOURCES = [os.path.join(_HERE, "csrc", name) for name in ("hstu_cache.hip", "hstu_cached_attn.hip")]
+SERVE_SOURCES = [os.path.join(_HERE, "csrc", name) for name in ("hstu_cache.hip", "hstu_cached_attn.hip", "hstu_log_probs.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 # the block's microbenchmark: a stand-alone program (its own main), evidence for what bounds the kernel
 MICRO_PATH = os.path.join(LIB_DIR, "micro_fwd_stream")

@@ -1,0 +1,578 @@
+// Log probabilities of given tokens from rows of logits, with the rows' entropy and their largest entries, and the
+// gradient of all of these, for gfx950 (MI355X): see include/hstu_serve.h.
+//
+//   lse = m + ln s,  s = sum_j exp(x_j - m),  m = max_j x_j        lp_c = (x_c - m) - ln s
+//   entropy = ln s - t / s,  t = sum_j (x_j - m) exp(x_j - m)
+//   d/dx_j = -p_j (G + g_e (x_j - lse + entropy)) + the gradients given for j,  G = their sum over the row
+//
+// Each pass reads the logits once.  A workgroup takes up to 8 vectors of 16 bytes per thread and keeps them in registers: the
+// maximum is known before the first exponential, so nothing is rescaled, and the largest entries are looked for without reading
+// again.  Rows that are longer are split; a second kernel joins the parts in their order.
+//
+// The largest entries of a part: the k-th largest of the threads' maxima bounds the k-th largest entry from below, few entries
+// reach it, and each of those finds its rank by counting who comes before it (by value, then by index).  The bound comes from
+// ballots on 16 bits of the ordered value.  Rows with more ties than the list holds take one entry after the other instead.
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "hstu_serve_common.h"
+
+namespace {
+
+constexpr int VECS = 8;              // vectors of 16 bytes that a thread holds
+constexpr int CAP = 1024;            // entries that reach the bound at most, on the short way
+constexpr int MAX_TOP = 256;
+
+struct Params {
+  const void* logits;
+  int64_t stride;
+  const int64_t* tokens;             // [rows][count]
+  float* log_probs;                  // [rows][count]
+  float* entropy;                    // [rows] or null
+  float* stats;                      // [rows][3]: m, ln s, entropy
+  float* top_log_probs;              // [rows][top]
+  int64_t* top_tokens;               // [rows][top]
+  // one part of a row: m, s, t, and its largest entries
+  float* part_stats;                 // [rows][parts][3]
+  float* part_value;                 // [rows][parts][top]
+  int32_t* part_index;
+  // the backward
+  const float* g_tokens;
+  const float* g_entropy;
+  const float* g_top;
+  void* d_logits;
+  int64_t d_stride;
+  int64_t rows;
+  int32_t vocab, count, top, parts, vecs;
+};
+
+// ordered bits: larger floats have larger ones, any NaN the largest; -0 and 0 are one value
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+  return x != x ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// an entry's place in the order: by value, then by the lower index
+__device__ __forceinline__ uint64_t place_of(float x, int index) { return (uint64_t)ordered(x) << 32 | (uint32_t)(0x7fffffff - index); }
+
+template <bool F32>
+struct Vec {
+  static constexpr int N = F32 ? 4 : 8;
+  uint4 raw;
+  __device__ __forceinline__ float at(int i) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    if constexpr (F32) return __builtin_bit_cast(float, w[i]);
+    else return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+
+// Where a row's vectors lie: the row may start anywhere, its vectors are the memory's 16-byte pieces.  Vector v holds entries
+// v N - shift ..., those outside [0, vocab) belong to somebody else and are neither read nor written.
+template <bool F32>
+struct Row {
+  const char* base;
+  int shift, vectors, vocab;
+  __device__ __forceinline__ Row(const void* logits, int64_t stride, int64_t row, int n) {
+    constexpr int N = Vec<F32>::N, SIZE = F32 ? 4 : 2;
+    const char* at = (const char*)logits + row * stride * SIZE;
+    shift = (int)((uintptr_t)at & 15u) / SIZE;
+    base = at - shift * SIZE;
+    vocab = n;
+    vectors = (int)(((int64_t)n + shift + N - 1) / N);
+  }
+  __device__ __forceinline__ int first(int v) const { return v * Vec<F32>::N - shift; }
+  __device__ __forceinline__ bool whole(int v) const { return first(v) >= 0 && (int64_t)first(v) + Vec<F32>::N <= vocab; }
+  __device__ __forceinline__ Vec<F32> load(int v) const {
+    constexpr int N = Vec<F32>::N;
+    Vec<F32> r;
+    if (whole(v)) {
+      r.raw = *(const uint4*)(base + (int64_t)v * 16);
+      return r;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = F32 ? 0xff800000u : 0xff80ff80u;     // -inf
+    const int e = first(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (v >= vectors || e + i < 0 || e + i >= vocab) continue;
+      if constexpr (F32) w[i] = *(const uint32_t*)(base + (int64_t)v * 16 + 4 * i);
+      else {
+        const uint32_t half = *(const uint16_t*)(base + (int64_t)v * 16 + 2 * i);
+        w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | half << 16 : (w[i / 2] & 0xffff0000u) | half;
+      }
+    }
+    r.raw = uint4{w[0], w[1], w[2], w[3]};
+    return r;
+  }
+};
+
+template <int NT, typename F>
+__device__ __forceinline__ float block_reduce(float x, float* lds, F op) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) x = op(x, __shfl_xor(x, m, 64));
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) x = op(x, lds[w]);
+  }
+  return x;
+}
+
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+
+struct Chosen {
+  float value[CAP];
+  int32_t index[CAP];
+  float bound[4][2];
+  uint64_t best[4];
+  int n;
+};
+
+// The k-th largest of a wave's values by the upper 16 of their ordered bits, lower bits zero (0: there are fewer).
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t next = found | 1u << bit;
+    if (__popcll(__ballot(key >= next)) >= k) found = next;
+  }
+  return found;
+}
+
+// The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  each(f) calls f(x, index) for a
+// thread's entries; there are at least k.
+template <int NT, typename Each, typename Out>
+__device__ __forceinline__ void select_top(int k, Chosen& c, Each each, Out out) {
+  constexpr int W = NT / 64;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  uint32_t most = 0;                       // (0: no entry; the least of an entry is that of -inf)
+  each([&](float x, int) { const uint32_t o = ordered(x); most = o > most ? o : most; });
+  // every wave has its share of the k, or one wave has all of them: either way k entries reach the bound
+  const uint32_t share = kth_of_wave(most, (k + W - 1) / W), all = W > 1 && k <= 64 ? kth_of_wave(most, k) : 0;
+  __syncthreads();
+  if (threadIdx.x == 0) c.n = 0;
+  if (lane == 0) {
+    c.bound[wave][0] = __builtin_bit_cast(float, share);
+    c.bound[wave][1] = __builtin_bit_cast(float, all);
+  }
+  __syncthreads();
+  uint32_t least = 0xffffffffu, best = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, c.bound[w][0]), b = __builtin_bit_cast(uint32_t, c.bound[w][1]);
+    least = a < least ? a : least;
+    best = b > best ? b : best;
+  }
+  const uint32_t bound = least > best ? least : best;
+  if (most != 0 && most >= bound) {
+    each([&](float x, int index) {
+      if (ordered(x) >= bound) {
+        const int at = atomicAdd(&c.n, 1);
+        if (at < CAP) { c.value[at] = x; c.index[at] = index; }
+      }
+    });
+  }
+  __syncthreads();
+  const int n = c.n;
+  if (n <= CAP) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const float x = c.value[i];
+      const int index = c.index[i];
+      const uint64_t mine = place_of(x, index);
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += place_of(c.value[j], c.index[j]) > mine;
+      if (rank < k) out(rank, x, index);
+    }
+    __syncthreads();
+    return;
+  }
+  // one after the other: the largest that comes behind the last one
+  uint64_t last = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    uint64_t mine = 0;
+    float value = 0.f;
+    int at = 0;
+    each([&](float x, int index) {
+      const uint64_t p = place_of(x, index);
+      if (p < last && p > mine) { mine = p; value = x; at = index; }
+    });
+    uint64_t all_best = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint64_t o = __shfl_xor(all_best, m, 64);
+      all_best = o > all_best ? o : all_best;
+    }
+    __syncthreads();
+    if (lane == 0) c.best[wave] = all_best;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) all_best = c.best[w] > all_best ? c.best[w] : all_best;
+    if (mine == all_best && mine != 0) out(r, value, at);
+    last = all_best;
+  }
+  __syncthreads();
+}
+
+// m + ln s and the entropy of a row from its sums; m = -inf stands for a row without any finite entry.
+__device__ __forceinline__ float entropy_of(float log_s, float s, float t) { return log_s - t / s; }
+
+template <bool F32>
+__device__ __forceinline__ float logit_at(const Params& p, int64_t row, int64_t index) {
+  const int64_t at = row * p.stride + index;
+  if constexpr (F32) return ((const float*)p.logits)[at];
+  else return (float)((const bf16_t*)p.logits)[at];
+}
+
+// What is asked of a row once its sums are known.
+template <bool F32, int NT>
+__device__ __forceinline__ void finish(const Params& p, int64_t row, float m, float s, float t) {
+  const float log_s = __logf(s), entropy = entropy_of(log_s, s, t);
+  if (threadIdx.x == 0) {
+    if (p.stats) { p.stats[row * 3] = m; p.stats[row * 3 + 1] = log_s; p.stats[row * 3 + 2] = entropy; }
+    if (p.entropy) p.entropy[row] = entropy;
+  }
+  for (int c = threadIdx.x; c < p.count; c += NT) {
+    const int64_t token = p.tokens[row * p.count + c];
+    float y = 0.f;                                             // (nothing asked)
+    if (token >= p.vocab) y = __builtin_nanf("");
+    else if (token >= 0) y = (logit_at<F32>(p, row, token) - m) - log_s;
+    p.log_probs[row * p.count + c] = y;
+  }
+}
+
+template <bool F32, int NT>
+__global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
+  constexpr int N = Vec<F32>::N;
+  __shared__ Chosen chosen;
+  __shared__ float sums[4];
+  const int64_t row = blockIdx.x / p.parts;
+  const int part = blockIdx.x % p.parts;
+  const Row<F32> r(p.logits, p.stride, row, p.vocab);
+  const int v0 = part * p.vecs * NT + threadIdx.x;
+  Vec<F32> x[VECS];
+#pragma unroll
+  for (int c = 0; c < VECS; ++c)
+    if (c < p.vecs) x[c] = r.load(v0 + c * NT);
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int c = 0; c < VECS; ++c)
+    if (c < p.vecs) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = fmaxf(m, x[c].at(i));
+    }
+  m = block_reduce<NT>(m, sums, larger);
+  const float zero = m == -__builtin_inff() ? 0.f : m;         // (a part without any entry above -inf sums to nothing)
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int c = 0; c < VECS; ++c)
+    if (c < p.vecs) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = x[c].at(i) - zero, e = __builtin_amdgcn_exp2f(d * LOG2E);
+        s += e;
+        t += e > 0.f ? d * e : 0.f;
+      }
+    }
+  s = block_reduce<NT>(s, sums, add);
+  t = block_reduce<NT>(t, sums, add);
+  if (p.parts == 1) {
+    finish<F32, NT>(p, row, m, s, t);
+  } else if (threadIdx.x == 0) {
+    float* to = p.part_stats + (row * p.parts + part) * 3;
+    to[0] = m; to[1] = s; to[2] = t;
+  }
+  if (p.top == 0) return;
+  // a part shorter than `top` gives what it has
+  const int64_t e0 = (int64_t)part * p.vecs * NT * N - r.shift, e1 = e0 + (int64_t)p.vecs * NT * N;
+  const int64_t here = (e1 < p.vocab ? e1 : p.vocab) - (e0 > 0 ? e0 : 0);
+  const int k = here < p.top ? (here > 0 ? (int)here : 0) : p.top;
+  const float log_s = __logf(s);
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int c = 0; c < VECS; ++c)
+      if (c < p.vecs) {
+        const int e = r.first(v0 + c * NT);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (e + i >= 0 && e + i < p.vocab) f(x[c].at(i), e + i);
+      }
+  };
+  if (p.parts == 1) {
+    select_top<NT>(k, chosen, each, [&](int rank, float value, int index) {
+      p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
+      p.top_tokens[row * p.top + rank] = index;
+    });
+  } else {
+    const int64_t to = (row * p.parts + part) * p.top;
+    for (int i = k + threadIdx.x; i < p.top; i += NT) p.part_index[to + i] = -1;
+    if (k > 0)
+      select_top<NT>(k, chosen, each, [&](int rank, float value, int index) {
+        p.part_value[to + rank] = value;
+        p.part_index[to + rank] = index;
+      });
+  }
+}
+
+// One row's parts: their sums in order, and the largest of their largest.
+template <bool F32>
+__global__ __launch_bounds__(256) void hstu_log_probs_join(const Params p) {
+  constexpr int NT = 256, E = 4;
+  __shared__ Chosen chosen;
+  __shared__ float sums[4];
+  __shared__ float best_value[MAX_TOP];
+  __shared__ int32_t best_index[MAX_TOP];
+  const int64_t row = blockIdx.x;
+  const float* from = p.part_stats + row * p.parts * 3;
+  float m = -__builtin_inff();
+  for (int i = threadIdx.x; i < p.parts; i += NT) m = fmaxf(m, from[3 * i]);
+  m = block_reduce<NT>(m, sums, larger);
+  const float zero = m == -__builtin_inff() ? 0.f : m;
+  float s = 0.f, t = 0.f;
+  for (int i = threadIdx.x; i < p.parts; i += NT) {
+    // a part's sums are about its own maximum: sum (x - m) e = scale (t + (its m - m) s)
+    const float d = from[3 * i] - zero, scale = __builtin_amdgcn_exp2f(d * LOG2E), ps = from[3 * i + 1];
+    s += scale * ps;
+    t += scale > 0.f ? scale * (from[3 * i + 2] + d * ps) : ps == ps ? 0.f : ps;
+  }
+  s = block_reduce<NT>(s, sums, add);
+  t = block_reduce<NT>(t, sums, add);
+  finish<F32, NT>(p, row, m, s, t);
+  if (p.top == 0) return;
+  const float log_s = __logf(s);
+  const int64_t base = row * p.parts * p.top, total = (int64_t)p.parts * p.top;
+  int have = 0;                        // the best of the entries so far, in LDS
+  for (int64_t done = 0; done < total;) {
+    const int room = NT * E - have;
+    const int take = total - done < room ? (int)(total - done) : room;
+    float x[E];
+    int index[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = e * NT + threadIdx.x;
+      index[e] = -1;
+      x[e] = 0.f;
+      if (i < have) { x[e] = best_value[i]; index[e] = best_index[i]; }
+      else if (i < have + take) { index[e] = p.part_index[base + done + i - have]; if (index[e] >= 0) x[e] = p.part_value[base + done + i - have]; }
+    }
+    __syncthreads();
+    float there = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) there += index[e] >= 0 ? 1.f : 0.f;
+    const int n = (int)block_reduce<NT>(there, sums, add);
+    const int k = n < p.top ? n : p.top;
+    done += take;
+    const bool end = done >= total;
+    if (k > 0)
+      select_top<NT>(k, chosen, [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (index[e] >= 0) f(x[e], index[e]);
+      }, [&](int rank, float value, int at) {
+        if (end) {
+          p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
+          p.top_tokens[row * p.top + rank] = at;
+        } else {
+          best_value[rank] = value;
+          best_index[rank] = at;
+        }
+      });
+    have = k;
+    __syncthreads();
+  }
+}
+
+template <bool F32, int NT>
+__global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
+  constexpr int N = Vec<F32>::N, SIZE = F32 ? 4 : 2;
+  __shared__ uint32_t hit[NT * VECS * N / 32];
+  __shared__ float sums[4];
+  const int64_t row = blockIdx.x / p.parts;
+  const int part = blockIdx.x % p.parts;
+  const Row<F32> r(p.logits, p.stride, row, p.vocab);
+  const int v0 = part * p.vecs * NT;
+  // the gradients' sum, and which of the part's entries have one of their own
+  const int64_t e0 = (int64_t)v0 * N - r.shift;
+  for (int i = threadIdx.x; i < NT * p.vecs * N / 32; i += NT) hit[i] = 0;
+  __syncthreads();
+  float total = 0.f;
+  auto mark = [&](int64_t index) {
+    const int64_t at = index - e0;
+    if (at >= 0 && at < (int64_t)NT * p.vecs * N) atomicOr(&hit[at / 32], 1u << (at % 32));
+  };
+  if (p.g_tokens)
+    for (int c = threadIdx.x; c < p.count; c += NT) {
+      const int64_t token = p.tokens[row * p.count + c];
+      if (token < 0) continue;
+      total += token < p.vocab ? p.g_tokens[row * p.count + c] : __builtin_nanf("");
+      mark(token);
+    }
+  if (p.g_top)
+    for (int c = threadIdx.x; c < p.top; c += NT) {
+      total += p.g_top[row * p.top + c];
+      mark(p.top_tokens[row * p.top + c]);
+    }
+  total = block_reduce<NT>(total, sums, add);
+  __syncthreads();
+  const float m = p.stats[row * 3], log_s = p.stats[row * 3 + 1], entropy = p.stats[row * 3 + 2];
+  const float ge = p.g_entropy ? p.g_entropy[row] : 0.f;
+  char* const out = (char*)p.d_logits + row * p.d_stride * SIZE;
+  const bool apart = (((uintptr_t)out ^ (uintptr_t)((const char*)p.logits + row * p.stride * SIZE)) & 15u) != 0;
+  for (int c = 0; c < p.vecs; ++c) {
+    const int v = v0 + c * NT + threadIdx.x;
+    if (v >= r.vectors) break;
+    const Vec<F32> x = r.load(v);
+    float y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float lp = (x.at(i) - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
+      y[i] = -pr * (total + (pr == 0.f ? 0.f : ge * (lp + entropy)));
+    }
+    const int e = r.first(v), at = (c * NT + threadIdx.x) * N;
+    uint32_t mine = hit[at / 32] >> (at % 32) & ((1u << N) - 1u);
+    while (mine) {
+      const int i = __builtin_ctz(mine);
+      mine &= mine - 1;
+      float more = 0.f;
+      if (p.g_tokens)
+        for (int k = 0; k < p.count; ++k)
+          if (p.tokens[row * p.count + k] == e + i) more += p.g_tokens[row * p.count + k];
+      if (p.g_top)
+        for (int k = 0; k < p.top; ++k)
+          if (p.top_tokens[row * p.top + k] == e + i) more += p.g_top[row * p.top + k];
+#pragma unroll
+      for (int n = 0; n < N; ++n) y[n] += n == i ? more : 0.f;
+    }
+    if (r.whole(v) && !apart) {
+      uint4 w;
+      if constexpr (F32) w = __builtin_bit_cast(uint4, floatx4{y[0], y[1], y[2], y[3]});
+      else w = uint4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
+      *(uint4*)(out + (int64_t)e * SIZE) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (e + i >= 0 && e + i < p.vocab) {
+          if constexpr (F32) ((float*)out)[e + i] = y[i];
+          else ((bf16_t*)out)[e + i] = (bf16_t)y[i];
+        }
+    }
+  }
+}
+
+struct Split { int nt, vecs, parts; };
+
+// How rows are cut up, by their number and length.
+Split split_of(const HstuLogProbsArgs& a) {
+  const int64_t n = a.dtype == HSTU_SERVE_FP32 ? 4 : 8, vectors = ((int64_t)a.vocab + n - 1 + n - 1) / n;   // (a row may start anywhere)
+  Split s;
+  s.nt = vectors <= 64 * VECS && a.top <= 64 ? 64 : 256;
+  s.vecs = (int)std::min<int64_t>(VECS, (vectors + s.nt - 1) / s.nt);
+  s.parts = (int)((vectors + (int64_t)s.nt * s.vecs - 1) / ((int64_t)s.nt * s.vecs));
+  return s;
+}
+
+int check(const HstuLogProbsArgs* a) {
+  if (!a) return serve_fail(HSTU_SERVE_ERR_NULL, "args is null");
+  if (a->struct_size != sizeof(HstuLogProbsArgs) || a->version != HSTU_SERVE_ABI_VERSION)
+    return serve_fail(HSTU_SERVE_ERR_VERSION, "struct_size %u version %u, expected %zu and %d", a->struct_size, a->version, sizeof(HstuLogProbsArgs), HSTU_SERVE_ABI_VERSION);
+  if (a->dtype != HSTU_SERVE_BF16 && a->dtype != HSTU_SERVE_FP32) return serve_fail(HSTU_SERVE_ERR_SHAPE, "dtype %d", a->dtype);
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > 1 << 30 || a->count < 0) return serve_fail(HSTU_SERVE_ERR_SHAPE, "rows=%lld vocab=%d count=%d", (long long)a->rows, a->vocab, a->count);
+  if (a->top < 0 || a->top > MAX_TOP || a->top > a->vocab) return serve_fail(HSTU_SERVE_ERR_SHAPE, "top=%d: at most %d and the vocabulary", a->top, MAX_TOP);
+  return HSTU_SERVE_OK;
+}
+
+size_t part_bytes(const HstuLogProbsArgs& a, const Split& s) {
+  return s.parts == 1 ? 0 : (size_t)a.rows * s.parts * (3 * sizeof(float) + (size_t)a.top * (sizeof(float) + sizeof(int32_t)));
+}
+
+int fill(const HstuLogProbsArgs* a, const Split& s, Params* p) {
+  const size_t size = a->dtype == HSTU_SERVE_FP32 ? 4 : 2;
+  if (!a->logits || (a->count > 0 && !a->tokens)) return serve_fail(HSTU_SERVE_ERR_NULL, "logits or tokens is null");
+  if ((uintptr_t)a->logits % size) return serve_fail(HSTU_SERVE_ERR_SHAPE, "logits are not aligned to their type");
+  if (a->rows > 0x7fffffffll / s.parts) return serve_fail(HSTU_SERVE_ERR_SHAPE, "%lld rows of %d parts are too many for one call", (long long)a->rows, s.parts);
+  *p = Params{};
+  p->logits = a->logits; p->stride = a->stride; p->tokens = a->tokens;
+  p->log_probs = a->log_probs; p->entropy = a->entropy; p->stats = a->stats;
+  p->top_log_probs = a->top_log_probs; p->top_tokens = a->top_tokens;
+  p->rows = a->rows; p->vocab = a->vocab; p->count = a->count; p->top = a->top;
+  p->parts = s.parts; p->vecs = s.vecs;
+  return HSTU_SERVE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t hstu_log_probs_workspace_bytes(const HstuLogProbsArgs* a) {
+  serve_clear_error();
+  if (check(a) || a->rows == 0) return 0;
+  return part_bytes(*a, split_of(*a));
+}
+
+int hstu_log_probs_fwd(const HstuLogProbsArgs* a, void* stream) {
+  serve_clear_error();
+  if (const int rc = check(a)) return rc;
+  if (a->rows == 0) return HSTU_SERVE_OK;
+  const Split s = split_of(*a);
+  Params p;
+  if (const int rc = fill(a, s, &p)) return rc;
+  if ((a->count > 0 && !a->log_probs) || (a->top > 0 && (!a->top_log_probs || !a->top_tokens))) return serve_fail(HSTU_SERVE_ERR_NULL, "an output is null");
+  const size_t need = part_bytes(*a, s);
+  if (need && (!a->workspace || a->workspace_bytes < need || !serve_aligned16(a->workspace)))
+    return serve_fail(HSTU_SERVE_ERR_WORKSPACE, "workspace of %zu bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
+  p.part_stats = (float*)a->workspace;
+  p.part_value = p.part_stats + a->rows * s.parts * 3;
+  p.part_index = (int32_t*)(p.part_value + a->rows * s.parts * a->top);
+  hipStream_t st = (hipStream_t)stream;
+  const bool f32 = a->dtype == HSTU_SERVE_FP32;
+  const uint32_t grid = (uint32_t)(a->rows * s.parts);
+  if (s.nt == 64) {
+    if (f32) hstu_log_probs_part<true, 64><<<grid, 64, 0, st>>>(p);
+    else hstu_log_probs_part<false, 64><<<grid, 64, 0, st>>>(p);
+  } else {
+    if (f32) hstu_log_probs_part<true, 256><<<grid, 256, 0, st>>>(p);
+    else hstu_log_probs_part<false, 256><<<grid, 256, 0, st>>>(p);
+  }
+  if (const int rc = serve_launched("hstu_log_probs_part")) return rc;
+  if (s.parts > 1) {
+    if (f32) hstu_log_probs_join<true><<<(uint32_t)a->rows, 256, 0, st>>>(p);
+    else hstu_log_probs_join<false><<<(uint32_t)a->rows, 256, 0, st>>>(p);
+    return serve_launched("hstu_log_probs_join");
+  }
+  return HSTU_SERVE_OK;
+}
+
+int hstu_log_probs_bwd(const HstuLogProbsArgs* a, void* stream) {
+  serve_clear_error();
+  if (const int rc = check(a)) return rc;
+  if (a->rows == 0) return HSTU_SERVE_OK;
+  const Split s = split_of(*a);
+  Params p;
+  if (const int rc = fill(a, s, &p)) return rc;
+  const size_t size = a->dtype == HSTU_SERVE_FP32 ? 4 : 2;
+  if (!a->stats || !a->d_logits || (a->g_top && !a->top_tokens)) return serve_fail(HSTU_SERVE_ERR_NULL, "stats, d_logits or top_tokens is null");
+  if ((uintptr_t)a->d_logits % size) return serve_fail(HSTU_SERVE_ERR_SHAPE, "d_logits is not aligned to its type");
+  p.g_tokens = a->count > 0 ? a->g_tokens : nullptr; p.g_entropy = a->g_entropy; p.g_top = a->top > 0 ? a->g_top : nullptr;
+  p.d_logits = a->d_logits; p.d_stride = a->d_stride;
+  hipStream_t st = (hipStream_t)stream;
+  const bool f32 = a->dtype == HSTU_SERVE_FP32;
+  const uint32_t grid = (uint32_t)(a->rows * s.parts);
+  if (s.nt == 64) {
+    if (f32) hstu_log_probs_backward<true, 64><<<grid, 64, 0, st>>>(p);
+    else hstu_log_probs_backward<false, 64><<<grid, 64, 0, st>>>(p);
+  } else {
+    if (f32) hstu_log_probs_backward<true, 256><<<grid, 256, 0, st>>>(p);
+    else hstu_log_probs_backward<false, 256><<<grid, 256, 0, st>>>(p);
+  }
+  return serve_launched("hstu_log_probs_backward");
+}
+
+}

@@ -95,3 +95,31 @@ def attention_tolerance(out, logits_off, weights, length, dtype):
   tol = logits_off + (length + 8) * 2.0**-24 * weights
   half = torch.finfo(dtype).eps / 2
   return tol + half * (weights if dtype == torch.bfloat16 else 2 * weights) * 1.01 + half * out.abs() + 1e-30
+
+
+def log_probs(x, tokens, top, g_tokens=None, g_entropy=None, g_top=None):
+  """Rows x [R, V] in 64 bits: (log_probs, entropy, top_log_probs, top_tokens, d_logits), and the log-probabilities of all."""
+  x = x.double()
+  lp = torch.log_softmax(x, -1)
+  p = lp.exp()
+  bad = torch.isnan(lp).any(-1, keepdim=True)
+  plogp = torch.where(p > 0, p * lp, 0.0)
+  h = torch.where(bad[:, 0], math.nan, -plogp.sum(-1))
+  ask = tokens.clamp(0, x.shape[1] - 1)
+  picked = torch.where(tokens < 0, 0.0, torch.where(tokens >= x.shape[1], math.nan, lp.gather(1, ask)))
+  order = torch.where(torch.isnan(x), math.inf, x)
+  first = torch.sort(torch.where(torch.isnan(x), 1, 0), dim=-1, descending=True, stable=True).indices
+  first = first.gather(1, torch.sort(order.gather(1, first), dim=-1, descending=True, stable=True).indices)[:, :top]
+  g = torch.zeros_like(x)
+  total = torch.zeros((x.shape[0], 1), dtype=torch.float64)
+  if g_tokens is not None:
+    gt = torch.where(tokens < 0, 0.0, torch.where(tokens >= x.shape[1], math.nan, g_tokens.double()))
+    total = total + gt.sum(-1, keepdim=True)
+    g = g.scatter_add(1, ask, gt)
+  if g_top is not None:
+    total = total + g_top.double().sum(-1, keepdim=True)
+    g = g.scatter_add(1, first, g_top.double())
+  inner = total.expand(x.shape)
+  if g_entropy is not None:
+    inner = inner + g_entropy.double()[:, None] * torch.where(p > 0, lp + h[:, None], 0.0)
+  return picked, h, lp.gather(1, first), first, g - p * inner, lp, inner

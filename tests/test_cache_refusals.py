@@ -101,3 +101,34 @@ def test_header_and_binding_agree():
   header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "hstu_serve.h")).read()
   assert int(re.search(r"HSTU_SERVE_ABI_VERSION (\d+)", header).group(1)) == _lib_serve.ABI_VERSION
   assert set(re.findall(r"^(?:int|size_t|const char\*) (hstu_\w+)\(", header, re.M)) == set(_lib_serve.EXPORTS)
+
+
+def _score_args(**kw):
+  a = _lib_serve.HstuLogProbsArgs()
+  a.struct_size, a.version = C.sizeof(a), _lib_serve.ABI_VERSION
+  a.logits, a.rows, a.stride, a.vocab, a.dtype, a.count, a.top = 0x1000, 4, 100000, 100000, _lib_serve.BF16, 1, 5
+  a.tokens, a.log_probs, a.top_log_probs, a.top_tokens, a.stats, a.d_logits = 0x2000, 0x3000, 0x4000, 0x5000, 0x6000, 0x7000
+  for name, value in kw.items():
+    setattr(a, name, value)
+  return a
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(struct_size=8), -2, "struct_size"), (dict(version=2), -2, "version"), (dict(dtype=3), -4, "dtype"), (dict(vocab=0), -4, "vocab"), (dict(rows=-1), -4, "rows"),
+    (dict(top=257), -4, "top"), (dict(vocab=4), -4, "top"), (dict(logits=None), -1, "null"), (dict(tokens=None), -1, "null"), (dict(logits=0x1001), -4, "aligned"),
+    (dict(rows=1 << 31), -4, "too many")])
+def test_scores_refused(change, status, word):
+  lib = _lib_serve.load()
+  for fn in (lib.hstu_log_probs_fwd, lib.hstu_log_probs_bwd):
+    assert fn(C.byref(_score_args(**change)), None) == status
+    assert word in lib.hstu_serve_last_error().decode()
+
+
+def test_scores_forward_and_backward_refused():
+  lib = _lib_serve.load()
+  for change, status in ((dict(log_probs=None), -1), (dict(top_tokens=None), -1), (dict(), -5), (dict(workspace=0x9000, workspace_bytes=16), -5)):
+    assert lib.hstu_log_probs_fwd(C.byref(_score_args(**change)), None) == status
+  for change, status in ((dict(stats=None), -1), (dict(d_logits=None), -1), (dict(d_logits=0x7001), -4), (dict(g_top=0x100, top_tokens=None), -1)):
+    assert lib.hstu_log_probs_bwd(C.byref(_score_args(**change)), None) == status
+  assert lib.hstu_log_probs_fwd(None, None) == -1 and lib.hstu_log_probs_bwd(None, None) == -1
+  assert lib.hstu_log_probs_fwd(C.byref(_score_args(rows=0)), None) == 0 and lib.hstu_log_probs_workspace_bytes(C.byref(_score_args(rows=0))) == 0
