@@ -26,6 +26,8 @@ MICRO_SOURCES = [os.path.join(_HERE, "csrc", "micro_fwd_stream.hip")]
 # the native host side: a Python extension module over both libraries
 NATIVE_PATH = os.path.join(LIB_DIR, "_native.so")
 NATIVE_SOURCES = [os.path.join(_HERE, "csrc", "native.cpp")]
+NATIVE_SERVE_PATH = os.path.join(LIB_DIR, "_native_serve.so")
+NATIVE_SERVE_SOURCES = [os.path.join(_HERE, "csrc", "native_serve.cpp")]
 
 # -packed-fp32-ops is switched off for the device pass: packed fp32
 # instructions are not wanted in these kernels.  The host pass does not know
@@ -71,24 +73,33 @@ def build_serve_library(verbose: bool = False) -> str:
   return _compile(SERVE_SOURCES, SERVE_LIB_PATH, verbose=verbose)
 
 
-def build_native(verbose: bool = False) -> str:
-  """Compiles the native host side into recml_amd/lib/_native.so (host code only; links the two libraries above)."""
+def _compile_native(sources, out, libraries, verbose=False) -> str:
   import sysconfig
   import torch
   troot = os.path.dirname(torch.__file__)
   tinc = os.path.join(troot, "include")
-  tmp = NATIVE_PATH + ".tmp"
+  tmp = out + ".tmp"
   cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I", INCLUDE,
          "-I", tinc, "-I", os.path.join(tinc, "torch", "csrc", "api", "include"), "-I", "/opt/rocm/include",
-         "-I", sysconfig.get_paths()["include"], "-o", tmp, *NATIVE_SOURCES, "-L", LIB_DIR, "-l:libhstu_attn.so", "-l:libhstu_block.so",
+         "-I", sysconfig.get_paths()["include"], "-o", tmp, *sources, "-L", LIB_DIR, *(f"-l:{os.path.basename(lib)}" for lib in libraries),
          "-L", os.path.join(troot, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN"]
   res = subprocess.run(cmd, capture_output=True, text=True)
   if res.returncode != 0:
     raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
   if verbose:
     print(res.stderr)
-  os.replace(tmp, NATIVE_PATH)
-  return NATIVE_PATH
+  os.replace(tmp, out)
+  return out
+
+
+def build_native(verbose: bool = False) -> str:
+  """Compiles the native host side into recml_amd/lib/_native.so (host code only; links the two libraries above)."""
+  return _compile_native(NATIVE_SOURCES, NATIVE_PATH, (LIB_PATH, BLOCK_LIB_PATH), verbose)
+
+
+def build_native_serve(verbose: bool = False) -> str:
+  """Compiles the serving operators' native host side into recml_amd/lib/_native_serve.so (links their library)."""
+  return _compile_native(NATIVE_SERVE_SOURCES, NATIVE_SERVE_PATH, (SERVE_LIB_PATH,), verbose)
 
 
 def build_microbench(verbose: bool = False) -> str:
@@ -111,4 +122,5 @@ if __name__ == "__main__":
   print(build_block_library(verbose=True))
   print(build_serve_library(verbose=True))
   print(build_native(verbose=True))
+  print(build_native_serve(verbose=True))
   print(build_microbench(verbose=True))

@@ -48,6 +48,7 @@ struct Params {
   int64_t d_stride;
   int64_t rows;
   int32_t vocab, count, top, parts, vecs;
+  int32_t sums_t;                    // the entropy is wanted, now or by the backward
 };
 
 // ordered bits: larger floats have larger ones, any NaN the largest; -0 and 0 are one value
@@ -63,6 +64,9 @@ template <bool F32>
 struct Vec {
   static constexpr int N = F32 ? 4 : 8;
   uint4 raw;
+  // Keeps the entries packed: without it the compiler holds them unpacked from one pass over the registers to the next (256
+  // registers, one wave a SIMD).
+  __device__ __forceinline__ void hold() { asm volatile("" : "+v"(raw.x), "+v"(raw.y), "+v"(raw.z), "+v"(raw.w)); }
   __device__ __forceinline__ float at(int i) const {
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     if constexpr (F32) return __builtin_bit_cast(float, w[i]);
@@ -148,14 +152,13 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
   return found;
 }
 
-// The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  each(f) calls f(x, index) for a
-// thread's entries; there are at least k.
-template <int NT, typename Each, typename Out>
-__device__ __forceinline__ void select_top(int k, Chosen& c, Each each, Out out) {
+// The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  `most`: the ordered bits of a
+// thread's largest entry (0: it has none; the least of an entry is that of -inf); collect(bound, push) calls push(x, index) for
+// its entries that reach the bound, each(f) f(x, index) for all of them; there are at least k.
+template <int NT, typename Collect, typename Each, typename Out>
+__device__ __forceinline__ void select_top(int k, Chosen& c, uint32_t most, Collect collect, Each each, Out out) {
   constexpr int W = NT / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  uint32_t most = 0;                       // (0: no entry; the least of an entry is that of -inf)
-  each([&](float x, int) { const uint32_t o = ordered(x); most = o > most ? o : most; });
   // every wave has its share of the k, or one wave has all of them: either way k entries reach the bound
   const uint32_t share = kth_of_wave(most, (k + W - 1) / W), all = W > 1 && k <= 64 ? kth_of_wave(most, k) : 0;
   __syncthreads();
@@ -173,14 +176,11 @@ __device__ __forceinline__ void select_top(int k, Chosen& c, Each each, Out out)
     best = b > best ? b : best;
   }
   const uint32_t bound = least > best ? least : best;
-  if (most != 0 && most >= bound) {
-    each([&](float x, int index) {
-      if (ordered(x) >= bound) {
-        const int at = atomicAdd(&c.n, 1);
-        if (at < CAP) { c.value[at] = x; c.index[at] = index; }
-      }
+  if (most != 0 && most >= bound)
+    collect(bound, [&](float x, int index) {
+      const int at = atomicAdd(&c.n, 1);
+      if (at < CAP) { c.value[at] = x; c.index[at] = index; }
     });
-  }
   __syncthreads();
   const int n = c.n;
   if (n <= CAP) {
@@ -189,6 +189,7 @@ __device__ __forceinline__ void select_top(int k, Chosen& c, Each each, Out out)
       const int index = c.index[i];
       const uint64_t mine = place_of(x, index);
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += place_of(c.value[j], c.index[j]) > mine;
       if (rank < k) out(rank, x, index);
     }
@@ -249,10 +250,9 @@ __device__ __forceinline__ void finish(const Params& p, int64_t row, float m, fl
   }
 }
 
-template <bool F32, int NT>
+template <bool F32, int NT, bool TOP>
 __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
   constexpr int N = Vec<F32>::N;
-  __shared__ Chosen chosen;
   __shared__ float sums[4];
   const int64_t row = blockIdx.x / p.parts;
   const int part = blockIdx.x % p.parts;
@@ -268,46 +268,80 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
     if (c < p.vecs) {
 #pragma unroll
       for (int i = 0; i < N; ++i) m = fmaxf(m, x[c].at(i));
+      x[c].hold();
     }
+  const float mine = m;
   m = block_reduce<NT>(m, sums, larger);
   const float zero = m == -__builtin_inff() ? 0.f : m;         // (a part without any entry above -inf sums to nothing)
   float s = 0.f, t = 0.f;
+  if (p.sums_t) {
 #pragma unroll
-  for (int c = 0; c < VECS; ++c)
-    if (c < p.vecs) {
+    for (int c = 0; c < VECS; ++c)
+      if (c < p.vecs) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float d = x[c].at(i) - zero, e = __builtin_amdgcn_exp2f(d * LOG2E);
-        s += e;
-        t += e > 0.f ? d * e : 0.f;
+        for (int i = 0; i < N; ++i) {
+          const float d = x[c].at(i) - zero, e = __builtin_amdgcn_exp2f(d * LOG2E);
+          s += e;
+          t = __builtin_fmaf(fmaxf(d, -1e30f), e, t);          // (-inf times its 0 is nothing; a NaN is in s)
+        }
+        x[c].hold();
       }
-    }
+    t = block_reduce<NT>(t, sums, add);
+  } else {
+#pragma unroll
+    for (int c = 0; c < VECS; ++c)
+      if (c < p.vecs) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += __builtin_amdgcn_exp2f((x[c].at(i) - zero) * LOG2E);
+        x[c].hold();
+      }
+  }
+  const bool odd = s != s;             // (the thread holds a NaN, or +inf)
   s = block_reduce<NT>(s, sums, add);
-  t = block_reduce<NT>(t, sums, add);
   if (p.parts == 1) {
     finish<F32, NT>(p, row, m, s, t);
   } else if (threadIdx.x == 0) {
     float* to = p.part_stats + (row * p.parts + part) * 3;
     to[0] = m; to[1] = s; to[2] = t;
   }
-  if (p.top == 0) return;
+  if constexpr (!TOP) return;
+  __shared__ Chosen chosen;
   // a part shorter than `top` gives what it has
   const int64_t e0 = (int64_t)part * p.vecs * NT * N - r.shift, e1 = e0 + (int64_t)p.vecs * NT * N;
   const int64_t here = (e1 < p.vocab ? e1 : p.vocab) - (e0 > 0 ? e0 : 0);
   const int k = here < p.top ? (here > 0 ? (int)here : 0) : p.top;
   const float log_s = __logf(s);
+  // (read again: only rows with more ties than the list holds, or with NaNs, need all entries once more)
   auto each = [&](auto f) {
+    for (int c = 0; c < p.vecs; ++c) {
+      const int v = v0 + c * NT, e = r.first(v);
+      if (v >= r.vectors) break;
+      const Vec<F32> y = r.load(v);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (e + i >= 0 && e + i < p.vocab) f(y.at(i), e + i);
+    }
+  };
+  uint32_t most = v0 < r.vectors ? ordered(mine) : 0;
+  if (odd) each([&](float y, int) { const uint32_t o = ordered(y); most = o > most ? o : most; });
+  auto collect = [&](uint32_t bound, auto push) {
+    // not below the bound's float: where that is a NaN (no bound, or one among the NaNs) everything is looked at
+    const float least = __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
 #pragma unroll
     for (int c = 0; c < VECS; ++c)
       if (c < p.vecs) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) any |= !(x[c].at(i) < least);
+        if (!any) continue;
         const int e = r.first(v0 + c * NT);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (e + i >= 0 && e + i < p.vocab) f(x[c].at(i), e + i);
+          if (e + i >= 0 && e + i < p.vocab && ordered(x[c].at(i)) >= bound) push(x[c].at(i), e + i);
       }
   };
   if (p.parts == 1) {
-    select_top<NT>(k, chosen, each, [&](int rank, float value, int index) {
+    select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
       p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
       p.top_tokens[row * p.top + rank] = index;
     });
@@ -315,7 +349,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
     const int64_t to = (row * p.parts + part) * p.top;
     for (int i = k + threadIdx.x; i < p.top; i += NT) p.part_index[to + i] = -1;
     if (k > 0)
-      select_top<NT>(k, chosen, each, [&](int rank, float value, int index) {
+      select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
         p.part_value[to + rank] = value;
         p.part_index[to + rank] = index;
       });
@@ -323,9 +357,9 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
 }
 
 // One row's parts: their sums in order, and the largest of their largest.
-template <bool F32>
-__global__ __launch_bounds__(256) void hstu_log_probs_join(const Params p) {
-  constexpr int NT = 256, E = 4;
+template <bool F32, int NT>
+__global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
+  constexpr int E = 4;
   __shared__ Chosen chosen;
   __shared__ float sums[4];
   __shared__ float best_value[MAX_TOP];
@@ -371,12 +405,18 @@ __global__ __launch_bounds__(256) void hstu_log_probs_join(const Params p) {
     const int k = n < p.top ? n : p.top;
     done += take;
     const bool end = done >= total;
-    if (k > 0)
-      select_top<NT>(k, chosen, [&](auto f) {
+    auto each = [&](auto f) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (index[e] >= 0) f(x[e], index[e]);
-      }, [&](int rank, float value, int at) {
+      for (int e = 0; e < E; ++e)
+        if (index[e] >= 0) f(x[e], index[e]);
+    };
+    uint32_t most = 0;
+    each([&](float y, int) { const uint32_t o = ordered(y); most = o > most ? o : most; });
+    auto collect = [&](uint32_t bound, auto push) {
+      each([&](float y, int i) { if (ordered(y) >= bound) push(y, i); });
+    };
+    if (k > 0)
+      select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int at) {
         if (end) {
           p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
           p.top_tokens[row * p.top + rank] = at;
@@ -399,6 +439,10 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
   const int part = blockIdx.x % p.parts;
   const Row<F32> r(p.logits, p.stride, row, p.vocab);
   const int v0 = part * p.vecs * NT;
+  Vec<F32> x[VECS];
+#pragma unroll
+  for (int c = 0; c < VECS; ++c)
+    if (c < p.vecs) x[c] = r.load(v0 + c * NT + threadIdx.x);
   // the gradients' sum, and which of the part's entries have one of their own
   const int64_t e0 = (int64_t)v0 * N - r.shift;
   for (int i = threadIdx.x; i < NT * p.vecs * N / 32; i += NT) hit[i] = 0;
@@ -426,15 +470,20 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
   const float ge = p.g_entropy ? p.g_entropy[row] : 0.f;
   char* const out = (char*)p.d_logits + row * p.d_stride * SIZE;
   const bool apart = (((uintptr_t)out ^ (uintptr_t)((const char*)p.logits + row * p.stride * SIZE)) & 15u) != 0;
-  for (int c = 0; c < p.vecs; ++c) {
-    const int v = v0 + c * NT + threadIdx.x;
-    if (v >= r.vectors) break;
-    const Vec<F32> x = r.load(v);
-    float y[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float lp = (x.at(i) - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
-      y[i] = -pr * (total + (pr == 0.f ? 0.f : ge * (lp + entropy)));
+  for (int c = 0; c < VECS; ++c) {
+    const int v = v0 + c * NT + threadIdx.x;
+    if (c >= p.vecs || v >= r.vectors) continue;
+    float y[N];
+    if (p.g_entropy) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float lp = (x[c].at(i) - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
+        y[i] = -pr * __builtin_fmaf(ge, fmaxf(lp, -1e30f) + entropy, total);      // (-inf times its 0 is nothing)
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = -__builtin_amdgcn_exp2f(((x[c].at(i) - m) - log_s) * LOG2E) * total;
     }
     const int e = r.first(v), at = (c * NT + threadIdx.x) * N;
     uint32_t mine = hit[at / 32] >> (at % 32) & ((1u << N) - 1u);
@@ -475,6 +524,8 @@ Split split_of(const HstuLogProbsArgs& a) {
   Split s;
   s.nt = vectors <= 64 * VECS && a.top <= 64 ? 64 : 256;
   s.vecs = (int)std::min<int64_t>(VECS, (vectors + s.nt - 1) / s.nt);
+  // few rows: shorter parts, so that they fill the chip
+  while (s.vecs > 1 && a.rows * ((vectors + (int64_t)s.nt * s.vecs - 1) / ((int64_t)s.nt * s.vecs)) < 256 && vectors > s.nt) s.vecs = (s.vecs + 1) / 2;
   s.parts = (int)((vectors + (int64_t)s.nt * s.vecs - 1) / ((int64_t)s.nt * s.vecs));
   return s;
 }
@@ -503,7 +554,7 @@ int fill(const HstuLogProbsArgs* a, const Split& s, Params* p) {
   p->log_probs = a->log_probs; p->entropy = a->entropy; p->stats = a->stats;
   p->top_log_probs = a->top_log_probs; p->top_tokens = a->top_tokens;
   p->rows = a->rows; p->vocab = a->vocab; p->count = a->count; p->top = a->top;
-  p->parts = s.parts; p->vecs = s.vecs;
+  p->parts = s.parts; p->vecs = s.vecs; p->sums_t = a->entropy != nullptr;
   return HSTU_SERVE_OK;
 }
 
@@ -534,17 +585,21 @@ int hstu_log_probs_fwd(const HstuLogProbsArgs* a, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const bool f32 = a->dtype == HSTU_SERVE_FP32;
   const uint32_t grid = (uint32_t)(a->rows * s.parts);
-  if (s.nt == 64) {
-    if (f32) hstu_log_probs_part<true, 64><<<grid, 64, 0, st>>>(p);
-    else hstu_log_probs_part<false, 64><<<grid, 64, 0, st>>>(p);
-  } else {
-    if (f32) hstu_log_probs_part<true, 256><<<grid, 256, 0, st>>>(p);
-    else hstu_log_probs_part<false, 256><<<grid, 256, 0, st>>>(p);
-  }
+#define PART(F32, NT)                                                              \
+  do {                                                                             \
+    if (p.top) hstu_log_probs_part<F32, NT, true><<<grid, NT, 0, st>>>(p);         \
+    else hstu_log_probs_part<F32, NT, false><<<grid, NT, 0, st>>>(p);              \
+  } while (0)
+  if (s.nt == 64) { if (f32) PART(true, 64); else PART(false, 64); }
+  else { if (f32) PART(true, 256); else PART(false, 256); }
+#undef PART
   if (const int rc = serve_launched("hstu_log_probs_part")) return rc;
   if (s.parts > 1) {
-    if (f32) hstu_log_probs_join<true><<<(uint32_t)a->rows, 256, 0, st>>>(p);
-    else hstu_log_probs_join<false><<<(uint32_t)a->rows, 256, 0, st>>>(p);
+    // (a wave where its lanes hold all of a row's parts at once)
+    const bool small = s.parts <= 64 && (int64_t)s.parts * a->top <= 256 && a->top <= 64;
+    const uint32_t rows = (uint32_t)a->rows;
+    if (small) { if (f32) hstu_log_probs_join<true, 64><<<rows, 64, 0, st>>>(p); else hstu_log_probs_join<false, 64><<<rows, 64, 0, st>>>(p); }
+    else { if (f32) hstu_log_probs_join<true, 256><<<rows, 256, 0, st>>>(p); else hstu_log_probs_join<false, 256><<<rows, 256, 0, st>>>(p); }
     return serve_launched("hstu_log_probs_join");
   }
   return HSTU_SERVE_OK;

@@ -9,21 +9,7 @@
 // last axis, int32 lengths and ids, fp32 tables).  Anything else -- a conversion, a copy, an error to report -- comes back
 // as None, and the Python side (recml_amd/hstu_ops.py: build_args), which knows every form and every message, runs.
 
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <hip/hip_runtime.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPCachingAllocator.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/edge.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/grad_mode.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/autograd/variable.h>
+#include "native_common.h"
 
 #include <limits>
 #include <memory>
@@ -38,12 +24,7 @@
 
 namespace {
 
-using at::Tensor;
 using bf16_bits = uint16_t;
-
-void* stream_of(const Tensor& t) {
-  return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
 
 bool capturing(void* stream) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -53,31 +34,6 @@ bool capturing(void* stream) {
 // ---------------------------------------------------------------------------
 // arguments
 // ---------------------------------------------------------------------------
-
-// An optional tensor argument: false when it is something that the Python side has to look at.
-bool tensor_arg(PyObject* o, Tensor* out) {
-  if (o == Py_None) return true;
-  if (!THPVariable_Check(o)) return false;
-  *out = THPVariable_Unpack(o);
-  return true;
-}
-
-bool float_arg(PyObject* o, double* out) {
-  if (PyFloat_CheckExact(o)) { *out = PyFloat_AS_DOUBLE(o); return true; }
-  if (PyLong_CheckExact(o)) {
-    *out = PyLong_AsDouble(o);
-    if (*out == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
-    return true;
-  }
-  return false;
-}
-
-bool long_arg(PyObject* o, int64_t* out) {
-  if (!PyLong_CheckExact(o)) return false;
-  int overflow = 0;
-  *out = PyLong_AsLongLongAndOverflow(o, &overflow);
-  return overflow == 0;
-}
 
 // Everything of a call but q, k, v, the bias tables and the dense bias (which may carry gradients).
 struct Options {
@@ -90,18 +46,6 @@ struct Options {
   bool causal = true;
   Tensor mask_rows, bias_rows; // copies of the dense operands with rows of whole 16-byte pieces, where the call needs them
 };
-
-bool on(const Tensor& t, c10::Device dev) { return t.is_cuda() && t.device() == dev; }
-
-bool plain(const Tensor& t, c10::Device dev, at::ScalarType type) { return on(t, dev) && t.scalar_type() == type && t.is_contiguous(); }
-
-// fp32 [heads, width] or [width] table with heads in {1, H}
-bool table(const Tensor& t, c10::Device dev, int64_t H, int64_t* heads, int64_t* width) {
-  if (!plain(t, dev, at::kFloat) || t.dim() < 1 || t.dim() > 2) return false;
-  *heads = t.dim() == 2 ? t.size(0) : 1;
-  *width = t.size(t.dim() - 1);
-  return *heads == 1 || *heads == H;
-}
 
 // Fills the struct for tensors that are ready as they are; false: the Python side takes the call.
 bool fill(HstuAttnFwdArgs& a, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& pos, const Tensor& ts_tab,
@@ -454,33 +398,14 @@ struct AttentionBackward : public torch::autograd::Node {
   }
 };
 
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-
-// Whether a tensor carries a forward-mode tangent.  The kernels give none for their results: such a call goes the Python way, whose
-// torch steps carry tangents on and whose autograd functions refuse them.
-bool dual(std::initializer_list<const Tensor*> ts) {
-  for (const Tensor* t : ts)
-    if (t->defined() && t->_fw_grad(0).defined()) return true;
-  return false;
-}
-
 // ---------------------------------------------------------------------------
 // block steps
 // ---------------------------------------------------------------------------
 
 void block_check(int rc, const char* what) { TORCH_CHECK(rc == HSTU_BLOCK_OK, what, " failed (", rc, "): ", hstu_block_last_error()); }
 
-bool aligned(const Tensor& t) { return ((uintptr_t)t.const_data_ptr() & 15u) == 0; }
-
 // A contiguous, aligned bf16 GPU tensor.
 bool ready(const Tensor& t, c10::Device dev) { return t.defined() && plain(t, dev, at::kBFloat16) && aligned(t); }
-
-Tensor fresh(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().requires_grad(false)); }
 
 // rows of `width` elements, `stride` apart, as the kernels take them
 struct Rows { const void* p; int64_t stride; };
@@ -709,7 +634,7 @@ struct NormOp {
 
 // A tensor kept for the backward, the forward's own intermediates included: this way torch's saved-tensor hooks see it (checkpointing
 // and offloading replace it).
-torch::autograd::SavedVariable keep(const Tensor& t) { return torch::autograd::SavedVariable(t, false); }
+
 
 // How far back a block's backward has to go, by what wants a gradient (`wanted(i)`: the i-th of tokens, the parameters, pos, ts_tab).
 struct BlockWants {
@@ -1004,14 +929,6 @@ struct LinearBackward : public torch::autograd::Node {
 // Python
 // ---------------------------------------------------------------------------
 
-// Runs `f`; an exception becomes the Python one of its type (torch.OutOfMemoryError, IndexError, an error of a hook, ...).
-template <typename F>
-PyObject* guarded(F&& f) {
-  HANDLE_TH_ERRORS
-  return f();
-  END_HANDLE_TH_ERRORS
-}
-
 enum Arg { A_Q, A_K, A_V, A_SEQ_LENS, A_SEQ_OFFSETS, A_MAX_LEN, A_N, A_ALPHA, A_CAUSAL, A_POS, A_TS, A_TS_TAB, A_BUCKET, A_QSEG, A_KVSEG, A_WINDOW,
            A_MASK, A_BIAS, A_OUT, A_QSCALE, A_KSCALE, A_DROP_P, A_DROP_SEED, A_GRAD, A_COUNT };
 
@@ -1084,19 +1001,6 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
     return THPVariable_Wrap(std::move(out));
   });
 }
-
-// Runs `f` without the interpreter's lock, on the tensor's device, outside of any graph.
-template <typename F>
-auto without_lock(const Tensor& t, F&& f) {
-  struct Release {
-    PyThreadState* saved = PyEval_SaveThread();
-    ~Release() { PyEval_RestoreThread(saved); }
-  } release;
-  const c10::DeviceGuard guard(t.device());
-  const at::NoGradGuard no_grad;
-  return f();
-}
-
 
 // block(tokens [.., D], params, heads, head_dim, eps, alpha, n, seq_lens, seq_offsets, max_len, pos, timestamps, ts_tab, mask, bias,
 //       dropout_p, dropout_seed, prepared, workspace, differentiable) -> (out, signature, workspace, reused) or None

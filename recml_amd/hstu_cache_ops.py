@@ -55,6 +55,11 @@ class KVPages:
 
   def __init__(self, k, k_scales, v, v_scales, *, head_dim: int):
     d = int(head_dim)
+    put = lambda bits: [object.__setattr__(self, n, t) for n, t in zip(self.__slots__, (k, k_scales, v, v_scales, d, bits))]
+    for bits in (4, 8):
+      if _native.check_pages(k, k_scales, v, v_scales, d, bits):
+        put(bits)
+        return
     if d not in HEAD_DIMS:
       raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
     for name, t in (("k", k), ("k_scales", k_scales), ("v", v), ("v_scales", v_scales)):
@@ -74,8 +79,10 @@ class KVPages:
     if v.shape != k.shape or tuple(k_scales.shape) != scales or tuple(v_scales.shape) != scales:
       raise ValueError(f"k and v must share one shape and the scales be {scales}, got {tuple(k.shape)}, {tuple(v.shape)}, "
                        f"{tuple(k_scales.shape)}, {tuple(v_scales.shape)}")
-    self.k, self.k_scales, self.v, self.v_scales = k, k_scales, v, v_scales
-    self.head_dim, self.bits = d, 8 * width // d
+    put(8 * width // d)
+
+  def __setattr__(self, name, value):
+    raise AttributeError("KVPages are what they were made of: make new ones")
 
   @classmethod
   def empty(cls, pages: int, page_size: int, heads: int, head_dim: int, *, bits: int = 4, device=None) -> "KVPages":
@@ -178,6 +185,8 @@ def kv_write(pages, k, v, page_table, starts, *, offsets=None, max_new=None) -> 
   k, v: [B, n, H, d], or packed [T, H, d] with `offsets` [B + 1] and `max_new` (the most rows of one sequence); float32 or
   bfloat16.  Row t of sequence b goes to place starts[b] + t; rows whose place has no page are dropped.  Lengths are the
   caller's: writing the same rows again changes nothing.  Two sequences that share a page must not write it in one call."""
+  if _native.kv_write(pages, k, v, page_table, starts, offsets, max_new):
+    return
   table = _table(pages, page_table)
   B, device = table.shape[0], pages.k.device
   for name, t in (("k", k), ("v", v)):
@@ -198,6 +207,10 @@ def kv_read(pages, page_table, starts, *, count=None, offsets=None, max_new=None
   """The keys and values that the pages stand for: (k, v), [B, count, H, d] from place starts[b] on, or packed
   [total, H, d] with `offsets` [B + 1] and `max_new` (rows of no sequence are not written).  Exact in bfloat16 and float32.
   Places without a page read as zeros."""
+  if dtype is torch.bfloat16 or dtype is torch.float32:
+    got = _native.kv_read(pages, page_table, starts, count, offsets, max_new, total, dtype is torch.float32)
+    if got is not None:
+      return got
   table = _table(pages, page_table)
   B, device = table.shape[0], pages.k.device
   if dtype not in _DTYPES:
@@ -249,6 +262,9 @@ def cached_attention(q, pages, page_table, lengths, *, max_len, offsets=None, ma
     out: optional preallocated output.  Packed rows of no sequence are left as they were in it.
 
   Returns: a tensor shaped and typed like q.  Inference only: raises where a gradient is asked for."""
+  got = _native.cached_attention(q, pages, page_table, lengths, max_len, offsets, max_new, n, alpha, pos_bias, timestamps, ts_bias, ts_bucket_size, out)
+  if got is not None:
+    return got
   table = _table(pages, page_table)
   B, device, H = table.shape[0], pages.k.device, pages.heads
   _check_rows("q", q, pages, B, offsets, max_new)

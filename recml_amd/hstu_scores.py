@@ -105,6 +105,9 @@ def token_log_probs(logits, tokens=None, *, top: int = 0, entropy: bool = False)
 
   Entries of -inf are tokens that cannot occur.  A row with a NaN, with +inf, or with nothing but -inf is NaN throughout.
   Differentiable in the logits, through log_probs, entropy and top_log_probs."""
+  got = _native.token_log_probs(logits, tokens, top, entropy, True)
+  if got is not None:
+    return TokenLogProbs(*got)
   _check_gpu("logits", logits)
   if logits.dtype not in _DTYPES:
     raise ValueError(f"logits: unsupported dtype {logits.dtype}: use float32 or bfloat16")

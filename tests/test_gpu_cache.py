@@ -377,3 +377,62 @@ def test_a_step_as_it_is_served(gpu):
     # two bf16 results of the same sums, each off by 2^-8 of its weights' magnitude and of itself
     size = (vv.abs().float().amax() * L * 2.0) / L
     assert (out.float() - want.float()).abs().max() <= 2 * 2.0**-8 * size
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_the_python_way(gpu, monkeypatch, packed):
+  """What the native host side declines goes through the Python one: the same kernels, the same bits."""
+  from recml_amd import _native
+  counts = [3, 1] if packed else [2, 2]
+  got, rows, table, lens, call, want, counts = _case(B=2, H=2, d=64, bits=4, page=64, lengths=[700, 20], counts=counts, max_len=700, dtype=BF16,
+                                                     packed=packed, seed=8, pos="heads", ts="one")
+  how = dict(offsets=call["offsets"], max_new=call["max_new"]) if packed else {}
+  read = dict(how, total=rows.shape[0]) if packed else dict(count=2)
+  def step():
+    recml_amd.kv_write(got, rows, rows * 0.5, table, lens - 3, **how)
+    return [recml_amd.cached_attention(rows, got, table, lens, **call), *recml_amd.kv_read(got, table, lens - 3, **read)]
+  native = step()
+  for t in (got.k, got.v):
+    t[int(table[1, 0]), :, 17:18] = 0                      # (a row that the next step writes again)
+  for name in ("kv_write", "kv_read", "cached_attention"):
+    monkeypatch.setattr(_native, name, lambda *a: None)
+  T = sum(counts)
+  for a, b in zip(native, step()):
+    assert torch.equal(a[:T], b[:T])
+
+
+def test_python_conversions_and_refusals(gpu):
+  """64-bit lengths, misaligned and strided rows, tables of other types; and what is refused."""
+  got, rows, table, lens, call, want, counts = _case(B=2, H=2, d=64, bits=8, page=64, lengths=[130, 20], counts=[2, 2], max_len=130, dtype=BF16,
+                                                     packed=False, seed=9, pos="heads", ts="one")
+  native = recml_amd.cached_attention(rows, got, table, lens, **call)
+  odd = torch.zeros(rows.numel() + 1, dtype=BF16, device="cuda")[1:].view(rows.shape)
+  odd.copy_(rows)
+  other = dict(call, pos_bias=call["pos_bias"].double(), ts_bias=call["ts_bias"].double(), timestamps=call["timestamps"].t().contiguous().t())
+  assert torch.equal(native, recml_amd.cached_attention(odd, got, table.long(), lens.long(), **other))
+  assert torch.equal(native, recml_amd.cached_attention(rows.transpose(2, 3).contiguous().transpose(2, 3), got, table, lens, **call))
+  bad = [dict(q=rows[:1]), dict(q=rows[..., :32]), dict(q=rows.half()), dict(lengths=lens[:1]), dict(lengths=lens.float()), dict(max_len=0), dict(n=0.0), dict(n=-1),
+         dict(pos_bias=call["pos_bias"][:, 1:]), dict(timestamps=None), dict(timestamps=call["timestamps"][:, 1:]), dict(ts_bias=torch.zeros(130, device="cuda")),
+         dict(out=rows.float()), dict(out=odd), dict(page_table=table[0]), dict(page_table=table.float()), dict(max_new=7), dict(lengths=lens.cpu()),
+         dict(offsets=torch.tensor([0, 2, 4]).cuda())]
+  for change in bad:
+    args = dict(call, q=rows, page_table=table, lengths=lens)
+    args.update(change)
+    with pytest.raises(ValueError):
+      recml_amd.cached_attention(args.pop("q"), got, args.pop("page_table"), args.pop("lengths"), **args)
+  leaf = rows.clone().requires_grad_(True)
+  with pytest.raises(ValueError, match="no gradient"):
+    recml_amd.cached_attention(leaf, got, table, lens, **call)
+  with pytest.raises(ValueError, match="no gradient"):
+    recml_amd.kv_write(got, leaf, rows, table, lens)
+  with torch.no_grad():
+    assert torch.equal(native, recml_amd.cached_attention(leaf, got, table, lens, **call))
+  for how in (dict(), dict(count=-1), dict(count=2, total=3), dict(offsets=torch.tensor([0, 1, 2]).cuda()), dict(count=1, dtype=torch.float16)):
+    with pytest.raises(ValueError):
+      recml_amd.kv_read(got, table, lens, **how)
+  with pytest.raises(AttributeError):
+    got.k = got.v
+  for parts in ((got.k[:, :, :31], got.k_scales, got.v, got.v_scales), (got.k, got.k_scales[..., 1:], got.v, got.v_scales), (got.k.float(), got.k_scales, got.v, got.v_scales),
+                (got.k, got.k_scales, got.v[:1], got.v_scales)):
+    with pytest.raises(ValueError):
+      recml_amd.KVPages(*parts, head_dim=64)
