@@ -16,7 +16,10 @@
 //                 through LDS, and the cache keeps rows as they are written.
 // The contraction order along d and along the keys is free as long as both operands agree: K's lane takes a run of d / 4
 // dims (one block of exponents at d = 128), and Q is read the same way.
-// fp32 queries run as three bf16 parts (24 bits: all of them), activated weights as three as well.
+// Queries in fp32 run as three bf16 parts (24 bits: all of them); activated weights as two for bf16 results (2^-17 of a weight is
+// lost, where one part would lose 2^-9 and make half of the result's error), as three for fp32 ones.
+// Biases are worked out by the whole workgroup, a pair a thread, for up to 8192 pairs ahead: done where the logits lie, a single
+// query's would cost each wave 16 times the work, since its 16 columns hold one row.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -24,6 +27,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "hstu_serve_common.h"
 
@@ -33,6 +37,7 @@ constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int STEP = 32;             // keys of a wave's step
 constexpr int MAX_BUCKETS = 128;
+constexpr int BUCKET_FLOATS = 2 * MAX_BUCKETS + 4;   // the buckets' thresholds and values in LDS
 
 struct Params {
   HstuKvPages g;
@@ -47,7 +52,7 @@ struct Params {
   const float* ts_tab;
   float* partial;                    // [row][head][part][d], null with one part
   int32_t per_seq, max_len, pos_heads, ts_heads, ts_buckets;
-  int32_t chunk, parts, qblocks;
+  int32_t chunk, parts, qblocks, sub_log2;
   float alpha, inv_n, buckets_per_log2;
   int32_t thr[MAX_BUCKETS + 2];      // thr[b]: smallest time difference of bucket b or a later one
 };
@@ -121,6 +126,14 @@ __device__ __forceinline__ void pairs_of(const Bytes<N>& c, float power, uint32_
   }
 }
 
+template <int I, int N, typename F>
+__device__ __forceinline__ void each_pair(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each_pair<I + 1, N>(f);
+  }
+}
+
 __device__ __forceinline__ bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_bit_cast(bf16x8, uint4{a, b, c, d});
 }
@@ -150,72 +163,160 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]
   }
 }
 
+// The buckets of time differences, in LDS: thr[b] the smallest difference of bucket b or a later one, tab[b] its value.
+struct Buckets {
+  const int32_t* thr;
+  const float* tab;
+  int32_t count;
+  float per_log2;            // ln 2 over a bucket's size
+};
+
+__device__ __forceinline__ float bucket_value(const Buckets& t, int64_t gap) {
+  gap = gap < 0 ? -gap : gap;
+  const int dt = gap < 1 ? 1 : gap > 1000000000 ? 1000000000 : (int)gap;
+  int b = (int)(__builtin_amdgcn_logf((float)dt) * t.per_log2);
+  b = b < 0 ? 0 : b > t.count ? t.count : b;                // (off by one at most: its neighbours' borders decide)
+  const int lo = t.thr[b], hi = t.thr[b + 1];
+  b += (dt >= hi ? 1 : 0) - (dt < lo ? 1 : 0);
+  return t.tab[b];
+}
+
+// Waves a SIMD that the registers are cut for.
+constexpr int waves_of(int dp, bool f32, int nq) { return f32 || dp > 128 || nq == 4 ? 1 : nq == 1 || dp <= 64 ? 3 : 2; }
+
+// What a wave's step reads of its 32 keys.
+template <int DP, int BITS>
+struct Raw {
+  static constexpr int KB = DP / 4 * BITS / 8;       // bytes of a lane's run of a key
+  static constexpr int KBLK = DP > 128 ? 2 : 1;      // blocks of exponents in it
+  static constexpr int VN = DP / 16;                 // dims of a lane's run of a value
+  static constexpr int VB = VN * BITS / 8;
+  Bytes<KB> k[2];
+  uint32_t ke[2][KBLK];
+  Bytes<VB> v[8];
+  uint32_t ve[2];
+};
+
 template <int DP, int BITS, bool F32, int NQ>
-__global__ __launch_bounds__(THREADS) void hstu_cached_attn_kernel(const Params p) {
-  constexpr int QP = F32 ? 3 : 1;             // bf16 parts of queries and weights
+__global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_attn_kernel(const Params p) {
+  using R = Raw<DP, BITS>;
+  constexpr int QP = F32 ? 3 : 1;             // bf16 parts of queries
+  constexpr int WP = F32 ? 3 : 2;             // and of weights
   constexpr int KS = DP / 32;                 // matrix steps along d
-  constexpr int KB = DP / 4 * BITS / 8;       // bytes of a lane's run of a key
-  constexpr int KBLK = DP > 128 ? 2 : 1;      // blocks of exponents in it
-  constexpr int VN = DP / 16;                 // dims of a lane's run of a value
-  constexpr int VB = VN * BITS / 8;
+  constexpr int VN = R::VN;
   constexpr int ACC = VN * 4 * NQ;            // accumulators of a lane
-  extern __shared__ float lds[];              // sums of two waves [2][ACC][64]; before that the timestamp tables
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  // sums of two waves [2][ACC][64]; before that the buckets' thresholds and values, the queries' operands, and the biases [row][sub + 4]
+  extern __shared__ float lds[];
+  int32_t* const thr = (int32_t*)lds;
+  float* const tab = lds + MAX_BUCKETS + 2;
+  bf16x8* const queries = (bf16x8*)(lds + BUCKET_FLOATS);
+  float* const table = lds + BUCKET_FLOATS + NQ * KS * QP * 256;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int H = p.g.H, d = p.g.d, page = p.g.page_size;
+  // (parts last: most sequences are shorter than the longest, and those without work would otherwise come at a fixed distance, which
+  // leaves the working ones to a quarter of the chip: 64 sequences of power-law length up to 2048, 32 us that way)
   int idx = blockIdx.x;
   const int h = idx % H; idx /= H;
-  const int part = idx % p.parts; idx /= p.parts;
-  const int qb = idx % p.qblocks, b = idx / p.qblocks;
+  const int qb = idx % p.qblocks; idx /= p.qblocks;
+  const int b = idx % p.g.B, part = idx / p.g.B;
   const Seq s = seq_of(p, b);
   const int t0 = qb * 16 * NQ;
   if (t0 >= s.count) return;
-  const int t1 = t0 + 16 * NQ < s.count ? t0 + 16 * NQ : s.count;
-  // the block's keys: those of its last row that is there
-  int end = 0;
+  const int t1 = t0 + 16 * NQ < s.count ? t0 + 16 * NQ : s.count, rows = t1 - t0;
+  // the block's keys: those of its last row that is there; below `all` every row attends to every key
+  int end = 0, all = 0;
   {
     const int64_t last = s.place0 + t1 - 1;
-    end = last < 0 ? 0 : last < s.limit ? (int)last + 1 : s.limit;
-    if (s.place0 + t0 >= s.limit) end = 0;
+    end = last < 0 || s.place0 + t0 >= s.limit ? 0 : last < s.limit ? (int)last + 1 : s.limit;
+    all = last < s.limit ? keys_of(s, t0) : 0;
   }
   const int k0 = part * p.chunk;
   if (part > 0 && k0 >= end) return;
   const int k1 = end - k0 < p.chunk ? end : k0 + p.chunk;
 
-  if (p.ts) {
-    int32_t* const thr = (int32_t*)lds;
-    float* const tab = lds + MAX_BUCKETS + 2;
+  // (pos[j - i]: the head's entries from that of the same place on)
+  const float* const pos = p.pos ? p.pos + (int64_t)(p.pos_heads > 1 ? h : 0) * (2 * (int64_t)p.max_len - 1) + p.max_len - 1 : nullptr;
+  const int64_t* const ts = p.ts ? p.ts + (int64_t)b * p.max_len : nullptr;
+  const Buckets buckets{thr, tab, p.ts_buckets, p.buckets_per_log2};
+  if (ts) {
     for (int i = threadIdx.x; i < MAX_BUCKETS + 2; i += THREADS) thr[i] = p.thr[i];
     for (int i = threadIdx.x; i <= p.ts_buckets; i += THREADS) tab[i] = p.ts_tab[(int64_t)(p.ts_heads > 1 ? h : 0) * (p.ts_buckets + 1) + i];
-    __syncthreads();
   }
 
-  // queries: lane (r, g) has row r's dims g d/4 ... of each tile
-  bf16x8 q[NQ][KS][QP];
+  const int row_bytes = d * BITS / 8, blocks = (d + 31) / 32;
+  const bool k_there = g * (DP / 4) < d, v_there = r * VN < d;
+  const int vblk = r * VN / 32 < blocks ? r * VN / 32 : blocks - 1;
+  // a lane's places in a step's rows and exponents
+  const uint32_t k_at = (uint32_t)((8 * (r >> 2) + (r & 3)) * row_bytes + g * R::KB), v_at = (uint32_t)(8 * g * row_bytes + r * R::VB);
+  const uint32_t kx_at = (uint32_t)(g * (DP / 4) / 32 * page + 8 * (r >> 2) + (r & 3)), vx_at = (uint32_t)(vblk * page + 8 * g);
+
+  // the page of a step's keys; steps come in order, so their page is found by counting on
+  int step_page = k0 / page, step_key = k0, step_slot = k0 - step_page * page;
+  auto page_of = [&](int key) {
+    step_slot += key - step_key;
+    step_key = key;
+    while (step_slot >= page) { step_slot -= page; ++step_page; }
+    return p.g.page_table[(int64_t)b * p.g.table_pages + step_page];
+  };
+  R x = {};
+  auto load_k = [&](int id, int slot) {
+    const int64_t head = (int64_t)id * H + h;
+    const uint8_t* const kr = (const uint8_t*)p.g.k_codes + (head * page + slot) * row_bytes;
+    const uint8_t* const kx = (const uint8_t*)p.g.k_scales + head * blocks * page + slot;
+    if (k_there) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        x.k[t] = load_bytes<R::KB>(kr + (k_at + 4 * t * row_bytes));
+#pragma unroll
+        for (int m = 0; m < R::KBLK; ++m) x.ke[t][m] = kx[kx_at + m * page + 4 * t];
+      }
+    }
+  };
+  auto load_v = [&](int id, int slot) {
+    const int64_t head = (int64_t)id * H + h;
+    const uint8_t* const vr = (const uint8_t*)p.g.v_codes + (head * page + slot) * row_bytes;
+    const uint8_t* const vx = (const uint8_t*)p.g.v_scales + head * blocks * page + slot;
+    const uint2 e = *(const uint2*)(vx + vx_at);
+    x.ve[0] = e.x; x.ve[1] = e.y;
+    if (v_there) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.v[i] = load_bytes<R::VB>(vr + (v_at + i * row_bytes));
+    }
+  };
+
+  int next = k0 + STEP * wave, id = -1;
+  if (next < k1) id = __builtin_amdgcn_readfirstlane(page_of(next));
+  bool there = id >= 0 && id < p.g.n_pages;
+  if (there) {
+    load_k(id, step_slot);
+    load_v(id, step_slot);
+  }
+
+  // queries, in LDS as the operands that all four waves use: lane (r, g) has row r's dims g d/4 ... of each tile
   int keys[NQ];
-  int64_t tq[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) keys[n] = keys_of(s, t0 + 16 * n + r);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    const int t = t0 + 16 * n + r;
-    keys[n] = keys_of(s, t);
-    const int64_t row = (p.offsets ? s.first * p.q_st : (int64_t)b * p.q_sb) + (int64_t)t * p.q_st + (int64_t)h * p.q_sh;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
+    const int64_t row = (p.offsets ? s.first * p.q_st : (int64_t)b * p.q_sb) + (int64_t)(t0 + 16 * n + r) * p.q_st + (int64_t)h * p.q_sh;
+    for (int k = wave; k < KS; k += WAVES) {
       const int e = g * (DP / 4) + 8 * k;
-      float x[8] = {};
+      float y[8] = {};
       if (keys[n] > 0 && e < d) {
         if constexpr (F32) {
           const floatx4* at = (const floatx4*)((const float*)p.q + row + e);
           const floatx4 a = at[0], c = at[1];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = c[i]; }
+          for (int i = 0; i < 4; ++i) { y[i] = a[i]; y[4 + i] = c[i]; }
         } else {
-          unpack8(*(const uint4*)((const bf16_t*)p.q + row + e), x);
+          unpack8(*(const uint4*)((const bf16_t*)p.q + row + e), y);
         }
       }
-      split8<QP>(x, q[n][k]);
+      bf16x8 parts[QP];
+      split8<QP>(y, parts);
+#pragma unroll
+      for (int c = 0; c < QP; ++c) queries[((n * KS + k) * QP + c) * 64 + lane] = parts[c];
     }
-    tq[n] = 0;
-    if (p.ts && keys[n] > 0) tq[n] = p.ts[(int64_t)b * p.max_len + (keys[n] < s.last_ts ? keys[n] : s.last_ts)];
   }
 
   floatx4 acc[NQ][VN];
@@ -224,144 +325,156 @@ __global__ __launch_bounds__(THREADS) void hstu_cached_attn_kernel(const Params 
 #pragma unroll
     for (int j = 0; j < VN; ++j) acc[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int row_bytes = d * BITS / 8, blocks = (d + 31) / 32;
-  const uint8_t* const kc = (const uint8_t*)p.g.k_codes;
-  const uint8_t* const vc = (const uint8_t*)p.g.v_codes;
-  const uint8_t* const ks = (const uint8_t*)p.g.k_scales;
-  const uint8_t* const vs = (const uint8_t*)p.g.v_scales;
-  const bool k_there = g * (DP / 4) < d, v_there = r * VN < d;
-  const float* const pos = p.pos ? p.pos + (int64_t)(p.pos_heads > 1 ? h : 0) * (2 * (int64_t)p.max_len - 1) : nullptr;
+  const int sub = 1 << p.sub_log2, pitch = sub + 4;
+  __syncthreads();
+  for (int c0 = k0; c0 < k1; c0 += sub) {
+    const int c1 = k1 - c0 < sub ? k1 : c0 + sub;
+    if (pos || ts) {
+      // a thread has one key at a time and runs over the rows, or over every 2nd, 4th, ... of them
+      __syncthreads();
+      const int wide = p.sub_log2 < 8 ? p.sub_log2 : 8, every = THREADS >> wide;
+      for (int jj = threadIdx.x & ((1 << wide) - 1); jj < c1 - c0; jj += THREADS) {
+        const int j = c0 + jj;
+        const int place0 = (int)s.place0 + t0, first = threadIdx.x >> wide;      // (places of rows: lengths of at most 2^31)
+        if (ts) {
+          const int64_t tk = ts[j];
+#pragma unroll 1
+          for (int t = first; t < rows; t += every) {
+            const int i = place0 + t;
+            float x = 0.f;
+            if (i >= j && i < s.limit) x = (pos ? pos[j - i] : 0.f) + bucket_value(buckets, ts[i < s.last_ts ? i + 1 : s.last_ts] - tk);
+            table[t * pitch + jj] = x;
+          }
+        } else {
+#pragma unroll 4
+          for (int t = first; t < rows; t += every) {
+            const int i = place0 + t;
+            table[t * pitch + jj] = i >= j && i < s.limit ? pos[j - i] : 0.f;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int key0 = next; key0 < c1; key0 = next) {
+      const bool here = there, whole = key0 + STEP <= all;
+      next = key0 + STEP * WAVES;
+      id = -1;
+      if (next < k1) id = __builtin_amdgcn_readfirstlane(page_of(next));
+      there = id >= 0 && id < p.g.n_pages;
+      if (!here) {
+        if (there) {
+          load_k(id, step_slot);
+          load_v(id, step_slot);
+        }
+        continue;
+      }
 
-  for (int key0 = k0 + STEP * wave; key0 < k1; key0 += STEP * WAVES) {
-    const int at = key0 / page, slot0 = key0 - at * page;
-    const int id = __builtin_amdgcn_readfirstlane(p.g.page_table[(int64_t)b * p.g.table_pages + at]);
-    if (id < 0 || id >= p.g.n_pages) continue;
-    const int64_t head = (int64_t)id * H + h;
-    const uint8_t* const kr = kc + (head * page + slot0) * row_bytes;
-    const uint8_t* const vr = vc + (head * page + slot0) * row_bytes + r * VB;
-    const uint8_t* const kx = ks + head * blocks * page + slot0;
-    const uint8_t* const vx = vs + head * blocks * page + slot0 + 8 * g;
-
-    Bytes<KB> kraw[2] = {};
-    uint32_t ke[2][KBLK] = {};
-    if (k_there) {
+      floatx4 st[2][NQ];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int key = 8 * (r >> 2) + 4 * t + (r & 3);
-        kraw[t] = load_bytes<KB>(kr + key * row_bytes + g * KB);
+        uint32_t w[DP / 8];
 #pragma unroll
-        for (int m = 0; m < KBLK; ++m) ke[t][m] = kx[(g * (DP / 4) / 32 + m) * page + key];
-      }
-    }
-    Bytes<VB> vraw[8] = {};
-    uint32_t ve[2];
-    if (v_there) {
+        for (int m = 0; m < R::KBLK; ++m) {
+          const float power = x.ke[t][m] == 255u ? __builtin_nanf("") : power_of(x.ke[t][m]);
+          // (a run of two blocks: half of its bytes each)
+          constexpr int HALF = R::KB / R::KBLK;
+          Bytes<HALF> half;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vraw[i] = load_bytes<VB>(vr + (8 * g + i) * row_bytes);
-    }
-    {
-      const uint2 e = *(const uint2*)(vx + (r * VN / 32 < blocks ? r * VN / 32 : blocks - 1) * page);
-      ve[0] = e.x; ve[1] = e.y;
-    }
-    // rows past the block's last key hold anything: zeros in their place
-    if (key0 + STEP > k1) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (key0 + 8 * g + i >= k1) {
-#pragma unroll
-          for (uint32_t& w : vraw[i].w) w = 0;
-          ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
+          for (int i = 0; i < (HALF < 4 ? 1 : HALF / 4); ++i) half.w[i] = x.k[t].w[m * (HALF / 4) + i];
+          pairs_of<BITS, HALF, DP / 8 / R::KBLK>(half, power, w + m * (DP / 8 / R::KBLK));
         }
-    }
-    // a value row that is not finite makes the kept weights of its key NaN instead (0 times it would be NaN for the others)
-    uint32_t nan_keys = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) nan_keys |= ((ve[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu ? 1u << i : 0u;
-
-    floatx4 st[2][NQ];
+        for (int n = 0; n < NQ; ++n) st[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint32_t w[DP / 8];
+        for (int k = 0; k < KS; ++k) {
+          const bf16x8 a = operand(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 #pragma unroll
-      for (int m = 0; m < KBLK; ++m) {
-        const float power = ke[t][m] == 255u ? __builtin_nanf("") : power_of(ke[t][m]);
-        // (a run of two blocks: half of its bytes each)
-        constexpr int HALF = KB / KBLK;
-        Bytes<HALF> half;
+          for (int n = 0; n < NQ; ++n)
+            if (n == 0 || 16 * n < rows) {
 #pragma unroll
-        for (int i = 0; i < (HALF < 4 ? 1 : HALF / 4); ++i) half.w[i] = kraw[t].w[m * (HALF / 4) + i];
-        pairs_of<BITS, HALF, DP / 8 / KBLK>(half, power, w + m * (DP / 8 / KBLK));
+              for (int c = 0; c < QP; ++c) st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, queries[((n * KS + k) * QP + c) * 64 + lane], st[t][n], 0, 0, 0);
+            }
+        }
       }
+
+      // the next step's keys are on their way while this one's weights and values are worked on, and its values after that
+      if (there) load_k(id, step_slot);
+
+      // rows past the block's last key hold anything: zeros in their place
+      if (key0 + STEP > k1) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) st[t][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 8; ++i)
+          if (key0 + 8 * g + i >= k1) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const bf16x8 a = operand(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            for (uint32_t& w : x.v[i].w) w = 0;
+            x.ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
+          }
+      }
+      // a value row that is not finite makes the kept weights of its key NaN (0 times it would be NaN for the others too)
+      uint32_t nan_keys = 0;
+      const uint32_t odd = (((x.ve[0] & 0x7f7f7f7fu) + 0x01010101u) & x.ve[0]) | (((x.ve[1] & 0x7f7f7f7fu) + 0x01010101u) & x.ve[1]);
+      const bool any_nan = __any((odd & 0x80808080u) != 0);
+      if (any_nan) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (((x.ve[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu) {
+            nan_keys |= 1u << i;
+            x.ve[i / 4] ^= 0x80u << (8 * (i % 4));
+          }
+      }
+
+      bf16x8 w8[NQ][WP];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        if (n > 0 && 16 * n >= rows) continue;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = p.alpha * st[i / 4][n][i % 4];
+        if (pos || ts) {
+          const floatx4* const at = (const floatx4*)(table + (16 * n + r < rows ? 16 * n + r : rows - 1) * pitch + (key0 - c0) + 8 * g);
+          const floatx4 lo = at[0], hi = at[1];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = silu(y[i]);
+        if (!whole || any_nan) {
+          const int j0 = key0 + 8 * g;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (nan_keys >> i & 1u) y[i] = __builtin_nanf("");
+            y[i] = j0 + i < keys[n] ? y[i] : 0.f;
+          }
+        }
+        split8<WP>(y, w8[n]);
+      }
+
+      float power[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) power[i] = power_of((x.ve[i / 4] >> (8 * (i % 4))) & 0xffu);
+      // dims 2 m and 2 m + 1 of the lane's run: its keys' pairs, then one operand for each
+      each_pair<0, VN / 2>([&](auto m) {
+        constexpr int M = decltype(m)::value;
+        uint32_t pair[8], lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pair[i] = pair_at<BITS, M>(x.v[i], power[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i], 0x05040100u);
+          hi[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i], 0x07060302u);
+        }
+        const bf16x8 a0 = operand(lo[0], lo[1], lo[2], lo[3]), a1 = operand(hi[0], hi[1], hi[2], hi[3]);
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
+          if (n == 0 || 16 * n < rows) {
 #pragma unroll
-          for (int c = 0; c < QP; ++c) st[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[n][k][c], st[t][n], 0, 0, 0);
-      }
-    }
-
-    bf16x8 w8[NQ][QP];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p.alpha * st[i / 4][n][i % 4];
-      const int j0 = key0 + 8 * g;                       // the lane's keys: j0 .. j0 + 7
-      if (pos) {
-        // (kept pairs lie inside the table; the others read its ends)
-        const int64_t top = 2 * ((int64_t)p.max_len - 1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          int64_t e = (int64_t)p.max_len + j0 + i - keys[n];
-          e = e < 0 ? 0 : e > top ? top : e;
-          x[i] += pos[e];
-        }
-      }
-      if (p.ts) {
-        const int32_t* const thr = (const int32_t*)lds;
-        const float* const tab = lds + MAX_BUCKETS + 2;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = j0 + i < p.max_len ? j0 + i : p.max_len - 1;
-          int64_t gap = tq[n] - p.ts[(int64_t)b * p.max_len + j];
-          gap = gap < 0 ? -gap : gap;
-          const int dt = gap < 1 ? 1 : gap > 1000000000 ? 1000000000 : (int)gap;
-          int bk = (int)(__builtin_amdgcn_logf((float)dt) * p.buckets_per_log2);
-          bk = bk < 0 ? 0 : bk > p.ts_buckets ? p.ts_buckets : bk;
-          bk = dt < thr[bk] ? bk - 1 : dt >= thr[bk + 1] ? bk + 1 : bk;
-          x[i] += tab[bk];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float y = silu(x[i]);
-        if (nan_keys >> i & 1u) y = __builtin_nanf("");
-        x[i] = j0 + i < keys[n] ? y : 0.f;
-      }
-      split8<QP>(x, w8[n]);
-    }
-
-    uint32_t pairs[8][VN / 2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t e = (ve[i / 4] >> (8 * (i % 4))) & 0xffu;
-      pairs_of<BITS, VB, VN / 2>(vraw[i], power_of(e == 255u ? 127u : e), pairs[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < VN; ++j) {
-      uint32_t w[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        w[m] = __builtin_amdgcn_perm(pairs[2 * m + 1][j / 2], pairs[2 * m][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-      const bf16x8 a = operand(w[0], w[1], w[2], w[3]);
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int c = 0; c < QP; ++c) acc[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w8[n][c], acc[n][j], 0, 0, 0);
+            for (int c = 0; c < WP; ++c) {
+              acc[n][2 * M] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, w8[n][c], acc[n][2 * M], 0, 0, 0);
+              acc[n][2 * M + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, w8[n][c], acc[n][2 * M + 1], 0, 0, 0);
+            }
+          }
+      });
+      if (there) load_v(id, step_slot);
     }
   }
 
@@ -441,7 +554,7 @@ __global__ __launch_bounds__(THREADS) void hstu_cached_attn_join(const Params p)
 }
 
 // The bucket law's integer thresholds up to bucket `count`: thr[b] is the smallest time difference in [1, 1e9] whose bucket
-// floor(ln(fl32(dt)) / size) is b or more (INT32_MAX: none).
+// floor(ln(fl32(dt)) / size) is b or more (INT32_MAX: none).  The last size's are kept.
 void thresholds(float size, int count, int32_t* out) {
   static std::mutex lock;
   static float known = -1.f;
@@ -513,7 +626,9 @@ size_t workspace_of(const HstuCachedAttnArgs& a, const Split& s) {
 template <int DP, int BITS, bool F32, int NQ>
 void launch(const Params& p, uint32_t grid, hipStream_t st) {
   constexpr int ACC = DP / 16 * 4 * NQ;
-  const size_t lds = std::max<size_t>((size_t)2 * ACC * 64 * sizeof(float), (2 * MAX_BUCKETS + 4) * sizeof(float));
+  const int rows = std::min(p.per_seq, 16 * NQ);
+  const size_t biases = p.pos || p.ts ? (size_t)rows * ((1 << p.sub_log2) + 4) : 0;
+  const size_t lds = std::max<size_t>((size_t)2 * ACC * 64, BUCKET_FLOATS + NQ * (DP / 32) * (F32 ? 3 : 1) * 256 + biases) * sizeof(float);
   hstu_cached_attn_kernel<DP, BITS, F32, NQ><<<grid, THREADS, lds, st>>>(p);
 }
 
@@ -574,6 +689,9 @@ int hstu_cached_attn(const HstuCachedAttnArgs* a, void* stream) {
   p.partial = s.parts > 1 ? (float*)a->workspace : nullptr;
   p.per_seq = a->rows_per_seq; p.max_len = a->max_len; p.pos_heads = a->pos_heads; p.ts_heads = a->ts_heads; p.ts_buckets = a->ts_buckets;
   p.chunk = s.chunk; p.parts = s.parts; p.qblocks = s.qblocks;
+  // biases of 8192 pairs at a time, and of 2048 keys at most
+  p.sub_log2 = 11;
+  while (p.sub_log2 > 7 && ((int64_t)std::min(a->rows_per_seq, 16 * s.nq) << p.sub_log2) > 8192) --p.sub_log2;
   p.alpha = a->alpha; p.inv_n = a->inv_n; p.buckets_per_log2 = 0.f;
   if (a->timestamps) {
     thresholds(a->ts_bucket_size, a->ts_buckets, p.thr);
