@@ -33,6 +33,8 @@
 
 namespace {
 
+typedef __attribute__((address_space(4))) int32_t Constant;   // what no kernel writes while this one runs
+
 constexpr int WAVES = 4;
 constexpr int THREADS = 64 * WAVES;
 constexpr int STEP = 32;             // keys of a wave's step
@@ -80,6 +82,7 @@ __device__ __forceinline__ Seq seq_of(const Params& p, int b) {
   const int64_t held = (int64_t)p.g.table_pages * p.g.page_size;
   int limit = n < p.max_len ? n : p.max_len;
   limit = limit < held ? limit : (int)held;
+  if (p.g.n_pages == 0) limit = 0;
   s.limit = limit < 0 ? 0 : limit;
   s.last_ts = (n < p.max_len ? n : p.max_len) - 1;
   return s;
@@ -138,10 +141,9 @@ __device__ __forceinline__ bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, ui
   return __builtin_bit_cast(bf16x8, uint4{a, b, c, d});
 }
 
-__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
-
-// x as bf16 parts whose sum it is (the third one takes what is left to its last bit)
-template <int PARTS>
+// x as bf16 parts whose sum it is (the third one takes what is left to its last bit).  KEEP: an infinity stays one (without, it becomes
+// a NaN: weights, whose sum with others it would make one in any case).
+template <int PARTS, bool KEEP>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]) {
   float rest[8];
 #pragma unroll
@@ -153,10 +155,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&out)[PARTS]
     for (int i = 0; i < 4; ++i) {
       w[i] = pack2(rest[2 * i], rest[2 * i + 1]);
       if (n + 1 < PARTS) {
-        // (what is left of an infinity is nothing)
         const float lo = __builtin_bit_cast(float, w[i] << 16), hi = __builtin_bit_cast(float, w[i] & 0xffff0000u);
-        rest[2 * i] = __builtin_isinf(lo) ? 0.f : rest[2 * i] - lo;
-        rest[2 * i + 1] = __builtin_isinf(hi) ? 0.f : rest[2 * i + 1] - hi;
+        rest[2 * i] = KEEP && __builtin_isinf(lo) ? 0.f : rest[2 * i] - lo;
+        rest[2 * i + 1] = KEEP && __builtin_isinf(hi) ? 0.f : rest[2 * i + 1] - hi;
       }
     }
     out[n] = operand(w[0], w[1], w[2], w[3]);
@@ -197,7 +198,7 @@ struct Raw {
   uint32_t ve[2];
 };
 
-template <int DP, int BITS, bool F32, int NQ>
+template <int DP, bool EXACT, int BITS, bool F32, int NQ>
 __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_attn_kernel(const Params p) {
   using R = Raw<DP, BITS>;
   constexpr int QP = F32 ? 3 : 1;             // bf16 parts of queries
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
   bf16x8* const queries = (bf16x8*)(lds + BUCKET_FLOATS);
   float* const table = lds + BUCKET_FLOATS + NQ * KS * QP * 256;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int H = p.g.H, d = p.g.d, page = p.g.page_size;
+  const int H = p.g.H, d = EXACT ? DP : p.g.d, page = p.g.page_size;
   // (parts last: most sequences are shorter than the longest, and those without work would otherwise come at a fixed distance, which
   // leaves the working ones to a quarter of the chip: 64 sequences of power-law length up to 2048, 32 us that way)
   int idx = blockIdx.x;
@@ -244,52 +245,62 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
   }
 
   const int row_bytes = d * BITS / 8, blocks = (d + 31) / 32;
-  const bool k_there = g * (DP / 4) < d, v_there = r * VN < d;
-  const int vblk = r * VN / 32 < blocks ? r * VN / 32 : blocks - 1;
-  // a lane's places in a step's rows and exponents
-  const uint32_t k_at = (uint32_t)((8 * (r >> 2) + (r & 3)) * row_bytes + g * R::KB), v_at = (uint32_t)(8 * g * row_bytes + r * R::VB);
-  const uint32_t kx_at = (uint32_t)(g * (DP / 4) / 32 * page + 8 * (r >> 2) + (r & 3)), vx_at = (uint32_t)(vblk * page + 8 * g);
+  // a lane's places in a step's rows and exponents; lanes past the head's dims read its first ones (their part of Q is zeros, their rows
+  // of O^T go nowhere)
+  const int kg = g * (DP / 4) < d ? g : 0, vg = r * VN < d ? r : 0;
+  const uint32_t k_lane = (uint32_t)((8 * (r >> 2) + (r & 3)) * row_bytes + kg * R::KB), v_lane = (uint32_t)(8 * g * row_bytes + vg * R::VB);
+  const uint32_t kx_lane = (uint32_t)(kg * (DP / 4) / 32 * page + 8 * (r >> 2) + (r & 3)), vx_lane = (uint32_t)(vg * VN / 32 * page + 8 * g);
+  // the head's rows and exponents in page 0, and from one page to the next
+  const int64_t code_page = (int64_t)H * page * row_bytes, scale_page = (int64_t)H * blocks * page;
+  const uint8_t* const k_head = (const uint8_t*)p.g.k_codes + (int64_t)h * page * row_bytes;
+  const uint8_t* const v_head = (const uint8_t*)p.g.v_codes + (int64_t)h * page * row_bytes;
+  const uint8_t* const kx_head = (const uint8_t*)p.g.k_scales + (int64_t)h * blocks * page;
+  const uint8_t* const vx_head = (const uint8_t*)p.g.v_scales + (int64_t)h * blocks * page;
 
-  // the page of a step's keys; steps come in order, so their page is found by counting on
-  int step_page = k0 / page, step_key = k0, step_slot = k0 - step_page * page;
-  auto page_of = [&](int key) {
-    step_slot += key - step_key;
-    step_key = key;
-    while (step_slot >= page) { step_slot -= page; ++step_page; }
-    return p.g.page_table[(int64_t)b * p.g.table_pages + step_page];
+  // the page of a step's keys; steps come in order, so their page is found by counting on.  A page that is not there stands for page 0
+  // with all of its keys masked, a step past the last for the last one: every step loads, whatever comes of it.
+  int at_page = k0 / page, at_key = k0, slot = k0 - at_page * page, id = 0;
+  bool there = false;
+  auto go_to = [&](int key) {
+    if (key >= k1) return;
+    slot += key - at_key;
+    at_key = key;
+    while (slot >= page) { slot -= page; ++at_page; }
+    // (a scalar load: a vector one would be waited for behind all of the step's)
+    id = ((const Constant*)(uintptr_t)p.g.page_table)[(int64_t)b * p.g.table_pages + __builtin_amdgcn_readfirstlane(at_page)];
+    there = id >= 0 && id < p.g.n_pages;
+    id = there ? id : 0;
   };
   R x = {};
-  auto load_k = [&](int id, int slot) {
-    const int64_t head = (int64_t)id * H + h;
-    const uint8_t* const kr = (const uint8_t*)p.g.k_codes + (head * page + slot) * row_bytes;
-    const uint8_t* const kx = (const uint8_t*)p.g.k_scales + head * blocks * page + slot;
-    if (k_there) {
+  // (the lane's part of an address stays 32 bits beside a scalar base)
+  auto load_k = [&]() {
+    uint32_t at = k_lane, xat = kx_lane;
+    asm volatile("" : "+v"(at), "+v"(xat));
+    const uint8_t* const rows = k_head + (id * code_page + slot * row_bytes);
+    const uint8_t* const exps = kx_head + (id * scale_page + slot);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        x.k[t] = load_bytes<R::KB>(kr + (k_at + 4 * t * row_bytes));
+    for (int t = 0; t < 2; ++t) {
+      x.k[t] = load_bytes<R::KB>(rows + 4 * t * row_bytes + at);
 #pragma unroll
-        for (int m = 0; m < R::KBLK; ++m) x.ke[t][m] = kx[kx_at + m * page + 4 * t];
-      }
+      for (int m = 0; m < R::KBLK; ++m) x.ke[t][m] = (exps + m * page + 4 * t)[xat];
     }
   };
-  auto load_v = [&](int id, int slot) {
-    const int64_t head = (int64_t)id * H + h;
-    const uint8_t* const vr = (const uint8_t*)p.g.v_codes + (head * page + slot) * row_bytes;
-    const uint8_t* const vx = (const uint8_t*)p.g.v_scales + head * blocks * page + slot;
-    const uint2 e = *(const uint2*)(vx + vx_at);
+  auto load_v = [&]() {
+    uint32_t at = v_lane, xat = vx_lane;
+    asm volatile("" : "+v"(at), "+v"(xat));
+    const uint8_t* const rows = v_head + (id * code_page + slot * row_bytes);
+    const uint2 e = *(const uint2*)(vx_head + (id * scale_page + slot) + xat);
     x.ve[0] = e.x; x.ve[1] = e.y;
-    if (v_there) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x.v[i] = load_bytes<R::VB>(vr + (v_at + i * row_bytes));
-    }
+    for (int i = 0; i < 8; ++i) x.v[i] = load_bytes<R::VB>(rows + i * row_bytes + at);
   };
 
-  int next = k0 + STEP * wave, id = -1;
-  if (next < k1) id = __builtin_amdgcn_readfirstlane(page_of(next));
-  bool there = id >= 0 && id < p.g.n_pages;
-  if (there) {
-    load_k(id, step_slot);
-    load_v(id, step_slot);
+  const bool any = k0 < k1 && p.g.n_pages > 0;
+  int next = k0 + STEP * wave;
+  if (any) {
+    go_to(next);
+    load_k();
+    load_v();
   }
 
   // queries, in LDS as the operands that all four waves use: lane (r, g) has row r's dims g d/4 ... of each tile
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
         }
       }
       bf16x8 parts[QP];
-      split8<QP>(y, parts);
+      split8<QP, true>(y, parts);
 #pragma unroll
       for (int c = 0; c < QP; ++c) queries[((n * KS + k) * QP + c) * 64 + lane] = parts[c];
     }
@@ -356,18 +367,10 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
       __syncthreads();
     }
     for (int key0 = next; key0 < c1; key0 = next) {
-      const bool here = there, whole = key0 + STEP <= all;
+      const int last = there ? k1 : key0;                 // (no key of a missing page is there)
+      const bool whole = there && key0 + STEP <= all;
       next = key0 + STEP * WAVES;
-      id = -1;
-      if (next < k1) id = __builtin_amdgcn_readfirstlane(page_of(next));
-      there = id >= 0 && id < p.g.n_pages;
-      if (!here) {
-        if (there) {
-          load_k(id, step_slot);
-          load_v(id, step_slot);
-        }
-        continue;
-      }
+      go_to(next);
 
       floatx4 st[2][NQ];
 #pragma unroll
@@ -398,13 +401,13 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
       }
 
       // the next step's keys are on their way while this one's weights and values are worked on, and its values after that
-      if (there) load_k(id, step_slot);
+      load_k();
 
       // rows past the block's last key hold anything: zeros in their place
-      if (key0 + STEP > k1) {
+      if (key0 + STEP > last) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (key0 + 8 * g + i >= k1) {
+          if (key0 + 8 * g + i >= last) {
 #pragma unroll
             for (uint32_t& w : x.v[i].w) w = 0;
             x.ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
@@ -428,25 +431,35 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
       for (int n = 0; n < NQ; ++n) {
         if (n > 0 && 16 * n >= rows) continue;
         float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = p.alpha * st[i / 4][n][i % 4];
         if (pos || ts) {
           const floatx4* const at = (const floatx4*)(table + (16 * n + r < rows ? 16 * n + r : rows - 1) * pitch + (key0 - c0) + 8 * g);
           const floatx4 lo = at[0], hi = at[1];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { y[i] += lo[i]; y[4 + i] += hi[i]; }
-        }
+          for (int i = 0; i < 4; ++i) {
+            y[i] = __builtin_fmaf(p.alpha, st[0][n][i], lo[i]);
+            y[4 + i] = __builtin_fmaf(p.alpha, st[1][n][i], hi[i]);
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = silu(y[i]);
+          for (int i = 0; i < 8; ++i) y[i] = p.alpha * st[i / 4][n][i % 4];
+        }
+        // x sigmoid(x), a stage at a time: the transcendentals of eight keys wait for none of each other
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(-LOG2E * y[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_rcpf(1.0f + e[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= e[i];
         if (!whole || any_nan) {
           const int j0 = key0 + 8 * g;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (nan_keys >> i & 1u) y[i] = __builtin_nanf("");
-            y[i] = j0 + i < keys[n] ? y[i] : 0.f;
+            y[i] = j0 + i < keys[n] && j0 + i < last ? y[i] : 0.f;
           }
         }
-        split8<WP>(y, w8[n]);
+        split8<WP, false>(y, w8[n]);
       }
 
       float power[8];
@@ -474,7 +487,7 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
             }
           }
       });
-      if (there) load_v(id, step_slot);
+      load_v();
     }
   }
 
@@ -623,32 +636,39 @@ size_t workspace_of(const HstuCachedAttnArgs& a, const Split& s) {
   return (size_t)rows * a.pages.H * s.parts * a.pages.d * sizeof(float);
 }
 
-template <int DP, int BITS, bool F32, int NQ>
+template <int DP, bool EXACT, int BITS, bool F32, int NQ>
 void launch(const Params& p, uint32_t grid, hipStream_t st) {
   constexpr int ACC = DP / 16 * 4 * NQ;
   const int rows = std::min(p.per_seq, 16 * NQ);
   const size_t biases = p.pos || p.ts ? (size_t)rows * ((1 << p.sub_log2) + 4) : 0;
   const size_t lds = std::max<size_t>((size_t)2 * ACC * 64, BUCKET_FLOATS + NQ * (DP / 32) * (F32 ? 3 : 1) * 256 + biases) * sizeof(float);
-  hstu_cached_attn_kernel<DP, BITS, F32, NQ><<<grid, THREADS, lds, st>>>(p);
+  hstu_cached_attn_kernel<DP, EXACT, BITS, F32, NQ><<<grid, THREADS, lds, st>>>(p);
 }
 
-template <int DP, int BITS>
+template <int DP, bool EXACT, int BITS>
 void launch_nq(const Params& p, bool f32, int nq, uint32_t grid, hipStream_t st) {
   if (f32) {
-    if constexpr (DP <= 128) { if (nq == 2) return launch<DP, BITS, true, 2>(p, grid, st); }
-    return launch<DP, BITS, true, 1>(p, grid, st);
+    if constexpr (DP <= 128) { if (nq == 2) return launch<DP, EXACT, BITS, true, 2>(p, grid, st); }
+    return launch<DP, EXACT, BITS, true, 1>(p, grid, st);
   }
-  if constexpr (DP <= 128) { if (nq == 4) return launch<DP, BITS, false, 4>(p, grid, st); }
-  if (nq == 2) return launch<DP, BITS, false, 2>(p, grid, st);
-  launch<DP, BITS, false, 1>(p, grid, st);
+  if constexpr (DP <= 128) { if (nq == 4) return launch<DP, EXACT, BITS, false, 4>(p, grid, st); }
+  if (nq == 2) return launch<DP, EXACT, BITS, false, 2>(p, grid, st);
+  launch<DP, EXACT, BITS, false, 1>(p, grid, st);
+}
+
+// Head dims that are no power of two (and those below 32) run as the next one with the lanes' addresses cut off.
+template <int DP, int BITS>
+void launch_exact(const Params& p, bool f32, int nq, uint32_t grid, hipStream_t st) {
+  if (p.g.d == DP) launch_nq<DP, true, BITS>(p, f32, nq, grid, st);
+  else launch_nq<DP, false, BITS>(p, f32, nq, grid, st);
 }
 
 template <int BITS>
 void launch_width(const Params& p, bool f32, int nq, uint32_t grid, hipStream_t st) {
-  if (p.g.d <= 32) launch_nq<32, BITS>(p, f32, nq, grid, st);
-  else if (p.g.d <= 64) launch_nq<64, BITS>(p, f32, nq, grid, st);
-  else if (p.g.d <= 128) launch_nq<128, BITS>(p, f32, nq, grid, st);
-  else launch_nq<256, BITS>(p, f32, nq, grid, st);
+  if (p.g.d <= 32) launch_exact<32, BITS>(p, f32, nq, grid, st);
+  else if (p.g.d <= 64) launch_exact<64, BITS>(p, f32, nq, grid, st);
+  else if (p.g.d <= 128) launch_exact<128, BITS>(p, f32, nq, grid, st);
+  else launch_exact<256, BITS>(p, f32, nq, grid, st);
 }
 
 }  // namespace
