@@ -337,6 +337,9 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
     for (int j = 0; j < VN; ++j) acc[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int sub = 1 << p.sub_log2, pitch = sub + 4;
+  // (vmcnt(0), here and behind the biases: what the compiler does not know to have arrived when the loop begins it waits for in every
+  // round of it, and with it for the loads ahead)
+  __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
   for (int c0 = k0; c0 < k1; c0 += sub) {
     const int c1 = k1 - c0 < sub ? k1 : c0 + sub;
@@ -364,6 +367,7 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
           }
         }
       }
+      __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
     }
     for (int key0 = next; key0 < c1; key0 = next) {
@@ -403,26 +407,31 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
       // the next step's keys are on their way while this one's weights and values are worked on, and its values after that
       load_k();
 
+      // (copies: what the loads write stays untouched, or the compiler moves it while it is on its way and waits for it to do so)
+      Bytes<R::VB> v[8];
+      uint32_t ve[2] = {x.ve[0], x.ve[1]};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = x.v[i];
       // rows past the block's last key hold anything: zeros in their place
       if (key0 + STEP > last) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (key0 + 8 * g + i >= last) {
 #pragma unroll
-            for (uint32_t& w : x.v[i].w) w = 0;
-            x.ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
+            for (uint32_t& w : v[i].w) w = 0;
+            ve[i / 4] &= ~(0xffu << (8 * (i % 4)));
           }
       }
       // a value row that is not finite makes the kept weights of its key NaN (0 times it would be NaN for the others too)
       uint32_t nan_keys = 0;
-      const uint32_t odd = (((x.ve[0] & 0x7f7f7f7fu) + 0x01010101u) & x.ve[0]) | (((x.ve[1] & 0x7f7f7f7fu) + 0x01010101u) & x.ve[1]);
+      const uint32_t odd = (((ve[0] & 0x7f7f7f7fu) + 0x01010101u) & ve[0]) | (((ve[1] & 0x7f7f7f7fu) + 0x01010101u) & ve[1]);
       const bool any_nan = __any((odd & 0x80808080u) != 0);
       if (any_nan) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (((x.ve[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu) {
+          if (((ve[i / 4] >> (8 * (i % 4))) & 0xffu) == 0xffu) {
             nan_keys |= 1u << i;
-            x.ve[i / 4] ^= 0x80u << (8 * (i % 4));
+            ve[i / 4] ^= 0x80u << (8 * (i % 4));
           }
       }
 
@@ -464,13 +473,13 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
 
       float power[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) power[i] = power_of((x.ve[i / 4] >> (8 * (i % 4))) & 0xffu);
+      for (int i = 0; i < 8; ++i) power[i] = power_of((ve[i / 4] >> (8 * (i % 4))) & 0xffu);
       // dims 2 m and 2 m + 1 of the lane's run: its keys' pairs, then one operand for each
       each_pair<0, VN / 2>([&](auto m) {
         constexpr int M = decltype(m)::value;
         uint32_t pair[8], lo[4], hi[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pair[i] = pair_at<BITS, M>(x.v[i], power[i]);
+        for (int i = 0; i < 8; ++i) pair[i] = pair_at<BITS, M>(v[i], power[i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           lo[i] = __builtin_amdgcn_perm(pair[2 * i + 1], pair[2 * i], 0x05040100u);
