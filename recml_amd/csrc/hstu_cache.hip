@@ -3,7 +3,7 @@
 //   hstu_kv_write   rows of new events -> codes and block exponents
 //   hstu_kv_read    codes and exponents -> rows
 //
-// Both are passes over memory.  One workgroup takes 32 places of one (sequence, head): page sizes are multiples of 32 and
+// Both are passes over memory.  One workgroup takes 32 places of one (sequence, head), keys and values: page sizes are multiples of 32 and
 // the places start at a multiple of 32, so it stays inside one page, its codes are one run of 32 rows and its exponents one
 // run of 32 bytes per block.
 
@@ -37,7 +37,8 @@ int serve_launched(const char* what) {
 namespace {
 
 constexpr int TILE = 32;     // places of one workgroup
-constexpr int THREADS = 256;
+
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
 // One of the two tensors of a call.
 struct Side {
@@ -66,137 +67,208 @@ __device__ __forceinline__ void rows_of(const Params& p, int b, int64_t* first, 
   *count = (int)(o1 - o0 < p.per_seq ? o1 - o0 : p.per_seq);
 }
 
+// Eight values of a row as they lie in memory.
 template <bool F32>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]) {
+struct Eight { uint4 w[F32 ? 2 : 1]; };
+
+template <bool F32>
+__device__ __forceinline__ void load8(const void* base, int64_t at, Eight<F32>& x) {
+  const uint4* const from = (const uint4*)((const char*)base + at * (F32 ? 4 : 2));
+#pragma unroll
+  for (int i = 0; i < (F32 ? 2 : 1); ++i) x.w[i] = from[i];
+}
+
+// The largest of the eight magnitudes, as fp32 bits (0x7f800000 and more: an infinity, a NaN).
+template <bool F32>
+__device__ __forceinline__ uint32_t largest(const Eight<F32>& x) {
   if constexpr (F32) {
-    const floatx4* s = (const floatx4*)((const float*)base + at);
-    const floatx4 a = s[0], b = s[1];
+    const uint32_t w[8] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w, x.w[1].x, x.w[1].y, x.w[1].z, x.w[1].w};
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+    for (int i = 0; i < 8; ++i) m = (w[i] & 0x7fffffffu) > m ? w[i] & 0x7fffffffu : m;
+    return m;
   } else {
-    unpack8(*(const uint4*)((const bf16_t*)base + at), x);
+    const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
+    ushort2v m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2v, w[i] & 0x7fff7fffu));
+    return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
   }
 }
 
-// LPR lanes per row (8 values each); rows r, r + THREADS / LPR, ... of the tile.
-template <int BITS, bool F32, int LPR>
-__global__ __launch_bounds__(THREADS) void hstu_kv_write_kernel(const Params p) {
-  constexpr int ROWS = THREADS / LPR;
-  const int d = p.g.d, H = p.g.H, page = p.g.page_size;
-  const int h = blockIdx.x % H, tile = blockIdx.x / H % p.tiles, b = blockIdx.x / H / p.tiles;
-  const Side s = p.side[blockIdx.y];
-  int64_t first;
-  int count;
-  rows_of(p, b, &first, &count);
-  const int64_t start = p.starts[b];
-  // places of the tile: whole multiples of 32, the first one at or below `start` (which may be negative)
+// Their codes under the power 2^(e - 127).
+template <int BITS, bool F32>
+__device__ __forceinline__ uint2 codes_of(const Eight<F32>& x, uint32_t e) {
+  uint32_t code[2] = {0, 0};
+  if constexpr (BITS == 4) {
+    // the hardware's scaled conversion: to the nearest code, ties to the even one, past the largest to the largest
+    const float power = power_of(e);
+    if constexpr (F32) {
+      const float* const y = (const float*)&x;
+      uint32_t c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[0], y[1], power, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], power, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[4], y[5], power, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[6], y[7], power, 3);
+      code[0] = c;
+    } else {
+      uint32_t c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, x.w[0].x), power, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, x.w[0].y), power, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, x.w[0].z), power, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, x.w[0].w), power, 3);
+      code[0] = c;
+    }
+  } else {
+    float y[8];
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = ((const float*)&x)[i];
+    } else {
+      unpack8(x.w[0], y);
+    }
+    const float inverse = power_of(254 - e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(y[i] * inverse, -448.f, 448.f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+      code[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], c, true);
+    }
+  }
+  return uint2{code[0], code[1]};
+}
+
+constexpr int threads_of(int lpr) { return lpr < 8 ? TILE * lpr : 256; }
+
+// What a workgroup's 32 places are: the rows of one (sequence, head) from place `base` on.
+struct Tile {
+  int64_t t0;            // the sequence's row at the tile's first place (may be negative)
+  int64_t first;         // the sequence's first row
+  int count;             // and how many it has
+  int h, b;
+  int64_t row0;          // kv_row of the tile's first place
+};
+
+__device__ __forceinline__ bool tile_of(const Params& p, Tile* t) {
+  t->h = blockIdx.x % p.g.H;
+  const int tile = blockIdx.x / p.g.H % p.tiles;
+  t->b = blockIdx.x / p.g.H / p.tiles;
+  rows_of(p, t->b, &t->first, &t->count);
+  const int64_t start = p.starts[t->b];
+  // (the first tile's first place: the multiple of 32 at or below `start`, which may be negative)
   const int64_t base = (start - (((start % TILE) + TILE) % TILE)) + (int64_t)tile * TILE;
-  if (base >= start + count) return;
-  const int64_t row0 = kv_row(p.g, b, base);
-  if (row0 < 0) return;
-  const int lane = threadIdx.x % LPR;
+  t->t0 = base - start;
+  if (t->t0 >= t->count) return false;
+  t->row0 = kv_row(p.g, t->b, base);
+  return true;
+}
+
+// LPR lanes per row (8 values each); all of a thread's rows, of the keys and of the values, are on their way before the first is
+// worked on: 65.5 k rows of 8 x 128, in and out 340 MB: 128 us with one load at a time, WRITE_US so.
+template <int BITS, bool F32, int LPR>
+__global__ __launch_bounds__(threads_of(LPR)) void hstu_kv_write_kernel(const Params p) {
+  constexpr int ROWS = threads_of(LPR) / LPR, PASSES = TILE / ROWS;
+  Tile t;
+  if (!tile_of(p, &t) || t.row0 < 0) return;
+  const int d = p.g.d, page = p.g.page_size, lane = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
   const int blocks = (d + 31) / 32, row_bytes = d * BITS / 8;
-  const int64_t head0 = row0 + (int64_t)h * page;               // row of the tile's first place in its head's rows
-  // (codes: rows of row_bytes; exponents: [page, head, block, slot])
-  const int64_t page_head = (row0 / page) + h, slot0 = row0 % page;
-  for (int r = threadIdx.x / LPR; r < TILE; r += ROWS) {
-    const int64_t t = base + r - start;
-    const bool there = t >= 0 && t < count && lane * 8 < d;
-    float x[8] = {};
-    if (there) load8<F32>(s.rows, (p.offsets ? 0 : (int64_t)b * s.sb) + (first + t) * s.st + (int64_t)h * s.sh + lane * 8, x);
-    float top = 0.f;
-    uint32_t bad = 0;
+  Eight<F32> x[2][PASSES];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t m = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
-      bad |= m >= 0x7f800000u;
-      top = fmaxf(top, __builtin_bit_cast(float, m));
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n) {
+      const int64_t row = t.t0 + r0 + n * ROWS;
+      x[s][n] = Eight<F32>{};
+      if (row >= 0 && row < t.count && lane * 8 < d)
+        load8<F32>(p.side[s].rows, (p.offsets ? 0 : (int64_t)t.b * p.side[s].sb) + (t.first + row) * p.side[s].st + (int64_t)t.h * p.side[s].sh + lane * 8, x[s][n]);
     }
-    // a block's four lanes, then the row's
+  const int64_t head0 = t.row0 + (int64_t)t.h * page;               // row of the tile's first place in its head's rows
+  const int64_t page_head = t.row0 / page + t.h, slot0 = t.row0 % page;
 #pragma unroll
-    for (int m = 1; m < 4 && m < LPR; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int m = 1; m < LPR; m <<= 1) bad |= __shfl_xor(bad, m, 64);
-    // the exponent: floor(log2 top) less the largest code's, one more where top is past the middle above that code
-    const uint32_t bits = __builtin_bit_cast(uint32_t, top);
-    constexpr int TOP_EXP = BITS == 4 ? 2 : 8;
-    constexpr uint32_t PAST = BITS == 4 ? 0x600000u : 0x680000u;      // mantissas of 1.75 and 1.8125
-    int e = (int)(bits >> 23) - TOP_EXP + ((bits & 0x7fffffu) > PAST ? 1 : 0);
-    constexpr int MOST = BITS == 4 ? 252 : 246;                        // (no code stands for more than fp32 holds: such rows saturate)
-    e = e < 1 ? 1 : e > MOST ? MOST : e;                               // (top = 0 too)
-    const float inverse = power_of((uint32_t)(254 - e));
-    uint32_t code[2] = {0, 0};
-    if (!bad) {
+    for (int n = 0; n < PASSES; ++n) {
+      const int r = r0 + n * ROWS;
+      const int64_t row = t.t0 + r;
+      // a block's four lanes, then the row's
+      uint32_t top = largest<F32>(x[s][n]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = x[i] * inverse, m = __builtin_fabsf(y);
-        if constexpr (BITS == 4) {
-          // the grid's steps are 1/2 below 2, 1 below 4 and 2 from there: rint at each is to the nearest code, ties to even
-          const float c = m < 2.f ? __builtin_rintf(2.f * m) : m < 4.f ? __builtin_rintf(m) + 2.f : fminf(__builtin_rintf(0.5f * m) + 4.f, 7.f);
-          code[0] |= ((uint32_t)c | ((__builtin_bit_cast(uint32_t, y) >> 28) & 8u)) << (4 * i);
-        } else {
-          const float z = fminf(fmaxf(y, -448.f), 448.f);
-          const int byte = __builtin_amdgcn_cvt_pk_fp8_f32(z, z, 0, false) & 0xff;
-          code[i / 4] |= (uint32_t)byte << (8 * (i % 4));
-        }
+      for (int m = 1; m < 4; m <<= 1) {
+        const uint32_t o = __shfl_xor(top, m, 64);
+        top = o > top ? o : top;
       }
+      uint32_t bad = top >= 0x7f800000u;
+#pragma unroll
+      for (int m = 4; m < LPR; m <<= 1) bad |= __shfl_xor(bad, m, 64);
+      // the exponent: floor(log2 top) less the largest code's, one more where top is past the middle above that code
+      constexpr int TOP_EXP = BITS == 4 ? 2 : 8;
+      constexpr uint32_t PAST = BITS == 4 ? 0x600000u : 0x680000u;      // mantissas of 1.75 and 1.8125
+      constexpr int MOST = BITS == 4 ? 252 : 246;                       // (no code stands for more than fp32 holds: such rows saturate)
+      int e = (int)(top >> 23) - TOP_EXP + ((top & 0x7fffffu) > PAST ? 1 : 0);
+      e = e < 1 ? 1 : e > MOST ? MOST : e;                              // (top = 0 too)
+      const uint2 code = codes_of<BITS, F32>(x[s][n], (uint32_t)e);
+      if (row < 0 || row >= t.count || lane * 8 >= d) continue;
+      uint8_t* const to = p.side[s].codes + (head0 + r) * row_bytes + lane * BITS;
+      if constexpr (BITS == 4) *(uint32_t*)to = bad ? 0 : code.x;
+      else *(uint2*)to = bad ? uint2{0, 0} : code;
+      if (lane % 4 == 0) p.side[s].scales[(page_head * blocks + lane / 4) * page + slot0 + r] = (uint8_t)(bad ? 255 : e);
     }
-    if (!there) continue;
-    uint8_t* to = s.codes + (head0 + r) * row_bytes + lane * BITS;
-    if constexpr (BITS == 4) *(uint32_t*)to = code[0];
-    else *(uint2*)to = uint2{code[0], code[1]};
-    if (lane % 4 == 0) s.scales[(page_head * blocks + lane / 4) * page + slot0 + r] = (uint8_t)(bad ? 255 : e);
-  }
 }
 
 template <int BITS, bool F32, int LPR>
-__global__ __launch_bounds__(THREADS) void hstu_kv_read_kernel(const Params p) {
-  constexpr int ROWS = THREADS / LPR;
-  const int d = p.g.d, H = p.g.H, page = p.g.page_size;
-  const int h = blockIdx.x % H, tile = blockIdx.x / H % p.tiles, b = blockIdx.x / H / p.tiles;
-  const Side s = p.side[blockIdx.y];
-  int64_t first;
-  int count;
-  rows_of(p, b, &first, &count);
-  const int64_t start = p.starts[b];
-  const int64_t base = (start - (((start % TILE) + TILE) % TILE)) + (int64_t)tile * TILE;
-  if (base >= start + count) return;
-  const int64_t row0 = kv_row(p.g, b, base);
-  const int lane = threadIdx.x % LPR;
+__global__ __launch_bounds__(threads_of(LPR)) void hstu_kv_read_kernel(const Params p) {
+  constexpr int ROWS = threads_of(LPR) / LPR, PASSES = TILE / ROWS;
+  Tile t;
+  if (!tile_of(p, &t)) return;
+  const int d = p.g.d, page = p.g.page_size, lane = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
   if (lane * 8 >= d) return;
   const int blocks = (d + 31) / 32, row_bytes = d * BITS / 8;
-  const int64_t head0 = row0 + (int64_t)h * page, page_head = (row0 / page) + h, slot0 = row0 % page;
-  for (int r = threadIdx.x / LPR; r < TILE; r += ROWS) {
-    const int64_t t = base + r - start;
-    if (t < 0 || t >= count) continue;
-    float y[8] = {};
-    if (row0 >= 0) {
-      const uint8_t* from = s.codes + (head0 + r) * row_bytes + lane * BITS;
-      const uint32_t e = s.scales[(page_head * blocks + lane / 4) * page + slot0 + r];
-      const float power = e == 255u ? __builtin_nanf("") : power_of(e);
-      if constexpr (BITS == 4) {
-        const uint32_t w = *(const uint32_t*)from;
-        const floatx2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1),
-                      c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
-        y[0] = a[0]; y[1] = a[1]; y[2] = b2[0]; y[3] = b2[1]; y[4] = c[0]; y[5] = c[1]; y[6] = f[0]; y[7] = f[1];
-      } else {
-        const uint2 w = *(const uint2*)from;
-        const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), b2 = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true),
-                      c = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false), f = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true);
-        y[0] = a[0]; y[1] = a[1]; y[2] = b2[0]; y[3] = b2[1]; y[4] = c[0]; y[5] = c[1]; y[6] = f[0]; y[7] = f[1];
-      }
+  const int64_t head0 = t.row0 + (int64_t)t.h * page, page_head = t.row0 / page + t.h, slot0 = t.row0 % page;
+  uint2 code[2][PASSES];
+  uint32_t e[2][PASSES];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= power;
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n) {
+      const int r = r0 + n * ROWS;
+      const int64_t row = t.t0 + r;
+      code[s][n] = uint2{0, 0};
+      e[s][n] = 1;
+      if (t.row0 < 0 || row < 0 || row >= t.count) continue;
+      const uint8_t* const from = p.side[s].codes + (head0 + r) * row_bytes + lane * BITS;
+      if constexpr (BITS == 4) code[s][n].x = *(const uint32_t*)from;
+      else code[s][n] = *(const uint2*)from;
+      e[s][n] = p.side[s].scales[(page_head * blocks + lane / 4) * page + slot0 + r];
     }
-    const int64_t at = (p.offsets ? 0 : (int64_t)b * s.sb) + (first + t) * s.st + (int64_t)h * s.sh + lane * 8;
-    if constexpr (F32) {
-      floatx4* to = (floatx4*)((float*)s.rows + at);
-      to[0] = floatx4{y[0], y[1], y[2], y[3]};
-      to[1] = floatx4{y[4], y[5], y[6], y[7]};
-    } else {
-      *(uint4*)((bf16_t*)s.rows + at) = uint4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int n = 0; n < PASSES; ++n) {
+      const int64_t row = t.t0 + r0 + n * ROWS;
+      if (row < 0 || row >= t.count) continue;
+      const float power = e[s][n] == 255u ? __builtin_nanf("") : power_of(e[s][n]);
+      const uint2 w = code[s][n];
+      floatx2 y[4];
+      if constexpr (BITS == 4) {
+        y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w.x, 1.0f, 0); y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w.x, 1.0f, 1);
+        y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w.x, 1.0f, 2); y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w.x, 1.0f, 3);
+      } else {
+        y[0] = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false); y[1] = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true);
+        y[2] = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false); y[3] = __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true);
+      }
+      // (a product in fp32: exact, and a NaN for a row that is not finite, zeros included)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = floatx2{y[i][0] * power, y[i][1] * power};
+      const int64_t at = (p.offsets ? 0 : (int64_t)t.b * p.side[s].sb) + (t.first + row) * p.side[s].st + (int64_t)t.h * p.side[s].sh + lane * 8;
+      if constexpr (F32) {
+        floatx4* const to = (floatx4*)((float*)p.side[s].rows + at);
+        to[0] = floatx4{y[0][0], y[0][1], y[1][0], y[1][1]};
+        to[1] = floatx4{y[2][0], y[2][1], y[3][0], y[3][1]};
+      } else {
+        *(uint4*)((bf16_t*)p.side[s].rows + at) = uint4{pack2(y[0][0], y[0][1]), pack2(y[1][0], y[1][1]), pack2(y[2][0], y[2][1]), pack2(y[3][0], y[3][1])};
+      }
     }
-  }
 }
 
 bool head_dim_taken(int d) {
@@ -249,12 +321,12 @@ int kv_rows(const HstuKvRowsArgs* a, void* stream, bool write) {
   p.total = a->total_rows;
   p.per_seq = a->rows_per_seq;
   p.tiles = (int32_t)tiles;
-  const dim3 grid((uint32_t)(tiles * g.H * g.B), 2);
+  const uint32_t grid = (uint32_t)(tiles * g.H * g.B);
   hipStream_t st = (hipStream_t)stream;
 #define KV_LAUNCH(BITS, F32, LPR)                                                        \
   do {                                                                                   \
-    if (write) hstu_kv_write_kernel<BITS, F32, LPR><<<grid, THREADS, 0, st>>>(p);        \
-    else hstu_kv_read_kernel<BITS, F32, LPR><<<grid, THREADS, 0, st>>>(p);               \
+    if (write) hstu_kv_write_kernel<BITS, F32, LPR><<<grid, threads_of(LPR), 0, st>>>(p);        \
+    else hstu_kv_read_kernel<BITS, F32, LPR><<<grid, threads_of(LPR), 0, st>>>(p);               \
   } while (0)
 #define KV_WIDTH(BITS, F32)                              \
   do {                                                   \
