@@ -20,6 +20,7 @@ from recml_amd.hstu_cache_ops import KVPages, cached_attention, kv_read, kv_writ
 from recml_amd.hstu_scores import TokenLogProbs, token_log_probs  # noqa: F401
 from recml_amd.masks import make_attention_mask, make_causal_mask  # noqa: F401
 from recml_amd.hstu_layer import HSTU, HSTUBlock  # noqa: F401
+from recml_amd.hstu_serving import HSTUCache  # noqa: F401
 from recml_amd.hstu_bias import (  # noqa: F401
     RelativeBucketedTimeAndPositionBasedBias,
     RelativePositionalBias,

@@ -34,7 +34,10 @@ import torch.nn.functional as F
 
 from recml_amd import _native
 from recml_amd import hstu_block_ops
+from recml_amd import hstu_cache_ops
 from recml_amd import hstu_ops
+from recml_amd import hstu_scores
+from recml_amd import hstu_serving
 from recml_amd import masks
 
 
@@ -361,6 +364,33 @@ class HSTUBlock(torch.nn.Module):
                       pos_bias=pos_bias, timestamps=timestamps, ts_bias=ts_bias, batch=batch, **drop)
     return self._gate_and_output(attn.reshape(T, H * hd), u.reshape(T, H * hd), tokens, fused)
 
+  def forward_cached(self, tokens, pages, page_table, lengths, starts, max_len, *, offsets=None, max_new=None, pos_bias=None, timestamps=None,
+                     ts_bias=None, whole=False):
+    """The block on new events of kept histories, in inference: their keys and values go into `pages` (a hstu_cache_ops.KVPages) from
+    place starts[b] on, and they attend to what the cache then holds of their user.
+
+    tokens: [B, n, D], or packed [T, D] with `offsets` [B + 1] and `max_new`; lengths [B]: events of every user, the new ones included;
+    max_len: the length of the full call (the normaliser, the tables' extent); timestamps: the users' [B, max_len] kept times.
+    whole=True (packed rows): the new events are the whole histories and attend to their own keys and values as they are, through
+    hstu_attention, with `timestamps` [T] the rows' own."""
+    if self.training and self.dropout > 0.0:
+      raise ValueError("serving is inference: call eval() on the model first")
+    H, hd, D = self.num_heads, self.head_dim, self.hidden_dim
+    lead = tokens.shape[:-1]
+    with torch.no_grad():
+      rows = tokens.reshape(-1, D)
+      fused = self._fused_inference(rows)
+      u, q, k, v = self._project(self._input_norm(rows, fused), lead, fused).unbind(dim=-3)
+      hstu_cache_ops.kv_write(pages, k, v, page_table, starts, offsets=offsets, max_new=max_new)
+      alpha, n = self._alpha_n(max_len)
+      if whole:
+        attn = hstu_ops.hstu_attention(q, k, v, seq_offsets=offsets, max_len=max_len, n=n, alpha=alpha, pos_bias=pos_bias,
+                                       timestamps=timestamps, ts_bias=ts_bias)
+      else:
+        attn = hstu_cache_ops.cached_attention(q, pages, page_table, lengths, max_len=max_len, offsets=offsets, max_new=max_new, n=n, alpha=alpha,
+                                               pos_bias=pos_bias, timestamps=timestamps, ts_bias=ts_bias)
+      return self._gate_and_output(attn.reshape(-1, H * hd), u.reshape(-1, H * hd), rows, fused).reshape(*lead, D)
+
 
 _OWN_BLOCK_FORWARDS = HSTUBlock.forward, HSTUBlock.forward_jagged
 
@@ -580,3 +610,93 @@ class HSTU(torch.nn.Module):
     self._check_indices(outside)
     out = torch.zeros((B * L, x.shape[-1]), dtype=x.dtype, device=x.device)
     return out.index_copy(0, rows[:tokens].to(torch.int64), x).reshape(B, L, x.shape[-1])
+
+  def log_probs(self, inputs, tokens, *, top: int = 0, entropy: bool = False, **kw):
+    """Log probabilities of items under the model's head: token_log_probs on the logits of `forward(inputs, **kw)`.  tokens: one item a
+    position [B, L] (a training loss: the next items, -1 where there is none) or several [B, L, C]."""
+    if self.reverse_embedding is None:
+      raise ValueError("the model has no output head")
+    return hstu_scores.token_log_probs(self(inputs, **kw), tokens, top=top, entropy=entropy)
+
+  def new_cache(self, batch: int, max_len: int, *, bits: int = 4, page_size: int = 64, pages: int | None = None, page_table=None,
+                timestamps: bool = False):
+    """Room for `batch` users' histories of up to `max_len` events: an hstu_serving.HSTUCache."""
+    return hstu_serving.HSTUCache(self.decoder_blocks, batch, max_len, bits=bits, page_size=page_size, pages=pages, page_table=page_table,
+                                  timestamps=timestamps, device=self.item_embedding.device)
+
+  def prefill(self, inputs, cache, *, seq_lens, timestamps=None, pos_bias=None, ts_bias=None):
+    """Takes whole histories into an empty cache, in inference: item ids [B, L], `seq_lens` [B] of them valid, `timestamps` [B, L].
+    Returns what forward(inputs, seq_lens=seq_lens, jagged=True) does for a call of cache.max_len positions, but for the last bits:
+    [B, L, D or vocabulary], zeros past a history's end."""
+    B, L = inputs.shape
+    if L > cache.max_len or B != cache.batch:
+      raise ValueError(f"the cache holds {cache.batch} histories of up to {cache.max_len} events, got {tuple(inputs.shape)}")
+    if tuple(seq_lens.shape) != (B,):
+      raise ValueError(f"seq_lens must be [{B}], got {tuple(seq_lens.shape)}")
+    lens = seq_lens.to(torch.int64).clamp(0, L)
+    rows = (torch.arange(L, device=inputs.device)[None, :] < lens[:, None]).reshape(-1).nonzero().squeeze(1)
+    offsets = torch.zeros(B + 1, dtype=torch.int32, device=inputs.device)
+    offsets[1:] = torch.cumsum(lens, 0)
+    out = None
+    with torch.no_grad():
+      if rows.numel():
+        ts = None if timestamps is None else timestamps.reshape(-1)[rows]
+        x = self._extend(inputs.reshape(-1)[rows], cache, offsets, L, rows // L, rows % L, torch.zeros_like(cache.lengths), lens.to(torch.int32), ts,
+                         pos_bias, ts_bias, True)
+        out = torch.zeros((B * L, x.shape[-1]), dtype=x.dtype, device=x.device).index_copy_(0, rows, x).reshape(B, L, -1)
+      cache.lengths.copy_(lens)
+    return out if out is not None else torch.zeros((B, L, (self.item_embedding if self.reverse_embedding is None else self.reverse_embedding).shape[1]),
+                                                   dtype=self.item_embedding.dtype, device=inputs.device)
+
+  def extend(self, ids, cache, *, offsets=None, max_new=None, timestamps=None, pos_bias=None, ts_bias=None):
+    """New events of kept histories, in inference: item ids [B, n] (every user has n), or packed [T] with `offsets` [B + 1] and `max_new` (the
+    most events of one user); `timestamps` shaped like them.  Their keys and values join the cache, and every event attends to its
+    user's history up to itself.  Returns the model's outputs for the new events, [B, n, ...] or [T, ...]; token_log_probs makes log
+    probabilities and the items to recommend of logits.  Nothing in here waits for the GPU: a step can be captured into a graph
+    and replayed.  Events past cache.max_len are lost: they join nothing and attend to nothing."""
+    B, dev = cache.batch, ids.device
+    if offsets is None:
+      if ids.dim() != 2 or ids.shape[0] != B:
+        raise ValueError(f"ids must be [{B}, n], got {tuple(ids.shape)}; packed ids need `offsets` and `max_new`")
+      count = ids.shape[1]
+      steps = torch.arange(count, device=dev).expand(B, count)
+      users = torch.arange(B, device=dev)[:, None].expand(B, count)
+    else:
+      if ids.dim() != 1 or max_new is None or tuple(offsets.shape) != (B + 1,):
+        raise ValueError(f"packed ids are [T] with `offsets` [{B + 1}] and `max_new`, got {tuple(ids.shape)} and {tuple(offsets.shape)}")
+      offsets = offsets.to(torch.int32)
+      count = offsets[1:] - offsets[:-1]
+      at = torch.arange(ids.shape[0], device=dev)
+      users = (torch.searchsorted(offsets[1:].to(torch.int64), at, right=True)).clamp(max=B - 1)
+      steps = at - offsets[users]
+    with torch.no_grad():
+      starts = cache.lengths.clone()
+      lengths = starts + count
+      x = self._extend(ids, cache, offsets, max_new, users, starts[users] + steps, starts, lengths, timestamps, pos_bias, ts_bias, False)
+      cache.lengths.copy_(lengths)
+    return x
+
+  def _extend(self, ids, cache, offsets, max_new, users, places, starts, lengths, timestamps, pos_bias, ts_bias, whole):
+    """The model on new events at their places."""
+    if self.training and self.dropout > 0.0:
+      raise ValueError("serving is inference: call eval() on the model first")
+    if len(cache.layers) != len(self.decoder_blocks):
+      raise ValueError(f"the cache has {len(cache.layers)} layers, the model {len(self.decoder_blocks)}")
+    if (ts_bias is None) != (timestamps is None):
+      raise ValueError("Both or neither of `timestamps` and `ts_bias` must be provided.")
+    cache._note_times(timestamps, users, places)
+    table, positions, D = self.item_embedding, self.position_embedding, self.model_dim
+    scale = D ** 0.5 if self.scale_by_sqrt_dim else 1.0
+    at = None if positions is None else places.clamp(0, positions.shape[0] - 1).to(torch.int64)
+    if table.is_cuda and table.dtype == torch.bfloat16 and D % 8 == 0 and D <= 8192:
+      x = hstu_block_ops.embed_norm(ids.to(torch.int64), table, self.final_norm_gamma, self.final_norm_beta, self.eps, scale=scale, positions=at,
+                                    pos_table=positions)
+    else:
+      x = table[ids.clamp(0, table.shape[0] - 1)]
+      x = x * scale if self.scale_by_sqrt_dim else x
+      x = self._final_norm(x if positions is None else x + positions[at])
+    for block, pages in zip(self.decoder_blocks, cache.layers):
+      x = block.forward_cached(x, pages, cache.page_table, lengths, starts, cache.max_len, offsets=offsets, max_new=max_new, pos_bias=pos_bias,
+                               timestamps=timestamps if whole else cache.timestamps, ts_bias=ts_bias, whole=whole)
+    x = self._final_norm(x)
+    return x if self.reverse_embedding is None else self._head(x)
