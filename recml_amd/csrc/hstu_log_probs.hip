@@ -24,7 +24,6 @@
 namespace {
 
 constexpr int VECS = 8;              // vectors of 16 bytes that a thread holds
-constexpr int CAP = 1024;            // entries that reach the bound at most, on the short way
 constexpr int MAX_TOP = 256;
 
 struct Params {
@@ -133,10 +132,13 @@ __device__ __forceinline__ float block_reduce(float x, float* lds, F op) {
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 
+// What select_top shares; CAP: entries that reach the bound at most, on the short way.
+template <int CAP_>
 struct Chosen {
+  static constexpr int CAP = CAP_;
+  uint64_t place[CAP];
   float value[CAP];
-  int32_t index[CAP];
-  float bound[4][2];
+  uint32_t bound[4];
   uint64_t best[4];
   int n;
 };
@@ -155,43 +157,40 @@ __device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
 // The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  `most`: the ordered bits of a
 // thread's largest entry (0: it has none; the least of an entry is that of -inf); collect(bound, push) calls push(x, index) for
 // its entries that reach the bound, each(f) f(x, index) for all of them; there are at least k.
-template <int NT, typename Collect, typename Each, typename Out>
-__device__ __forceinline__ void select_top(int k, Chosen& c, uint32_t most, Collect collect, Each each, Out out) {
+template <int NT, typename C, typename Collect, typename Each, typename Out>
+__device__ __forceinline__ void select_top(int k, C& c, uint32_t most, Collect collect, Each each, Out out) {
   constexpr int W = NT / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  // every wave has its share of the k, or one wave has all of them: either way k entries reach the bound
-  const uint32_t share = kth_of_wave(most, (k + W - 1) / W), all = W > 1 && k <= 64 ? kth_of_wave(most, k) : 0;
-  __syncthreads();
-  if (threadIdx.x == 0) c.n = 0;
-  if (lane == 0) {
-    c.bound[wave][0] = __builtin_bit_cast(float, share);
-    c.bound[wave][1] = __builtin_bit_cast(float, all);
-  }
-  __syncthreads();
-  uint32_t least = 0xffffffffu, best = 0;
+  // what every wave has its share of the k of; where a wave has too few entries for that, what one wave has all k of
+  auto over_waves = [&](uint32_t mine, auto pick) {
+    if constexpr (W > 1) {
+      __syncthreads();
+      if (lane == 0) c.bound[wave] = mine;
+      __syncthreads();
+      mine = c.bound[0];
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, c.bound[w][0]), b = __builtin_bit_cast(uint32_t, c.bound[w][1]);
-    least = a < least ? a : least;
-    best = b > best ? b : best;
-  }
-  const uint32_t bound = least > best ? least : best;
+      for (int w = 1; w < W; ++w) mine = pick(mine, c.bound[w]);
+    }
+    return mine;
+  };
+  if (threadIdx.x == 0) c.n = 0;
+  uint32_t bound = over_waves(kth_of_wave(most, (k + W - 1) / W), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+  if (W > 1 && bound == 0 && k <= 64) bound = over_waves(kth_of_wave(most, k), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+  __syncthreads();
   if (most != 0 && most >= bound)
     collect(bound, [&](float x, int index) {
       const int at = atomicAdd(&c.n, 1);
-      if (at < CAP) { c.value[at] = x; c.index[at] = index; }
+      if (at < C::CAP) { c.place[at] = place_of(x, index); c.value[at] = x; }
     });
   __syncthreads();
   const int n = c.n;
-  if (n <= CAP) {
+  if (n <= C::CAP) {
     for (int i = threadIdx.x; i < n; i += NT) {
-      const float x = c.value[i];
-      const int index = c.index[i];
-      const uint64_t mine = place_of(x, index);
+      const uint64_t mine = c.place[i];
       int rank = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += place_of(c.value[j], c.index[j]) > mine;
-      if (rank < k) out(rank, x, index);
+      for (int j = 0; j < n; ++j) rank += c.place[j] > mine;
+      if (rank < k) out(rank, c.value[i], 0x7fffffff - (int)(uint32_t)mine);
     }
     __syncthreads();
     return;
@@ -305,7 +304,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
     to[0] = m; to[1] = s; to[2] = t;
   }
   if constexpr (!TOP) return;
-  __shared__ Chosen chosen;
+  __shared__ Chosen<NT == 64 ? 256 : 1024> chosen;
   // a part shorter than `top` gives what it has
   const int64_t e0 = (int64_t)part * p.vecs * NT * N - r.shift, e1 = e0 + (int64_t)p.vecs * NT * N;
   const int64_t here = (e1 < p.vocab ? e1 : p.vocab) - (e0 > 0 ? e0 : 0);
@@ -359,11 +358,11 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
 // One row's parts: their sums in order, and the largest of their largest.
 template <bool F32, int NT>
 __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
-  constexpr int E = 4;
-  __shared__ Chosen chosen;
+  constexpr int E = NT == 64 ? 4 : 8, TOP = NT == 64 ? 64 : MAX_TOP;
+  __shared__ Chosen<NT * E> chosen;
   __shared__ float sums[4];
-  __shared__ float best_value[MAX_TOP];
-  __shared__ int32_t best_index[MAX_TOP];
+  __shared__ float best_value[TOP];
+  __shared__ int32_t best_index[TOP];
   const int64_t row = blockIdx.x;
   const float* from = p.part_stats + row * p.parts * 3;
   float m = -__builtin_inff();
@@ -523,9 +522,10 @@ Split split_of(const HstuLogProbsArgs& a) {
   const int64_t n = a.dtype == HSTU_SERVE_FP32 ? 4 : 8, vectors = ((int64_t)a.vocab + n - 1 + n - 1) / n;   // (a row may start anywhere)
   Split s;
   s.nt = vectors <= 64 * VECS && a.top <= 64 ? 64 : 256;
-  s.vecs = (int)std::min<int64_t>(VECS, (vectors + s.nt - 1) / s.nt);
-  // few rows: shorter parts, so that they fill the chip
-  while (s.vecs > 1 && a.rows * ((vectors + (int64_t)s.nt * s.vecs - 1) / ((int64_t)s.nt * s.vecs)) < 256 && vectors > s.nt) s.vecs = (s.vecs + 1) / 2;
+  int64_t parts = (vectors + (int64_t)s.nt * VECS - 1) / ((int64_t)s.nt * VECS);
+  // few rows: more parts, so that they fill the chip, while the join holds all of a row's largest entries at once
+  while (a.rows * parts < 256 && parts * s.nt * 2 <= vectors && 2 * parts * a.top <= 2048) parts *= 2;
+  s.vecs = (int)((vectors + parts * s.nt - 1) / (parts * s.nt));
   s.parts = (int)((vectors + (int64_t)s.nt * s.vecs - 1) / ((int64_t)s.nt * s.vecs));
   return s;
 }
