@@ -18,8 +18,9 @@
 // dims (one block of exponents at d = 128), and Q is read the same way.
 // Queries in fp32 run as three bf16 parts (24 bits: all of them); activated weights as two for bf16 results (2^-17 of a weight is
 // lost, where one part would lose 2^-9 and make half of the result's error), as three for fp32 ones.
-// Biases are worked out by the whole workgroup, a pair a thread, for up to 8192 pairs ahead: done where the logits lie, a single
-// query's would cost each wave 16 times the work, since its 16 columns hold one row.
+// Biases with timestamps are worked out by the whole workgroup, a pair a thread, for up to 8192 pairs ahead: done where the logits
+// lie, a single query's would cost each wave 16 times the work, since its 16 columns hold one row.  Positions alone are the entries
+// of the table that the block's places span, once.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -337,35 +338,36 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
     for (int j = 0; j < VN; ++j) acc[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int sub = 1 << p.sub_log2, pitch = sub + 4;
+  const int place0 = (int)s.place0 + t0;              // (places of rows: lengths of at most 2^31)
   // (vmcnt(0), here and behind the biases: what the compiler does not know to have arrived when the loop begins it waits for in every
   // round of it, and with it for the loads ahead)
   __builtin_amdgcn_s_waitcnt(0x0f70);
   __syncthreads();
   for (int c0 = k0; c0 < k1; c0 += sub) {
     const int c1 = k1 - c0 < sub ? k1 : c0 + sub;
-    if (pos || ts) {
-      // a thread has one key at a time and runs over the rows, or over every 2nd, 4th, ... of them
+    if (ts) {
+      // a pair's bias each: a thread has one key at a time and runs over the rows, or over every 2nd, 4th, ... of them
       __syncthreads();
       const int wide = p.sub_log2 < 8 ? p.sub_log2 : 8, every = THREADS >> wide;
       for (int jj = threadIdx.x & ((1 << wide) - 1); jj < c1 - c0; jj += THREADS) {
         const int j = c0 + jj;
-        const int place0 = (int)s.place0 + t0, first = threadIdx.x >> wide;      // (places of rows: lengths of at most 2^31)
-        if (ts) {
-          const int64_t tk = ts[j];
+        const int64_t tk = ts[j];
 #pragma unroll 1
-          for (int t = first; t < rows; t += every) {
-            const int i = place0 + t;
-            float x = 0.f;
-            if (i >= j && i < s.limit) x = (pos ? pos[j - i] : 0.f) + bucket_value(buckets, ts[i < s.last_ts ? i + 1 : s.last_ts] - tk);
-            table[t * pitch + jj] = x;
-          }
-        } else {
-#pragma unroll 4
-          for (int t = first; t < rows; t += every) {
-            const int i = place0 + t;
-            table[t * pitch + jj] = i >= j && i < s.limit ? pos[j - i] : 0.f;
-          }
+        for (int t = threadIdx.x >> wide; t < rows; t += every) {
+          const int i = place0 + t;
+          float x = 0.f;
+          if (i >= j && i < s.limit) x = (pos ? pos[j - i] : 0.f) + bucket_value(buckets, ts[i < s.last_ts ? i + 1 : s.last_ts] - tk);
+          table[t * pitch + jj] = x;
         }
+      }
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      __syncthreads();
+    } else if (pos) {
+      // the position's alone depends on j - i: the table's entries from the last row's first key on
+      __syncthreads();
+      for (int e = threadIdx.x; e < c1 - c0 + rows; e += THREADS) {
+        const int diff = c0 - (place0 + rows - 1) + e;
+        table[e] = diff <= 0 && diff > -p.max_len ? pos[diff] : 0.f;
       }
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
@@ -440,14 +442,11 @@ __global__ __launch_bounds__(THREADS, waves_of(DP, F32, NQ)) void hstu_cached_at
       for (int n = 0; n < NQ; ++n) {
         if (n > 0 && 16 * n >= rows) continue;
         float y[8];
-        if (pos || ts) {
-          const floatx4* const at = (const floatx4*)(table + (16 * n + r < rows ? 16 * n + r : rows - 1) * pitch + (key0 - c0) + 8 * g);
-          const floatx4 lo = at[0], hi = at[1];
+        if (ts || pos) {
+          const int t = 16 * n + r < rows ? 16 * n + r : rows - 1, jj = key0 - c0 + 8 * g;
+          const float* const at = table + (ts ? t * pitch + jj : rows - 1 - t + jj);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            y[i] = __builtin_fmaf(p.alpha, st[0][n][i], lo[i]);
-            y[4 + i] = __builtin_fmaf(p.alpha, st[1][n][i], hi[i]);
-          }
+          for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(p.alpha, st[i / 4][n][i % 4], at[i]);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) y[i] = p.alpha * st[i / 4][n][i % 4];
@@ -649,7 +648,7 @@ template <int DP, bool EXACT, int BITS, bool F32, int NQ>
 void launch(const Params& p, uint32_t grid, hipStream_t st) {
   constexpr int ACC = DP / 16 * 4 * NQ;
   const int rows = std::min(p.per_seq, 16 * NQ);
-  const size_t biases = p.pos || p.ts ? (size_t)rows * ((1 << p.sub_log2) + 4) : 0;
+  const size_t biases = p.ts ? (size_t)rows * ((1 << p.sub_log2) + 4) : p.pos ? (size_t)std::min(1 << p.sub_log2, p.chunk) + rows + 8 : 0;
   const size_t lds = std::max<size_t>((size_t)2 * ACC * 64, BUCKET_FLOATS + NQ * (DP / 32) * (F32 ? 3 : 1) * 256 + biases) * sizeof(float);
   hstu_cached_attn_kernel<DP, EXACT, BITS, F32, NQ><<<grid, THREADS, lds, st>>>(p);
 }
@@ -718,9 +717,9 @@ int hstu_cached_attn(const HstuCachedAttnArgs* a, void* stream) {
   p.partial = s.parts > 1 ? (float*)a->workspace : nullptr;
   p.per_seq = a->rows_per_seq; p.max_len = a->max_len; p.pos_heads = a->pos_heads; p.ts_heads = a->ts_heads; p.ts_buckets = a->ts_buckets;
   p.chunk = s.chunk; p.parts = s.parts; p.qblocks = s.qblocks;
-  // biases of 8192 pairs at a time, and of 2048 keys at most
-  p.sub_log2 = 11;
-  while (p.sub_log2 > 7 && ((int64_t)std::min(a->rows_per_seq, 16 * s.nq) << p.sub_log2) > 8192) --p.sub_log2;
+  // biases of 8192 pairs at a time, and of 2048 keys at most; of positions alone, of 8192 keys
+  p.sub_log2 = a->timestamps ? 11 : 13;
+  while (a->timestamps && p.sub_log2 > 7 && ((int64_t)std::min(a->rows_per_seq, 16 * s.nq) << p.sub_log2) > 8192) --p.sub_log2;
   p.alpha = a->alpha; p.inv_n = a->inv_n; p.buckets_per_log2 = 0.f;
   if (a->timestamps) {
     thresholds(a->ts_bucket_size, a->ts_buckets, p.thr);

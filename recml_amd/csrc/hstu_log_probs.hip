@@ -11,7 +11,8 @@
 //
 // The largest entries of a part: the k-th largest of the threads' maxima bounds the k-th largest entry from below, few entries
 // reach it, and each of those finds its rank by counting who comes before it (by value, then by index).  The bound comes from
-// ballots on 16 bits of the ordered value.  Rows with more ties than the list holds take one entry after the other instead.
+// ballots on 16 bits of the ordered value.  Where more reach it than the lists hold (ties, mostly), the k-th entry is found exactly,
+// bit by bit.
 
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -138,86 +139,113 @@ struct Chosen {
   static constexpr int CAP = CAP_;
   uint64_t place[CAP];
   float value[CAP];
-  uint32_t bound[4];
-  uint64_t best[4];
-  int n;
+  uint32_t bound[4][2];
+  int n, vectors;
 };
 
-// The k-th largest of a wave's values by the upper 16 of their ordered bits, lower bits zero (0: there are fewer).
-__device__ __forceinline__ uint32_t kth_of_wave(uint32_t key, int k) {
-  uint32_t found = 0;
+// The j-th and the k-th largest of a wave's values by the upper 16 of their ordered bits, lower bits zero (0: there are fewer).
+__device__ __forceinline__ void kth_of_wave(uint32_t key, int j, int k, uint32_t* jth, uint32_t* kth) {
+  uint32_t a = 0, b = 0;
 #pragma unroll
   for (int bit = 31; bit >= 16; --bit) {
-    const uint32_t next = found | 1u << bit;
-    if (__popcll(__ballot(key >= next)) >= k) found = next;
+    const uint32_t na = a | 1u << bit, nb = b | 1u << bit;
+    a = __popcll(__ballot(key >= na)) >= j ? na : a;
+    b = __popcll(__ballot(key >= nb)) >= k ? nb : b;
   }
-  return found;
+  *jth = a;
+  *kth = b;
+}
+
+// The k entries themselves, where too many reach the bound: the k-th largest value bit by bit, then, among its equals, the index up
+// to which they belong to the k.
+template <int NT, typename C, typename Each>
+__device__ __forceinline__ void exactly(int k, C& c, Each each) {
+  constexpr int W = NT / 64;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  auto count = [&](auto counts) {
+    int mine = 0;
+    each([&](float x, int index) { mine += counts(ordered(x), index) ? 1 : 0; });
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) mine += __shfl_xor(mine, m, 64);
+    if constexpr (W > 1) {
+      __syncthreads();
+      if (lane == 0) c.bound[wave][0] = (uint32_t)mine;
+      __syncthreads();
+      mine = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mine += (int)c.bound[w][0];
+    }
+    return mine;
+  };
+  uint32_t value = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = value | 1u << bit;
+    if (count([&](uint32_t o, int) { return o >= next; }) >= k) value = next;
+  }
+  const int ties = k - count([&](uint32_t o, int) { return o > value; });
+  int below = 0;                           // the largest index with fewer than `ties` equals below it
+#pragma unroll 1
+  for (int bit = 30; bit >= 0; --bit) {
+    const int next = below | 1 << bit;
+    if (count([&](uint32_t o, int index) { return o == value && index < next; }) < ties) below = next;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) c.n = 0;
+  __syncthreads();
+  each([&](float x, int index) {
+    const uint32_t o = ordered(x);
+    if (o > value || (o == value && index <= below)) {
+      const int at = atomicAdd(&c.n, 1);
+      c.place[at] = place_of(x, index);    // (k of them)
+      c.value[at] = x;
+    }
+  });
+  __syncthreads();
 }
 
 // The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  `most`: the ordered bits of a
-// thread's largest entry (0: it has none; the least of an entry is that of -inf); collect(bound, push) calls push(x, index) for
-// its entries that reach the bound, each(f) f(x, index) for all of them; there are at least k.
+// thread's largest entry (0: it has none; the least of an entry is that of -inf); collect(bound, reaches, push), called by all threads,
+// calls push(x, index) for the entries that reach the bound, each(f) f(x, index) for all of a thread's; there are at least k.
 template <int NT, typename C, typename Collect, typename Each, typename Out>
 __device__ __forceinline__ void select_top(int k, C& c, uint32_t most, Collect collect, Each each, Out out) {
   constexpr int W = NT / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  // what every wave has its share of the k of; where a wave has too few entries for that, what one wave has all k of
-  auto over_waves = [&](uint32_t mine, auto pick) {
-    if constexpr (W > 1) {
-      __syncthreads();
-      if (lane == 0) c.bound[wave] = mine;
-      __syncthreads();
-      mine = c.bound[0];
-#pragma unroll
-      for (int w = 1; w < W; ++w) mine = pick(mine, c.bound[w]);
-    }
-    return mine;
-  };
-  if (threadIdx.x == 0) c.n = 0;
-  uint32_t bound = over_waves(kth_of_wave(most, (k + W - 1) / W), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-  if (W > 1 && bound == 0 && k <= 64) bound = over_waves(kth_of_wave(most, k), [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-  __syncthreads();
-  if (most != 0 && most >= bound)
-    collect(bound, [&](float x, int index) {
-      const int at = atomicAdd(&c.n, 1);
-      if (at < C::CAP) { c.place[at] = place_of(x, index); c.value[at] = x; }
-    });
-  __syncthreads();
-  const int n = c.n;
-  if (n <= C::CAP) {
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const uint64_t mine = c.place[i];
-      int rank = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += c.place[j] > mine;
-      if (rank < k) out(rank, c.value[i], 0x7fffffff - (int)(uint32_t)mine);
-    }
+  // every wave has its share of the k, or one wave has all of them: either way k entries reach the bound.  (The shares bound well
+  // where all waves are full, the wave's k where one of them holds little.)
+  uint32_t share, all;
+  kth_of_wave(most, (k + W - 1) / W, k, &share, &all);
+  uint32_t bound = share;
+  if constexpr (W > 1) {
+    if (lane == 0) { c.bound[wave][0] = share; c.bound[wave][1] = all; }
     __syncthreads();
-    return;
+    uint32_t best = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      bound = c.bound[w][0] < bound ? c.bound[w][0] : bound;
+      best = c.bound[w][1] > best ? c.bound[w][1] : best;
+    }
+    bound = best > bound ? best : bound;
   }
-  // one after the other: the largest that comes behind the last one
-  uint64_t last = ~0ull;
-  for (int r = 0; r < k; ++r) {
-    uint64_t mine = 0;
-    float value = 0.f;
-    int at = 0;
-    each([&](float x, int index) {
-      const uint64_t p = place_of(x, index);
-      if (p < last && p > mine) { mine = p; value = x; at = index; }
-    });
-    uint64_t all_best = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint64_t o = __shfl_xor(all_best, m, 64);
-      all_best = o > all_best ? o : all_best;
-    }
-    __syncthreads();
-    if (lane == 0) c.best[wave] = all_best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) all_best = c.best[w] > all_best ? c.best[w] : all_best;
-    if (mine == all_best && mine != 0) out(r, value, at);
-    last = all_best;
+  if (threadIdx.x == 0) c.n = c.vectors = 0;
+  __syncthreads();
+  collect(bound, most != 0 && most >= bound, [&](float x, int index) {
+    const int at = atomicAdd(&c.n, 1);
+    if (at < C::CAP) { c.place[at] = place_of(x, index); c.value[at] = x; }
+  });
+  __syncthreads();
+  int n = c.n;
+  if (n > C::CAP) {
+    exactly<NT>(k, c, each);
+    n = k;
+  }
+  // who comes before an entry is its rank
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t mine = c.place[i];
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) before += c.place[j] > mine;
+    if (before < k) out(before, c.value[i], 0x7fffffff - (int)(uint32_t)mine);
   }
   __syncthreads();
 }
@@ -305,54 +333,71 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
   }
   if constexpr (!TOP) return;
   __shared__ Chosen<NT == 64 ? 256 : 1024> chosen;
+  constexpr int HELD = NT == 64 ? 64 : 512;                    // vectors with entries that reach the bound
+  __shared__ uint4 held[HELD];
+  __shared__ int32_t held_at[HELD];
   // a part shorter than `top` gives what it has
   const int64_t e0 = (int64_t)part * p.vecs * NT * N - r.shift, e1 = e0 + (int64_t)p.vecs * NT * N;
   const int64_t here = (e1 < p.vocab ? e1 : p.vocab) - (e0 > 0 ? e0 : 0);
   const int k = here < p.top ? (here > 0 ? (int)here : 0) : p.top;
   const float log_s = __logf(s);
-  // (read again: only rows with more ties than the list holds, or with NaNs, need all entries once more)
+  // (read again: from the registers the long way would hold their ordered bits too, and cost the short one a third of its waves)
   auto each = [&](auto f) {
+#pragma unroll 1
     for (int c = 0; c < p.vecs; ++c) {
       const int v = v0 + c * NT, e = r.first(v);
-      if (v >= r.vectors) break;
       const Vec<F32> y = r.load(v);
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (e + i >= 0 && e + i < p.vocab) f(y.at(i), e + i);
+        if (v < r.vectors && e + i >= 0 && e + i < p.vocab) f(y.at(i), e + i);
     }
   };
   uint32_t most = v0 < r.vectors ? ordered(mine) : 0;
   if (odd) each([&](float y, int) { const uint32_t o = ordered(y); most = o > most ? o : most; });
-  auto collect = [&](uint32_t bound, auto push) {
-    // not below the bound's float: where that is a NaN (no bound, or one among the NaNs) everything is looked at
+  auto collect = [&](uint32_t bound, bool reaches, auto push) {
+    // vectors with an entry that is not below the bound's float (where that is a NaN, all of them), then their entries: the code that
+    // an entry takes is there once, not 64 times (which is fetched on every launch, a third of a small call's time)
     const float least = __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
+    if (reaches) {
 #pragma unroll
-    for (int c = 0; c < VECS; ++c)
-      if (c < p.vecs) {
-        bool any = false;
+      for (int c = 0; c < VECS; ++c)
+        if (c < p.vecs) {
+          bool any = false;
+          x[c].hold();
 #pragma unroll
-        for (int i = 0; i < N; ++i) any |= !(x[c].at(i) < least);
-        if (!any) continue;
-        const int e = r.first(v0 + c * NT);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (e + i >= 0 && e + i < p.vocab && ordered(x[c].at(i)) >= bound) push(x[c].at(i), e + i);
-      }
+          for (int i = 0; i < N; ++i) any |= !(x[c].at(i) < least);
+          if (any) {
+            const int at = atomicAdd(&chosen.vectors, 1);
+            if (at < HELD) { held[at] = x[c].raw; held_at[at] = r.first(v0 + c * NT); }
+          }
+        }
+    }
+    __syncthreads();
+    const int n = chosen.vectors;
+    if (n > HELD) {                                            // (all the same to the bound: the long way)
+      if (threadIdx.x == 0) chosen.n = 1 << 30;
+      return;
+    }
+    for (int i = threadIdx.x; i < n * N; i += NT) {
+      const int e = held_at[i / N] + i % N;
+      const uint32_t w = ((const uint32_t*)held)[F32 ? i : i / 2];
+      const float y = __builtin_bit_cast(float, F32 ? w : i % 2 ? w & 0xffff0000u : w << 16);
+      if (e >= 0 && e < p.vocab && ordered(y) >= bound) push(y, e);
+    }
   };
-  if (p.parts == 1) {
-    select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
-      p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
-      p.top_tokens[row * p.top + rank] = index;
-    });
-  } else {
-    const int64_t to = (row * p.parts + part) * p.top;
+  const int64_t to = (row * p.parts + part) * p.top;
+  if (p.parts > 1)
     for (int i = k + threadIdx.x; i < p.top; i += NT) p.part_index[to + i] = -1;
-    if (k > 0)
-      select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
+  if (k > 0)
+    select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
+      if (p.parts == 1) {
+        p.top_log_probs[to + rank] = (value - m) - log_s;
+        p.top_tokens[to + rank] = index;
+      } else {
         p.part_value[to + rank] = value;
         p.part_index[to + rank] = index;
-      });
-  }
+      }
+    });
 }
 
 // One row's parts: their sums in order, and the largest of their largest.
@@ -411,8 +456,8 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
     };
     uint32_t most = 0;
     each([&](float y, int) { const uint32_t o = ordered(y); most = o > most ? o : most; });
-    auto collect = [&](uint32_t bound, auto push) {
-      each([&](float y, int i) { if (ordered(y) >= bound) push(y, i); });
+    auto collect = [&](uint32_t bound, bool reaches, auto push) {
+      if (reaches) each([&](float y, int i) { if (ordered(y) >= bound) push(y, i); });
     };
     if (k > 0)
       select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int at) {
@@ -521,7 +566,8 @@ struct Split { int nt, vecs, parts; };
 Split split_of(const HstuLogProbsArgs& a) {
   const int64_t n = a.dtype == HSTU_SERVE_FP32 ? 4 : 8, vectors = ((int64_t)a.vocab + n - 1 + n - 1) / n;   // (a row may start anywhere)
   Split s;
-  s.nt = vectors <= 64 * VECS && a.top <= 64 ? 64 : 256;
+  // (a wave for short rows: its 64 maxima bound a few of their largest entries well)
+  s.nt = vectors <= 64 * VECS && a.top <= 16 ? 64 : 256;
   int64_t parts = (vectors + (int64_t)s.nt * VECS - 1) / ((int64_t)s.nt * VECS);
   // few rows: more parts, so that they fill the chip, while the join holds all of a row's largest entries at once
   while (a.rows * parts < 256 && parts * s.nt * 2 <= vectors && 2 * parts * a.top <= 2048) parts *= 2;

@@ -245,3 +245,18 @@ def test_second_derivatives(gpu):
   picked = torch.where(ids < 0, 0.0, lp.gather(1, ids.clamp(min=0)))
   ref = second(b, picked, -(lp.exp() * safe).sum(-1), lp.gather(1, got.top_tokens.cpu()))
   assert (mine.cpu().double() - ref).abs().max() <= 1e-4        # (fp32 sums of 50 terms, two derivatives of values up to 10)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("vocab", [300, 4000, 16000, 40000])
+def test_many_alternatives_and_many_ties(gpu, vocab, dtype):
+  """Rows of a few values only: more entries reach the bound than the lists hold, and the lowest indices win."""
+  few = torch.randint(0, 3, (4, vocab), generator=_gen(1)).float()
+  few[1] = torch.where(torch.rand(vocab, generator=_gen(2)) < 0.9, 1.0, few[1])
+  few[2, : vocab // 2] = -math.inf
+  few[3] = -math.inf
+  few[3, vocab // 2 :: 7] = -2.0
+  x = few.to(dtype)
+  tokens = torch.randint(0, vocab, (4, 1), generator=_gen(3))
+  for top in (1, 16, 17, 64, 65, 200, 256):
+    _check(recml_amd.token_log_probs(x.cuda(), tokens.cuda(), top=top), x, tokens, top, False)
