@@ -24,6 +24,8 @@
 
 namespace {
 
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
 constexpr int VECS = 8;              // vectors of 16 bytes that a thread holds
 constexpr int MAX_TOP = 256;
 
@@ -94,7 +96,7 @@ struct Row {
     constexpr int N = Vec<F32>::N;
     Vec<F32> r;
     if (whole(v)) {
-      r.raw = *(const uint4*)(base + (int64_t)v * 16);
+      r.raw = __builtin_bit_cast(uint4, __builtin_nontemporal_load((const uint4v*)(base + (int64_t)v * 16)));
       return r;
     }
     uint32_t w[4];
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
       uint4 w;
       if constexpr (F32) w = __builtin_bit_cast(uint4, floatx4{y[0], y[1], y[2], y[3]});
       else w = uint4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
-      *(uint4*)(out + (int64_t)e * SIZE) = w;
+      __builtin_nontemporal_store(__builtin_bit_cast(uint4v, w), (uint4v*)(out + (int64_t)e * SIZE));
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
