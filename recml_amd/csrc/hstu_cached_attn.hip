@@ -610,8 +610,11 @@ Split split_of(const HstuCachedAttnArgs& a) {
   s.qblocks = (a.rows_per_seq + 16 * s.nq - 1) / (16 * s.nq);
   const int64_t cap = std::min<int64_t>(a.max_len, (int64_t)a.pages.table_pages * a.pages.page_size);
   const int64_t base = (int64_t)a.pages.B * a.pages.H * s.qblocks;
-  int64_t parts = (2048 + base - 1) / base;
-  parts = std::max<int64_t>(1, std::min(parts, (cap + 255) / 256));
+  // 2048 workgroups, of 256 keys at least and of 1024 where there are many without splitting: a part costs its start and the join's launch
+  // (8 us of 13 at 512 sequences of 512 keys), a long one that the others wait for it.  64 sequences x 8 heads, up to 2048 keys of 128 in 4
+  // bits: 4 parts 16.4 us at power-law lengths and 36.4 at full ones, 2 parts 18.4 and 33.4, one 20.4 and 33.7, 8 parts 18.2 and 43.
+  const int64_t least = std::max<int64_t>(256, std::min<int64_t>(base, 1024));
+  const int64_t parts = std::max<int64_t>(1, std::min((2048 + base - 1) / base, (cap + least - 1) / least));
   const int64_t chunk = std::max<int64_t>(128, ((cap + parts - 1) / parts + 127) / 128 * 128);
   s.chunk = (int)std::min<int64_t>(chunk, 1 << 30);
   s.parts = (int)std::max<int64_t>(1, (cap + s.chunk - 1) / s.chunk);
