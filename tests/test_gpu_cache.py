@@ -436,3 +436,43 @@ def test_python_conversions_and_refusals(gpu):
                 (got.k, got.k_scales, got.v[:1], got.v_scales)):
     with pytest.raises(ValueError):
       recml_amd.KVPages(*parts, head_dim=64)
+
+
+def test_pages_past_four_gigabytes(gpu):
+  """Codes at offsets that 32 bits do not hold."""
+  H, d, page, pages, n = 2, 256, 128, 70_000, 300                 # (64 KB a page: 4.6 GB of codes, keys and values each)
+  got = recml_amd.KVPages.empty(pages, page, H, d, bits=8, device="cuda:0")
+  assert got.k.numel() > 2**32
+  table = torch.tensor([[69_999, 3, 69_998]], dtype=torch.int32)
+  k, v = (torch.randn((1, n, H, d), generator=_gen(s)) * 0.4 for s in (1, 2))
+  q = torch.randn((1, 2, H, d), generator=_gen(3)) * 0.4
+  zero = torch.zeros(1, dtype=torch.int32).cuda()
+  recml_amd.kv_write(got, k.cuda(), v.cuda(), table.cuda(), zero)
+  for r, x in zip(recml_amd.kv_read(got, table.cuda(), zero, count=n, dtype=F32), (k, v)):
+    assert torch.equal(r.cpu().double(), R.stored(x, 8))
+  assert got.k[69_999].any() and got.k[3].any() and not got.k[69_997].any() and not got.k[0].any()
+  out = recml_amd.cached_attention(q.cuda(), got, table.cuda(), torch.tensor([n]).cuda(), max_len=n)
+  want = R.attention(q[0], R.stored(k, 8)[0], R.stored(v, 8)[0], length=n, held=torch.ones(n, dtype=torch.bool), max_len=n)
+  assert ((out[0].cpu().double() - want[0]).abs() <= R.attention_tolerance(*want, n, F32)).all()
+
+
+def test_calls_from_two_threads(gpu):
+  """Two threads, each on a stream of its own, reading one cache."""
+  import threading
+  c = [_case(B=2, H=2, d=64, bits=4, page=64, lengths=[700, 90], counts=[1, 1], max_len=700, dtype=BF16, packed=False, seed=8, ts="heads",
+             bucket_size=size) for size in (0.301, 0.5)]
+  want = [recml_amd.cached_attention(x[1], x[0], x[2], x[3], **x[4]) for x in c]
+  torch.cuda.synchronize()
+  bad = []
+  def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+      outs = [recml_amd.cached_attention(c[i][1], c[i][0], c[i][2], c[i][3], **c[i][4]) for _ in range(50)]
+      torch.cuda.current_stream().synchronize()
+      if not all(torch.equal(o, want[i]) for o in outs):
+        bad.append(i)
+  threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  assert not bad

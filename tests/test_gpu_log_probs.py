@@ -260,3 +260,31 @@ def test_many_alternatives_and_many_ties(gpu, vocab, dtype):
   tokens = torch.randint(0, vocab, (4, 1), generator=_gen(3))
   for top in (1, 16, 17, 64, 65, 200, 256):
     _check(recml_amd.token_log_probs(x.cuda(), tokens.cuda(), top=top), x, tokens, top, False)
+
+
+def test_logits_past_four_billion_entries(gpu):
+  """A last row whose entries lie past 2^32."""
+  rows, vocab = 4300, 1_000_003
+  x = torch.zeros((rows, vocab), dtype=BF16, device="cuda")
+  last = _logits(1, vocab, BF16, 5)
+  x[-1] = last[0].cuda()
+  ids = torch.zeros((rows, 2), dtype=torch.int64, device="cuda")
+  ids[-1, 1] = vocab - 1
+  leaf = x.requires_grad_(True)
+  got = recml_amd.token_log_probs(leaf, ids, top=4, entropy=True)
+  _check(recml_amd.TokenLogProbs(*(t[-1:].detach() for t in got)), last, ids[-1:].cpu(), 4, True)
+  d = torch.autograd.grad(got.log_probs[-1].sum(), leaf)[0]
+  want = R.log_probs(last, ids[-1:].cpu(), 0, torch.ones((1, 2)))[4]
+  assert not d[-2].any() and (d[-1].cpu().double() - want[0]).abs().max() <= 2.0**-7 + 1e-5      # (a gradient of 1 in bf16: 2^-8 of it, twice)
+
+
+def test_a_loss_that_asks_for_some_rows_only(gpu):
+  """Gradients that arrive as views: expanded, strided, of some outputs only."""
+  x = _logits(6, 3000, F32, 3).cuda().requires_grad_(True)
+  ids = torch.randint(0, 3000, (6, 4), generator=_gen(1)).cuda()
+  got = recml_amd.token_log_probs(x, ids, top=3, entropy=True)
+  a = torch.autograd.grad(got.log_probs.mean(), x, retain_graph=True)[0]                          # (an expanded scalar)
+  b = torch.autograd.grad(got.log_probs, x, torch.full((4, 6), 1 / 24, device="cuda").t(), retain_graph=True)[0]
+  assert torch.equal(a, b)
+  c = torch.autograd.grad(got.top_log_probs[2, 1] + got.entropy[5], x)[0]
+  assert c[2].any() and c[5].any() and not c[[0, 1, 3, 4]].any()
