@@ -49,7 +49,7 @@ typedef enum HstuServeStatus {
 
 typedef enum HstuServeDtype { HSTU_SERVE_BF16 = 0, HSTU_SERVE_FP32 = 1 } HstuServeDtype;
 
-/* The pages of one layer.  Pointers 16-byte aligned; page_size a multiple of 32; d one of 8, 16, 24, 32, 48, 64, 96,
+/* The pages of one layer.  Pointers 16-byte aligned; page_size a multiple of 32, at most 2^20; d one of 8, 16, 24, 32, 48, 64, 96,
  * 128, 192, 256; bits 4 or 8. */
 typedef struct HstuKvPages {
   void* k_codes;

@@ -295,7 +295,8 @@ int serve_check_pages(const HstuKvPages& g) {
   if (g.B > 0 && g.table_pages > 0 && !g.page_table) return serve_fail(HSTU_SERVE_ERR_NULL, "page_table is null");
   if (g.bits != 4 && g.bits != 8) return serve_fail(HSTU_SERVE_ERR_SHAPE, "bits=%d: 4 or 8", g.bits);
   if (!head_dim_taken(g.d)) return serve_fail(HSTU_SERVE_ERR_SHAPE, "d=%d: 8, 16, 24, 32, 48, 64, 96, 128, 192 or 256", g.d);
-  if (g.page_size < 32 || g.page_size % 32) return serve_fail(HSTU_SERVE_ERR_SHAPE, "page_size=%d: a multiple of 32", g.page_size);
+  // (a head's part of a page stays within 32 bits)
+  if (g.page_size < 32 || g.page_size % 32 || g.page_size > 1 << 20) return serve_fail(HSTU_SERVE_ERR_SHAPE, "page_size=%d: a multiple of 32, at most 2^20", g.page_size);
   for (const void* t : {g.k_codes, g.k_scales, g.v_codes, g.v_scales})
     if (!serve_aligned16(t)) return serve_fail(HSTU_SERVE_ERR_SHAPE, "codes and scales start on 16-byte boundaries");
   return HSTU_SERVE_OK;

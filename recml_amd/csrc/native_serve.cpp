@@ -42,7 +42,7 @@ bool fill_pages(const Pages& p, HstuKvPages* g) {
   for (const Tensor& t : p.t)
     if (!t.defined() || !plain(t, dev, at::kByte) || t.dim() != 4 || !aligned(t)) return false;
   const int64_t n = k.size(0), H = k.size(1), size = k.size(2), width = k.size(3), blocks = (p.d + 31) / 32;
-  if (8 * width != p.bits * p.d || (p.bits != 4 && p.bits != 8) || size < 32 || size % 32 || H < 1 || n > MOST || H > MOST || size > MOST) return false;
+  if (8 * width != p.bits * p.d || (p.bits != 4 && p.bits != 8) || size < 32 || size % 32 || size > 1 << 20 || H < 1 || n > MOST || H > MOST) return false;
   if (p.t[2].sizes() != k.sizes()) return false;
   for (int i : {1, 3})
     if (p.t[i].size(0) != n || p.t[i].size(1) != H || p.t[i].size(2) != blocks || p.t[i].size(3) != size) return false;
@@ -78,6 +78,13 @@ bool table_arg(PyObject* o, c10::Device dev, Tensor* keep, HstuKvPages* g) {
 
 bool ints_arg(PyObject* o, c10::Device dev, int64_t n, Tensor* keep) {
   return tensor_arg(o, keep) && keep->defined() && plain(*keep, dev, at::kInt) && keep->dim() == 1 && keep->size(0) == n;
+}
+
+// Whether every entry has memory of its own, as far as strides of zero tell.
+bool apart(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return false;
+  return true;
 }
 
 struct RowStrides { int64_t b, t, h; };
@@ -148,7 +155,7 @@ PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (!tensor_arg(a[1], &k) || !tensor_arg(a[2], &v) || !k.defined() || !v.defined() || !table_arg(a[3], dev, &table, &args.pages) ||
         !ints_arg(a[4], dev, args.pages.B, &starts)) Py_RETURN_NONE;
     const bool packed = a[5] != Py_None;
-    if (packed && (!ints_arg(a[5], dev, (int64_t)args.pages.B + 1, &offsets) || !long_arg(a[6], &max_new) || max_new < 0 || max_new > MOST)) Py_RETURN_NONE;
+    if (packed && (!ints_arg(a[5], dev, (int64_t)args.pages.B + 1, &offsets) || !long_arg(a[6], &max_new) || max_new < 0 || max_new > 1 << 30)) Py_RETURN_NONE;
     if (!packed && a[6] != Py_None) Py_RETURN_NONE;
     if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || !rows_ready(k, dev, args.pages, packed, &ks) || !rows_ready(v, dev, args.pages, packed, &vs) ||
         wants_grad({&k, &v}) || dual({&k, &v})) Py_RETURN_NONE;
@@ -182,7 +189,7 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t count) {
     } else if (!long_arg(a[3], &n) || a[5] != Py_None || a[6] != Py_None) {
       Py_RETURN_NONE;
     }
-    if (n < 0 || n > MOST || total < 0 || total > MOST) Py_RETURN_NONE;
+    if (n < 0 || n > 1 << 30 || total < 0 || total > MOST) Py_RETURN_NONE;
     const auto type = a[7] == Py_True ? at::kFloat : at::kBFloat16;
     without_lock(pages.t[0], [&] {
       const int64_t B = args.pages.B, H = args.pages.H, d = args.pages.d;
@@ -223,7 +230,7 @@ PyObject* cached_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (!packed && a[6] != Py_None) Py_RETURN_NONE;
     if ((a[7] != Py_None && (!float_arg(a[7], &n) || !(n > 0.0))) || !float_arg(a[8], &alpha) || !float_arg(a[12], &bucket)) Py_RETURN_NONE;
     if (!tensor_arg(a[9], &pos) || !tensor_arg(a[10], &ts) || !tensor_arg(a[11], &ts_tab) || !tensor_arg(a[13], &out)) Py_RETURN_NONE;
-    if (!rows_ready(q, dev, args.pages, packed, &qs) || wants_grad({&q, &pos, &ts_tab}) || dual({&q, &pos, &ts_tab})) Py_RETURN_NONE;
+    if (!rows_ready(q, dev, args.pages, packed, &qs) || wants_grad({&q, &pos, &ts_tab, &out}) || dual({&q, &pos, &ts_tab})) Py_RETURN_NONE;
     if (!packed) max_new = q.size(1);
     if (max_new < 0 || max_new > 1 << 30) Py_RETURN_NONE;
     args.lengths = lengths.const_data_ptr<int32_t>();
@@ -243,7 +250,7 @@ PyObject* cached_attention(PyObject*, PyObject* const* a, Py_ssize_t count) {
       args.ts_tab = ts_tab.const_data_ptr<float>();
       args.ts_heads = (int32_t)heads; args.ts_buckets = (int32_t)width - 1; args.ts_bucket_size = (float)bucket;
     }
-    if (out.defined() && (out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes() || !rows_ready(out, dev, args.pages, packed, &os))) Py_RETURN_NONE;
+    if (out.defined() && (out.scalar_type() != q.scalar_type() || out.sizes() != q.sizes() || !apart(out) || !rows_ready(out, dev, args.pages, packed, &os))) Py_RETURN_NONE;
     without_lock(q, [&] {
       if (!out.defined()) {
         out = at::empty(q.sizes(), q.options().requires_grad(false));
@@ -370,6 +377,7 @@ PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t count) {
     Tensor x, tokens;
     int64_t top, rows, stride;
     if (!tensor_arg(a[0], &x) || !tensor_arg(a[1], &tokens) || !x.defined() || !long_arg(a[2], &top) || !logits_rows(x, &rows, &stride)) Py_RETURN_NONE;
+    if (a[3] != Py_True && a[3] != Py_False) Py_RETURN_NONE;
     const bool entropy = a[3] == Py_True;
     const int64_t V = x.size(-1);
     if (top < 0 || top > std::min<int64_t>(V, 256) || rows < 1 || dual({&x})) Py_RETURN_NONE;

@@ -19,6 +19,7 @@ from recml_amd import _lib_serve
 from recml_amd import _native
 
 HEAD_DIMS = (8, 16, 24, 32, 48, 64, 96, 128, 192, 256)
+MOST_ROWS = 1 << 30          # of one sequence, and of a call's max_len: the kernels count in 32 bits
 _DTYPES = {torch.bfloat16: _lib_serve.BF16, torch.float32: _lib_serve.FP32}
 
 
@@ -71,8 +72,8 @@ class KVPages:
     pages, heads, size, width = k.shape
     if 8 * width not in (4 * d, 8 * d):
       raise ValueError(f"rows of {width} bytes do not hold {d} codes of 4 or 8 bits")
-    if size < 32 or size % 32:
-      raise ValueError(f"page_size must be a multiple of 32, got {size}")
+    if size < 32 or size % 32 or size > 1 << 20:
+      raise ValueError(f"page_size must be a multiple of 32, at most 2^20, got {size}")
     if heads < 1:
       raise ValueError("there must be at least one head")
     scales = (pages, heads, (d + 31) // 32, size)
@@ -156,8 +157,8 @@ def _check_rows(name, t, pages, B, offsets, max_new):
       raise ValueError(f"max_new={max_new} does not match the {t.shape[1]} rows of a sequence")
   elif t.dim() != 3 or tuple(t.shape[1:]) != tail:
     raise ValueError(f"packed {name} must be [T, {tail[0]}, {tail[1]}], got {tuple(t.shape)}")
-  elif max_new is None or int(max_new) < 0:
-    raise ValueError("packed rows need `max_new`, the most rows that one sequence has")
+  elif max_new is None or not 0 <= int(max_new) <= MOST_ROWS:
+    raise ValueError(f"packed rows need `max_new`, the most rows that one sequence has (up to {MOST_ROWS}), got {max_new}")
 
 
 def _fill_rows(a, pages, table, B, starts, offsets, per_seq, total, k, v):
@@ -217,11 +218,11 @@ def kv_read(pages, page_table, starts, *, count=None, offsets=None, max_new=None
     raise ValueError(f"unsupported dtype {dtype}: use float32 or bfloat16")
   starts = _ints("starts", starts, device, (B,))
   if offsets is None:
-    if count is None or int(count) < 0 or total is not None or max_new is not None:
+    if count is None or not 0 <= int(count) <= MOST_ROWS or total is not None or max_new is not None:
       raise ValueError("pass `count`, or `offsets` with `max_new` and `total`")
     shape, per_seq = (B, int(count)), int(count)
   else:
-    if count is not None or max_new is None or total is None or int(max_new) < 0 or int(total) < 0:
+    if count is not None or max_new is None or total is None or not 0 <= int(max_new) <= MOST_ROWS or int(total) < 0:
       raise ValueError("pass `count`, or `offsets` with `max_new` and `total`")
     offsets = _ints("offsets", offsets, device, (B + 1,))
     shape, per_seq = (int(total),), int(max_new)
@@ -268,12 +269,12 @@ def cached_attention(q, pages, page_table, lengths, *, max_len, offsets=None, ma
   table = _table(pages, page_table)
   B, device, H = table.shape[0], pages.k.device, pages.heads
   _check_rows("q", q, pages, B, offsets, max_new)
-  _no_gradient("cached_attention", q, pos_bias, ts_bias)
+  _no_gradient("cached_attention", q, pos_bias, ts_bias, out)
   lengths = _ints("lengths", lengths, device, (B,))
   offsets = None if offsets is None else _ints("offsets", offsets, device, (B + 1,))
   L = int(max_len)
-  if L < 1:
-    raise ValueError(f"max_len must be positive, got {max_len}")
+  if not 1 <= L <= MOST_ROWS:
+    raise ValueError(f"max_len must lie between 1 and {MOST_ROWS}, got {max_len}")
   n = L if n is None else n
   if not n > 0:
     raise ValueError(f"normaliser n must be positive, got {n}")
@@ -285,8 +286,8 @@ def cached_attention(q, pages, page_table, lengths, *, max_len, offsets=None, ma
     _check_gpu("out", out)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
       raise ValueError(f"out must be a {q.dtype} tensor of shape {tuple(q.shape)} on {device}")
-    if _rows(out, unit) is not out:
-      raise ValueError("out's rows must be contiguous and start on 16-byte boundaries")
+    if _rows(out, unit) is not out or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+      raise ValueError("out's rows must be contiguous, start on 16-byte boundaries and lie apart")
   a = _lib_serve.HstuCachedAttnArgs()
   a.struct_size, a.version = C.sizeof(a), _lib_serve.ABI_VERSION
   pages._fill(a.pages, table, B)

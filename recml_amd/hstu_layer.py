@@ -409,6 +409,14 @@ def _is_plain_call(block, jagged) -> bool:
                    or m._global_forward_hooks or m._global_forward_pre_hooks or m._global_backward_hooks or m._global_backward_pre_hooks))
 
 
+def _serves(block) -> bool:
+  """Whether the block's forward_cached stands for its forward: both HSTUBlock's own, or a subclass's that has one of its own."""
+  own, kind = block.__dict__, type(block)
+  same = (kind.forward is HSTUBlock.forward and kind.forward_jagged is HSTUBlock.forward_jagged
+          and "forward" not in own and "forward_jagged" not in own)
+  return same or kind.forward_cached is not HSTUBlock.forward_cached or "forward_cached" in own
+
+
 class HSTU(torch.nn.Module):
   """The HSTU model forward (recml/layers/keras/hstu.py:585-621): item
   embedding (x sqrt(D)) + position embedding -> final_norm -> blocks ->
@@ -633,6 +641,8 @@ class HSTU(torch.nn.Module):
       raise ValueError(f"the cache holds {cache.batch} histories of up to {cache.max_len} events, got {tuple(inputs.shape)}")
     if tuple(seq_lens.shape) != (B,):
       raise ValueError(f"seq_lens must be [{B}], got {tuple(seq_lens.shape)}")
+    if timestamps is not None and timestamps.shape != inputs.shape:
+      raise ValueError(f"timestamps must be {tuple(inputs.shape)}, got {tuple(timestamps.shape)}")
     lens = seq_lens.to(torch.int64).clamp(0, L)
     rows = (torch.arange(L, device=inputs.device)[None, :] < lens[:, None]).reshape(-1).nonzero().squeeze(1)
     offsets = torch.zeros(B + 1, dtype=torch.int32, device=inputs.device)
@@ -653,7 +663,8 @@ class HSTU(torch.nn.Module):
     most events of one user); `timestamps` shaped like them.  Their keys and values join the cache, and every event attends to its
     user's history up to itself.  Returns the model's outputs for the new events, [B, n, ...] or [T, ...]; token_log_probs makes log
     probabilities and the items to recommend of logits.  Nothing in here waits for the GPU: a step can be captured into a graph
-    and replayed.  Events past cache.max_len are lost: they join nothing and attend to nothing."""
+    and replayed.  Events past cache.max_len are lost: they join nothing and attend to nothing.  So are a user's packed events past
+    `max_new`, and packed rows of no user: what comes back for those means nothing."""
     B, dev = cache.batch, ids.device
     if offsets is None:
       if ids.dim() != 2 or ids.shape[0] != B:
@@ -665,10 +676,12 @@ class HSTU(torch.nn.Module):
       if ids.dim() != 1 or max_new is None or tuple(offsets.shape) != (B + 1,):
         raise ValueError(f"packed ids are [T] with `offsets` [{B + 1}] and `max_new`, got {tuple(ids.shape)} and {tuple(offsets.shape)}")
       offsets = offsets.to(torch.int32)
-      count = offsets[1:] - offsets[:-1]
+      ends = offsets.to(torch.int64).clamp(0, ids.shape[0])
+      count = (ends[1:] - ends[:-1]).clamp(0, int(max_new)).to(torch.int32)
       at = torch.arange(ids.shape[0], device=dev)
-      users = (torch.searchsorted(offsets[1:].to(torch.int64), at, right=True)).clamp(max=B - 1)
-      steps = at - offsets[users]
+      users = torch.searchsorted(ends[1:], at, right=True).clamp(max=B - 1)
+      steps = at - ends[users]
+      steps = torch.where((steps >= 0) & (steps < count[users]), steps, cache.max_len)      # (past every history's end)
     with torch.no_grad():
       starts = cache.lengths.clone()
       lengths = starts + count
@@ -682,6 +695,9 @@ class HSTU(torch.nn.Module):
       raise ValueError("serving is inference: call eval() on the model first")
     if len(cache.layers) != len(self.decoder_blocks):
       raise ValueError(f"the cache has {len(cache.layers)} layers, the model {len(self.decoder_blocks)}")
+    if type(self)._front_end is not HSTU._front_end or not all(_serves(block) for block in self.decoder_blocks):
+      raise ValueError("serving runs HSTU's own front end and HSTUBlock.forward_cached: a block with a forward of its own needs a "
+                       "forward_cached of its own too")
     if (ts_bias is None) != (timestamps is None):
       raise ValueError("Both or neither of `timestamps` and `ts_bias` must be provided.")
     cache._note_times(timestamps, users, places)

@@ -19,6 +19,7 @@ from recml_amd import _native
 from recml_amd.hstu_cache_ops import _DTYPES, _call, _check_gpu
 
 MAX_TOP = 256
+MAX_VOCAB = 1 << 30
 
 
 class TokenLogProbs(NamedTuple):
@@ -111,8 +112,8 @@ def token_log_probs(logits, tokens=None, *, top: int = 0, entropy: bool = False)
   _check_gpu("logits", logits)
   if logits.dtype not in _DTYPES:
     raise ValueError(f"logits: unsupported dtype {logits.dtype}: use float32 or bfloat16")
-  if logits.dim() < 1 or logits.shape[-1] < 1:
-    raise ValueError(f"logits must be [..., V] with V at least 1, got {tuple(logits.shape)}")
+  if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
+    raise ValueError(f"logits must be [..., V] with V from 1 to {MAX_VOCAB}, got {tuple(logits.shape)}")
   lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
   top = int(top)
   if not 0 <= top <= min(MAX_TOP, V):
@@ -125,6 +126,8 @@ def token_log_probs(logits, tokens=None, *, top: int = 0, entropy: bool = False)
     shape = tuple(tokens.shape)
     if shape != lead and not (len(shape) == len(lead) + 1 and shape[:-1] == lead):
       raise ValueError(f"tokens must be {lead} or {lead + ('C',)}, got {shape}")
+    if shape != lead and shape[-1] > MAX_VOCAB:
+      raise ValueError(f"at most {MAX_VOCAB} tokens a row, got {shape}")
     if tokens.numel():
       ids = tokens.to(torch.int64).reshape(-1, 1 if shape == lead else shape[-1]).contiguous()
   elif not top and not entropy:

@@ -132,3 +132,10 @@ def test_scores_forward_and_backward_refused():
     assert lib.hstu_log_probs_bwd(C.byref(_score_args(**change)), None) == status
   assert lib.hstu_log_probs_fwd(None, None) == -1 and lib.hstu_log_probs_bwd(None, None) == -1
   assert lib.hstu_log_probs_fwd(C.byref(_score_args(rows=0)), None) == 0 and lib.hstu_log_probs_workspace_bytes(C.byref(_score_args(rows=0))) == 0
+
+
+def test_pages_that_32_bits_do_not_reach_are_refused():
+  lib = _lib_serve.load()
+  for size in ((1 << 20) + 32, 1 << 30):
+    assert lib.hstu_kv_write(C.byref(_rows_args(page_size=size)), None) == -4 and "2^20" in lib.hstu_serve_last_error().decode()
+    assert lib.hstu_cached_attn(C.byref(_attn_args(page_size=size)), None) == -4

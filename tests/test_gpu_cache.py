@@ -476,3 +476,22 @@ def test_calls_from_two_threads(gpu):
   for t in threads:
     t.join()
   assert not bad
+
+
+def test_numbers_past_32_bits_and_outputs_that_overlap_are_refused(gpu):
+  """Counts that the kernels' 32 bits would cut off, an output whose rows share memory, an output that wants a gradient."""
+  got, rows, table, lens, call, want, counts = _case(B=2, H=2, d=64, bits=8, page=64, lengths=[130, 20], counts=[2, 2], max_len=130, dtype=BF16,
+                                                     packed=False, seed=9)
+  flat, offsets = rows.reshape(4, 2, 64), torch.tensor([0, 2, 4], dtype=torch.int32).cuda()
+  for change in (dict(max_len=2**32 + 130), dict(max_len=2**30 + 1), dict(out=rows[:, :1].expand_as(rows)), dict(out=rows.clone().requires_grad_(True))):
+    with pytest.raises(ValueError):
+      recml_amd.cached_attention(rows, got, table, lens, **dict(call, **change))
+  for many in (2**32 + 2, 2**30 + 1, -1):
+    with pytest.raises(ValueError, match="max_new"):
+      recml_amd.cached_attention(flat, got, table, lens, **dict(call, offsets=offsets, max_new=many))
+    with pytest.raises(ValueError, match="max_new"):
+      recml_amd.kv_write(got, flat, flat, table, lens, offsets=offsets, max_new=many)
+    with pytest.raises(ValueError):
+      recml_amd.kv_read(got, table, lens, offsets=offsets, max_new=many, total=4)
+    with pytest.raises(ValueError):
+      recml_amd.kv_read(got, table, lens, count=many)

@@ -288,3 +288,14 @@ def test_a_loss_that_asks_for_some_rows_only(gpu):
   assert torch.equal(a, b)
   c = torch.autograd.grad(got.top_log_probs[2, 1] + got.entropy[5], x)[0]
   assert c[2].any() and c[5].any() and not c[[0, 1, 3, 4]].any()
+
+
+def test_a_vocabulary_past_32_bits_is_refused_and_entropy_by_any_truth(gpu):
+  x = torch.zeros((1, 1), device="cuda").expand(1, 2**32 + 8)           # (no memory behind it; refused before a copy is made)
+  with pytest.raises(ValueError, match="V from 1"):
+    recml_amd.token_log_probs(x, torch.zeros(1, dtype=torch.int64, device="cuda"))
+  y, ids = torch.randn((3, 50), generator=_gen(1)).cuda(), torch.arange(3).cuda()
+  want = recml_amd.token_log_probs(y, ids, entropy=True)
+  got = recml_amd.token_log_probs(y, ids, entropy=1)
+  assert torch.equal(got.entropy, want.entropy) and torch.equal(got.log_probs, want.log_probs)
+  assert recml_amd.token_log_probs(y, ids, entropy=0).entropy is None

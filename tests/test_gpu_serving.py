@@ -249,3 +249,59 @@ def test_what_serving_refuses(gpu):
     dropped.extend(ids, dropped.new_cache(2, 32))
   with pytest.raises(ValueError, match="head_dim"):
     recml_amd.HSTU(vocab_size=10, model_dim=40, num_heads=1, num_layers=1, device="cuda:0").new_cache(2, 32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_without_events(gpu, dtype):
+  model = _model(dtype)
+  cache = model.new_cache(2, 32)
+  assert model.extend(torch.zeros((2, 0), dtype=torch.int64).cuda(), cache).shape == (2, 0, 300)
+  none = torch.zeros(3, dtype=torch.int32).cuda()
+  assert model.extend(torch.zeros(0, dtype=torch.int64).cuda(), cache, offsets=none, max_new=4).shape == (0, 300)
+  out = model.prefill(torch.zeros((2, 5), dtype=torch.int64).cuda(), cache, seq_lens=torch.zeros(2, dtype=torch.int64).cuda())
+  assert out.shape == (2, 5, 300) and not out.any() and cache.lengths.tolist() == [0, 0]
+
+
+def test_packed_rows_of_no_user_and_past_max_new(gpu):
+  """Rows before the first user's, behind the last one's and past `max_new` join no history: neither its length, nor its keys, nor its times."""
+  model = _model(F32)
+  pos, tab = (torch.randn((127,), generator=_gen(3)) * 0.2).cuda(), (torch.randn((129,), generator=_gen(4)) * 0.2).cuda()
+  ids = torch.randint(1, 300, (2, 12), generator=_gen(1)).cuda()
+  ts = (1_600_000_000 + torch.randint(1, 10**5, (2, 12), generator=_gen(2)).cumsum(1)).cuda()
+  odd, plain = (model.new_cache(2, 64, bits=8, page_size=32, timestamps=True) for _ in range(2))
+  for c in (odd, plain):
+    model.prefill(ids[:, :6], c, seq_lens=torch.tensor([6, 4]).cuda(), timestamps=ts[:, :6], pos_bias=pos, ts_bias=tab)
+  # user 0: rows 2 and 3; user 1: rows 4, 5 and 6, of which the third is past max_new; rows 0, 1, 7, 8: nobody's
+  rows, when = torch.randint(1, 300, (9,), generator=_gen(5)).cuda(), (1_700_000_000 + torch.arange(9)).cuda()
+  a = model.extend(rows, odd, offsets=torch.tensor([2, 4, 7]).cuda(), max_new=2, timestamps=when, pos_bias=pos, ts_bias=tab)
+  b = model.extend(rows[2:6], plain, offsets=torch.tensor([0, 2, 4]).cuda(), max_new=2, timestamps=when[2:6], pos_bias=pos, ts_bias=tab)
+  assert torch.equal(a[2:6], b)
+  assert odd.lengths.tolist() == plain.lengths.tolist() == [8, 6]
+  assert torch.equal(odd.timestamps, plain.timestamps)
+  for x, y in zip(odd.layers, plain.layers):
+    assert torch.equal(x.k, y.k) and torch.equal(x.v_scales, y.v_scales)
+  step = dict(timestamps=ts[:, 6:7], pos_bias=pos, ts_bias=tab)
+  assert torch.equal(model.extend(ids[:, 6:7], odd, **step), model.extend(ids[:, 6:7], plain, **step))
+
+
+def test_times_of_another_shape_and_blocks_of_another_kind_are_refused(gpu):
+  model = _model(F32, layers=1)
+  ids, lens = torch.zeros((2, 4), dtype=torch.int64).cuda(), torch.tensor([4, 2]).cuda()
+  timed = model.new_cache(2, 32, timestamps=True)
+  with pytest.raises(ValueError, match="timestamps"):
+    model.prefill(ids, timed, seq_lens=lens, timestamps=torch.zeros((2, 9), dtype=torch.int64).cuda(), ts_bias=torch.zeros(129).cuda())
+
+  class Doubled(recml_amd.HSTUBlock):
+    def forward(self, *args, **kw):
+      return 2 * super().forward(*args, **kw)
+
+  class Served(Doubled):
+    def forward_cached(self, *args, **kw):
+      return 2 * super().forward_cached(*args, **kw)
+
+  block = model.decoder_blocks[0]
+  block.__class__ = Doubled
+  with pytest.raises(ValueError, match="forward_cached"):
+    model.extend(ids, model.new_cache(2, 32))
+  block.__class__ = Served
+  assert model.extend(ids, model.new_cache(2, 32)).shape == (2, 4, 300)
