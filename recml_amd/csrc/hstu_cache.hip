@@ -321,7 +321,7 @@ int kv_rows(const HstuKvRowsArgs* a, void* stream, bool write) {
   for (const int64_t s : {a->k_stride_t, a->k_stride_h, a->v_stride_t, a->v_stride_h, a->offsets ? (int64_t)0 : a->k_stride_b, a->offsets ? (int64_t)0 : a->v_stride_b})
     if (s % unit) return serve_fail(HSTU_SERVE_ERR_SHAPE, "a stride of %lld elements: rows start on 16-byte boundaries", (long long)s);
   const int64_t tiles = ((int64_t)a->rows_per_seq + 31 + 31) / 32;   // (the first place may lie anywhere in its 32)
-  if (tiles * g.H > 0x7fffffffll || tiles * g.H * g.B > 0x7fffffffll) return serve_fail(HSTU_SERVE_ERR_SHAPE, "%lld x %d x %d tiles are too many for one call", (long long)tiles, g.H, g.B);
+  if (tiles * g.H > SERVE_THREADS / 256 / g.B) return serve_fail(HSTU_SERVE_ERR_SHAPE, "%lld x %d x %d tiles are too many for one call", (long long)tiles, g.H, g.B);
   Params p;
   p.g = g;
   p.side[0] = Side{(uint8_t*)g.k_codes, (uint8_t*)g.k_scales, a->k, a->k_stride_b, a->k_stride_t, a->k_stride_h};

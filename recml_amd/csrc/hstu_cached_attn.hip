@@ -706,7 +706,7 @@ int hstu_cached_attn(const HstuCachedAttnArgs* a, void* stream) {
   const size_t need = workspace_of(*a, s);
   if (need && (!a->workspace || a->workspace_bytes < need || !serve_aligned16(a->workspace)))
     return serve_fail(HSTU_SERVE_ERR_WORKSPACE, "workspace of %zu bytes on a 16-byte boundary needed, got %zu", need, a->workspace_bytes);
-  const int64_t grid = (int64_t)a->pages.B * a->pages.H * s.qblocks, most = 0x7fffffff;
+  const int64_t grid = (int64_t)a->pages.B * a->pages.H * s.qblocks, most = SERVE_THREADS / THREADS;
   const int64_t per = (int64_t)a->rows_per_seq * a->pages.H * (a->pages.d / 4), join = (per + THREADS - 1) / THREADS * a->pages.B;
   if (grid > most / s.parts || join > most) return serve_fail(HSTU_SERVE_ERR_SHAPE, "too many workgroups for one call");
   Params p;

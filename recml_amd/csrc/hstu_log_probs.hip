@@ -311,7 +311,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
         for (int i = 0; i < N; ++i) {
           const float d = x[c].at(i) - zero, e = __builtin_amdgcn_exp2f(d * LOG2E);
           s += e;
-          t = __builtin_fmaf(fmaxf(d, -1e30f), e, t);          // (-inf times its 0 is nothing; a NaN is in s)
+          t = __builtin_fmaf(fmaxf(d, -1e4f), e, t);           // (e is 0 long before: -inf times its 0 is nothing; a NaN is in s)
         }
         x[c].hold();
       }
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float lp = (x[c].at(i) - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
-        y[i] = -pr * __builtin_fmaf(ge, fmaxf(lp, -1e30f) + entropy, total);      // (-inf times its 0 is nothing)
+        y[i] = -pr * __builtin_fmaf(ge, fmaxf(lp, -1e4f) + entropy, total);      // (-inf times its 0 is nothing)
       }
     } else {
 #pragma unroll
@@ -596,7 +596,7 @@ int fill(const HstuLogProbsArgs* a, const Split& s, Params* p) {
   const size_t size = a->dtype == HSTU_SERVE_FP32 ? 4 : 2;
   if (!a->logits || (a->count > 0 && !a->tokens)) return serve_fail(HSTU_SERVE_ERR_NULL, "logits or tokens is null");
   if ((uintptr_t)a->logits % size) return serve_fail(HSTU_SERVE_ERR_SHAPE, "logits are not aligned to their type");
-  if (a->rows > 0x7fffffffll / s.parts) return serve_fail(HSTU_SERVE_ERR_SHAPE, "%lld rows of %d parts are too many for one call", (long long)a->rows, s.parts);
+  if (a->rows > SERVE_THREADS / s.nt / s.parts) return serve_fail(HSTU_SERVE_ERR_SHAPE, "%lld rows of %d parts are too many for one call", (long long)a->rows, s.parts);
   *p = Params{};
   p->logits = a->logits; p->stride = a->stride; p->tokens = a->tokens;
   p->log_probs = a->log_probs; p->entropy = a->entropy; p->stats = a->stats;

@@ -27,6 +27,8 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+constexpr int64_t SERVE_THREADS = 0xffffffffll;      // of one launch: a dimension's threads are counted in 32 bits
+
 inline bool serve_aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {

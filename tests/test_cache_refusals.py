@@ -139,3 +139,15 @@ def test_pages_that_32_bits_do_not_reach_are_refused():
   for size in ((1 << 20) + 32, 1 << 30):
     assert lib.hstu_kv_write(C.byref(_rows_args(page_size=size)), None) == -4 and "2^20" in lib.hstu_serve_last_error().decode()
     assert lib.hstu_cached_attn(C.byref(_attn_args(page_size=size)), None) == -4
+
+
+def test_more_threads_than_a_launch_has_are_refused():
+  """A launch counts its threads in 32 bits: 2^24 workgroups of 256, 2^26 of 64."""
+  lib = _lib_serve.load()
+  for fn in (lib.hstu_kv_write, lib.hstu_kv_read):
+    assert fn(C.byref(_rows_args(B=1 << 20, H=16, k_stride_h=64, rows_per_seq=1)), None) == -4 and "too many" in lib.hstu_serve_last_error().decode()
+  assert lib.hstu_cached_attn(C.byref(_attn_args(B=1 << 20, H=16, workspace=0x10, workspace_bytes=1 << 40)), None) == -4
+  assert "too many" in lib.hstu_serve_last_error().decode()
+  small = dict(vocab=16, stride=16, top=0, workspace=0x10, workspace_bytes=1 << 40)
+  for change in (dict(small, rows=1 << 26), dict(small, vocab=16384, stride=16384, rows=1 << 24)):
+    assert lib.hstu_log_probs_fwd(C.byref(_score_args(**change)), None) == -4 and "too many" in lib.hstu_serve_last_error().decode()

@@ -299,3 +299,14 @@ def test_a_vocabulary_past_32_bits_is_refused_and_entropy_by_any_truth(gpu):
   got = recml_amd.token_log_probs(y, ids, entropy=1)
   assert torch.equal(got.entropy, want.entropy) and torch.equal(got.log_probs, want.log_probs)
   assert recml_amd.token_log_probs(y, ids, entropy=0).entropy is None
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_large_gradient_of_the_entropy_beside_masked_entries(gpu, dtype):
+  """Masked entries get none of it, however large it is."""
+  x = (torch.randn((2, 70), generator=_gen(3))).to(dtype)
+  x[0, 5:30] = -math.inf
+  x = x.cuda().requires_grad_(True)
+  d = torch.autograd.grad(recml_amd.token_log_probs(x, entropy=True).entropy, x, torch.full((2,), 2.0**40).cuda())[0]
+  one = torch.autograd.grad(recml_amd.token_log_probs(x, entropy=True).entropy, x, torch.ones(2).cuda())[0]
+  assert torch.equal(d, one * 2.0**40) and not d[0, 5:30].any() and d.isfinite().all()
