@@ -479,7 +479,13 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
 template <bool F32, int NT>
 __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
   constexpr int N = Vec<F32>::N, SIZE = F32 ? 4 : 2;
-  __shared__ uint32_t hit[NT * VECS * N / 32];
+  __shared__ uint32_t hit[NT * VECS * N / 32], several[NT * VECS * N / 32];
+  constexpr int LIST = 4 * NT;
+  // the places of the first outputs' entries in the part, and their gradients
+  __shared__ __attribute__((aligned(16))) int list[LIST];
+  __shared__ __attribute__((aligned(16))) float gradient[LIST];
+  __shared__ uint16_t queue[LIST];     // those whose entries are others' too
+  __shared__ int queued, repeated;
   __shared__ float sums[4];
   const int64_t row = blockIdx.x / p.parts;
   const int part = blockIdx.x % p.parts;
@@ -489,64 +495,102 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
 #pragma unroll
   for (int c = 0; c < VECS; ++c)
     if (c < p.vecs) x[c] = r.load(v0 + c * NT + threadIdx.x);
-  // the gradients' sum, and which of the part's entries have one of their own
+  // the gradients' sum, and which of the part's entries have one of their own, or several
   const int64_t e0 = (int64_t)v0 * N - r.shift;
-  for (int i = threadIdx.x; i < NT * p.vecs * N / 32; i += NT) hit[i] = 0;
+  const int entries = NT * p.vecs * N, asked = (p.g_tokens ? p.count : 0) + (p.g_top ? p.top : 0), given = p.g_tokens ? p.count : 0;
+  for (int i = threadIdx.x; i < entries / 32; i += NT) hit[i] = several[i] = 0;
+  if (threadIdx.x == 0) queued = repeated = 0;
   __syncthreads();
+  // (the c-th of the outputs: the tokens', then the largest entries')
+  auto index_of = [&](int c) { return c < given ? p.tokens[row * p.count + c] : p.top_tokens[row * p.top + c - given]; };
+  auto gradient_of = [&](int c) { return c < given ? p.g_tokens[row * p.count + c] : p.g_top[row * p.top + c - given]; };
   float total = 0.f;
-  auto mark = [&](int64_t index) {
-    const int64_t at = index - e0;
-    if (at >= 0 && at < (int64_t)NT * p.vecs * N) atomicOr(&hit[at / 32], 1u << (at % 32));
+  // (which of the part's entries an index is; -1: none)
+  auto place_in = [&](int64_t index) { return index >= 0 && index < p.vocab && index >= e0 && index - e0 < entries ? (int)(index - e0) : -1; };
+  auto mark = [&](int c) {
+    const int64_t index = index_of(c);
+    const int at = place_in(index);
+    const float g = index < 0 ? 0.f : index < p.vocab ? gradient_of(c) : __builtin_nanf("");
+    total += g;
+    if (at >= 0) {
+      const uint32_t bit = 1u << (at % 32);
+      if (atomicOr(&hit[at / 32], bit) & bit) {
+        atomicOr(&several[at / 32], bit);
+        repeated = 1;
+      }
+    }
+    if (c < LIST) { list[c] = at; gradient[c] = g; }
+    return at;
   };
-  if (p.g_tokens)
-    for (int c = threadIdx.x; c < p.count; c += NT) {
-      const int64_t token = p.tokens[row * p.count + c];
-      if (token < 0) continue;
-      total += token < p.vocab ? p.g_tokens[row * p.count + c] : __builtin_nanf("");
-      mark(token);
-    }
-  if (p.g_top)
-    for (int c = threadIdx.x; c < p.top; c += NT) {
-      total += p.g_top[row * p.top + c];
-      mark(p.top_tokens[row * p.top + c]);
-    }
+  // (the thread's first one outside the loop: its logit is on its way from here on)
+  int mine = -1;
+  float early = 0.f;
+  if (threadIdx.x < asked) mine = mark(threadIdx.x);
+  if (mine >= 0) early = logit_at<F32>(p, row, e0 + mine);
+  for (int c = threadIdx.x + NT; c < asked; c += NT) mark(c);
+  for (int c = asked + threadIdx.x; c < LIST && c < (asked + 7) / 8 * 8; c += NT) { list[c] = -1; gradient[c] = 0.f; }
   total = block_reduce<NT>(total, sums, add);
   __syncthreads();
   const float m = p.stats[row * 3], log_s = p.stats[row * 3 + 1], entropy = p.stats[row * 3 + 2];
   const float ge = p.g_entropy ? p.g_entropy[row] : 0.f;
+  auto rest_of = [&](float x) {
+    const float lp = (x - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
+    return p.g_entropy ? -pr * __builtin_fmaf(ge, fmaxf(lp, -1e4f) + entropy, total) : -pr * total;      // (-inf times its 0 is nothing)
+  };
   char* const out = (char*)p.d_logits + row * p.d_stride * SIZE;
+  auto put = [&](int64_t e, float y) {
+    if constexpr (F32) ((float*)out)[e] = y;
+    else ((bf16_t*)out)[e] = (bf16_t)y;
+  };
+  // Entries with gradients of their own are written by the first output that asks for them, with the others' in their order, and the rest
+  // below.  (Entry by entry, each looking through all outputs, 100 tokens of 2000 rows of 10000 took 183 us.)
+  const bool dense = asked > 2 * NT;     // (so many that they are worth a list of those that look through the others)
+  auto one = [&](int at) { return (several[at / 32] >> (at % 32) & 1u) == 0; };
+  for (int c = threadIdx.x; c < asked; c += NT) {
+    const int at = c < NT ? mine : c < LIST ? list[c] : place_in(index_of(c));
+    if (at < 0) continue;
+    if (one(at)) put(e0 + at, rest_of(c < NT ? early : logit_at<F32>(p, row, e0 + at)) + (c < LIST ? gradient[c] : gradient_of(c)));
+    else if (dense && c < LIST) queue[atomicAdd(&queued, 1)] = (uint16_t)c;
+  }
+  if (repeated) {
+    if (dense) __syncthreads();
+    const int listed = asked < LIST ? (asked + 7) / 8 * 8 : LIST, n = dense ? queued : 0, rest = dense ? LIST : 0;
+    for (int i = threadIdx.x; i < n || i - n + rest < asked; i += NT) {
+      const int c = i < n ? queue[i] : i - n + rest, at = c < LIST ? list[c] : place_in(index_of(c));
+      if (at < 0 || one(at)) continue;
+      float own = c < LIST ? gradient[c] : gradient_of(c);
+      bool first = true;
+      for (int k0 = 0; k0 < listed; k0 += 8) {
+        int l[8];
+        float g[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { l[k] = list[k0 + k]; g[k] = gradient[k0 + k]; }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool met = l[k] == at && k0 + k != c;
+          own += met ? g[k] : 0.f;
+          first &= !met || k0 + k > c;
+        }
+      }
+      for (int k = LIST; k < asked; ++k) {
+        if (k == c || place_in(index_of(k)) != at) continue;
+        own += gradient_of(k);
+        first &= k > c;
+      }
+      if (first) put(e0 + at, rest_of(logit_at<F32>(p, row, e0 + at)) + own);
+    }
+  }
   const bool apart = (((uintptr_t)out ^ (uintptr_t)((const char*)p.logits + row * p.stride * SIZE)) & 15u) != 0;
 #pragma unroll
   for (int c = 0; c < VECS; ++c) {
     const int v = v0 + c * NT + threadIdx.x;
     if (c >= p.vecs || v >= r.vectors) continue;
     float y[N];
-    if (p.g_entropy) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float lp = (x[c].at(i) - m) - log_s, pr = __builtin_amdgcn_exp2f(lp * LOG2E);
-        y[i] = -pr * __builtin_fmaf(ge, fmaxf(lp, -1e4f) + entropy, total);      // (-inf times its 0 is nothing)
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = -__builtin_amdgcn_exp2f(((x[c].at(i) - m) - log_s) * LOG2E) * total;
-    }
+    for (int i = 0; i < N; ++i) y[i] = rest_of(x[c].at(i));
     const int e = r.first(v), at = (c * NT + threadIdx.x) * N;
-    uint32_t mine = hit[at / 32] >> (at % 32) & ((1u << N) - 1u);
-    while (mine) {
-      const int i = __builtin_ctz(mine);
-      mine &= mine - 1;
-      float more = 0.f;
-      if (p.g_tokens)
-        for (int k = 0; k < p.count; ++k)
-          if (p.tokens[row * p.count + k] == e + i) more += p.g_tokens[row * p.count + k];
-      if (p.g_top)
-        for (int k = 0; k < p.top; ++k)
-          if (p.top_tokens[row * p.top + k] == e + i) more += p.g_top[row * p.top + k];
-#pragma unroll
-      for (int n = 0; n < N; ++n) y[n] += n == i ? more : 0.f;
-    }
-    if (r.whole(v) && !apart) {
+    const uint32_t taken = hit[at / 32] >> (at % 32) & ((1u << N) - 1u);
+    if (r.whole(v) && !apart && taken == 0) {
       uint4 w;
       if constexpr (F32) w = __builtin_bit_cast(uint4, floatx4{y[0], y[1], y[2], y[3]});
       else w = uint4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
@@ -554,10 +598,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_backward(const Params p) {
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (e + i >= 0 && e + i < p.vocab) {
-          if constexpr (F32) ((float*)out)[e + i] = y[i];
-          else ((bf16_t*)out)[e + i] = (bf16_t)y[i];
-        }
+        if (e + i >= 0 && e + i < p.vocab && !(taken >> i & 1u)) put(e + i, y[i]);
     }
   }
 }

@@ -310,3 +310,38 @@ def test_a_large_gradient_of_the_entropy_beside_masked_entries(gpu, dtype):
   d = torch.autograd.grad(recml_amd.token_log_probs(x, entropy=True).entropy, x, torch.full((2,), 2.0**40).cuda())[0]
   one = torch.autograd.grad(recml_amd.token_log_probs(x, entropy=True).entropy, x, torch.ones(2).cuda())[0]
   assert torch.equal(d, one * 2.0**40) and not d[0, 5:30].any() and d.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,vocab,count,top", [(3, 29, 100, 5), (2, 300, 129, 0), (2, 300, 700, 16), (2, 700, 513, 50), (3, 9001, 1000, 50), (2, 20011, 1500, 100), (1, 5000, 3001, 256)])
+def test_gradients_of_many_tokens(gpu, rows, vocab, count, top, dtype):
+  """More tokens a row than a workgroup has threads and than it lists, many of them the same: each entry gets the sum of its own in their order."""
+  x = _logits(rows, vocab, dtype, vocab + 3)
+  tokens = torch.randint(-1, vocab, (rows, count), generator=_gen(2))
+  tokens[:, 5:9] = tokens[:, 3:4]
+  tokens[:, -1] = tokens[:, 3]
+  g = [torch.randn(s, generator=_gen(3 + i)) for i, s in enumerate([(rows, count), (rows,), (rows, top)])]
+  xs = x.cuda().requires_grad_(True)
+  def run():
+    got = recml_amd.token_log_probs(xs, tokens.cuda(), top=top, entropy=True)
+    return torch.autograd.grad([got.log_probs, got.entropy] + ([got.top_log_probs] if top else []), xs, [t.cuda() for t in g[: 3 if top else 2]])[0].cpu()
+  d = run()
+  assert torch.equal(d, run())
+  want = R.log_probs(x, tokens, top, *(g if top else g[:2]))
+  lp, inner = want[5], want[6]
+  p = lp.exp()
+  # an entry's own gradients: as many roundings of partial sums up to their size as it has; the rest as in test_gradient
+  size = sum(t.double().abs().reshape(rows, -1).sum(-1, keepdim=True) for t in g)
+  off = 8 * STEP * lp.abs().nan_to_num(posinf=0) + 3 * _sums_off(vocab)
+  tol = p * (inner.abs() * off + size * (8 * _sums_off(vocab) * (1 + math.log(vocab + 1)))) + 4 * STEP * (size * p + want[4].abs()) + 2.0**-132
+  tol = tol + torch.finfo(dtype).eps / 2 * want[4].abs() + STEP * (count + top) * size * p
+  ids = tokens.clamp(min=0)
+  mine = torch.zeros((rows, vocab), dtype=torch.float64)
+  mine.scatter_add_(1, ids, g[0].double().abs() * (tokens >= 0))
+  times = torch.zeros((rows, vocab), dtype=torch.float64).scatter_add_(1, ids, (tokens >= 0).double())
+  if top:
+    mine.scatter_add_(1, want[3], g[2].double().abs())
+    times.scatter_add_(1, want[3], torch.ones_like(g[2].double()))
+  tol = tol + STEP * times * mine
+  bad = (d.double() - want[4]).abs() > tol
+  assert not bad.any(), (float((d.double() - want[4]).abs().max()), int(bad.sum()))
