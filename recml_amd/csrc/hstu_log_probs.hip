@@ -335,7 +335,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
   }
   if constexpr (!TOP) return;
   __shared__ Chosen<NT == 64 ? 256 : 1024> chosen;
-  constexpr int HELD = NT == 64 ? 64 : 512;                    // vectors with entries that reach the bound
+  constexpr int HELD = NT == 64 ? 192 : 512;                   // vectors with entries that reach the bound
   __shared__ uint4 held[HELD];
   __shared__ int32_t held_at[HELD];
   // a part shorter than `top` gives what it has
@@ -609,8 +609,10 @@ struct Split { int nt, vecs, parts; };
 Split split_of(const HstuLogProbsArgs& a) {
   const int64_t n = a.dtype == HSTU_SERVE_FP32 ? 4 : 8, vectors = ((int64_t)a.vocab + n - 1 + n - 1) / n;   // (a row may start anywhere)
   Split s;
-  // (a wave for short rows: its 64 maxima bound a few of their largest entries well)
-  s.nt = vectors <= 64 * VECS && a.top <= 16 ? 64 : 256;
+  // a wave for short rows where there are enough of them to fill the chip, four waves otherwise: forward and backward of 16000 rows of 2000
+  // (bf16) with the 10 largest 27 + 35 us against 62 + 49, of 100 rows 11 + 6 against 7 + 6.  Its 64 maxima bound up to 50 of a row's largest
+  // entries well: 100 of them reach the bound, with 60 it is 180.
+  s.nt = vectors <= 64 * VECS && (a.rows >= 1024 ? a.top <= 50 : vectors <= 128 && a.top <= 16) ? 64 : 256;
   int64_t parts = (vectors + (int64_t)s.nt * VECS - 1) / ((int64_t)s.nt * VECS);
   // few rows: more parts, so that they fill the chip, while the join holds all of a row's largest entries at once
   while (a.rows * parts < 256 && parts * s.nt * 2 <= vectors && 2 * parts * a.top <= 2048) parts *= 2;
