@@ -265,19 +265,31 @@ __device__ __forceinline__ float logit_at(const Params& p, int64_t row, int64_t 
   else return (float)((const bf16_t*)p.logits)[at];
 }
 
+// A thread's first token of a row and its logit, asked for ahead of the sums.
+struct First { int64_t token; float logit; };
+
+template <bool F32>
+__device__ __forceinline__ First first_of(const Params& p, int64_t row) {
+  First f = {-1, 0.f};
+  if ((int)threadIdx.x < p.count) f.token = p.tokens[row * p.count + threadIdx.x];
+  if (f.token >= 0 && f.token < p.vocab) f.logit = logit_at<F32>(p, row, f.token);
+  return f;
+}
+
 // What is asked of a row once its sums are known.
 template <bool F32, int NT>
-__device__ __forceinline__ void finish(const Params& p, int64_t row, float m, float s, float t) {
+__device__ __forceinline__ void finish(const Params& p, int64_t row, float m, float s, float t, const First& first) {
   const float log_s = __logf(s), entropy = entropy_of(log_s, s, t);
   if (threadIdx.x == 0) {
     if (p.stats) { p.stats[row * 3] = m; p.stats[row * 3 + 1] = log_s; p.stats[row * 3 + 2] = entropy; }
     if (p.entropy) p.entropy[row] = entropy;
   }
   for (int c = threadIdx.x; c < p.count; c += NT) {
-    const int64_t token = p.tokens[row * p.count + c];
+    const bool early = c < NT;
+    const int64_t token = early ? first.token : p.tokens[row * p.count + c];
     float y = 0.f;                                             // (nothing asked)
     if (token >= p.vocab) y = __builtin_nanf("");
-    else if (token >= 0) y = (logit_at<F32>(p, row, token) - m) - log_s;
+    else if (token >= 0) y = ((early ? first.logit : logit_at<F32>(p, row, token)) - m) - log_s;
     p.log_probs[row * p.count + c] = y;
   }
 }
@@ -331,7 +343,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
   const bool odd = s != s;             // (the thread holds a NaN, or +inf)
   s = block_reduce<NT>(s, sums, add);
   if (p.parts == 1) {
-    finish<F32, NT>(p, row, m, s, t);
+    finish<F32, NT>(p, row, m, s, t, first_of<F32>(p, row));     // (earlier, it costs a wave a SIMD)
   } else if (threadIdx.x == 0) {
     float* to = p.part_stats + (row * p.parts + part) * 3;
     to[0] = m; to[1] = s; to[2] = t;
@@ -415,6 +427,23 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
   __shared__ int32_t best_index[TOP];
   const int64_t row = blockIdx.x;
   const float* from = p.part_stats + row * p.parts * 3;
+  // (a row is a chain of latencies: what does not depend on the sums is asked for ahead of them)
+  const int64_t base = row * p.parts * p.top, total = (int64_t)p.parts * p.top;
+  float x[E];
+  int index[E];
+  auto fetch = [&](int64_t done, int have, int take) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = e * NT + threadIdx.x - have;
+      if (i < 0) continue;
+      index[e] = -1;
+      x[e] = 0.f;
+      if (i < take) { index[e] = p.part_index[base + done + i]; x[e] = p.part_value[base + done + i]; }
+    }
+  };
+  int take = total < NT * E ? (int)total : NT * E;
+  fetch(0, 0, take);
+  const First first = first_of<F32>(p, row);
   float m = -__builtin_inff();
   for (int i = threadIdx.x; i < p.parts; i += NT) m = fmaxf(m, from[3 * i]);
   m = block_reduce<NT>(m, sums, larger);
@@ -428,25 +457,21 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
   }
   s = block_reduce<NT>(s, sums, add);
   t = block_reduce<NT>(t, sums, add);
-  finish<F32, NT>(p, row, m, s, t);
+  finish<F32, NT>(p, row, m, s, t, first);
   if (p.top == 0) return;
   const float log_s = __logf(s);
-  const int64_t base = row * p.parts * p.top, total = (int64_t)p.parts * p.top;
   int have = 0;                        // the best of the entries so far, in LDS
   for (int64_t done = 0; done < total;) {
-    const int room = NT * E - have;
-    const int take = total - done < room ? (int)(total - done) : room;
-    float x[E];
-    int index[E];
+    if (done > 0) {
+      take = total - done < NT * E - have ? (int)(total - done) : NT * E - have;
+      fetch(done, have, take);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = e * NT + threadIdx.x;
-      index[e] = -1;
-      x[e] = 0.f;
-      if (i < have) { x[e] = best_value[i]; index[e] = best_index[i]; }
-      else if (i < have + take) { index[e] = p.part_index[base + done + i - have]; if (index[e] >= 0) x[e] = p.part_value[base + done + i - have]; }
+      for (int e = 0; e < E; ++e) {
+        const int i = e * NT + threadIdx.x;
+        if (i < have) { x[e] = best_value[i]; index[e] = best_index[i]; }
+      }
+      __syncthreads();
     }
-    __syncthreads();
     float there = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) there += index[e] >= 0 ? 1.f : 0.f;

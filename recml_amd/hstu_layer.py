@@ -12,6 +12,9 @@ backward regenerate the same keep pattern from a seed drawn per call), and the m
 entries with torch's dropout; in eval mode neither does anything.  Parameters are created frozen:
 `requires_grad_(True)` makes them trainable.
 
+For serving, HSTU.new_cache, prefill and extend keep users' histories (hstu_serving.HSTUCache, hstu_cache_ops) and run the
+model on new events alone; HSTU.log_probs scores items under the head, differentiably (hstu_scores).
+
 Mirrors, name for name:
   HSTUBlock   recml/layers/keras/hstu.py:240-474 (weights :281-354, call :422-474)
   HSTU        recml/layers/keras/hstu.py:492-621 (call :585-621)
