@@ -26,11 +26,6 @@ namespace {
 
 using bf16_bits = uint16_t;
 
-bool capturing(void* stream) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing((hipStream_t)stream, &st) == hipSuccess && st != hipStreamCaptureStatusNone;
-}
-
 // ---------------------------------------------------------------------------
 // arguments
 // ---------------------------------------------------------------------------

@@ -12,6 +12,7 @@
 #include <limits>
 #include <memory>
 #include <mutex>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -366,6 +367,28 @@ struct LogProbsBackward : public torch::autograd::Node {
   }
 };
 
+// A backward pass into a graph waits for the streams of the leaves' accumulators.  Those that an eager graph of the same leaves made, and
+// keeps alive, belong to a stream that is not captured: the wait fails on the engine's thread and takes the process with it.
+void refuse_mixed_graphs(const Tensor& x) {
+  if (!capturing(stream_of(x))) return;
+  const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+  std::vector<torch::autograd::Node*> todo{torch::autograd::impl::gradient_edge(x).function.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    torch::autograd::Node* const node = todo.back();
+    todo.pop_back();
+    if (!node || !seen.insert(node).second) continue;
+    for (const auto& e : node->next_edges()) todo.push_back(e.function.get());
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) continue;
+    const auto stream = node->stream();
+    if (!stream || *stream == here) continue;
+    // (the default stream may not be asked while another is captured)
+    void* const other = (void*)c10::hip::HIPStreamMasqueradingAsCUDA(*stream).stream();
+    TORCH_CHECK_VALUE(other && capturing(other),
+                      "token_log_probs is captured with a gradient while an eager graph of the same leaves lives: let go of its outputs first");
+  }
+}
+
 // token_log_probs(logits, tokens, top, entropy, differentiable) -> (log_probs, entropy, top_log_probs, top_tokens), each a tensor or None;
 // or None
 PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t count) {
@@ -376,7 +399,9 @@ PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t count) {
   return guarded([&]() -> PyObject* {
     Tensor x, tokens;
     int64_t top, rows, stride;
-    if (!tensor_arg(a[0], &x) || !tensor_arg(a[1], &tokens) || !x.defined() || !long_arg(a[2], &top) || !logits_rows(x, &rows, &stride)) Py_RETURN_NONE;
+    if (!tensor_arg(a[0], &x) || !x.defined()) Py_RETURN_NONE;
+    if (x.is_cuda() && wants_grad({&x})) refuse_mixed_graphs(x);
+    if (!tensor_arg(a[1], &tokens) || !long_arg(a[2], &top) || !logits_rows(x, &rows, &stride)) Py_RETURN_NONE;
     if (a[3] != Py_True && a[3] != Py_False) Py_RETURN_NONE;
     const bool entropy = a[3] == Py_True;
     const int64_t V = x.size(-1);

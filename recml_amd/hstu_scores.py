@@ -105,7 +105,8 @@ def token_log_probs(logits, tokens=None, *, top: int = 0, entropy: bool = False)
     entropy: whether to return the rows' entropy, -sum p log p.
 
   Entries of -inf are tokens that cannot occur.  A row with a NaN, with +inf, or with nothing but -inf is NaN throughout.
-  Differentiable in the logits, through log_probs, entropy and top_log_probs."""
+  Differentiable in the logits, through log_probs, entropy and top_log_probs.  Captured into a graph with a gradient, it raises where an
+  eager graph of the same leaves lives: their accumulators are not the captured stream's, and the backward pass would end the process."""
   got = _native.token_log_probs(logits, tokens, top, entropy, True)
   if got is not None:
     return TokenLogProbs(*got)

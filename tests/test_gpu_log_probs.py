@@ -345,3 +345,40 @@ def test_gradients_of_many_tokens(gpu, rows, vocab, count, top, dtype):
   tol = tol + STEP * times * mine
   bad = (d.double() - want[4]).abs() > tol
   assert not bad.any(), (float((d.double() - want[4]).abs().max()), int(bad.sum()))
+
+
+def test_a_captured_backward_beside_an_eager_graph_is_refused(gpu):
+  """The leaves' accumulators of an eager graph that lives belong to a stream that is not captured.  Refused before the engine meets it,
+  through the operator's own leaf and through one further up; without the eager graph the same step is captured and replayed."""
+  ids = torch.tensor([3, 4, 5]).cuda()
+  h = torch.randn((3, 16), generator=_gen(1)).cuda()
+  w = (torch.randn((16, 40), generator=_gen(2))).cuda().requires_grad_(True)
+  x = torch.randn((3, 40), generator=_gen(3)).cuda().requires_grad_(True)
+  one = torch.ones(3).cuda()
+  for leaf, logits in ((x, lambda: x), (w, lambda: h @ w)):
+    def step():
+      return torch.autograd.grad(recml_amd.token_log_probs(logits(), ids).log_probs, leaf, one)[0]
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+      step()
+    torch.cuda.current_stream().wait_stream(s)
+    lives = recml_amd.token_log_probs(logits(), ids)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      h.clone()
+      with pytest.raises(ValueError, match="eager graph"):
+        recml_amd.token_log_probs(logits(), ids)
+      with torch.no_grad():
+        recml_amd.token_log_probs(logits(), ids)
+    del lives, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      got = step()
+    for _ in range(3):
+      got.zero_()
+      graph.replay()
+      assert torch.equal(step(), want)
+      torch.cuda.synchronize()
+      assert torch.equal(got, want)
