@@ -10,7 +10,7 @@
 // again.  Rows that are longer are split; a second kernel joins the parts in their order.  Memory bounds all of it where there is much:
 // 8192 rows of 100000 in bf16, with the entropy, forward in 305 us (5.4 TB/s) and the join in 7, backward in 600 (5.5 TB/s, as much
 // written as read; both streams go past the caches, through them the three took 920 together and 850 so).  Few rows are chains of
-// latencies: one of a million with its 10 largest 7.9 us and 8.0 for the join.
+// latencies: one of a million with its 10 largest 7.7 us and 5.5 for the join.
 //
 // The largest entries of a part: the k-th largest of the threads' maxima bounds the k-th largest entry from below, few entries
 // reach it, and each of those finds its rank by counting who comes before it (by value, then by index).  The bound comes from
