@@ -206,8 +206,8 @@ def kv_write(pages, k, v, page_table, starts, *, offsets=None, max_new=None) -> 
 
 def kv_read(pages, page_table, starts, *, count=None, offsets=None, max_new=None, total=None, dtype=torch.bfloat16):
   """The keys and values that the pages stand for: (k, v), [B, count, H, d] from place starts[b] on, or packed
-  [total, H, d] with `offsets` [B + 1] and `max_new` (rows of no sequence are not written).  Exact in bfloat16 and float32.
-  Places without a page read as zeros."""
+  [total, H, d] with `offsets` [B + 1] and `max_new` (rows of no sequence are not written).  Exact in float32, and in bfloat16
+  down to its smallest values.  Places without a page read as zeros."""
   if dtype is torch.bfloat16 or dtype is torch.float32:
     got = _native.kv_read(pages, page_table, starts, count, offsets, max_new, total, dtype is torch.float32)
     if got is not None:
