@@ -162,9 +162,9 @@ __device__ __forceinline__ void kth_of_wave(uint32_t key, int j, int k, uint32_t
 }
 
 // The k entries themselves, where too many reach the bound: the k-th largest value bit by bit, then, among its equals, the index up
-// to which they belong to the k.
-template <int NT, typename C, typename Each>
-__device__ __forceinline__ void exactly(int k, C& c, Each each) {
+// to which they belong to the k.  Each bit is a pass over the entries: bf16's values have their upper 16 only, indices those of `vocab`.
+template <bool F32, int NT, typename C, typename Each>
+__device__ __forceinline__ void exactly(int k, int vocab, C& c, Each each) {
   constexpr int W = NT / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   auto count = [&](auto counts) {
@@ -184,14 +184,15 @@ __device__ __forceinline__ void exactly(int k, C& c, Each each) {
   };
   uint32_t value = 0;
 #pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= (F32 ? 0 : 16); --bit) {
     const uint32_t next = value | 1u << bit;
     if (count([&](uint32_t o, int) { return o >= next; }) >= k) value = next;
   }
+  if (!F32 && (value < 0x80000000u || value == 0xffff0000u)) value |= 0xffffu;      // (negative ones' lower bits, and a NaN's)
   const int ties = k - count([&](uint32_t o, int) { return o > value; });
   int below = 0;                           // the largest index with fewer than `ties` equals below it
 #pragma unroll 1
-  for (int bit = 30; bit >= 0; --bit) {
+  for (int bit = 31 - __builtin_clz(vocab); bit >= 0; --bit) {
     const int next = below | 1 << bit;
     if (count([&](uint32_t o, int index) { return o == value && index < next; }) < ties) below = next;
   }
@@ -212,8 +213,8 @@ __device__ __forceinline__ void exactly(int k, C& c, Each each) {
 // The k largest of the workgroup's entries, the r-th of them given to out(r, value, index).  `most`: the ordered bits of a
 // thread's largest entry (0: it has none; the least of an entry is that of -inf); collect(bound, reaches, push), called by all threads,
 // calls push(x, index) for the entries that reach the bound, each(f) f(x, index) for all of a thread's; there are at least k.
-template <int NT, typename C, typename Collect, typename Each, typename Out>
-__device__ __forceinline__ void select_top(int k, C& c, uint32_t most, Collect collect, Each each, Out out) {
+template <bool F32, int NT, typename C, typename Collect, typename Each, typename Out>
+__device__ __forceinline__ void select_top(int k, int vocab, C& c, uint32_t most, Collect collect, Each each, Out out) {
   constexpr int W = NT / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   // every wave has its share of the k, or one wave has all of them: either way k entries reach the bound.  (The shares bound well
@@ -241,7 +242,7 @@ __device__ __forceinline__ void select_top(int k, C& c, uint32_t most, Collect c
   __syncthreads();
   int n = c.n;
   if (n > C::CAP) {
-    exactly<NT>(k, c, each);
+    exactly<F32, NT>(k, vocab, c, each);
     n = k;
   }
   // who comes before an entry is its rank
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_part(const Params p) {
   if (p.parts > 1)
     for (int i = k + threadIdx.x; i < p.top; i += NT) p.part_index[to + i] = -1;
   if (k > 0)
-    select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int index) {
+    select_top<F32, NT>(k, p.vocab, chosen, most, collect, each, [&](int rank, float value, int index) {
       if (p.parts == 1) {
         p.top_log_probs[to + rank] = (value - m) - log_s;
         p.top_tokens[to + rank] = index;
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(NT) void hstu_log_probs_join(const Params p) {
       if (reaches) each([&](float y, int i) { if (ordered(y) >= bound) push(y, i); });
     };
     if (k > 0)
-      select_top<NT>(k, chosen, most, collect, each, [&](int rank, float value, int at) {
+      select_top<F32, NT>(k, p.vocab, chosen, most, collect, each, [&](int rank, float value, int at) {
         if (end) {
           p.top_log_probs[row * p.top + rank] = (value - m) - log_s;
           p.top_tokens[row * p.top + rank] = at;

@@ -382,3 +382,17 @@ def test_a_captured_backward_beside_an_eager_graph_is_refused(gpu):
       assert torch.equal(step(), want)
       torch.cuda.synchronize()
       assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(2, 700), (1100, 700), (2, 3001), (2, 40000)])
+def test_rows_of_one_value(gpu, rows, vocab, dtype):
+  """Everything ties: the lowest tokens, after the two that are larger; negative values, zeros of both signs, -inf and NaN."""
+  for value in (0.0, -0.0, -1.5, 2.75, -math.inf, math.nan):
+    x = torch.full((rows, vocab), value, dtype=dtype)
+    if value == value:
+      x[:, 650], x[:, 333] = 3.0, 4.0
+    got = recml_amd.token_log_probs(x.cuda(), top=20)
+    want = [333, 650, *range(18)] if value == value else list(range(20))
+    assert torch.equal(got.top_tokens.cpu(), torch.tensor(want).expand(rows, 20)), value
+    assert bool(got.top_log_probs.isnan().all()) == (value != value)
