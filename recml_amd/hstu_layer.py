@@ -373,7 +373,8 @@ class HSTUBlock(torch.nn.Module):
     place starts[b] on, and they attend to what the cache then holds of their user.
 
     tokens: [B, n, D], or packed [T, D] with `offsets` [B + 1] and `max_new`; lengths [B]: events of every user, the new ones included;
-    max_len: the length of the full call (the normaliser, the tables' extent); timestamps: the users' [B, max_len] kept times.
+    max_len: the length of the full call (the normaliser, the tables' extent); timestamps: the users' [B, max_len] kept times.  Rows at
+    places below 0 join nothing and attend to nothing.
     whole=True (packed rows): the new events are the whole histories and attend to their own keys and values as they are, through
     hstu_attention, with `timestamps` [T] the rows' own."""
     if self.training and self.dropout > 0.0:
@@ -667,7 +668,12 @@ class HSTU(torch.nn.Module):
     user's history up to itself.  Returns the model's outputs for the new events, [B, n, ...] or [T, ...]; token_log_probs makes log
     probabilities and the items to recommend of logits.  Nothing in here waits for the GPU: a step can be captured into a graph
     and replayed.  Events past cache.max_len are lost: they join nothing and attend to nothing.  So are a user's packed events past
-    `max_new`, and packed rows of no user: what comes back for those means nothing."""
+    `max_new`, and packed rows of no user: what comes back for those means nothing.
+
+    The outputs are forward's on the events so far, but for the rounding of the kept keys and values, whatever calls the events come in
+    by.  With timestamps and more than one block the last kept event of every user with new ones is run again for that (its time bias
+    reads the next event's time), and its keys and values are written again: two users may share the pages of a common beginning only if
+    it ends before either's last event."""
     B, dev = cache.batch, ids.device
     if offsets is None:
       if ids.dim() != 2 or ids.shape[0] != B:
@@ -678,6 +684,8 @@ class HSTU(torch.nn.Module):
     else:
       if ids.dim() != 1 or max_new is None or tuple(offsets.shape) != (B + 1,):
         raise ValueError(f"packed ids are [T] with `offsets` [{B + 1}] and `max_new`, got {tuple(ids.shape)} and {tuple(offsets.shape)}")
+      if int(max_new) < 0:
+        raise ValueError(f"max_new must not be negative, got {max_new}")
       offsets = offsets.to(torch.int32)
       ends = offsets.to(torch.int64).clamp(0, ids.shape[0])
       count = (ends[1:] - ends[:-1]).clamp(0, int(max_new)).to(torch.int32)
@@ -703,7 +711,10 @@ class HSTU(torch.nn.Module):
                        "forward_cached of its own too")
     if (ts_bias is None) != (timestamps is None):
       raise ValueError("Both or neither of `timestamps` and `ts_bias` must be provided.")
-    cache._note_times(timestamps, users, places)
+    cache._note(ids, timestamps, users, places)
+    last, packed, rows = not whole and cache.ids is not None and ids.numel() > 0, offsets is not None, None
+    if last:
+      ids, places, starts, offsets, max_new, rows = cache._with_last(ids, places, starts, lengths, offsets, max_new)
     table, positions, D = self.item_embedding, self.position_embedding, self.model_dim
     scale = D ** 0.5 if self.scale_by_sqrt_dim else 1.0
     at = None if positions is None else places.clamp(0, positions.shape[0] - 1).to(torch.int64)
@@ -717,5 +728,7 @@ class HSTU(torch.nn.Module):
     for block, pages in zip(self.decoder_blocks, cache.layers):
       x = block.forward_cached(x, pages, cache.page_table, lengths, starts, cache.max_len, offsets=offsets, max_new=max_new, pos_bias=pos_bias,
                                timestamps=timestamps if whole else cache.timestamps, ts_bias=ts_bias, whole=whole)
+    if last:
+      x = x[rows] if packed else x[:, 1:].contiguous()
     x = self._final_norm(x)
     return x if self.reverse_embedding is None else self._head(x)
