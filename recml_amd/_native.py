@@ -65,6 +65,6 @@ _FUNCTIONS = ("attention", "block", "blocks", "embed", "final_norm", "linear", "
 attention, block, blocks, embed, final_norm, linear, pack, mask_lengths, raised, norm_gate_bwd, has_room = (
     _first_call(n, _FUNCTIONS, lambda: _load("_native", _lib, _lib_block), _other_library) for n in _FUNCTIONS)
 
-_SERVE_FUNCTIONS = ("check_pages", "kv_write", "kv_read", "cached_attention", "token_log_probs")
-check_pages, kv_write, kv_read, cached_attention, token_log_probs = (
+_SERVE_FUNCTIONS = ("check_pages", "kv_write", "kv_read", "cached_attention", "token_log_probs", "accumulators")
+check_pages, kv_write, kv_read, cached_attention, token_log_probs, accumulators = (
     _first_call(n, _SERVE_FUNCTIONS, lambda: _load("_native_serve", _lib_serve), _other_serve_library) for n in _SERVE_FUNCTIONS)

@@ -367,26 +367,49 @@ struct LogProbsBackward : public torch::autograd::Node {
   }
 };
 
-// A backward pass into a graph waits for the streams of the leaves' accumulators.  Those that an eager graph of the same leaves made, and
-// keeps alive, belong to a stream that is not captured: the wait fails on the engine's thread and takes the process with it.
-void refuse_mixed_graphs(const Tensor& x) {
-  if (!capturing(stream_of(x))) return;
-  const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
-  std::vector<torch::autograd::Node*> todo{torch::autograd::impl::gradient_edge(x).function.get()};
+// Gives `f` every accumulator of a leaf that a backward pass from x would reach.  (A leaf's own is there for as long as
+// somebody holds it, and may be made for this walk: the edge is held until the end.)
+template <typename F>
+void each_accumulator(const Tensor& x, F&& f) {
+  const torch::autograd::Edge root = torch::autograd::impl::gradient_edge(x);
+  std::vector<torch::autograd::Node*> todo{root.function.get()};
   std::unordered_set<torch::autograd::Node*> seen;
   while (!todo.empty()) {
     torch::autograd::Node* const node = todo.back();
     todo.pop_back();
     if (!node || !seen.insert(node).second) continue;
     for (const auto& e : node->next_edges()) todo.push_back(e.function.get());
-    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node)) f(node);
+  }
+}
+
+// A backward pass into a graph waits for the streams of the leaves' accumulators.  Those that an eager graph of the same leaves made, and
+// keeps alive, belong to a stream that is not captured: the wait fails on the engine's thread and takes the process with it.
+void refuse_mixed_graphs(const Tensor& x) {
+  if (!capturing(stream_of(x))) return;
+  const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+  each_accumulator(x, [&](torch::autograd::Node* node) {
     const auto stream = node->stream();
-    if (!stream || *stream == here) continue;
+    if (!stream || *stream == here) return;
     // (the default stream may not be asked while another is captured)
     void* const other = (void*)c10::hip::HIPStreamMasqueradingAsCUDA(*stream).stream();
     TORCH_CHECK_VALUE(other && capturing(other),
                       "token_log_probs is captured with a gradient while an eager graph of the same leaves lives: let go of its outputs first");
+  });
+}
+
+// accumulators(tensor) -> how many leaves' accumulators a backward pass from it reaches
+PyObject* accumulators(PyObject*, PyObject* const* a, Py_ssize_t count) {
+  if (count != 1 || !THPVariable_Check(a[0])) {
+    PyErr_SetString(PyExc_TypeError, "accumulators takes a tensor");
+    return nullptr;
   }
+  return guarded([&]() -> PyObject* {
+    const Tensor x = THPVariable_Unpack(a[0]);
+    int64_t n = 0;
+    if (x.requires_grad()) each_accumulator(x, [&](torch::autograd::Node*) { ++n; });
+    return PyLong_FromLongLong(n);
+  });
 }
 
 // token_log_probs(logits, tokens, top, entropy, differentiable) -> (log_probs, entropy, top_log_probs, top_tokens), each a tensor or None;
@@ -473,6 +496,7 @@ PyMethodDef methods[] = {
     HSTU_FAST(kv_read, "The keys and values that pages stand for."),
     HSTU_FAST(cached_attention, "The attention of new events over a cache."),
     HSTU_FAST(token_log_probs, "Log probabilities of tokens (differentiable)."),
+    HSTU_FAST(accumulators, "How many leaves a backward pass from a tensor reaches."),
     {nullptr, nullptr, 0, nullptr},
 };
 
