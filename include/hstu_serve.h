@@ -124,7 +124,8 @@ int hstu_cached_attn(const HstuCachedAttnArgs* args, void* stream);
  *   top_log_probs, top_tokens: the `top` largest entries (at most 256) in falling order, ties by the lower token; NaN
  *                  comes before all others
  * A row whose sum of exponentials is not finite and positive (a NaN, +inf, nothing but -inf) has NaN for all of them.
- * stats: [rows][3], what the backward needs (or null).
+ * stats: [rows][3], what the backward needs (or null); for a backward with g_entropy the forward has to have `entropy` too (its sum is
+ * made for that alone: without it such a backward's rows are NaN).
  * The backward writes d_logits (typed like the logits) = sum over the outputs of their gradients times theirs by the
  * logits: g_tokens [rows][count], g_entropy [rows], g_top [rows][top], each or null; tokens, top_tokens and stats as the
  * forward had and left them.  The same token twice gets both gradients; negative tokens none; one past the vocabulary

@@ -53,7 +53,7 @@ struct Params {
   int64_t d_stride;
   int64_t rows;
   int32_t vocab, count, top, parts, vecs;
-  int32_t sums_t;                    // the entropy is wanted, now or by the backward
+  int32_t sums_t;                    // the entropy is wanted
 };
 
 // ordered bits: larger floats have larger ones, any NaN the largest; -0 and 0 are one value
@@ -280,7 +280,8 @@ __device__ __forceinline__ First first_of(const Params& p, int64_t row) {
 // What is asked of a row once its sums are known.
 template <bool F32, int NT>
 __device__ __forceinline__ void finish(const Params& p, int64_t row, float m, float s, float t, const First& first) {
-  const float log_s = __logf(s), entropy = entropy_of(log_s, s, t);
+  // (NaN where t was not summed: a backward that asks for the entropy's part all the same shows it)
+  const float log_s = __logf(s), entropy = p.sums_t ? entropy_of(log_s, s, t) : __builtin_nanf("");
   if (threadIdx.x == 0) {
     if (p.stats) { p.stats[row * 3] = m; p.stats[row * 3 + 1] = log_s; p.stats[row * 3 + 2] = entropy; }
     if (p.entropy) p.entropy[row] = entropy;

@@ -396,3 +396,36 @@ def test_rows_of_one_value(gpu, rows, vocab, dtype):
     want = [333, 650, *range(18)] if value == value else list(range(20))
     assert torch.equal(got.top_tokens.cpu(), torch.tensor(want).expand(rows, 20)), value
     assert bool(got.top_log_probs.isnan().all()) == (value != value)
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 70), (1100, 90), (2, 40000)])
+def test_statistics_without_the_entropy(gpu, rows, vocab):
+  """From C: a forward without an entropy serves a backward without its gradient; one with it is told so by NaN, never by another number."""
+  import ctypes as C
+  from recml_amd import _lib_serve
+  lib = _lib_serve.load()
+  x = _logits(rows, vocab, F32, 3).cuda()
+  ids = torch.randint(0, vocab, (rows, 1), generator=_gen(1)).cuda()
+  ones = torch.ones(rows).cuda()
+  def run(entropy, g_tokens, g_entropy):
+    lp, ent, stats, d = torch.empty(rows).cuda(), torch.empty(rows).cuda(), torch.full((rows, 3), 7.0).cuda(), torch.full((rows, vocab), 7.0).cuda()
+    a = _lib_serve.HstuLogProbsArgs()
+    a.struct_size, a.version = C.sizeof(a), _lib_serve.ABI_VERSION
+    a.logits, a.rows, a.stride, a.vocab, a.dtype, a.count = x.data_ptr(), rows, vocab, vocab, _lib_serve.FP32, 1
+    a.tokens, a.log_probs, a.stats, a.entropy = ids.data_ptr(), lp.data_ptr(), stats.data_ptr(), ent.data_ptr() if entropy else None
+    work = torch.empty(max(16, lib.hstu_log_probs_workspace_bytes(C.byref(a))), dtype=torch.uint8).cuda()
+    a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.hstu_log_probs_fwd(C.byref(a), stream) == 0
+    a.d_logits, a.d_stride = d.data_ptr(), vocab
+    a.g_tokens, a.g_entropy = ones.data_ptr() if g_tokens else None, ones.data_ptr() if g_entropy else None
+    assert lib.hstu_log_probs_bwd(C.byref(a), stream) == 0
+    torch.cuda.synchronize()
+    return d
+  xs = x.clone().requires_grad_(True)
+  got = recml_amd.token_log_probs(xs, ids, entropy=True)
+  plain = torch.autograd.grad(got.log_probs, xs, torch.ones_like(got.log_probs), retain_graph=True)[0]
+  both = torch.autograd.grad([got.log_probs, got.entropy], xs, [torch.ones_like(got.log_probs), ones])[0]
+  assert torch.equal(run(False, True, False), plain) and torch.equal(run(True, True, False), plain)
+  assert torch.equal(run(True, True, True), both)
+  assert run(False, True, True).isnan().all() and run(False, False, True).isnan().all()
