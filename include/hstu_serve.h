@@ -117,7 +117,8 @@ typedef struct HstuCachedAttnArgs {
 size_t hstu_cached_attn_workspace_bytes(const HstuCachedAttnArgs* args);
 int hstu_cached_attn(const HstuCachedAttnArgs* args, void* stream);
 
-/* Of each of `rows` rows of `vocab` logits (bf16 or fp32, row stride in elements, any alignment of the type):
+/* Of each of `rows` rows of `vocab` logits (bf16 or fp32, row stride in elements, any alignment of the type; at
+ * most 2^30 of them, and of `count` tokens, a row):
  *   log_probs[row][c] = x[tokens[row][c]] - ln sum_j exp x_j; 0 where the token is negative (nothing asked), NaN where it
  *                  is past the vocabulary
  *   entropy[row]   = -sum_j p_j ln p_j (or null)

@@ -656,7 +656,8 @@ int check(const HstuLogProbsArgs* a) {
   if (a->struct_size != sizeof(HstuLogProbsArgs) || a->version != HSTU_SERVE_ABI_VERSION)
     return serve_fail(HSTU_SERVE_ERR_VERSION, "struct_size %u version %u, expected %zu and %d", a->struct_size, a->version, sizeof(HstuLogProbsArgs), HSTU_SERVE_ABI_VERSION);
   if (a->dtype != HSTU_SERVE_BF16 && a->dtype != HSTU_SERVE_FP32) return serve_fail(HSTU_SERVE_ERR_SHAPE, "dtype %d", a->dtype);
-  if (a->rows < 0 || a->vocab < 1 || a->vocab > 1 << 30 || a->count < 0) return serve_fail(HSTU_SERVE_ERR_SHAPE, "rows=%lld vocab=%d count=%d", (long long)a->rows, a->vocab, a->count);
+  // (a thread's next token, and the tokens and the largest entries together, are counted in 32 bits)
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > 1 << 30 || a->count < 0 || a->count > 1 << 30) return serve_fail(HSTU_SERVE_ERR_SHAPE, "rows=%lld vocab=%d count=%d (each row's at most 2^30)", (long long)a->rows, a->vocab, a->count);
   if (a->top < 0 || a->top > MAX_TOP || a->top > a->vocab) return serve_fail(HSTU_SERVE_ERR_SHAPE, "top=%d: at most %d and the vocabulary", a->top, MAX_TOP);
   return HSTU_SERVE_OK;
 }

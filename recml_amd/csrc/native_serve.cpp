@@ -438,7 +438,7 @@ PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t count) {
       for (int64_t i = 0; i < lead; ++i)
         if (tokens.size(i) != x.size(i)) Py_RETURN_NONE;
       per_row = tokens.dim() == lead ? 1 : tokens.size(lead);
-      if (per_row > MOST) Py_RETURN_NONE;
+      if (per_row > 1 << 30) Py_RETURN_NONE;
     }
     const bool graph = wants_grad({&x});
     Tensor lp, ent, stats, tl, ti;

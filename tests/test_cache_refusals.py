@@ -151,3 +151,13 @@ def test_more_threads_than_a_launch_has_are_refused():
   small = dict(vocab=16, stride=16, top=0, workspace=0x10, workspace_bytes=1 << 40)
   for change in (dict(small, rows=1 << 26), dict(small, vocab=16384, stride=16384, rows=1 << 24)):
     assert lib.hstu_log_probs_fwd(C.byref(_score_args(**change)), None) == -4 and "too many" in lib.hstu_serve_last_error().decode()
+
+
+def test_more_tokens_a_row_than_the_kernels_count_are_refused():
+  """2^30 of them at most: a thread's next token, and the tokens and largest entries together, are counted in 32 bits."""
+  lib = _lib_serve.load()
+  for count in ((1 << 30) + 1, (1 << 31) - 1):
+    for fn in (lib.hstu_log_probs_fwd, lib.hstu_log_probs_bwd):
+      assert fn(C.byref(_score_args(count=count, logits=None)), None) == -4 and "count" in lib.hstu_serve_last_error().decode()
+    assert lib.hstu_log_probs_workspace_bytes(C.byref(_score_args(count=count))) == 0
+  assert lib.hstu_log_probs_fwd(C.byref(_score_args(count=1 << 30, logits=None)), None) == -1
