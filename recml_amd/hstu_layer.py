@@ -197,7 +197,7 @@ class HSTUBlock(torch.nn.Module):
     return dict(dropout_p=self.dropout, dropout_seed=int(dropout_seed))
 
   def forward(self, inputs, *, seq_lens=None, pos_bias=None, timestamps=None, ts_bias=None,
-              attention_mask=None, attention_bias=None, batch=None, dropout_seed=None):
+              attention_mask=None, attention_bias=None, batch=None, dropout_seed=None, kept=None):
     """inputs [B, L, D] -> [B, L, D].
 
     Give `seq_lens` [B] (keys and rows at or past the length are masked, as
@@ -206,8 +206,11 @@ class HSTUBlock(torch.nn.Module):
     [B, L, L] and optional `attention_bias` [B, L, L]
     (recml/layers/keras/hstu.py:422-440), beside which lengths and tables are not looked at.  `batch`: an `hstu_ops.AttentionBatch` shared with the
     other blocks that see the same lengths, timestamps and tables.  `dropout_seed`: in training mode
-    with a dropout rate, the seed of this call's keep pattern (default: drawn from torch's generator).
+    with a dropout rate, the seed of this call's keep pattern (default: drawn from torch's generator).  `kept`: forward_cached's
+    other arguments, (args, kwargs); it is then what is called (serving comes by here where the block has hooks).
     """
+    if kept is not None:
+      return self.forward_cached(inputs, *kept[0], **kept[1])
     drop = self._dropout_kw(dropout_seed)
     B, L, D = inputs.shape
     H, hd = self.num_heads, self.head_dim
@@ -414,11 +417,18 @@ def _is_plain_call(block, jagged) -> bool:
 
 
 def _serves(block) -> bool:
-  """Whether the block's forward_cached stands for its forward: both HSTUBlock's own, or a subclass's that has one of its own."""
+  """Whether the block's forward_cached stands for its forward: both HSTUBlock's own, or a subclass's that has one of its own.  With hooks on
+  the block, or on all modules, its forward has to be HSTUBlock's: they run around that."""
   own, kind = block.__dict__, type(block)
-  same = (kind.forward is HSTUBlock.forward and kind.forward_jagged is HSTUBlock.forward_jagged
-          and "forward" not in own and "forward_jagged" not in own)
-  return same or kind.forward_cached is not HSTUBlock.forward_cached or "forward_cached" in own
+  plain = kind.forward is HSTUBlock.forward and "forward" not in own
+  same = plain and kind.forward_jagged is HSTUBlock.forward_jagged and "forward_jagged" not in own
+  return (same or kind.forward_cached is not HSTUBlock.forward_cached or "forward_cached" in own) and (plain or not _hooked(block))
+
+
+def _hooked(block) -> bool:
+  """Whether hooks run where the block is called as a module in inference."""
+  m, own = torch.nn.modules.module, block.__dict__
+  return bool(own["_forward_hooks"] or own["_forward_pre_hooks"] or m._global_forward_hooks or m._global_forward_pre_hooks)
 
 
 class HSTU(torch.nn.Module):
@@ -639,7 +649,8 @@ class HSTU(torch.nn.Module):
   def prefill(self, inputs, cache, *, seq_lens, timestamps=None, pos_bias=None, ts_bias=None):
     """Takes whole histories into an empty cache, in inference: item ids [B, L], `seq_lens` [B] of them valid, `timestamps` [B, L].
     Returns what forward(inputs, seq_lens=seq_lens, jagged=True) does for a call of cache.max_len positions, but for the last bits:
-    [B, L, D or vocabulary], zeros past a history's end."""
+    [B, L, D or vocabulary], zeros past a history's end.  (Hooks on the blocks run, on packed rows [T, D]; that form of forward passes
+    them by.)"""
     B, L = inputs.shape
     if L > cache.max_len or B != cache.batch:
       raise ValueError(f"the cache holds {cache.batch} histories of up to {cache.max_len} events, got {tuple(inputs.shape)}")
@@ -673,7 +684,7 @@ class HSTU(torch.nn.Module):
     The outputs are forward's on the events so far, but for the rounding of the kept keys and values, whatever calls the events come in
     by.  With timestamps and more than one block the last kept event of every user with new ones is run again for that (its time bias
     reads the next event's time), and its keys and values are written again: two users may share the pages of a common beginning only if
-    it ends before either's last event."""
+    it ends before either's last event.  Hooks on the blocks run and see that event's row too."""
     B, dev = cache.batch, ids.device
     if offsets is None:
       if ids.dim() != 2 or ids.shape[0] != B:
@@ -708,7 +719,7 @@ class HSTU(torch.nn.Module):
       raise ValueError(f"the cache has {len(cache.layers)} layers, the model {len(self.decoder_blocks)}")
     if type(self)._front_end is not HSTU._front_end or not all(_serves(block) for block in self.decoder_blocks):
       raise ValueError("serving runs HSTU's own front end and HSTUBlock.forward_cached: a block with a forward of its own needs a "
-                       "forward_cached of its own too")
+                       "forward_cached of its own too, and no hooks")
     if (ts_bias is None) != (timestamps is None):
       raise ValueError("Both or neither of `timestamps` and `ts_bias` must be provided.")
     cache._note(ids, timestamps, users, places)
@@ -725,9 +736,10 @@ class HSTU(torch.nn.Module):
       x = table[ids.clamp(0, table.shape[0] - 1)]
       x = x * scale if self.scale_by_sqrt_dim else x
       x = self._final_norm(x if positions is None else x + positions[at])
+    kw = dict(offsets=offsets, max_new=max_new, pos_bias=pos_bias, timestamps=timestamps if whole else cache.timestamps, ts_bias=ts_bias, whole=whole)
     for block, pages in zip(self.decoder_blocks, cache.layers):
-      x = block.forward_cached(x, pages, cache.page_table, lengths, starts, cache.max_len, offsets=offsets, max_new=max_new, pos_bias=pos_bias,
-                               timestamps=timestamps if whole else cache.timestamps, ts_bias=ts_bias, whole=whole)
+      kept = pages, cache.page_table, lengths, starts, cache.max_len
+      x = block(x, kept=(kept, kw)) if _hooked(block) else block.forward_cached(x, *kept, **kw)
     if last:
       x = x[rows] if packed else x[:, 1:].contiguous()
     x = self._final_norm(x)

@@ -214,3 +214,69 @@ def test_rewound_and_begun_again():
   out = model.extend(pick(mixed), cache, timestamps=pick(at), **kw)
   full = _full(model, mixed, at, [n + 2 for n in lens], kw, True)
   _same(out, torch.stack([full[b, n : n + 2] for b, n in enumerate(lens)]))
+
+
+@pytest.mark.parametrize("everywhere", [False, True])
+def test_hooks_run(everywhere):
+  """Hooks on the blocks, or on all modules, do in serving what they do in the model's call."""
+  model, (ids, ts, pos, tab) = _model(2), _data()
+  kw = dict(pos_bias=pos, ts_bias=tab)
+  seen = []
+  def before(module, args):
+    if isinstance(module, recml_amd.HSTUBlock):
+      return (args[0] * 1.5,)
+  def after(module, args, out):
+    if isinstance(module, recml_amd.HSTUBlock):
+      seen.append(tuple(out.shape))
+      return out - 0.25
+  m = torch.nn.modules.module
+  if everywhere:
+    handles = [m.register_module_forward_pre_hook(before), m.register_module_forward_hook(after)]
+  else:
+    handles = [model.decoder_blocks[0].register_forward_pre_hook(before), model.decoder_blocks[1].register_forward_hook(after)]
+  try:
+    cache = model.new_cache(3, L, page_size=4, timestamps=True)
+    out = model.prefill(ids[:, :9], cache, seq_lens=torch.tensor([9, 0, 4]), timestamps=ts[:, :9], **kw)
+    assert seen == [(13, D)] * len(seen) and len(seen) == (2 if everywhere else 1)
+    full = _full(model, ids, ts, [9, 0, 4], kw, True)
+    _same(out[0], full[0, :9])
+    new = lambda x: torch.stack([x[0, 9:11], x[1, 0:2], x[2, 4:6]])
+    out = model.extend(new(ids), cache, timestamps=new(ts), **kw)
+    _same(out, new(_full(model, ids, ts, [11, 2, 6], kw, True)))
+  finally:
+    for h in handles:
+      h.remove()
+  plain = model.new_cache(3, L, page_size=4, timestamps=True)
+  assert not torch.equal(model.extend(ids[:, :1], plain, timestamps=ts[:, :1], **kw), out[:, :1])
+
+
+def test_pruned_weights_are_served():
+  """Pruning works its weights out in a hook ahead of each call."""
+  from torch.nn.utils import prune
+  model, (ids, _, pos, _) = _model(2), _data()
+  prune.l1_unstructured(model.decoder_blocks[0], "v_kernel", amount=0.5)
+  with torch.no_grad():
+    model.decoder_blocks[0].v_kernel_orig.mul_(1.25)
+  cache = model.new_cache(3, L, page_size=4)
+  out = model.extend(ids[:, :4], cache, pos_bias=pos)
+  _same(out, _full(model, ids, None, [4, 4, 4], dict(pos_bias=pos), False)[:, :4])
+
+
+def test_hooks_around_another_forward_are_refused():
+  """A subclass that serves through a forward_cached of its own: the hooks' place is around its forward, which is not run."""
+  class Served(recml_amd.HSTUBlock):
+    def forward(self, *args, **kw):
+      return 2 * super().forward(*args, **kw)
+
+    def forward_cached(self, *args, **kw):
+      return 2 * super().forward_cached(*args, **kw)
+
+  model, (ids, _, _, _) = _model(2), _data()
+  model.decoder_blocks[1].__class__ = Served
+  _same(model.extend(ids[:, :4], model.new_cache(3, L, page_size=4)), _full(model, ids, None, [4, 4, 4], dict(pos_bias=None), False)[:, :4])
+  handle = model.decoder_blocks[1].register_forward_hook(lambda *a: None)
+  with pytest.raises(ValueError, match="hooks"):
+    model.extend(ids[:, :4], model.new_cache(3, L, page_size=4))
+  handle.remove()
+  model.decoder_blocks[0].register_forward_hook(lambda *a: None)
+  assert model.extend(ids[:, :4], model.new_cache(3, L, page_size=4)).shape == (3, 4, VOCAB)
