@@ -641,8 +641,11 @@ Split split_of(const HstuLogProbsArgs& a) {
   Split s;
   // a wave for short rows where there are enough of them to fill the chip, four waves otherwise: forward and backward of 16000 rows of 2000
   // (bf16) with the 10 largest 27 + 35 us against 62 + 49, of 100 rows 11 + 6 against 7 + 6.  Its 64 maxima bound up to 50 of a row's largest
-  // entries well: 100 of them reach the bound, with 60 it is 180.
-  s.nt = vectors <= 64 * VECS && (a.rows >= 1024 ? a.top <= 50 : vectors <= 128 && a.top <= 16) ? 64 : 256;
+  // entries well: 100 of them reach the bound, with 60 it is 180.  A row of fewer vectors than entries asked for has no bound: all of its entries
+  // are ranked, and past the one wave's list of 256 found bit by bit, where four waves pay for
+  // longer: 300 wide with the 50 largest, 1024 rows 49 us against 22, 4096 rows 55 against 62, 16384 rows 201 against 216.
+  const bool bounded = a.vocab <= 256 || a.vocab / n >= a.top;
+  s.nt = vectors <= 64 * VECS && (a.rows >= (bounded ? 1024 : 4096) ? a.top <= 50 : vectors <= 128 && a.top <= 16) ? 64 : 256;
   int64_t parts = (vectors + (int64_t)s.nt * VECS - 1) / ((int64_t)s.nt * VECS);
   // few rows: more parts, so that they fill the chip, while the join holds all of a row's largest entries at once
   while (a.rows * parts < 256 && parts * s.nt * 2 <= vectors && 2 * parts * a.top <= 2048) parts *= 2;
