@@ -412,11 +412,10 @@ PyObject* accumulators(PyObject*, PyObject* const* a, Py_ssize_t count) {
   });
 }
 
-// token_log_probs(logits, tokens, top, entropy, differentiable) -> (log_probs, entropy, top_log_probs, top_tokens), each a tensor or None;
-// or None
+// token_log_probs(logits, tokens, top, entropy) -> (log_probs, entropy, top_log_probs, top_tokens), each a tensor or None; or None
 PyObject* token_log_probs(PyObject*, PyObject* const* a, Py_ssize_t count) {
-  if (count != 5) {
-    PyErr_SetString(PyExc_TypeError, "token_log_probs takes 5 arguments");
+  if (count != 4) {
+    PyErr_SetString(PyExc_TypeError, "token_log_probs takes 4 arguments");
     return nullptr;
   }
   return guarded([&]() -> PyObject* {

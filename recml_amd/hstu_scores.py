@@ -107,7 +107,7 @@ def token_log_probs(logits, tokens=None, *, top: int = 0, entropy: bool = False)
   Entries of -inf are tokens that cannot occur.  A row with a NaN, with +inf, or with nothing but -inf is NaN throughout.
   Differentiable in the logits, through log_probs, entropy and top_log_probs.  Captured into a graph with a gradient, it raises where an
   eager graph of the same leaves lives: their accumulators are not the captured stream's, and the backward pass would end the process."""
-  got = _native.token_log_probs(logits, tokens, top, entropy, True)
+  got = _native.token_log_probs(logits, tokens, top, entropy)
   if got is not None:
     return TokenLogProbs(*got)
   _check_gpu("logits", logits)

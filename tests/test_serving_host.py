@@ -1,5 +1,6 @@
 """The native host side of the serving operators, where it can be looked at without a GPU."""
 
+import pytest
 import torch
 
 from recml_amd import _native
@@ -21,3 +22,12 @@ def test_a_leafs_accumulator_outlives_the_walk_over_its_graph():
   # (the walk leaves nothing behind and nothing out: gradients are what they were)
   (x * w).sum().backward()
   assert torch.equal(x.grad, w.detach()) and torch.equal(w.grad, x.detach())
+
+
+def test_the_native_call_takes_what_it_reads():
+  """A graph is made where the logits want a gradient: there is no argument for it."""
+  x = torch.randn(2, 5)
+  assert _native.token_log_probs(x, None, 1, False) is None           # (CPU tensors are for the Python side to refuse)
+  for args in ((x, None, 1, False, True), (x, None, 1)):
+    with pytest.raises(TypeError, match="4 arguments"):
+      _native.token_log_probs(*args)
