@@ -339,3 +339,59 @@ def test_two_blocks_with_times_event_by_event(gpu, bits):
   assert float((together - full[:, n0:]).norm() / full[:, n0:].norm()) <= 4 * (2.0**-2 if bits == 4 else 2.0**-4)
   for last in (one[:, -1], some.reshape(B, m, -1)[:, -1]):
     assert float((last - full[:, -1]).norm() / full[:, -1].norm()) <= 4 * (2.0**-2 if bits == 4 else 2.0**-4)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_prefill_with_times_is_the_forward(gpu, dtype, bits):
+  """Both tables, two blocks, histories of every length up to the cache's; what is kept does not come into it."""
+  model = _model(dtype)
+  B, L, long = 5, 50, 44
+  ids = torch.randint(1, 300, (B, long), generator=_gen(1)).cuda()
+  ts = (1_600_000_000 + torch.exp(torch.rand((B, long), generator=_gen(2)) * 15).long().cumsum(1)).cuda()
+  lens = torch.tensor([44, 1, 0, 33, 2]).cuda()
+  kw = dict(pos_bias=(torch.randn((2, 2 * L - 1), generator=_gen(3)) * 0.2).cuda(), ts_bias=torch.randn((2, 129), generator=_gen(4)).cuda())
+  cache = model.new_cache(B, L, bits=bits, page_size=32, timestamps=True)
+  out = model.prefill(ids, cache, seq_lens=lens, timestamps=ts, **kw)
+  # the full call of the cache's length: its normaliser and its tables' extent
+  pad = lambda x: torch.cat([x, torch.zeros((B, L - long), dtype=x.dtype, device=x.device)], 1)
+  want = model(pad(ids), seq_lens=lens, jagged=True, timestamps=pad(ts), **kw)[:, :long]
+  # two runs of the same steps, rounded in other places: 2^-8 a step in bf16, sums in other orders in fp32
+  assert (out.double() - want.double()).norm() / want.double().norm() <= (1e-5 if dtype == F32 else 8 * 2.0**-8)
+  valid = torch.arange(long).cuda()[None] < lens[:, None]
+  assert not out[~valid].any() and torch.equal(cache.lengths, lens.int()) and torch.equal(cache.timestamps[:, :long][valid], ts[valid])
+  assert torch.equal(cache.ids[:, :long][valid], ids[valid])
+
+
+def test_the_gradient_of_the_head_against_differences(gpu):
+  """Along the gradient itself the loss rises by its norm: an error of one in a hundred shows."""
+  model = _model(F32, vocab=97)
+  model.requires_grad_(True)
+  ids = torch.randint(1, 97, (3, 12), generator=_gen(1)).cuda()
+  lens = torch.tensor([12, 5, 1]).cuda()
+  nxt = torch.where(torch.arange(12, device="cuda")[None] < (lens - 1)[:, None], ids.roll(-1, 1), -1)
+  def loss():
+    got = model.log_probs(ids, nxt, entropy=True, seq_lens=lens)
+    return -(got.log_probs.double().sum() + 0.1 * got.entropy.double().sum()) / 15
+  w = model.reverse_embedding
+  g = torch.autograd.grad(loss(), w)[0]
+  size = float(g.double().norm())
+  d, h = g / g.norm(), 4e-3
+  with torch.no_grad():
+    before = model(ids, seq_lens=lens)
+    ends = []
+    for s in (h, -2 * h):
+      w.add_(s * d)
+      ends.append(float(loss()))
+      after = model(ids, seq_lens=lens) if s > 0 else after
+    w.add_(h * d)
+  # A row's logits move by up to m for a step of 1 along d: third derivatives of ln sum exp stay below (2 m)^3 / 10 (a third central moment of
+  # values in a span of 2 m), the entropy's, a product of it with log probabilities of up to 12, below ten times that, of which a tenth counts.
+  m = ((after - before) / h).abs().amax(-1).double()
+  smooth = h * h / 6 * float(((2 * m) ** 3).sum()) * 0.2 / 15
+  # 15 log probabilities and 36 tenths of an entropy, each off by 89 steps of 2^-24 and four of its size (up to 12), twice over 2 h; weights that
+  # moved by h d and were rounded to 2^-24 of about 0.1, 64 of them a logit with rows of norm 8
+  rounding = (15 + 3.6) / 15 * ((89 + 4 * 12) * 2.0**-24 + 8 * 0.1 * 2.0**-24) / h
+  tol = smooth + rounding + 1e-4 * size
+  assert tol <= 0.02 * size, (smooth, rounding, size)
+  assert abs((ends[0] - ends[1]) / (2 * h) - size) <= tol, (ends, size, tol)
