@@ -20,7 +20,11 @@
 
 namespace {
 
-void serve_check(int rc, const char* what) { TORCH_CHECK(rc == HSTU_SERVE_OK, what, " failed (", rc, "): ", hstu_serve_last_error()); }
+// What the Python side raises for these: arguments that are refused are a ValueError.
+void serve_check(int rc, const char* what) {
+  TORCH_CHECK_VALUE(rc != HSTU_SERVE_ERR_NULL && rc != HSTU_SERVE_ERR_SHAPE, what, " rejected the arguments (", rc, "): ", hstu_serve_last_error());
+  TORCH_CHECK(rc == HSTU_SERVE_OK, what, " failed (", rc, "): ", hstu_serve_last_error());
+}
 
 constexpr int64_t MOST = std::numeric_limits<int32_t>::max();
 

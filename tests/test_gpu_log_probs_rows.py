@@ -75,3 +75,36 @@ def test_gradients_of_many_rows(gpu, dtype, vocab, count, top):
   bad = (d.double() - want[4]).abs() > tol
   assert not bad.any(), (float((d.double() - want[4]).abs().max()), int(bad.sum()))
   assert not d[9, vocab // 2 :].any()
+
+
+def test_a_refused_call_raises_the_same_either_way(gpu):
+  """More threads than a launch counts, through the native call and through Python's; and a bucket size that is nothing in fp32."""
+  x = torch.zeros((1, 1)).cuda().expand(1 << 26, 1)
+  for entropy in (True, 1):                          # (1: not the native call's)
+    with pytest.raises(ValueError, match="too many"):
+      recml_amd.token_log_probs(x, entropy=entropy)
+  pages = recml_amd.KVPages.empty(1, 32, 1, 8)
+  table, q = torch.zeros((1, 1), dtype=torch.int32).cuda(), torch.zeros((1, 1, 1, 8)).cuda()
+  for lengths in (torch.ones(1, dtype=torch.int32).cuda(), torch.ones(1, dtype=torch.int64).cuda()):     # (the second is Python's)
+    with pytest.raises(ValueError, match="ts_bucket_size"):
+      recml_amd.cached_attention(q, pages, table, lengths, max_len=4, timestamps=torch.zeros((1, 4), dtype=torch.int64).cuda(), ts_bias=torch.zeros(9).cuda(),
+                                 ts_bucket_size=1e-60)
+
+
+def test_inside_inference_mode(gpu):
+  """Tensors that keep no version: the same results."""
+  x = _logits(3, 500, BF16, 1).cuda()
+  want = recml_amd.token_log_probs(x, torch.tensor([1, 2, 3]).cuda(), top=4, entropy=True)
+  with torch.inference_mode():
+    y = x.clone()
+    got = recml_amd.token_log_probs(y, torch.tensor([1, 2, 3]).cuda(), top=4, entropy=True)
+    model = recml_amd.HSTU(vocab_size=50, max_positions=32, model_dim=16, num_heads=2, num_layers=2, device="cuda:0", seed=3).eval()
+    ids, ts = torch.randint(0, 50, (2, 8), generator=_gen(2)).cuda(), torch.arange(16).reshape(2, 8).cuda() * 1000
+    tab = torch.randn((129,), generator=_gen(3)).cuda()
+    cache = model.new_cache(2, 32, timestamps=True)
+    model.prefill(ids[:, :4], cache, seq_lens=torch.tensor([4, 2]).cuda(), timestamps=ts[:, :4], ts_bias=tab)
+    out = model.extend(ids[:, 4:], cache, timestamps=ts[:, 4:], ts_bias=tab)
+  assert all(torch.equal(a, b) for a, b in zip(got, want))
+  cache = model.new_cache(2, 32, timestamps=True)
+  model.prefill(ids[:, :4], cache, seq_lens=torch.tensor([4, 2]).cuda(), timestamps=ts[:, :4], ts_bias=tab)
+  assert torch.equal(out, model.extend(ids[:, 4:], cache, timestamps=ts[:, 4:], ts_bias=tab))
