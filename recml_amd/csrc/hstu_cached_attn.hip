@@ -610,6 +610,11 @@ Split split_of(const HstuCachedAttnArgs& a) {
   Split s;
   const bool f32 = a.dtype == HSTU_SERVE_FP32;
   const int most = a.pages.d > 128 ? (f32 ? 1 : 2) : f32 ? 2 : 4;
+  // blocks of 16, 32 or 64 rows, by how many a sequence has: a step of keys is converted once for a block's rows, and the more they are the fewer
+  // waves a SIMD holds.  128 sequences of 1024 keys, 8 heads, 4 bits, bf16, both tables, on blocks of 16 / 32 / 64: head dims of 64, 24 rows
+  // 89 / 73 / 107 us, 64 rows 168 / 154 / 221; of 128, 24 rows 103 / 108 / 220, 64 rows 191 / 198 / 450; 4 heads of 256, 24 rows 94 / 143, 64 rows
+  // 179 / 270.  With positions alone: 64, 24 rows 37 / 32 / 47; 128, 24 rows 49 / 51 / 106, 64 rows 91 / 84 / 144.  So two blocks of 32 beat one of 64
+  // wherever it is taken, and 16 rows beat 32 at head dims of 256 and, with times, mostly at 128.
   s.nq = a.rows_per_seq > 32 ? 4 : a.rows_per_seq > 16 ? 2 : 1;
   s.nq = std::min(s.nq, most);
   s.qblocks = (a.rows_per_seq + 16 * s.nq - 1) / (16 * s.nq);

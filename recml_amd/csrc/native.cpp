@@ -627,10 +627,6 @@ struct NormOp {
   }
 };
 
-// A tensor kept for the backward, the forward's own intermediates included: this way torch's saved-tensor hooks see it (checkpointing
-// and offloading replace it).
-
-
 // How far back a block's backward has to go, by what wants a gradient (`wanted(i)`: the i-th of tokens, the parameters, pos, ts_tab).
 struct BlockWants {
   bool kernels = false, input, projections, attention, gate;

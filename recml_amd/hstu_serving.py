@@ -71,7 +71,7 @@ class HSTUCache:
     """New events with each user's last kept one in front of them: (ids, places, starts, offsets, max_new, rows), laid out like the new events
     alone, `rows` where those are among them (packed; padded ones are all but each user's first).  A user without a kept event has a row
     at place -1 there, which joins nothing; one without a new event, or past max_len, gets `starts` under which none of its rows does."""
-    at = starts.to(torch.int64) - 1
+    at, full = starts.to(torch.int64) - 1, starts >= self.max_len
     last = self.ids.gather(1, at.clamp(0, self.max_len - 1)[:, None])
     ids = ids.to(torch.int64)
     if offsets is None:
@@ -88,6 +88,6 @@ class HSTUCache:
       together[:, firsts] = torch.stack([last[:, 0], at])
       ids, places = together
       offsets, most = (ends + torch.arange(B + 1, device=ids.device)).to(torch.int32), min(int(max_new), T) + 1
-      max_new = most
-    starts = torch.where((starts >= self.max_len) | (lengths == starts), -1 - most, starts - 1)
+      max_new, full = most, full | (lengths == starts)
+    starts = torch.where(full, -1 - most, starts - 1)
     return ids, places, starts, offsets, max_new, rows
