@@ -395,3 +395,41 @@ def test_the_gradient_of_the_head_against_differences(gpu):
   tol = smooth + rounding + 1e-4 * size
   assert tol <= 0.02 * size, (smooth, rounding, size)
   assert abs((ends[0] - ends[1]) / (2 * h) - size) <= tol, (ends, size, tol)
+
+
+def test_a_packed_step_with_times_in_a_graph(gpu):
+  """Offsets, ids and times are copied in between replays: users with no, one or several new events, as the eager calls have them."""
+  model = _model(BF16)
+  pos, tab = (torch.randn((2, 127), generator=_gen(3)) * 0.2).cuda(), torch.randn((2, 129), generator=_gen(4)).cuda()
+  kw = dict(pos_bias=pos, ts_bias=tab)
+  T, B = 5, 4
+  seq, when0 = torch.randint(1, 300, (B, 10), generator=_gen(1)).cuda(), 1_600_000_000 + torch.arange(10 * B).reshape(B, 10).cuda() * 977
+  caches = [model.new_cache(B, 64, bits=8, page_size=32, timestamps=True) for _ in range(2)]
+  for c in caches:
+    model.prefill(seq, c, seq_lens=torch.tensor([10, 0, 3, 7]).cuda(), timestamps=when0, **kw)
+  ids, when, offsets = torch.ones(T, dtype=torch.int64).cuda(), torch.full((T,), 1_700_000_000).cuda(), torch.tensor([0, 1, 2, 3, 5], dtype=torch.int32).cuda()
+  def step(cache):
+    return model.extend(ids, cache, offsets=offsets, max_new=3, timestamps=when, **kw)
+  keep = caches[1].lengths.clone()
+  s = torch.cuda.Stream()
+  s.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(s):
+    step(caches[1])
+  torch.cuda.current_stream().wait_stream(s)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    out = step(caches[1])
+  caches[1].lengths.copy_(keep)
+  # (what the warm-up wrote past the kept lengths is the past of nobody)
+  for n, ends in enumerate(([0, 1, 2, 3, 5], [0, 0, 3, 3, 5], [0, 2, 2, 2, 2], [1, 2, 2, 4, 5], [0, 3, 4, 5, 5])):
+    ids.copy_(torch.randint(1, 300, (T,), generator=_gen(20 + n)))
+    when.copy_(1_700_000_000 + 100_000 * n + torch.arange(T) * 333)
+    offsets.copy_(torch.tensor(ends))
+    graph.replay()
+    want = step(caches[0])
+    torch.cuda.synchronize()
+    rows = slice(ends[0], ends[-1])
+    assert torch.equal(out[rows], want[rows]), n
+    assert torch.equal(caches[0].lengths, caches[1].lengths)
+    for b, m in enumerate(caches[0].lengths.tolist()):
+      assert torch.equal(caches[0].ids[b, :m], caches[1].ids[b, :m]) and torch.equal(caches[0].timestamps[b, :m], caches[1].timestamps[b, :m])
