@@ -327,7 +327,7 @@ def test_two_blocks_with_times_event_by_event(gpu, bits):
     m = new.shape[1]
     some = model.extend(new.reshape(-1), caches[2], offsets=m * torch.arange(B + 1).cuda(), max_new=m, timestamps=when.reshape(-1), **kw)
   # Sums in another order move a value by 1e-5 of itself at most (the tolerance of the tests of one block), codes are at least 2^-4 of it apart:
-  # of the first block's 30720 values less than 2e-5 * 2^4 of each, 10 in all, change their code.  One that does moves what later events get there by less
+  # of the first block's 30 thousand values less than 2e-5 * 2^4 of each, 10 in all, change their code.  One that does moves what later events get there by less
   # than 2^-3 of one of its 64 * 32 terms, 1e-3 of the sum's norm with its neighbours' signs, and with it 2 * 1e-3 * 2^4 = 3 in 100 of the second block's
   # codes.  (Kept as if each event were the last: 19 in 100 of the codes of 4 bits, 48 of those of 8.)
   for c in caches[1:]:
