@@ -1,5 +1,5 @@
 """Loads the native host sides (recml_amd/lib/_native.so, built from recml_amd/csrc/native.cpp, and, for the serving operators,
-_native_serve.so from native_serve.cpp).
+_native_serve.so from native_serve.cpp; for the steps on rows in 8 bits, _native_rows8.so from native_rows8.cpp).
 
 Its functions take a call whose arguments are ready for the kernels as they are, and return None for any other, which
 the Python side then checks, converts or reports.
@@ -13,7 +13,7 @@ import os
 import torch
 from torch.autograd import forward_ad
 
-from recml_amd import _lib, _lib_block, _lib_serve
+from recml_amd import _lib, _lib_block, _lib_rows8, _lib_serve
 
 PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_native.so")
 
@@ -45,6 +45,10 @@ def _other_serve_library() -> bool:
   return bool(os.environ.get("RECML_AMD_SERVE_LIB"))
 
 
+def _other_rows8_library() -> bool:
+  return bool(os.environ.get("RECML_AMD_ROWS8_LIB"))
+
+
 def _decline(*args):
   return None
 
@@ -68,3 +72,7 @@ attention, block, blocks, embed, final_norm, linear, pack, mask_lengths, raised,
 _SERVE_FUNCTIONS = ("check_pages", "kv_write", "kv_read", "cached_attention", "token_log_probs", "accumulators")
 check_pages, kv_write, kv_read, cached_attention, token_log_probs, accumulators = (
     _first_call(n, _SERVE_FUNCTIONS, lambda: _load("_native_serve", _lib_serve), _other_serve_library) for n in _SERVE_FUNCTIONS)
+
+_ROWS8_FUNCTIONS = ("check_rows8", "norm_rows8", "read_rows8", "gemm_rows8")
+check_rows8, norm_rows8, read_rows8, gemm_rows8 = (
+    _first_call(n, _ROWS8_FUNCTIONS, lambda: _load("_native_rows8", _lib_rows8), _other_rows8_library) for n in _ROWS8_FUNCTIONS)

@@ -18,6 +18,9 @@ BLOCK_SOURCES = [os.path.join(_HERE, "csrc", "hstu_block.hip"), os.path.join(_HE
 # serving from kept histories and scoring of logits
 SERVE_LIB_PATH = os.path.join(LIB_DIR, "libhstu_serve.so")
 SERVE_SOURCES = [os.path.join(_HERE, "csrc", name) for name in ("hstu_cache.hip", "hstu_cached_attn.hip", "hstu_log_probs.hip")]
+# a block's steps on rows in 8 bits
+ROWS8_LIB_PATH = os.path.join(LIB_DIR, "libhstu_rows8.so")
+ROWS8_SOURCES = [os.path.join(_HERE, "csrc", name) for name in ("hstu_rows8.hip", "hstu_rows8_gemm.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 # the block's microbenchmark: a stand-alone program (its own main), evidence for what bounds the kernel
 MICRO_PATH = os.path.join(LIB_DIR, "micro_fwd_stream")
@@ -28,6 +31,8 @@ NATIVE_PATH = os.path.join(LIB_DIR, "_native.so")
 NATIVE_SOURCES = [os.path.join(_HERE, "csrc", "native.cpp")]
 NATIVE_SERVE_PATH = os.path.join(LIB_DIR, "_native_serve.so")
 NATIVE_SERVE_SOURCES = [os.path.join(_HERE, "csrc", "native_serve.cpp")]
+NATIVE_ROWS8_PATH = os.path.join(LIB_DIR, "_native_rows8.so")
+NATIVE_ROWS8_SOURCES = [os.path.join(_HERE, "csrc", "native_rows8.cpp")]
 
 # -packed-fp32-ops is switched off for the device pass: packed fp32
 # instructions are not wanted in these kernels.  The host pass does not know
@@ -73,6 +78,11 @@ def build_serve_library(verbose: bool = False) -> str:
   return _compile(SERVE_SOURCES, SERVE_LIB_PATH, verbose=verbose)
 
 
+def build_rows8_library(verbose: bool = False) -> str:
+  """Compiles the steps on rows in 8 bits into recml_amd/lib/libhstu_rows8.so."""
+  return _compile(ROWS8_SOURCES, ROWS8_LIB_PATH, verbose=verbose)
+
+
 def _compile_native(sources, out, libraries, verbose=False) -> str:
   import sysconfig
   import torch
@@ -102,6 +112,11 @@ def build_native_serve(verbose: bool = False) -> str:
   return _compile_native(NATIVE_SERVE_SOURCES, NATIVE_SERVE_PATH, (SERVE_LIB_PATH,), verbose)
 
 
+def build_native_rows8(verbose: bool = False) -> str:
+  """Compiles the native host side of the steps on rows in 8 bits into recml_amd/lib/_native_rows8.so (links their library)."""
+  return _compile_native(NATIVE_ROWS8_SOURCES, NATIVE_ROWS8_PATH, (ROWS8_LIB_PATH,), verbose)
+
+
 def build_microbench(verbose: bool = False) -> str:
   """Compiles the forward block's microbenchmark into recml_amd/lib/micro_fwd_stream (an executable)."""
   os.makedirs(LIB_DIR, exist_ok=True)
@@ -121,6 +136,8 @@ if __name__ == "__main__":
   print(build_library(verbose=True))
   print(build_block_library(verbose=True))
   print(build_serve_library(verbose=True))
+  print(build_rows8_library(verbose=True))
   print(build_native(verbose=True))
   print(build_native_serve(verbose=True))
+  print(build_native_rows8(verbose=True))
   print(build_microbench(verbose=True))

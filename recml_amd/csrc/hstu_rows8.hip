@@ -1,0 +1,354 @@
+// Rows of activations and weights in 8 bits, for gfx950 (MI355X): see include/hstu_rows8.h.
+//
+//   hstu_rows8_norm   rows, normed or as they are -> codes and block exponents
+//   hstu_rows8_read   codes and exponents -> rows
+//
+// Both are passes over memory: a row is read once, stays in registers as fp32 through the sum, the statistics (the mean, then the squares
+// about it), the gate and the blocks' maxima, and leaves as one byte a value.
+
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "hstu_rows8_common.h"
+
+namespace {
+thread_local char g_err[512] = "";
+}
+
+int rows8_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+void rows8_clear_error() { g_err[0] = 0; }
+
+int rows8_launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? HSTU_ROWS8_OK : rows8_fail(HSTU_ROWS8_ERR_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+}
+
+int rows8_check(const HstuRows8& r, const char* name) {
+  if (r.rows < 0 || r.rows > 0x7fffffffll) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%s: %lld rows", name, (long long)r.rows);
+  if (r.width < 1 || r.width > HSTU_ROWS8_MAX_WIDTH) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%s: width=%d: 1 to %d", name, r.width, HSTU_ROWS8_MAX_WIDTH);
+  if (r.rows == 0) return HSTU_ROWS8_OK;
+  if (!r.codes || !r.exponents) return rows8_fail(HSTU_ROWS8_ERR_NULL, "%s: codes or exponents are null", name);
+  if (!rows8_aligned16(r.codes) || ((uintptr_t)r.exponents & 3u)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%s: codes start on a 16-byte boundary, exponents on a 4-byte one", name);
+  return HSTU_ROWS8_OK;
+}
+
+namespace {
+
+struct Params {
+  const void *x, *add, *gate, *gamma, *beta;
+  void* sum;
+  uint8_t* codes;
+  uint8_t* exponents;
+  int64_t x_stride, add_stride, gate_stride, sum_stride;
+  int64_t rows;
+  int32_t width;
+  float eps;
+};
+
+// Eight values of a row in fp32; past the width zeros.  VEC: a width and places of whole vectors.
+template <bool F32, bool VEC>
+__device__ __forceinline__ void load8(const void* base, int64_t at, int col, int width, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = 0.f;
+  if constexpr (VEC) {
+    if (col >= width) return;
+    if constexpr (F32) {
+      const floatx4* const from = (const floatx4*)((const float*)base + at + col);
+      const floatx4 lo = from[0], hi = from[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
+    } else {
+      unpack8(*(const uint4v*)((const bf16_t*)base + at + col), f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < width) f[i] = F32 ? ((const float*)base)[at + col + i] : (float)((const bf16_t*)base)[at + col + i];
+  }
+}
+
+template <bool F32, bool VEC>
+__device__ __forceinline__ void store8(void* base, int64_t at, int col, int width, const float (&f)[8]) {
+  if constexpr (VEC) {
+    if (col >= width) return;
+    if constexpr (F32) {
+      floatx4* const to = (floatx4*)((float*)base + at + col);
+      to[0] = floatx4{f[0], f[1], f[2], f[3]};
+      to[1] = floatx4{f[4], f[5], f[6], f[7]};
+    } else {
+      *(uint4v*)((bf16_t*)base + at + col) = pack8(f);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < width) {
+        if constexpr (F32) ((float*)base)[at + col + i] = f[i];
+        else ((bf16_t*)base)[at + col + i] = (bf16_t)f[i];
+      }
+  }
+}
+
+// a value of the lane's neighbour in a row of 16: quad_perm [1,0,3,2] and [2,3,0,1], row_half_mirror, row_mirror
+template <int CTRL>
+__device__ __forceinline__ uint32_t of_neighbour(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
+template <int CTRL>
+__device__ __forceinline__ float add_neighbour(float v) { return v + __builtin_bit_cast(float, of_neighbour<CTRL>(__builtin_bit_cast(uint32_t, v))); }
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_neighbour(uint32_t v) {
+  const uint32_t o = of_neighbour<CTRL>(v);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  return max_neighbour<0x140>(max_neighbour<0x141>(max_neighbour<0x4E>(max_neighbour<0xB1>(v))));
+}
+
+// the sum over a row's T threads, the same bits in each of them
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float* parts) {
+  v = add_neighbour<0x140>(add_neighbour<0x141>(add_neighbour<0x4E>(add_neighbour<0xB1>(v))));
+  if constexpr (T >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (T >= 64) v += __shfl_xor(v, 32, 64);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) v += parts[w];
+    __syncthreads();
+  }
+  return v;
+}
+
+constexpr int threads_of(int t) { return t < 256 ? 256 : t; }
+
+// T threads a row, V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
+template <bool F32, bool VEC, int NORM, int T, int V>
+__global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Params p) {
+  __shared__ float parts[T > 64 ? T / 64 : 1];
+  const int t = threadIdx.x % T;
+  const int64_t row = (int64_t)blockIdx.x * (threads_of(T) / T) + threadIdx.x / T;
+  if (row >= p.rows) return;                       // (T > 64: a row is the whole workgroup)
+  const int W = p.width, blocks = rows8_blocks(W);
+  float y[V][8];
+#pragma unroll
+  for (int v = 0; v < V; ++v) load8<F32, VEC>(p.x, row * p.x_stride, 8 * (v * T + t), W, y[v]);
+  if (p.add) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int col = 8 * (v * T + t);
+      float a[8];
+      load8<F32, VEC>(p.add, row * p.add_stride, col, W, a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[v][i] += a[i];
+        if constexpr (!F32) y[v][i] = (float)(bf16_t)y[v][i];
+      }
+      if (p.sum) store8<F32, VEC>(p.sum, row * p.sum_stride, col, W, y[v]);
+    }
+  }
+  if constexpr (NORM != HSTU_ROWS8_AS_IS) {
+    // (divided, not multiplied by 1 / W: the mean of equal values is that value, and their differences from it are zeros)
+    const float count = (float)W;
+    float mean = 0.f;
+    if constexpr (NORM == HSTU_ROWS8_LAYER) {
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i & 1] += y[v][i];
+      mean = row_sum<T>(s[0] + s[1], parts) / count;
+    }
+    float ss[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = 8 * (v * T + t) + i < W ? y[v][i] - mean : 0.f;
+        ss[i & 1] = __builtin_fmaf(d, d, ss[i & 1]);
+      }
+    const float rstd = __builtin_amdgcn_rsqf(row_sum<T>(ss[0] + ss[1], parts) / count + p.eps);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int col = 8 * (v * T + t);
+      float g[8], b[8];
+      load8<F32, VEC>(p.gamma, 0, col, W, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[i] = 0.f;
+      if (p.beta) load8<F32, VEC>(p.beta, 0, col, W, b);
+      // (past the width: gamma and beta are zeros there, and a mean or rstd that is not finite stays out)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[v][i] = col + i < W ? __builtin_fmaf((y[v][i] - mean) * rstd, g[i], b[i]) : 0.f;
+    }
+  }
+  if (p.gate) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float u[8];
+      load8<F32, VEC>(p.gate, row * p.gate_stride, 8 * (v * T + t), W, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[v][i] *= u[i];
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int piece = v * T + t, block = piece / 16;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t m = __builtin_bit_cast(uint32_t, y[v][i]) & 0x7fffffffu;
+      top = m > top ? m : top;
+    }
+    top = max16(top);
+    // floor(log2 top) less the largest code's 8, one more where top is past 464 = 1.8125 * 2^8 powers
+    int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x680000u ? 1 : 0);
+    e = e < 1 ? 1 : e > 246 ? 246 : e;              // (top = 0 too)
+    const bool bad = top >= 0x7f800000u;
+    const float inverse = power_of(254 - (uint32_t)e);
+    uint2 code;
+    {
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = __builtin_amdgcn_fmed3f(y[v][i] * inverse, -448.f, 448.f);
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+      code.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
+      code.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], c, true);
+    }
+    if (block < blocks) *(uint2*)(p.codes + row * ((int64_t)blocks * BLOCK) + 8 * piece) = bad ? uint2{0u, 0u} : code;
+    if (t % 16 == 0 && block < (blocks + 3) / 4 * 4)
+      p.exponents[((int64_t)(block / 4) * p.rows + row) * 4 + block % 4] = block >= blocks ? (uint8_t)1 : bad ? (uint8_t)255 : (uint8_t)e;
+    // (groups whose last blocks no thread has)
+    if (v == V - 1 && t == T - 1) {
+      for (int more = block + 1; more < (blocks + 3) / 4 * 4; ++more) p.exponents[((int64_t)(more / 4) * p.rows + row) * 4 + more % 4] = 1;
+    }
+  }
+}
+
+struct ReadParams {
+  const uint8_t* codes;
+  const uint8_t* exponents;
+  void* out;
+  int64_t out_stride, rows;
+  int32_t width;
+  int32_t pieces;          // of 8 values, in a row's codes
+};
+
+// a piece of 8 values a thread
+template <bool F32, bool VEC>
+__global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / p.pieces;
+  const int piece = (int)(at - row * p.pieces);
+  if (row >= p.rows || 8 * piece >= p.width) return;
+  const uint2 w = *(const uint2*)(p.codes + at * 8);
+  const int block = piece / 16;
+  const uint32_t e = p.exponents[((int64_t)(block / 4) * p.rows + row) * 4 + block % 4];
+  const float power = e == 255u ? __builtin_nanf("") : power_of(e);
+  const floatx2 y[4] = {__builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)w.x, true),
+                        __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)w.y, true)};
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = y[i / 2][i % 2] * power;
+  store8<F32, VEC>(p.out, row * p.out_stride, 8 * piece, p.width, f);
+}
+
+template <bool F32, bool VEC, int NORM>
+void launch_norm(const Params& p, hipStream_t st) {
+#define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, VEC, NORM, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
+  if (p.width <= 128) ROWS8_LAUNCH(16, 1);
+  else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
+  else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
+  else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
+  else if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
+  else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+  else ROWS8_LAUNCH(1024, 4);
+#undef ROWS8_LAUNCH
+}
+
+int norm_rows(const HstuRows8NormArgs* a, void* stream) {
+  rows8_clear_error();
+  if (!a) return rows8_fail(HSTU_ROWS8_ERR_NULL, "args is null");
+  if (a->struct_size != sizeof(HstuRows8NormArgs) || a->version != HSTU_ROWS8_ABI_VERSION)
+    return rows8_fail(HSTU_ROWS8_ERR_VERSION, "struct_size %u version %u, expected %zu and %d", a->struct_size, a->version, sizeof(HstuRows8NormArgs), HSTU_ROWS8_ABI_VERSION);
+  if (const int rc = rows8_check(a->rows, "rows")) return rc;
+  if (a->dtype != HSTU_ROWS8_BF16 && a->dtype != HSTU_ROWS8_FP32) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "dtype %d", a->dtype);
+  if (a->norm < HSTU_ROWS8_AS_IS || a->norm > HSTU_ROWS8_RMS) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "norm %d", a->norm);
+  if (a->sum && !a->add) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a sum needs something to add");
+  if (a->rows.rows == 0) return HSTU_ROWS8_OK;
+  if (!a->x) return rows8_fail(HSTU_ROWS8_ERR_NULL, "x is null");
+  if (a->norm != HSTU_ROWS8_AS_IS && !a->gamma) return rows8_fail(HSTU_ROWS8_ERR_NULL, "gamma is null");
+  // (a workgroup a row at most)
+  const int64_t threads = a->rows.width <= 2048 ? 64 : a->rows.width <= 8192 ? 256 : 1024;
+  if (a->rows.rows > ROWS8_THREADS / threads - 16) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)a->rows.rows, a->rows.width);
+  const bool f32 = a->dtype == HSTU_ROWS8_FP32;
+  const int unit = f32 ? 4 : 8;
+  bool vec = a->rows.width % 8 == 0;
+  auto rows_of = [&](const void* t, int64_t stride) {
+    if (t && ((uintptr_t)t & (f32 ? 3u : 1u))) return false;
+    vec = vec && (!t || (rows8_aligned16(t) && (stride % unit == 0 || a->rows.rows == 1)));
+    return true;
+  };
+  if (!rows_of(a->x, a->x_stride) || !rows_of(a->add, a->add_stride) || !rows_of(a->gate, a->gate_stride) || !rows_of(a->sum, a->sum_stride) ||
+      !rows_of(a->gamma, 0) || !rows_of(a->beta, 0)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a pointer is not aligned to its type");
+  Params p;
+  p.x = a->x; p.add = a->add; p.gate = a->gate; p.gamma = a->gamma; p.beta = a->beta; p.sum = a->sum;
+  p.codes = (uint8_t*)a->rows.codes; p.exponents = (uint8_t*)a->rows.exponents;
+  p.x_stride = a->x_stride; p.add_stride = a->add_stride; p.gate_stride = a->gate_stride; p.sum_stride = a->sum_stride;
+  p.rows = a->rows.rows; p.width = a->rows.width; p.eps = a->eps;
+  hipStream_t st = (hipStream_t)stream;
+#define ROWS8_NORM(F32, VEC)                                                                  \
+  do {                                                                                        \
+    if (a->norm == HSTU_ROWS8_LAYER) launch_norm<F32, VEC, HSTU_ROWS8_LAYER>(p, st);          \
+    else if (a->norm == HSTU_ROWS8_RMS) launch_norm<F32, VEC, HSTU_ROWS8_RMS>(p, st);         \
+    else launch_norm<F32, VEC, HSTU_ROWS8_AS_IS>(p, st);                                      \
+  } while (0)
+  if (f32) { if (vec) ROWS8_NORM(true, true); else ROWS8_NORM(true, false); }
+  else { if (vec) ROWS8_NORM(false, true); else ROWS8_NORM(false, false); }
+#undef ROWS8_NORM
+  return rows8_launched("hstu_rows8_norm");
+}
+
+int read_rows(const HstuRows8ReadArgs* a, void* stream) {
+  rows8_clear_error();
+  if (!a) return rows8_fail(HSTU_ROWS8_ERR_NULL, "args is null");
+  if (a->struct_size != sizeof(HstuRows8ReadArgs) || a->version != HSTU_ROWS8_ABI_VERSION)
+    return rows8_fail(HSTU_ROWS8_ERR_VERSION, "struct_size %u version %u, expected %zu and %d", a->struct_size, a->version, sizeof(HstuRows8ReadArgs), HSTU_ROWS8_ABI_VERSION);
+  if (const int rc = rows8_check(a->rows, "rows")) return rc;
+  if (a->dtype != HSTU_ROWS8_BF16 && a->dtype != HSTU_ROWS8_FP32) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "dtype %d", a->dtype);
+  if (a->rows.rows == 0) return HSTU_ROWS8_OK;
+  if (!a->out) return rows8_fail(HSTU_ROWS8_ERR_NULL, "out is null");
+  const bool f32 = a->dtype == HSTU_ROWS8_FP32;
+  if ((uintptr_t)a->out & (f32 ? 3u : 1u)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "out is not aligned to its type");
+  ReadParams p;
+  p.codes = (const uint8_t*)a->rows.codes; p.exponents = (const uint8_t*)a->rows.exponents;
+  p.out = a->out; p.out_stride = a->out_stride; p.rows = a->rows.rows; p.width = a->rows.width;
+  p.pieces = rows8_blocks(p.width) * (BLOCK / 8);
+  const int64_t all = p.rows * p.pieces;
+  if (all > ROWS8_THREADS - 256) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)p.rows, p.width);
+  const bool vec = p.width % 8 == 0 && rows8_aligned16(a->out) && (p.out_stride % (f32 ? 4 : 8) == 0 || p.rows == 1);
+  const uint32_t grid = (uint32_t)((all + 255) / 256);
+  hipStream_t st = (hipStream_t)stream;
+  if (f32) { if (vec) hstu_rows8_read_kernel<true, true><<<grid, 256, 0, st>>>(p); else hstu_rows8_read_kernel<true, false><<<grid, 256, 0, st>>>(p); }
+  else { if (vec) hstu_rows8_read_kernel<false, true><<<grid, 256, 0, st>>>(p); else hstu_rows8_read_kernel<false, false><<<grid, 256, 0, st>>>(p); }
+  return rows8_launched("hstu_rows8_read");
+}
+
+}  // namespace
+
+extern "C" {
+
+int hstu_rows8_norm(const HstuRows8NormArgs* args, void* stream) { return norm_rows(args, stream); }
+int hstu_rows8_read(const HstuRows8ReadArgs* args, void* stream) { return read_rows(args, stream); }
+int hstu_rows8_abi_version(void) { return HSTU_ROWS8_ABI_VERSION; }
+const char* hstu_rows8_last_error(void) { return g_err; }
+
+}
