@@ -186,7 +186,11 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
       if (p.beta) load8<F32, VEC>(p.beta, 0, col, W, b);
       // (past the width: gamma and beta are zeros there, and a mean or rstd that is not finite stays out)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[v][i] = col + i < W ? __builtin_fmaf((y[v][i] - mean) * rstd, g[i], b[i]) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+#pragma clang fp contract(off)      // (every step rounded, as it is in separate operations: half as many codes differ from theirs, 5e-7 of them)
+        const float z = (y[v][i] - mean) * rstd * g[i];
+        y[v][i] = col + i < W ? z + b[i] : 0.f;
+      }
     }
   }
   if (p.gate) {

@@ -14,6 +14,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "hstu_rows8_common.h"
 
 namespace {
@@ -100,6 +103,28 @@ __device__ __forceinline__ void row_store8(void* base, int64_t at, int col, int 
     }
 }
 
+// Four values of a row added, from column `at` on; none past `cols`.
+template <bool F32>
+__device__ __forceinline__ void add4(const void* base, int64_t row, int at, int cols, bool vec, floatx4& y) {
+  if (vec) {
+    if constexpr (F32) {
+      const floatx4 v = *(const floatx4*)((const float*)base + row + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] += v[i];
+    } else {
+      const uint2 v = *(const uint2*)((const bf16_t*)base + row + at);
+      y[0] += __builtin_bit_cast(float, v.x << 16);
+      y[1] += __builtin_bit_cast(float, v.x & 0xffff0000u);
+      y[2] += __builtin_bit_cast(float, v.y << 16);
+      y[3] += __builtin_bit_cast(float, v.y & 0xffff0000u);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < cols) y[i] += F32 ? ((const float*)base)[row + at + i] : (float)((const bf16_t*)base)[row + at + i];
+}
+
 // Eight of a lane's 32 codes as the values that they stand for, exact in bf16.
 __device__ __forceinline__ bf16x8 values8(const intx8& codes, int q, float power) {
   const uint32_t lo = (uint32_t)codes[2 * q], hi = (uint32_t)codes[2 * q + 1];
@@ -121,13 +146,15 @@ constexpr int lds_bytes(int mb, int nb, int wm, int wn, int stages) {
 // lane then holds four consecutive columns of one output row.
 //   A row's 128 bytes lie in LDS as eight 16-byte chunks, chunk c of row r at c ^ (r / 2 % 8): 16 rows reach all 64 banks.  Which
 // contraction elements a lane holds does not matter as long as both operands' lanes hold the same ones.
+//   128 x 64 a wave for the reason of the bf16 products: with 64 x 64 the four SIMDs' fragments take all of the LDS bandwidth at full matrix
+// rate, with 128 x 64 three quarters of it.  16384 x 8192 by 8192 in 870 us (2530 TFLOP/s), in tiles of 128 x 128 940, of 64 x 64 1580.
 template <int MB, int NB, int WM, int WN, int STAGES, bool F32>
 __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const GemmParams g) {
   constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN, WAVES = WM * WN;
   constexpr int X_BYTES = TM * BLOCK, CODES = (TM + TN) * BLOCK, STAGE = stage_bytes(TM, TN);
-  constexpr int LX = TM / 8 / WAVES, LW = TN / 8 / WAVES, LE = (TM + TN) / 64;      // direct loads of 8 rows; of 64 rows' exponents
-  static_assert(LX * 8 * WAVES == TM && LW * 8 * WAVES == TN && TM % 64 == 0 && TN % 64 == 0 && LE <= WAVES, "whole loads a wave");
-  constexpr int NLOAD = LX + LW + 1;
+  constexpr int LX = TM / 8 / WAVES, LW = TN / 8 / WAVES, LE = (TM + TN) / 64, LEW = (LE + WAVES - 1) / WAVES;      // direct loads of 8 rows; of 64 rows' exponents
+  static_assert(LX * 8 * WAVES == TM && LW * 8 * WAVES == TN && TM % 64 == 0 && TN % 64 == 0, "whole loads a wave");
+  constexpr int NLOAD = LX + LW + LEW;
   static_assert(STAGES >= 2 && (STAGES - 1) * NLOAD <= 63, "vmcnt range");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const uint32_t smem_lds = __builtin_amdgcn_groupstaticsize();
@@ -158,24 +185,37 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
     const int r = 8 * (w * LW + i) + (lane >> 3), at = n0 + r < g.cols ? r : g.cols - 1 - n0;
     wo[i] = (uint32_t)(at * (int)pitch + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
   }
-  const int piece = w % LE;                                     // (more waves than pieces: some load the same)
-  const bool piece_x = 64 * piece < TM;
-  const int e_row = (piece_x ? 64 * piece : 64 * piece - TM) + lane, e_last = (piece_x ? g.rows - 1 - m0 : g.cols - 1 - n0);
-  const uint32_t eo = 4u * (uint32_t)(e_row < e_last ? e_row : e_last);
+  // (more waves than pieces of exponents: some load the same)
+  uint32_t eo[LEW], e_to[LEW];
+  const uint8_t* e_base[LEW];
+  int64_t e_step[LEW];
+#pragma unroll
+  for (int i = 0; i < LEW; ++i) {
+    const int piece = (w + WAVES * i) % LE;
+    const bool of_x = 64 * piece < TM;
+    const int row = (of_x ? 64 * piece : 64 * piece - TM) + lane, last = of_x ? g.rows - 1 - m0 : g.cols - 1 - n0;
+    eo[i] = 4u * (uint32_t)(row < last ? row : last);
+    e_to[i] = CODES + 256u * piece;
+    e_base[i] = scalar_ptr(of_x ? g.xe + (int64_t)m0 * 4 : g.we + (int64_t)n0 * 4);
+    e_step[i] = 4 * (int64_t)(of_x ? g.rows : g.cols);
+  }
   const uint8_t* x_base = scalar_ptr(g.x + (int64_t)m0 * pitch);
   const uint8_t* w_base = scalar_ptr(g.w + (int64_t)n0 * pitch);
-  const uint8_t* e_base = scalar_ptr(piece_x ? g.xe + (int64_t)m0 * 4 : g.we + (int64_t)n0 * 4);
-  const int64_t e_step = 4 * (int64_t)(piece_x ? g.rows : g.cols);
   int loaded = 0;                                               // stages asked for
   auto issue_one = [&](int st, int i) __attribute__((always_inline)) {
     const uint32_t base = smem_lds + (uint32_t)st * STAGE;
     if (i < LX) lds_dma16(x_base, xo[i < LX ? i : 0], base + 1024u * (w * LX + i));
     else if (i < LX + LW) lds_dma16(w_base, wo[i < LX ? 0 : i < LX + LW ? i - LX : 0], base + X_BYTES + 1024u * (w * LW + i - LX));
     else {
-      lds_dma4(e_base, eo, base + CODES + 256u * piece);
+      constexpr int FROM = LX + LW;
+      lds_dma4(e_base[i < FROM ? 0 : i - FROM], eo[i < FROM ? 0 : i - FROM], base + e_to[i < FROM ? 0 : i - FROM]);
+    }
+    if (i == NLOAD - 1) {       // on to the next block; every four blocks to the next group of exponents
       x_base += BLOCK;
       w_base += BLOCK;
-      if ((++loaded & 3) == 0) e_base += e_step;
+      if ((++loaded & 3) == 0)
+#pragma unroll
+        for (int e = 0; e < LEW; ++e) e_base[e] += e_step[e];
     }
   };
 
@@ -325,6 +365,318 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   }
 }
 
+// f(0), f(1), ..., f(N - 1), each index a constant
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) { each_of(std::make_integer_sequence<int, N>{}, f); }
+
+// The products of contractions of KB blocks with many outputs.  A wave keeps 32 rows of x as fragments in its registers, and the weight
+// goes by in LDS, 32 of its columns and the whole contraction a stage.  A workgroup is eight waves; it takes a run of pieces of (256 rows,
+// 64 columns), rows by rows: its ring of stages never empties, and x is read once, or twice where a tile is two workgroups'.
+//   What bounds hstu_rows8_gemm_kernel at a short contraction is that a tile's loads, products, epilogue and stores take turns.  Here the
+// products of a column block stand beside the epilogue of the one before it and a second wave of the SIMD beside both, and the stores go
+// on meanwhile.  73728 x 512 to 2048 with SiLU 148 us in tiles of 256 x 256, 90 so (1710 TFLOP/s, 3.8 TB/s), plain 129 and 80; 16398 x 1024 to
+// 4096 109 and 78; added to other rows, 73728 x 512 to 512 48 and 40; 73728 x 256 to 1024 56 and 41, x 64 to 256 16 and 13.  SiLU's two
+// quarter-rate instructions a value are as much work as the products are.  Two blocks of 32 rows a wave halve the reads of LDS and are no
+// faster (97 and 77).
+enum { ROWS_PLAIN, ROWS_SILU, ROWS_ADD };
+template <int KB, int OUT>
+__global__ __launch_bounds__(512, 2) void hstu_rows8_rows_kernel(const GemmParams g) {
+  constexpr int NS = 2 * KB, AHEAD = 1, STAGES = 3, GROUPS = (KB + 3) / 4, PITCH = KB * BLOCK;
+  constexpr int CODES = 32 * PITCH, STAGE = CODES + 256;
+  constexpr int LP = (4 * KB + 7) / 8, NLOAD = LP + 1;              // direct loads of 1 KB per wave and stage, and of exponents
+  constexpr int STORES = 4;
+  constexpr bool ADD = OUT == ROWS_ADD;
+  static_assert(KB <= 8 && NS % (AHEAD + 1) == 0 && STAGES == 3, "fragments keep their registers from step to step");
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const uint32_t smem_lds = __builtin_amdgcn_groupstaticsize();
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+
+  // this workgroup's run of pairs of column blocks, XCD by XCD
+  const int pairs = g.cols >> 6;
+  const int64_t all = (int64_t)g.row_tiles * pairs;
+  const int64_t me = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int64_t first = all * me / gridDim.x, last = all * (me + 1) / gridDim.x;
+  if (first >= last) return;
+  // (scalars, which a division leaves in vector registers)
+  int rt = __builtin_amdgcn_readfirstlane((int)(first / pairs)), pc = __builtin_amdgcn_readfirstlane((int)(first - (int64_t)rt * pairs));
+  int todo = __builtin_amdgcn_readfirstlane((int)(last - first));
+
+  // ---- the weight's stages: KB panels of 32 rows of 128 bytes, chunk c of row r at c ^ (r / 2 % 8); then the rows' exponents by groups
+  uint32_t po[LP], p_to[LP];
+#pragma unroll
+  for (int i = 0; i < LP; ++i) {
+    const int piece = (w + 8 * i) % (4 * KB), r = 8 * (piece & 3) + (lane >> 3);      // (more waves than pieces: some load the same)
+    po[i] = (uint32_t)(r * PITCH + BLOCK * (piece >> 2) + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+    p_to[i] = 1024u * piece;
+  }
+  const uint32_t eo = 4u * (uint32_t)l32 + (GROUPS > 1 ? (uint32_t)hh * 4u * (uint32_t)g.cols : 0u);
+  int column = 64 * pc, left = 2 * todo;               // of the next stage to load; stages left to load
+  auto load_stage = [&](int st) __attribute__((always_inline)) {
+    const uint32_t base = smem_lds + (uint32_t)st * STAGE;
+    const uint8_t* const from = scalar_ptr(g.w + (int64_t)column * PITCH);
+#pragma unroll
+    for (int i = 0; i < LP; ++i) lds_dma16(from, po[i], base + p_to[i]);
+    lds_dma4(scalar_ptr(g.we + (int64_t)column * 4), eo, base + CODES);
+    column = column + 32 == g.cols ? 0 : column + 32;
+    --left;
+  };
+  uint32_t fo[2][2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) fo[s][h] = (uint32_t)(l32 * BLOCK + 16 * ((4 * s + 2 * hh + h) ^ ((l32 >> 1) & 7)));
+  intx8 f[AHEAD + 1];
+  int we[2][GROUPS];                                   // of the stage at work, and of the one after it
+  auto ask = [&](int st, auto s_) __attribute__((always_inline)) {
+    constexpr int s = decltype(s_)::value;
+    const uint8_t* const at = smem + st * STAGE + 4096 * (s / 2);
+    struct { uint4v a, b; } both = {*(const uint4v*)(at + fo[s & 1][0]), *(const uint4v*)(at + fo[s & 1][1])};
+    f[s % (AHEAD + 1)] = __builtin_bit_cast(intx8, both);
+  };
+  auto exponents = [&](int st, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) we[to][i] = *(const int*)(smem + st * STAGE + CODES + 128 * i + 4 * l32);
+  };
+
+  intx8 xf[NS];
+  int xe[GROUPS];
+  auto load_rows = [&](int tile) __attribute__((always_inline)) {
+    int row = 256 * tile + 32 * w + l32;
+    row = row < g.rows ? row : g.rows - 1;             // (what a row past the end gives is not stored)
+    const uint8_t* const at = g.x + (int64_t)row * PITCH + 32 * hh;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      struct { uint4v a, b; } both = {*(const uint4v*)(at + 64 * s), *(const uint4v*)(at + 64 * s + 16)};
+      xf[s] = __builtin_bit_cast(intx8, both);
+    }
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) xe[i] = *(const int*)(g.xe + ((int64_t)i * g.rows + row) * 4);
+    // (waited for here: left to their first use, the waits would stand in the loop and be for every younger load and store in each round)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(xf[s]));
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) asm volatile("" : "+v"(xe[i]));
+  };
+
+  // ---- ADD: what is added is where a column block's sum begins, four columns of a lane's row at a time, a step ahead.  (Rows past the
+  // end: a buffer's loads past its last byte are zeros, its stores nothing, and all of them count.)
+  typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+  uint2v cv[4];
+  const uint32_t c_at = ADD ? (uint32_t)((32 * w + l32) * (int)g.c_stride + 4 * hh) * 2u : 0u;
+  auto bytes_of = [&](int tile, int64_t stride, int from) __attribute__((always_inline)) {
+    const int rows = g.rows - 256 * tile < 256 ? g.rows - 256 * tile : 256;
+    return (int)(((int64_t)(rows - 1) * stride + (g.cols - from)) * 2);
+  };
+  auto ask_added = [&](int tile, int from) __attribute__((always_inline)) {
+    const bf16_t* const base = (const bf16_t*)g.c + (int64_t)256 * tile * g.c_stride + from;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)scalar_ptr((const uint8_t*)base), 0, bytes_of(tile, g.c_stride, from), 0x00020000);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) cv[q] = __builtin_amdgcn_raw_buffer_load_b64(r, (int)c_at + 16 * q, 0, 0);
+  };
+  auto added_here = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(cv[q]));
+  };
+
+  // ---- the epilogue: 32 rows x 64 columns through the wave's own LDS in bf16, rows of 128 bytes, 8-byte piece c of row r at
+  // c ^ (r / 2 % 16) (written a column piece of all rows at a time, read a row at a time: all banks both ways)
+  uint8_t* const out_lds = smem + STAGES * STAGE + w * 4096;
+  const int wslot = (l32 >> 1) & 15;
+  floatx16 acc[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[1][i] = 0.f;        // (finished once before there is anything in it: into LDS, and not stored)
+  // part `q4` of 4 of a column block: four columns of a lane's row
+  auto finish = [&](auto par_, auto q_) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_)::value, q4 = decltype(q_)::value;
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = acc[par][4 * q4 + i];
+    if constexpr (OUT == ROWS_SILU) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = silu(z[i]);
+    }
+    *(uint2*)(out_lds + l32 * 128 + (((8 * par + 2 * q4 + hh) ^ wslot) * 8)) = uint2{pack2(z[0], z[1]), pack2(z[2], z[3])};
+  };
+  const bool halves = (lane >> 4) & 1;                 // (of 16 bytes, in the other order)
+  const uint32_t out_at = (uint32_t)((32 * w + (lane >> 3)) * (int)g.out_stride + 8 * (lane & 7)) * 2u;
+  const uint32_t out_step = 16u * (uint32_t)g.out_stride;
+  const uint8_t* to_out = (const uint8_t*)g.out;       // where the pair in LDS goes
+  int to_bytes = 0;
+  auto store = [&]() __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)scalar_ptr(to_out), 0, to_bytes, 0x00020000);
+    uint4v u[STORES];
+#pragma unroll
+    for (int i = 0; i < STORES; ++i) {
+      const int row = (lane >> 3) + 8 * i;
+      const uint4v v = *(const uint4v*)(out_lds + row * 128 + (((lane & 7) ^ ((row >> 2) & 7)) * 16));
+      u[i] = uint4v{halves ? v[2] : v[0], halves ? v[3] : v[1], halves ? v[0] : v[2], halves ? v[1] : v[3]};
+    }
+#pragma unroll
+    for (int i = 0; i < STORES; ++i) __builtin_amdgcn_raw_buffer_store_b128(u[i], r, (int)(out_at + i * out_step), 0, 2);
+  };
+
+  // ---- the run
+#pragma unroll
+  for (int t = 0; t < STAGES; ++t)
+    if (left > 0) load_stage(t);
+  load_rows(rt);
+  if constexpr (ADD) {
+    ask_added(rt, 64 * pc);
+    added_here();
+  }
+  ROWS8_WAIT_VMCNT(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  int st = 0;
+  exponents(0, 0);
+  each<AHEAD>([&](auto s) __attribute__((always_inline)) { ask(0, s); });
+  // One step: the products of a column block, the epilogue of the one before it, the stage after the next two on its way; in a pair's second
+  // step the rows of the pair before are stored.
+  auto step = [&](auto par_) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_)::value;
+    const int next = st + 1 == STAGES ? 0 : st + 1;
+    floatx16 begin;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) begin[i] = !ADD ? 0.f : __builtin_bit_cast(float, i % 2 ? cv[i / 4][i % 4 / 2] & 0xffff0000u : cv[i / 4][i % 4 / 2] << 16);
+    if constexpr (ADD) {
+      const bool turn = par == 1 && pc + 1 == pairs;
+      ask_added(turn ? (todo > 1 ? rt + 1 : rt) : rt, turn ? 0 : 64 * pc + (par == 0 ? 32 : 64));
+    }
+    if constexpr (par == 1) {
+      store();
+      to_out = (const uint8_t*)((const bf16_t*)g.out + (int64_t)256 * rt * g.out_stride + 64 * pc);
+      to_bytes = bytes_of(rt, g.out_stride, 64 * pc);
+    }
+    each<NS>([&](auto s_) __attribute__((always_inline)) {
+      constexpr int s = decltype(s_)::value, kb = s / 2;
+      if constexpr (s + AHEAD < NS) {
+        ask(st, std::integral_constant<int, s + AHEAD>{});
+      } else {
+        if constexpr (s + AHEAD == NS) {
+          // everyone's last read of this stage is done, the next stage is here, and this one's place can be filled again.  Younger than the
+          // next stage's loads: those of the one after it, and one pair's stores (in this step or the one before).
+          if constexpr (ADD) added_here();
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (left > 0) ROWS8_WAIT_VMCNT(NLOAD + STORES);
+          else ROWS8_WAIT_VMCNT(0);
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (left > 0) load_stage(st);
+          exponents(next, par ^ 1);
+        }
+        ask(next, std::integral_constant<int, s + AHEAD - NS>{});
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      acc[par] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f[s % (AHEAD + 1)], xf[s], s == 0 ? begin : acc[par], 0, 0, kb % 4, we[par][kb / 4], kb % 4, xe[kb / 4]);
+      // the block before this one, a share of it behind each product
+      each<4>([&](auto q) __attribute__((always_inline)) {
+        if constexpr (decltype(q)::value * NS / 4 == s) finish(std::integral_constant<int, par ^ 1>{}, q);
+      });
+      asm volatile("" : "+v"(acc[par]));               // (the product stays here: the compiler would move it to where its result is used)
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    st = next;
+  };
+  while (true) {
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    if (--todo == 0) break;
+    if (++pc == pairs) {
+      pc = 0;
+      load_rows(++rt);
+    }
+  }
+  each<4>([&](auto q) __attribute__((always_inline)) { finish(std::integral_constant<int, 1>{}, q); });
+  store();
+}
+
+// The products of up to 16 MT rows: a step of serving, where a call is a chain of latencies.  A workgroup takes 16 output columns and its
+// waves one block of the contraction each in turn, straight from memory into their registers; their sums are added in LDS in the waves'
+// order.  1 x 1024 to 4096 3.0 us (in tiles of 64 x 64, whose stages follow each other, 4.7), 1 x 8192 to 8192 14 us (4.6 TB/s).
+constexpr int FEW_WAVES = 8;
+template <int MT, bool F32>
+__global__ __launch_bounds__(64 * FEW_WAVES) void hstu_rows8_few_kernel(const GemmParams g) {
+  __shared__ floatx4 sums[FEW_WAVES][MT][64];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int l16 = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int64_t pitch = (int64_t)g.blocks * BLOCK;
+  // (rows past an operand's end are its last one: what they give is not stored)
+  const int n = n0 + l16 < g.cols ? n0 + l16 : g.cols - 1;
+  const uint8_t* const wr = g.w + n * pitch + 32 * q;
+  const uint8_t* xr[MT];
+  int m[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t] = 16 * t + l16 < g.rows ? 16 * t + l16 : g.rows - 1;
+    xr[t] = g.x + m[t] * pitch + 32 * q;
+  }
+  floatx4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto codes_of = [&](const uint8_t* at) __attribute__((always_inline)) {
+    struct { uint4v a, b; } both = {*(const uint4v*)at, *(const uint4v*)(at + 16)};
+    return __builtin_bit_cast(intx8, both);
+  };
+#pragma unroll 2
+  for (int kb = w; kb < g.blocks; kb += waves) {
+    const intx8 wf = codes_of(wr + kb * BLOCK);
+    const int ws = g.we[((int64_t)(kb >> 2) * g.cols + n) * 4 + (kb & 3)];
+    intx8 xf[MT];
+    int xs[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      xf[t] = codes_of(xr[t] + kb * BLOCK);
+      xs[t] = g.xe[((int64_t)(kb >> 2) * g.rows + m[t]) * 4 + (kb & 3)];
+    }
+    if constexpr (F32) {
+      const float wp = power_of((uint32_t)ws);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values8(wf, i, wp), values8(xf[t], i, power_of((uint32_t)xs[t])), acc[t], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[t], acc[t], 0, 0, 0, ws, 0, xs[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) sums[w][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = w; t < MT; t += waves) {
+    floatx4 y = sums[0][t][lane];
+    for (int i = 1; i < waves; ++i) {
+      const floatx4 v = sums[i][t][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += v[e];
+    }
+    // the lane's four columns of row 16 t + l16
+    const int row = 16 * t + l16, at = n0 + 4 * q;
+    if (row >= g.rows || at >= g.cols) continue;
+    if (g.c) add4<F32>(g.c, (int64_t)row * g.c_stride, at, g.cols, g.vec, y);
+    if (g.bias) add4<F32>(g.bias, 0, at, g.cols, g.vec, y);
+    if (g.activation) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = silu(y[e]);
+    }
+    if (g.vec) {
+      if constexpr (F32) *(floatx4*)((float*)g.out + (int64_t)row * g.out_stride + at) = y;
+      else *(uint2*)((bf16_t*)g.out + (int64_t)row * g.out_stride + at) = uint2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at + e < g.cols) {
+          if constexpr (F32) ((float*)g.out)[(int64_t)row * g.out_stride + at + e] = y[e];
+          else ((bf16_t*)g.out)[(int64_t)row * g.out_stride + at + e] = (bf16_t)y[e];
+        }
+    }
+  }
+}
+
 // Raises a kernel's limit of dynamic LDS, once per device.
 int allow_lds(const void* fn, int bytes, int* granted) {
   int dev = 0;
@@ -351,12 +703,77 @@ int launch_tiles(GemmParams g, hipStream_t st) {
   return rows8_launched("hstu_rows8_gemm");
 }
 
+template <int MT, bool F32>
+int launch_few(const GemmParams& g, hipStream_t st) {
+  const int waves = g.blocks < FEW_WAVES ? g.blocks : FEW_WAVES;
+  hstu_rows8_few_kernel<MT, F32><<<(uint32_t)((g.cols + 15) / 16), 64 * waves, 0, st>>>(g);
+  return rows8_launched("hstu_rows8_gemm");
+}
+
+template <int KB, int OUT>
+int launch_rows(GemmParams g, hipStream_t st) {
+  constexpr int LDS = 3 * (32 * KB * BLOCK + 256) + 8 * 4096;
+  static int granted[64];
+  const void* const fn = (const void*)hstu_rows8_rows_kernel<KB, OUT>;
+  if (const int rc = allow_lds(fn, LDS, granted)) return rc;
+  g.row_tiles = (g.rows + 255) / 256;
+  hstu_rows8_rows_kernel<KB, OUT><<<256, 512, LDS, st>>>(g);
+  return rows8_launched("hstu_rows8_gemm");
+}
+
+template <int OUT>
+int launch_rows(const GemmParams& g, hipStream_t st) {
+  switch (g.blocks) {
+    case 1: return launch_rows<1, OUT>(g, st);
+    case 2: return launch_rows<2, OUT>(g, st);
+    case 3: return launch_rows<3, OUT>(g, st);
+    case 4: return launch_rows<4, OUT>(g, st);
+    case 5: return launch_rows<5, OUT>(g, st);
+    case 6: return launch_rows<6, OUT>(g, st);
+    case 7: return launch_rows<7, OUT>(g, st);
+    default: return launch_rows<8, OUT>(g, st);
+  }
+}
+
+// Whether the weight goes by rows kept in registers: bf16 results of contractions of up to 1024, whole pieces of 64 columns, at least three
+// pieces for each of the 256 workgroups (two: 4000 x 512 to 2048 12 us either way, 8000 x 512 to 2048, four of them, 16 against 19 in
+// tiles), and a quarter of the last rows' tile wasted at most.  What it does behind the product is one of three.
+bool rows_take(const GemmParams& g) {
+  const int64_t tiles = ((int64_t)g.rows + 255) / 256, pieces = tiles * (g.cols / 64);
+  return g.blocks <= 8 && g.cols % 64 == 0 && g.vec && !g.bias && !(g.c && g.activation) && pieces >= 768 && 4 * (int64_t)g.rows >= 3 * 256 * tiles &&
+         g.out_stride < 1 << 21 && g.c_stride < 1 << 21 && g.cols < 1 << 29;
+}
+
+// Up to 16 rows, or 32 where the weight is a small one, are latencies: 16 x 1024 to 4096 3.4 us, in tiles 4.8; 32 of them 3.7.  They are not where
+// a great many columns of a short contraction read their rows of x anew every 16 columns: 8 x 512 to 100000 13.1 us, in tiles 10.9;
+// 20000 columns 3.8 and 4.3, 1 x 8192 to 8192 14 and 20.
+int few_take(const GemmParams& g) {
+  if (g.rows <= 16 && (g.cols <= 32768 || g.blocks >= 16)) return 1;
+  return g.rows <= 32 && g.cols <= 8192 && g.blocks <= 16 ? 2 : 0;
+}
+
 template <bool F32>
 int launch(const GemmParams& g, hipStream_t st) {
-  auto tiles = [&](int64_t t) { return ((g.rows + t - 1) / t) * ((g.cols + t - 1) / t); };
-  if (tiles(256) >= 192) return launch_tiles<4, 2, 2, 4, 2, F32>(g, st);
-  if (tiles(128) >= 192) return launch_tiles<2, 2, 2, 2, 2, F32>(g, st);
-  return launch_tiles<1, 1, 2, 2, 4, F32>(g, st);
+  if (const int few = few_take(g)) return few == 1 ? launch_few<1, F32>(g, st) : launch_few<2, F32>(g, st);
+  if constexpr (!F32) {
+    if (rows_take(g)) return g.c ? launch_rows<ROWS_ADD>(g, st) : g.activation ? launch_rows<ROWS_SILU>(g, st) : launch_rows<ROWS_PLAIN>(g, st);
+  }
+  // The tile under which the call is shortest: rounds of as many tiles as the chip holds (1, 2 and 4 to a CU), each of them a fixed time and one
+  // for each block of the contraction, in us as 73728 x 512 to 2048 and 16384 x 8192 by 8192 measure them.
+  const float fixed[3] = {F32 ? 13.3f : 8.5f, F32 ? 6.1f : 4.1f, F32 ? 2.9f : 1.8f}, block[3] = {F32 ? 3.0f : 1.76f, F32 ? 1.7f : 0.92f, F32 ? 1.1f : 0.77f};
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t t = 256 >> i, tiles = (((int64_t)g.rows + t - 1) / t) * (((int64_t)g.cols + t - 1) / t), chip = 256 << i;
+    const float us = (float)((tiles + chip - 1) / chip) * (fixed[i] + block[i] * (float)g.blocks);
+    if (i == 0 || us < least) { best = i; least = us; }
+  }
+  if (best == 0) return launch_tiles<4, 2, 2, 4, 2, F32>(g, st);
+  if (best == 1) return launch_tiles<2, 2, 2, 2, 2, F32>(g, st);
+  // Four stages instead of two halve the workgroups of a CU: that pays where long rows come from past the L2s (64 x 8192 to 8192 20 us
+  // against 30, 200 x 4096 to 4096 12.7 and 12.2, 64 x 512 to 100000 14.6 and 12.6).
+  const bool far = g.blocks >= 16 && ((int64_t)g.rows + g.cols) * g.blocks * BLOCK > 32 << 20;
+  return far ? launch_tiles<1, 1, 2, 2, 4, F32>(g, st) : launch_tiles<1, 1, 2, 2, 2, F32>(g, st);
 }
 
 int gemm(const HstuRows8GemmArgs* a, void* stream) {

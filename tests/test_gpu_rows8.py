@@ -1,11 +1,13 @@
 """Rows in 8 bits: quantising, norms into them, what they stand for, and their products, against 64 bits."""
 
+import ctypes as C
 import threading
 
 import pytest
 import torch
 
 import recml_amd
+from recml_amd import _lib_rows8
 from tests import rows8_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -182,6 +184,41 @@ def test_large_product(gpu, rows, depth, cols, dtype):
     off = R.product_off(y, before, size, depth, dtype, False)
     got = recml_amd.gemm_rows8(x, w, residual=c, dtype=dtype)
     assert float(((got.double() - y).abs() - off).max()) <= 0
+
+
+@pytest.mark.parametrize("how", ["plain", "silu", "added"])
+@pytest.mark.parametrize("depth", [40, 256, 300, 512, 640, 700, 896, 1024])
+def test_many_outputs_of_short_contractions(gpu, depth, how):
+  """Rows kept in registers: every number of blocks, a last tile that is not whole, runs that begin and end inside a tile."""
+  rows, cols = 256 * 11 - 37, 64 * 75
+  x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
+  c = torch.randn((rows, cols + 8), generator=_gen(depth)).to(BF16).to(gpu)[:, :cols] if how == "added" else None
+  got = recml_amd.gemm_rows8(x, w, None, how == "silu", residual=c)
+  y, before, sizes = R.product(R.values(x.codes, x.exponents, depth).to(gpu), R.values(w.codes, w.exponents, depth).to(gpu), None, c, how == "silu")
+  assert float(((got.double() - y).abs() - R.product_off(y, before, sizes, depth, BF16, how == "silu")).max()) <= 0
+  assert torch.equal(got, recml_amd.gemm_rows8(x, w, None, how == "silu", residual=c))
+  if c is None:                                # (with a bias the call goes by tiles, whose sums are the same)
+    assert torch.equal(got, recml_amd.gemm_rows8(x, w, torch.zeros(cols, dtype=BF16, device=gpu), how == "silu"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,depth,cols", [(1, 128, 24), (20, 300, 40), (50, 300, 72), (300, 200, 136), (2000, 200, 1032), (7000, 200, 2120), (2779, 500, 4800)])
+def test_leaves_what_is_not_its_own(gpu, rows, depth, cols, dtype):
+  """Rows with a stride of their own in the middle of a buffer: what stands between, before and behind them stays."""
+  x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
+  stride, unit = cols + 8, 16
+  buffer = torch.full((unit + rows * stride + unit,), 7.0, dtype=dtype, device=gpu)
+  a = _lib_rows8.HstuRows8GemmArgs()
+  a.struct_size, a.version = C.sizeof(a), _lib_rows8.ABI_VERSION
+  x._fill(a.x)
+  w._fill(a.w)
+  a.dtype, a.out, a.out_stride = (_lib_rows8.FP32 if dtype == F32 else _lib_rows8.BF16), buffer[unit:].data_ptr(), stride
+  assert _lib_rows8.load().hstu_rows8_gemm(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+  torch.cuda.synchronize()
+  assert (buffer[:unit] == 7).all() and (buffer[-unit:] == 7).all()
+  body = buffer[unit:-unit].view(rows, stride)
+  assert (body[:, cols:] == 7).all()
+  assert torch.equal(body[:, :cols], recml_amd.gemm_rows8(x, w, dtype=dtype))
 
 
 def test_sums_in_fp32(gpu):
