@@ -13,7 +13,8 @@ entries with torch's dropout; in eval mode neither does anything.  Parameters ar
 `requires_grad_(True)` makes them trainable.
 
 For serving, HSTU.new_cache, prefill and extend keep users' histories (hstu_serving.HSTUCache, hstu_cache_ops) and run the
-model on new events alone; HSTU.log_probs scores items under the head, differentiably (hstu_scores).
+model on new events alone; HSTU.log_probs scores items under the head, differentiably (hstu_scores).  HSTU.quantize keeps the
+blocks' weights in 8 bits for inference: norms, products and gate then go through hstu_rows8, whatever form the call has.
 
 Mirrors, name for name:
   HSTUBlock   recml/layers/keras/hstu.py:240-474 (weights :281-354, call :422-474)
@@ -39,6 +40,7 @@ from recml_amd import _native
 from recml_amd import hstu_block_ops
 from recml_amd import hstu_cache_ops
 from recml_amd import hstu_ops
+from recml_amd import hstu_rows8
 from recml_amd import hstu_scores
 from recml_amd import hstu_serving
 from recml_amd import masks
@@ -134,6 +136,16 @@ def _glorot_uniform(shape, fan_in, fan_out, generator, dtype, device):
   return w.to(device=device, dtype=dtype)
 
 
+def _versions(tensors):
+  """Which tensors they are, and how often they were written to (so that a copy of them knows whether it still is one)."""
+  return tuple((t, 0 if t.is_inference() else t._version) for t in tensors if t is not None)
+
+
+def _unchanged(kept, tensors) -> bool:
+  now = _versions(tensors)
+  return len(now) == len(kept) and all(a is b and m == n for (a, m), (b, n) in zip(kept, now))
+
+
 class HSTUBlock(torch.nn.Module):
   """One HSTU block: LN -> U,Q,K,V = act(x W) -> pointwise attention -> LN over
   (heads, head_dim) -> U * normed -> output projection -> + inputs
@@ -186,6 +198,35 @@ class HSTUBlock(torch.nn.Module):
       rf *= s
     return shape[-2] * rf, shape[-1] * rf
 
+  _rows8 = None      # the weights in 8 bits: projections, their bias, output product, and what they were made of
+
+  def quantize(self) -> None:
+    """Keeps the projections' and the output product's weights in 8 bits (hstu_rows8.Rows8): every call of the block then runs its norms,
+    products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
+    a change to them quantize() has to be called again (a call notices and raises).  `dequantize` goes back."""
+    with torch.no_grad():
+      w, b = self._uqkv_weights()
+      out = self.output_kernel.reshape(-1, self.hidden_dim)
+      kept = hstu_rows8.quantize_rows(w.t()), b, hstu_rows8.quantize_rows(out.t())
+    self._rows8 = (*kept, _versions(self._quantized_weights()))
+
+  def dequantize(self) -> None:
+    """Back to the parameters' own type."""
+    self._rows8 = None
+
+  def _quantized_weights(self):
+    """The parameters that quantize copied (not those that something else, a parametrization say, makes anew for each call)."""
+    P = self._parameters
+    names = [f"{n}_{kind}" for kind in (("kernel", "bias") if self.use_bias else ("kernel",)) for n in ("u", "q", "k", "v")] + ["output_kernel"]
+    return [P[n] for n in names if n in P]
+
+  def _check_rows8(self, *inputs):
+    """Whether a call of a block with weights in 8 bits can be one; raises if not."""
+    if self._wants_grad(*inputs):
+      raise ValueError("a block with its weights in 8 bits has no gradient: call it under torch.no_grad(), or dequantize() it first")
+    if not _unchanged(self._rows8[3], self._quantized_weights()):
+      raise ValueError("the block's weights have changed since quantize(): call it again")
+
   def _dropout_kw(self, dropout_seed=None) -> dict:
     """The attention's dropout arguments for this call: none in eval mode or at rate 0; in training mode the
     block's rate and a seed from torch's CPU generator (so torch.manual_seed makes a run repeatable, and no GPU
@@ -226,7 +267,7 @@ class HSTUBlock(torch.nn.Module):
       return self._train_steps(inputs.reshape(B * L, D), (B, L), pos_bias, ts_bias, batch,
                                dict(seq_lens=seq_lens, n=n, alpha=alpha, timestamps=timestamps, **drop)).reshape(B, L, D)
     fused = self._fused_inference(inputs, pos_bias, ts_bias, attention_bias)
-    u, q, k, v = self._project(self._input_norm(inputs, fused).reshape(B * L, D), (B, L), fused).unbind(dim=2)
+    u, q, k, v = self._uqkv(inputs.reshape(B * L, D), (B, L), fused).unbind(dim=2)
     if attention_mask is not None:
       # the reference's calling convention: a dense [B, L, L] mask and bias (training: forward and backward kernels,
       # the gradient of a dense bias included)
@@ -256,10 +297,21 @@ class HSTUBlock(torch.nn.Module):
       uqkv = F.silu(uqkv if b is None else uqkv + b)
     return uqkv.reshape(*lead, 4, self.num_heads, self.head_dim)
 
+  def _uqkv(self, rows, lead, fused):
+    """U, Q, K, V of rows [T, D] as they come in: norm and projections."""
+    if self._rows8 is None:
+      return self._project(self._input_norm(rows, fused), lead, fused)
+    w, b = self._rows8[:2]
+    normed = hstu_rows8.norm_rows8(rows, self.input_ln_gamma, self.input_ln_beta, self.eps)
+    return hstu_rows8.gemm_rows8(normed, w, b, True, dtype=rows.dtype).reshape(*lead, 4, self.num_heads, self.head_dim)
+
   def _gate_and_output(self, attn, u, residual, fused):
     """Attention norm, U gate, output product and residual, on rows.  `fused`: norm and gate in one pass, rounded once, and the
     residual as the product's C operand."""
     W = attn.shape[-1]
+    if self._rows8 is not None:
+      gated = hstu_rows8.norm_rows8(attn, self.attn_ln_gamma, self.attn_ln_beta, self.eps, gate=u)
+      return hstu_rows8.gemm_rows8(gated, self._rows8[2], self.output_bias if self.use_bias else None, residual=residual, dtype=residual.dtype)
     gamma, beta, w = self.attn_ln_gamma.reshape(-1), self.attn_ln_beta.reshape(-1), self.output_kernel.reshape(W, self.hidden_dim)
     if fused:
       return hstu_block_ops.gemm_silu(hstu_block_ops.norm_gate(attn, u, gamma, beta, self.eps), w, self.output_bias, False, residual=residual)
@@ -313,6 +365,9 @@ class HSTUBlock(torch.nn.Module):
                     attention_mask=None, attention_bias=None):
     """The block through its HIP kernels, forward and backward, as one native call (recml_amd/csrc/native.cpp: block): bf16 on a
     GPU, parameters ready as they are.  None where it does not apply: fp32, a dense mask or bias with gradients, ..."""
+    if self._rows8 is not None:
+      self._check_rows8(tokens, pos_bias, ts_bias, attention_bias)
+      return None
     if tokens.dtype != torch.bfloat16 or not tokens.is_cuda:
       return None
     weights = self._weights()
@@ -365,7 +420,7 @@ class HSTUBlock(torch.nn.Module):
       return self._train_steps(tokens, (T,), pos_bias, ts_bias, batch,
                                dict(seq_offsets=seq_offsets, max_len=max_len, n=n, alpha=alpha, timestamps=timestamps, **drop))
     fused = self._fused_inference(tokens, pos_bias, ts_bias)
-    u, q, k, v = self._project(self._input_norm(tokens, fused), (T,), fused).unbind(dim=1)
+    u, q, k, v = self._uqkv(tokens, (T,), fused).unbind(dim=1)
     attn = _attention(q, k, v, seq_offsets=seq_offsets, max_len=max_len, n=n, alpha=alpha,
                       pos_bias=pos_bias, timestamps=timestamps, ts_bias=ts_bias, batch=batch, **drop)
     return self._gate_and_output(attn.reshape(T, H * hd), u.reshape(T, H * hd), tokens, fused)
@@ -386,8 +441,10 @@ class HSTUBlock(torch.nn.Module):
     lead = tokens.shape[:-1]
     with torch.no_grad():
       rows = tokens.reshape(-1, D)
+      if self._rows8 is not None:
+        self._check_rows8()
       fused = self._fused_inference(rows)
-      u, q, k, v = self._project(self._input_norm(rows, fused), lead, fused).unbind(dim=-3)
+      u, q, k, v = self._uqkv(rows, lead, fused).unbind(dim=-3)
       hstu_cache_ops.kv_write(pages, k, v, page_table, starts, offsets=offsets, max_new=max_new)
       alpha, n = self._alpha_n(max_len)
       if whole:
@@ -405,7 +462,7 @@ _OWN_BLOCK_FORWARDS = HSTUBlock.forward, HSTUBlock.forward_jagged
 def _is_plain_call(block, jagged) -> bool:
   """Whether a call of the block is a call of HSTUBlock's own forward and nothing else: no subclass, no forward put in its place, and, where
   it is called as a module (the packed form calls forward_jagged itself), no hooks on it or on all modules, and not compiled."""
-  if type(block) is not HSTUBlock or (HSTUBlock.forward, HSTUBlock.forward_jagged) != _OWN_BLOCK_FORWARDS:
+  if type(block) is not HSTUBlock or block._rows8 is not None or (HSTUBlock.forward, HSTUBlock.forward_jagged) != _OWN_BLOCK_FORWARDS:
     return False
   own = block.__dict__
   if jagged:
@@ -456,6 +513,26 @@ class HSTU(torch.nn.Module):
     self.eps = norm_eps
     self.scale_by_sqrt_dim = scale_by_sqrt_dim
     self.dropout = float(dropout)      # on the embeddings here (hstu.py:541-543, 602), on the attention weights in the blocks
+
+  _head8 = None      # the head's weight in 8 bits, and what it was made of
+
+  def quantize(self, *, head: bool = False) -> None:
+    """Keeps the blocks' weights in 8 bits (HSTUBlock.quantize), and with `head` the head's: forward, prefill and extend then run their
+    products on them, in inference only, on a GPU.  The parameters stay as they are; call it again after a change to them."""
+    if head and self.reverse_embedding is None:
+      raise ValueError("the model has no output head")
+    for block in self.decoder_blocks:
+      block.quantize()
+    self._head8 = None
+    if head:
+      with torch.no_grad():
+        self._head8 = hstu_rows8.quantize_rows(self.reverse_embedding.t()), _versions([self.reverse_embedding])
+
+  def dequantize(self) -> None:
+    """Back to the parameters' own type."""
+    for block in self.decoder_blocks:
+      block.dequantize()
+    self._head8 = None
 
   def count_params(self) -> int:
     return sum(p.numel() for p in self.parameters())
@@ -533,6 +610,13 @@ class HSTU(torch.nn.Module):
                           None if offsets is None else length, pos_bias, gamma, beta, self.eps)
 
   def _head(self, x):
+    if self._head8 is not None:
+      w, made_of = self._head8
+      if not _unchanged(made_of, [self.reverse_embedding]):
+        raise ValueError("the head's weight has changed since quantize(): call it again")
+      if _differentiates(x, self.reverse_embedding):
+        raise ValueError("a head with its weight in 8 bits has no gradient: call it under torch.no_grad(), or dequantize() the model first")
+      return hstu_rows8.gemm_rows8(hstu_rows8.quantize_rows(x), w, dtype=x.dtype).reshape(*x.shape[:-1], w.rows)
     out = _native.linear(x, self.reverse_embedding, True)
     return x @ self.reverse_embedding if out is None else out
 

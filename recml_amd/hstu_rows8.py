@@ -101,6 +101,9 @@ class Rows8:
   def __setattr__(self, name, value):
     raise AttributeError("Rows8 are what they were made of: make new ones")
 
+  def __reduce__(self):
+    return Rows8, (self.codes, self.exponents, self.width)
+
   def __repr__(self):
     return f"Rows8({self.rows} rows of {self.width} on {self.codes.device})"
 
