@@ -60,47 +60,32 @@ __device__ __forceinline__ float silu(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
 
-// Eight values of a row of the output's type from column `col` on; past `cols` zeros, and nothing stored.
 template <bool F32>
-__device__ __forceinline__ void row_load8(const void* base, int64_t at, int col, int cols, bool vec, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 0.f;
-  if (vec) {
-    if (col >= cols) return;
-    if constexpr (F32) {
-      const floatx4* const from = (const floatx4*)((const float*)base + at + col);
-      const floatx4 lo = from[0], hi = from[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
-    } else {
-      unpack8(*(const uint4v*)((const bf16_t*)base + at + col), f);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < cols) f[i] = F32 ? ((const float*)base)[at + col + i] : (float)((const bf16_t*)base)[at + col + i];
+__device__ __forceinline__ float value_of(const void* base, int64_t at) {
+  return F32 ? ((const float*)base)[at] : (float)((const bf16_t*)base)[at];
 }
 
+// Eight values of the output's type, side by side on a 16-byte boundary.
 template <bool F32>
-__device__ __forceinline__ void row_store8(void* base, int64_t at, int col, int cols, bool vec, const float (&f)[8]) {
-  if (vec) {
-    if (col >= cols) return;
-    if constexpr (F32) {
-      floatx4* const to = (floatx4*)((float*)base + at + col);
-      to[0] = floatx4{f[0], f[1], f[2], f[3]};
-      to[1] = floatx4{f[4], f[5], f[6], f[7]};
-    } else {
-      *(uint4v*)((bf16_t*)base + at + col) = pack8(f);
-    }
-    return;
-  }
+__device__ __forceinline__ void row_load8(const void* base, int64_t at, float (&f)[8]) {
+  if constexpr (F32) {
+    const floatx4* const from = (const floatx4*)((const float*)base + at);
+    const floatx4 lo = from[0], hi = from[1];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (col + i < cols) {
-      if constexpr (F32) ((float*)base)[at + col + i] = f[i];
-      else ((bf16_t*)base)[at + col + i] = (bf16_t)f[i];
-    }
+    for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
+  } else {
+    unpack8(*(const uint4v*)((const bf16_t*)base + at), f);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ void row_store8(void* base, int64_t at, const float (&f)[8]) {
+  if constexpr (F32) {
+    floatx4* const to = (floatx4*)((float*)base + at);
+    to[0] = floatx4{f[0], f[1], f[2], f[3]};
+    to[1] = floatx4{f[4], f[5], f[6], f[7]};
+  } else {
+    *(uint4v*)((bf16_t*)base + at) = pack8(f);      // (past the L2s, as the bf16 products store large outputs, it is no faster)
+  }
 }
 
 // Four values of a row added, from column `at` on; none past `cols`.
@@ -122,7 +107,7 @@ __device__ __forceinline__ void add4(const void* base, int64_t row, int at, int 
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (at + i < cols) y[i] += F32 ? ((const float*)base)[row + at + i] : (float)((const bf16_t*)base)[row + at + i];
+    if (at + i < cols) y[i] += value_of<F32>(base, row + at + i);
 }
 
 // Eight of a lane's 32 codes as the values that they stand for, exact in bf16.
@@ -140,14 +125,116 @@ constexpr int lds_bytes(int mb, int nb, int wm, int wn, int stages) {
   return ring > out ? ring : out;
 }
 
+// Which tile a workgroup has; false: none.  Workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, which go by eight
+// rows of tiles at a time.
+__device__ __forceinline__ bool tile_of(const GemmParams& g, int* rt, int* ct) {
+  const int all = g.row_tiles * g.col_tiles, each = (all + 7) >> 3;
+  const int tile = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= each || tile >= all) return false;
+  const int band = tile / (8 * g.col_tiles), in_band = tile - band * 8 * g.col_tiles;
+  const int high = g.row_tiles - 8 * band < 8 ? g.row_tiles - 8 * band : 8;
+  *ct = in_band / high;
+  *rt = 8 * band + in_band - *ct * high;
+  return true;
+}
+
+// A wave's sums on their way out: blocks of 32 rows x 32 NB columns from (m0, n0) on, through the wave's own LDS (fp32, rows 16 bytes apart
+// from a multiple of 128), then pieces of 8 columns of a row per lane; where rows are not whole vectors, one column per lane (1237 x 1001 to
+// 777 in fp32 12.9 us with pieces of single values, 9.5 so).
+template <int MB, int NB, bool F32>
+__device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&acc)[NB][MB], uint8_t* stage, int m0, int n0) {
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
+  constexpr int W = 32 * NB, PITCH = W * 4 + 16;
+  auto put = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < NB; ++a)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *(floatx4*)(stage + l32 * PITCH + (32 * a + 8 * q4 + 4 * hh) * 4) =
+            floatx4{acc[a][b][4 * q4], acc[a][b][4 * q4 + 1], acc[a][b][4 * q4 + 2], acc[a][b][4 * q4 + 3]};
+    __builtin_amdgcn_wave_barrier();
+  };
+  if (!g.vec) {
+    constexpr int ROWS = 64 / W;                       // of an instruction
+    const int col = lane % W, n = n0 + col;
+    const bool in = n < g.cols;
+    const float bias = g.bias && in ? value_of<F32>(g.bias, n) : 0.f;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      put(b);
+#pragma unroll 8
+      for (int i = 0; i < 32 / ROWS; ++i) {
+        const int row = ROWS * i + lane / W, m = m0 + 32 * b + row;
+        if (!in || m >= g.rows) continue;
+        float y = *(const float*)(stage + row * PITCH + 4 * col);
+        if (g.c) y += value_of<F32>(g.c, (int64_t)m * g.c_stride + n);
+        y += bias;
+        if (g.activation) y = silu(y);
+        const int64_t to = (int64_t)m * g.out_stride + n;
+        if constexpr (F32) ((float*)g.out)[to] = y;
+        else ((bf16_t*)g.out)[to] = (bf16_t)y;
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    return;
+  }
+  constexpr int LPR = W / 8, RPI = 64 / LPR, PIECES = 32 / RPI;        // lanes per row, rows per instruction
+  const int rr = lane / LPR, cc = lane - rr * LPR;
+  const int n = n0 + 8 * cc;
+  float bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = 0.f;
+  if (g.bias && n < g.cols) row_load8<F32>(g.bias, n, bias);
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    put(b);
+    float y[PIECES][8];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const uint8_t* at = stage + (RPI * i + rr) * PITCH + 32 * cc;
+      const floatx4 lo = *(const floatx4*)at, hi = *(const floatx4*)(at + 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { y[i][e] = lo[e]; y[i][4 + e] = hi[e]; }
+    }
+    const int mb = m0 + 32 * b + rr;      // the lane's row of piece 0
+    auto inside = [&](int i) __attribute__((always_inline)) { return mb + RPI * i < g.rows && n < g.cols; };
+    if (g.c) {
+      float cv[PIECES][8];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cv[i][e] = 0.f;
+        if (inside(i)) row_load8<F32>(g.c, (int64_t)(mb + RPI * i) * g.c_stride + n, cv[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[i][e] += cv[i][e];
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[i][e] += bias[e];
+    if (g.activation) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[i][e] = silu(y[i][e]);
+    }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+      if (inside(i)) row_store8<F32>(g.out, (int64_t)(mb + RPI * i) * g.out_stride + n, y[i]);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // One workgroup: a tile of 32 MB WM rows of x by 32 NB WN rows of w (output columns), WM x WN waves of 32 MB x 32 NB.  The contraction runs
 // in stages of one block of 128 through an LDS ring filled by direct loads; a stage is the codes of both operands and their rows' exponents
 // (the four of a group at once: one byte of them is read).  The product is formed transposed (columns as the matrix instruction's rows): a
 // lane then holds four consecutive columns of one output row.
 //   A row's 128 bytes lie in LDS as eight 16-byte chunks, chunk c of row r at c ^ (r / 2 % 8): 16 rows reach all 64 banks.  Which
 // contraction elements a lane holds does not matter as long as both operands' lanes hold the same ones.
-//   128 x 64 a wave for the reason of the bf16 products: with 64 x 64 the four SIMDs' fragments take all of the LDS bandwidth at full matrix
-// rate, with 128 x 64 three quarters of it.  16384 x 8192 by 8192 in 870 us (2530 TFLOP/s), in tiles of 128 x 128 940, of 64 x 64 1580.
+//   For results in bf16 the tiles are of 128 x 128 and less (hstu_rows8_turns_kernel has the larger ones).
 template <int MB, int NB, int WM, int WN, int STAGES, bool F32>
 __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const GemmParams g) {
   constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN, WAVES = WM * WN;
@@ -162,13 +249,8 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
 
-  // Workgroups go to the eight XCDs in turn: each XCD takes a run of the tiles, which go by eight rows of tiles at a time.
-  const int all = g.row_tiles * g.col_tiles, each = (all + 7) >> 3;
-  const int tile = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= each || tile >= all) return;
-  const int band = tile / (8 * g.col_tiles), in_band = tile - band * 8 * g.col_tiles;
-  const int high = g.row_tiles - 8 * band < 8 ? g.row_tiles - 8 * band : 8;
-  const int ct = in_band / high, rt = 8 * band + in_band - ct * high;
+  int rt, ct;
+  if (!tile_of(g, &rt, &ct)) return;
   const int m0 = rt * TM, n0 = ct * TN, nt = g.blocks;
 
   // ---- what each lane loads: piece i of an operand is 8 rows, lane l of it the 16 bytes at row l / 8, place l % 8.  Rows past an operand's
@@ -309,60 +391,153 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
     st = st + 1 >= STAGES ? 0 : st + 1;
   }
 
-  // ---- out: blocks of 32 rows x 32 NB columns through the wave's own LDS (fp32, rows 16 bytes apart from a multiple of 128), then
-  // pieces of 8 columns of a row per lane
-  constexpr int W = 32 * NB, PITCH = W * 4 + 16;
-  uint8_t* stage = smem + w * (32 * PITCH);
-  constexpr int LPR = W / 8, RPI = 64 / LPR, PIECES = 32 / RPI;        // lanes per row, rows per instruction
-  const int rr = lane / LPR, cc = lane - rr * LPR;
-  const int n = n0 + wn * W + 8 * cc;
-  const bool vec = g.vec;
-  float bias[8];
+  tile_out<MB, NB, F32>(g, acc, smem + w * (32 * (32 * NB * 4 + 16)), m0 + 32 * MB * wm, n0 + 32 * NB * wn);
+}
+
+// The same product where there is work for tiles of 256 x 256 and a contraction to stream.  Eight waves of 128 x 64 in two halves, one wave of
+// each to a SIMD, that take turns: while one half forms a stage's products the other reads its fragments of the next from LDS and asks for
+// more of it, and a barrier changes them over.  So the matrix pipe and LDS are both at work all the time, where waves that go in step leave
+// each idle in turn.  16384 x 8192 by 8192 in 829 us (2650 TFLOP/s; in step 941), 8192 of each 421 (in step 497), 16384 x 2048 to 8192 249
+// (282).  What bounds it is power: the matrix pipe is at work two thirds of the time, at a clock of 1.8 GHz that waves in step, 58 %, find at
+// 2.0.  Four waves of 128 x 128, which read a third less of LDS, one to a SIMD, with the loads between their products, took 914.
+__global__ __launch_bounds__(512, 2) void hstu_rows8_turns_kernel(const GemmParams g) {
+  constexpr int T = 256, X_BYTES = T * BLOCK, CODES = 2 * X_BYTES, STAGE = stage_bytes(T, T);
+  constexpr int L = T / 8 / 8, NLOAD = 2 * L + 1;              // direct loads of 8 rows a wave and operand; of 64 rows' exponents
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const uint32_t smem_lds = __builtin_amdgcn_groupstaticsize();
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  int rt, ct;
+  if (!tile_of(g, &rt, &ct)) return;
+  const int m0 = rt * T, n0 = ct * T, nt = g.blocks;
+
+  // ---- what each lane loads, as hstu_rows8_gemm_kernel has it
+  const int64_t pitch = (int64_t)g.blocks * BLOCK;
+  uint32_t xo[L], wo[L];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bias[i] = 0.f;
-  if (g.bias) row_load8<F32>(g.bias, 0, n, g.cols, vec, bias);
-#pragma unroll
-  for (int b = 0; b < MB; ++b) {
-#pragma unroll
-    for (int a = 0; a < NB; ++a)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *(floatx4*)(stage + l32 * PITCH + (32 * a + 8 * q4 + 4 * hh) * 4) =
-            floatx4{acc[a][b][4 * q4], acc[a][b][4 * q4 + 1], acc[a][b][4 * q4 + 2], acc[a][b][4 * q4 + 3]};
-    __builtin_amdgcn_wave_barrier();
-    float y[PIECES][8];
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const uint8_t* at = stage + (RPI * i + rr) * PITCH + 32 * cc;
-      const floatx4 lo = *(const floatx4*)at, hi = *(const floatx4*)(at + 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { y[i][e] = lo[e]; y[i][4 + e] = hi[e]; }
-    }
-    const int mb = m0 + wm * 32 * MB + 32 * b + rr;      // the lane's row of piece 0
-    if (g.c) {
-      float cv[PIECES][8];
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-        row_load8<F32>(g.c, (int64_t)(mb + RPI * i) * g.c_stride, n, mb + RPI * i < g.rows ? g.cols : 0, vec, cv[i]);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] += cv[i][e];
-    }
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] += bias[e];
-    if (g.activation) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] = silu(y[i][e]);
-    }
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) row_store8<F32>(g.out, (int64_t)(mb + RPI * i) * g.out_stride, n, mb + RPI * i < g.rows ? g.cols : 0, vec, y[i]);
-    __builtin_amdgcn_wave_barrier();
+  for (int i = 0; i < L; ++i) {
+    const int r = 8 * (w * L + i) + (lane >> 3);
+    const uint32_t chunk = 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    xo[i] = (uint32_t)((m0 + r < g.rows ? r : g.rows - 1 - m0) * (int)pitch) + chunk;
+    wo[i] = (uint32_t)((n0 + r < g.cols ? r : g.cols - 1 - n0) * (int)pitch) + chunk;
   }
+  const bool of_x = w < 4;
+  const int e_row = 64 * (w & 3) + lane, e_last = of_x ? g.rows - 1 - m0 : g.cols - 1 - n0;
+  const uint32_t eo = 4u * (uint32_t)(e_row < e_last ? e_row : e_last);
+  const uint8_t* x_base = scalar_ptr(g.x + (int64_t)m0 * pitch);
+  const uint8_t* w_base = scalar_ptr(g.w + (int64_t)n0 * pitch);
+  const uint8_t* e_base = scalar_ptr(of_x ? g.xe + (int64_t)m0 * 4 : g.we + (int64_t)n0 * 4);
+  const int64_t e_step = 4 * (int64_t)(of_x ? g.rows : g.cols);
+  int loaded = 0;                                               // stages asked for
+  auto issue_one = [&](int st, int i) __attribute__((always_inline)) {
+    const uint32_t base = smem_lds + (uint32_t)st * STAGE;
+    if (i < L) lds_dma16(x_base, xo[i < L ? i : 0], base + 1024u * (w * L + i));
+    else if (i < 2 * L) lds_dma16(w_base, wo[i < L ? 0 : i < 2 * L ? i - L : 0], base + X_BYTES + 1024u * (w * L + i - L));
+    else {
+      lds_dma4(e_base, eo, base + CODES + 256u * w);
+      // (past the last block it is loaded again, into a place that nobody reads)
+      const bool more = ++loaded < nt;
+      x_base += more ? BLOCK : 0;
+      w_base += more ? BLOCK : 0;
+      e_base += more && (loaded & 3) == 0 ? e_step : 0;
+    }
+  };
+  auto issue = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) issue_one(st, i);
+  };
+
+  const int wm = w & 1, wn = w >> 1;
+  uint32_t fo[2][2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) fo[s][h] = (uint32_t)(l32 * BLOCK + 16 * ((4 * s + 2 * hh + h) ^ ((l32 >> 1) & 7)));
+  intx8 wf[2][2], xf[2][4];
+  int ws[2], xs[4];
+  auto take = [&](int st, int t) __attribute__((always_inline)) {
+    const uint8_t* const at = smem + st * STAGE;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      auto frag = [&](int row0) __attribute__((always_inline)) {
+        struct { uint4v a, b; } both = {*(const uint4v*)(at + row0 * BLOCK + fo[s][0]), *(const uint4v*)(at + row0 * BLOCK + fo[s][1])};
+        return __builtin_bit_cast(intx8, both);
+      };
+#pragma unroll
+      for (int a = 0; a < 2; ++a) wf[s][a] = frag(T + 64 * wn + 32 * a);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) xf[s][b] = frag(128 * wm + 32 * b);
+    }
+    const uint8_t* const e = at + CODES + 4 * l32 + (t & 3);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) ws[a] = e[4 * (T + 64 * wn + 32 * a)];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) xs[b] = e[4 * (128 * wm + 32 * b)];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+
+  floatx16 acc[2][4];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+  auto products = [&](auto refill_, int st) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int s = i >> 3, b = (i >> 1) & 3, a = i & 1;
+      acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[s][a], xf[s][b], acc[a][b], 0, 0, 0, ws[a], 0, xs[b]);
+      asm volatile("" : "+v"(acc[a][b]));              // (the product stays here: the compiler would move it to where its result is used)
+      if constexpr (decltype(refill_)::value) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i >= 2 && i < 2 + NLOAD) issue_one(st, i - 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto change = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // The first half reads stage t in turn 2 t and forms its products in turn 2 t + 1, the second half a turn later.  A stage's place is free
+  // behind turn 2 t + 1: the first half asks for its share of stage t + 2 in turn 2 t + 2, beside the fragments of stage t + 1, the second half
+  // in the same turn between the products of stage t.  Each waits for its share before the barrier behind turn 2 t + 3.
+  issue(0);
+  if (w >= 4) issue(1);
+  if (w >= 4) ROWS8_WAIT_VMCNT(NLOAD);
+  else ROWS8_WAIT_VMCNT(0);
+  change();
+  if (w < 4) {
+    for (int t = 0; t < nt; ++t) {
+      issue((t + 1) & 1);
+      take(t & 1, t);
+      change();
+      products(std::false_type{}, 0);
+      ROWS8_WAIT_VMCNT(0);
+      change();
+    }
+    change();
+  } else {
+    change();
+    for (int t = 0; t < nt; ++t) {
+      take(t & 1, t);
+      ROWS8_WAIT_VMCNT(0);
+      change();
+      products(std::true_type{}, t & 1);
+      change();
+    }
+  }
+  ROWS8_WAIT_VMCNT(0);
+  __syncthreads();
+  tile_out<4, 2, false>(g, acc, smem + w * (32 * (32 * 2 * 4 + 16)), m0 + 128 * wm, n0 + 64 * wn);
 }
 
 // f(0), f(1), ..., f(N - 1), each index a constant
@@ -703,6 +878,18 @@ int launch_tiles(GemmParams g, hipStream_t st) {
   return rows8_launched("hstu_rows8_gemm");
 }
 
+int launch_turns(GemmParams g, hipStream_t st) {
+  constexpr int LDS = 2 * stage_bytes(256, 256);
+  static int granted[64];
+  const int64_t rt = ((int64_t)g.rows + 255) / 256, ct = ((int64_t)g.cols + 255) / 256;
+  if ((rt * ct + 7) / 8 * 8 * 512 > ROWS8_THREADS) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%d x %d outputs are too many for one call", g.rows, g.cols);
+  g.row_tiles = (int32_t)rt;
+  g.col_tiles = (int32_t)ct;
+  if (const int rc = allow_lds((const void*)hstu_rows8_turns_kernel, LDS, granted)) return rc;
+  hstu_rows8_turns_kernel<<<(uint32_t)((rt * ct + 7) / 8 * 8), 512, LDS, st>>>(g);
+  return rows8_launched("hstu_rows8_gemm");
+}
+
 template <int MT, bool F32>
 int launch_few(const GemmParams& g, hipStream_t st) {
   const int waves = g.blocks < FEW_WAVES ? g.blocks : FEW_WAVES;
@@ -760,7 +947,7 @@ int launch(const GemmParams& g, hipStream_t st) {
   }
   // The tile under which the call is shortest: rounds of as many tiles as the chip holds (1, 2 and 4 to a CU), each of them a fixed time and one
   // for each block of the contraction, in us as 73728 x 512 to 2048 and 16384 x 8192 by 8192 measure them.
-  const float fixed[3] = {F32 ? 13.3f : 8.5f, F32 ? 6.1f : 4.1f, F32 ? 2.9f : 1.8f}, block[3] = {F32 ? 3.0f : 1.76f, F32 ? 1.7f : 0.92f, F32 ? 1.1f : 0.77f};
+  const float fixed[3] = {F32 ? 13.3f : 9.3f, F32 ? 6.1f : 4.1f, F32 ? 2.9f : 1.8f}, block[3] = {F32 ? 3.0f : 1.46f, F32 ? 1.7f : 0.92f, F32 ? 1.1f : 0.77f};
   int best = 0;
   float least = 0.f;
   for (int i = 0; i < 3; ++i) {
@@ -768,7 +955,10 @@ int launch(const GemmParams& g, hipStream_t st) {
     const float us = (float)((tiles + chip - 1) / chip) * (fixed[i] + block[i] * (float)g.blocks);
     if (i == 0 || us < least) { best = i; least = us; }
   }
-  if (best == 0) return launch_tiles<4, 2, 2, 4, 2, F32>(g, st);
+  if (best == 0) {
+    if constexpr (F32) return launch_tiles<4, 2, 2, 4, 2, true>(g, st);
+    else return launch_turns(g, st);
+  }
   if (best == 1) return launch_tiles<2, 2, 2, 2, 2, F32>(g, st);
   // Four stages instead of two halve the workgroups of a CU: that pays where long rows come from past the L2s (64 x 8192 to 8192 20 us
   // against 30, 200 x 4096 to 4096 12.7 and 12.2, 64 x 512 to 100000 14.6 and 12.6).

@@ -169,7 +169,8 @@ def test_product(gpu, rows, depth, cols, dtype):
     _check_product(got, x, w, b, c, act, dtype)
 
 
-LARGE = [(700, 512, 2048), (2100, 256, 1030), (9000, 200, 520), (64, 512, 9000), (16, 1024, 5000), (3000, 1024, 4096)]
+LARGE = [(700, 512, 2048), (2100, 256, 1030), (9000, 200, 520), (64, 512, 9000), (16, 1024, 5000), (3000, 1024, 4096),
+         (4000, 1500, 4000), (4000, 650, 4090)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
