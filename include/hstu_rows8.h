@@ -52,9 +52,9 @@ typedef struct HstuRows8 {
 /* s = x (+ add, rounded to their type: it is stored at `sum` if that is given, and the norm is of the rounded rows)
  *   HSTU_ROWS8_LAYER  y = (s - mean) * rstd * gamma + beta   mean and (biased) variance of the row, rstd = 1 / sqrt(variance + eps)
  *   HSTU_ROWS8_RMS    y = s * rstd * gamma + beta            rstd = 1 / sqrt(mean of s^2 + eps)
- *   HSTU_ROWS8_AS_IS  y = s
+ *   HSTU_ROWS8_AS_IS  y = x, with nothing added and no gate
  * rows = (gate *) y in 8 bits.  Statistics and products in fp32, one rounding to the codes.  x, add, gate, sum: [rows, width] of `dtype`
- * with row strides in elements (any alignment of the type; whole 16 bytes everywhere, and a width of whole 16 bytes, run faster); add and
+ * with row strides in elements (any alignment of the type); add and
  * gate may be null, sum with add; sum may be x or add, otherwise no output may overlap an input.  gamma [width] of `dtype` (a norm needs
  * it), beta likewise or null. */
 typedef struct HstuRows8NormArgs {

@@ -54,42 +54,98 @@ struct Params {
   float eps;
 };
 
-// Eight values of a row in fp32; past the width zeros.  VEC: a width and places of whole vectors.
-template <bool F32, bool VEC>
-__device__ __forceinline__ void load8(const void* base, int64_t at, int col, int width, float (&f)[8]) {
+// Eight values of a row as they lie in memory, at any place that the type may have: the wide accesses of this chip need no more.
+typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float floats4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool F32>
+struct Eight {
+  uint4v w[F32 ? 2 : 1];
+};
+
+// How rows go into pieces of 8: evenly, or with a last piece that is not whole, or into one that is not.
+enum { FIT_EVEN, FIT_REST, FIT_PART };
+
+// Eight values from column `col` on; past the width zeros.  No branch: a piece that is not whole is the row's last eight values, moved down.
+template <bool F32, int FIT>
+__device__ __forceinline__ Eight<F32> load8(const void* base, int64_t at, int col, int width) {
+  constexpr int N = F32 ? 8 : 4;                   // words
+  Eight<F32> x = {};
+  uint32_t w[N];
+  if constexpr (FIT == FIT_PART) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 0.f;
-  if constexpr (VEC) {
-    if (col >= width) return;
-    if constexpr (F32) {
-      const floatx4* const from = (const floatx4*)((const float*)base + at + col);
-      const floatx4 lo = from[0], hi = from[1];
+    for (int i = 0; i < N; ++i) w[i] = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
-    } else {
-      unpack8(*(const uint4v*)((const bf16_t*)base + at + col), f);
-    }
+    for (int i = 0; i < 7; ++i)
+      if (col + i < width) {
+        if constexpr (F32) w[i] = ((const uint32_t*)base)[at + col + i];
+        else w[i / 2] |= (uint32_t)((const uint16_t*)base)[at + col + i] << (16 * (i % 2));
+      }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) x.w[i] = uint4v{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    return x;
+  }
+  const int from = col < width - 8 ? col : width - 8, down = col - from;
+  if constexpr (F32) {
+    const floats4* const p = (const floats4*)((const float*)base + at + from);
+    x.w[0] = __builtin_bit_cast(uint4v, (floatx4)p[0]);
+    x.w[1] = __builtin_bit_cast(uint4v, (floatx4)p[1]);
   } else {
+    x.w[0] = *(const words4*)((const bf16_t*)base + at + from);
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < width) f[i] = F32 ? ((const float*)base)[at + col + i] : (float)((const bf16_t*)base)[at + col + i];
+  for (int i = 0; i < N; ++i) w[i] = x.w[i / 4][i % 4];
+  if constexpr (FIT == FIT_REST) {
+    auto move = [&](int words, bool on) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t v = i + words < N ? w[i + words < N ? i + words : 0] : 0u;
+        w[i] = on ? v : w[i];
+      }
+    };
+    if constexpr (!F32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t v = __builtin_amdgcn_alignbit(i + 1 < N ? w[i + 1 < N ? i + 1 : 0] : 0u, w[i], 16);
+        w[i] = down & 1 ? v : w[i];
+      }
+      move(1, down & 2);
+      move(2, down & 4);
+    } else {
+      move(1, down & 1);
+      move(2, down & 2);
+      move(4, down & 4);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = down < 8 ? w[i] : 0u;
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) x.w[i] = uint4v{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+  return x;
+}
+template <bool F32>
+__device__ __forceinline__ void values_of(const Eight<F32>& x, float (&f)[8]) {
+  if constexpr (F32) {
+    const floatx4 lo = __builtin_bit_cast(floatx4, x.w[0]), hi = __builtin_bit_cast(floatx4, x.w[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
+  } else {
+    unpack8(x.w[0], f);
   }
 }
 
-template <bool F32, bool VEC>
+template <bool F32>
 __device__ __forceinline__ void store8(void* base, int64_t at, int col, int width, const float (&f)[8]) {
-  if constexpr (VEC) {
-    if (col >= width) return;
+  if (col + 8 <= width) {
     if constexpr (F32) {
-      floatx4* const to = (floatx4*)((float*)base + at + col);
-      to[0] = floatx4{f[0], f[1], f[2], f[3]};
-      to[1] = floatx4{f[4], f[5], f[6], f[7]};
+      floats4* const to = (floats4*)((float*)base + at + col);
+      to[0] = floats4{f[0], f[1], f[2], f[3]};
+      to[1] = floats4{f[4], f[5], f[6], f[7]};
     } else {
-      *(uint4v*)((bf16_t*)base + at + col) = pack8(f);
+      *(words4*)((bf16_t*)base + at + col) = pack8(f);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 7; ++i)
       if (col + i < width) {
         if constexpr (F32) ((float*)base)[at + col + i] = f[i];
         else ((bf16_t*)base)[at + col + i] = (bf16_t)f[i];
@@ -131,28 +187,43 @@ __device__ __forceinline__ float row_sum(float v, float* parts) {
 constexpr int threads_of(int t) { return t < 256 ? 256 : t; }
 
 // T threads a row, V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
-template <bool F32, bool VEC, int NORM, int T, int V>
+// Everything that a row needs is asked for at once: gamma, beta and gate behind the statistics would be a second latency.  MORE: there is
+// something to add or a gate; what is not there (nor beta) is read from x (gamma) once more and left out, so that no branch parts the loads.
+template <bool F32, int NORM, bool MORE, int FIT, int T, int V>
 __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Params p) {
   __shared__ float parts[T > 64 ? T / 64 : 1];
   const int t = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * (threads_of(T) / T) + threadIdx.x / T;
   if (row >= p.rows) return;                       // (T > 64: a row is the whole workgroup)
   const int W = p.width, blocks = rows8_blocks(W);
+  Eight<F32> x[V], added[V], gate[V], gamma[V], beta[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int col = 8 * (v * T + t);
+    x[v] = load8<F32, FIT>(p.x, row * p.x_stride, col, W);
+    if constexpr (MORE) {
+      added[v] = load8<F32, FIT>(p.add ? p.add : p.x, row * (p.add ? p.add_stride : p.x_stride), col, W);
+      gate[v] = load8<F32, FIT>(p.gate ? p.gate : p.x, row * (p.gate ? p.gate_stride : p.x_stride), col, W);
+    }
+    if constexpr (NORM != HSTU_ROWS8_AS_IS) {
+      gamma[v] = load8<F32, FIT>(p.gamma, 0, col, W);
+      beta[v] = load8<F32, FIT>(p.beta ? p.beta : p.gamma, 0, col, W);
+    }
+  }
   float y[V][8];
 #pragma unroll
-  for (int v = 0; v < V; ++v) load8<F32, VEC>(p.x, row * p.x_stride, 8 * (v * T + t), W, y[v]);
-  if (p.add) {
+  for (int v = 0; v < V; ++v) values_of<F32>(x[v], y[v]);
+  if (MORE && p.add) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int col = 8 * (v * T + t);
       float a[8];
-      load8<F32, VEC>(p.add, row * p.add_stride, col, W, a);
+      values_of<F32>(added[v], a);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[v][i] += a[i];
         if constexpr (!F32) y[v][i] = (float)(bf16_t)y[v][i];
       }
-      if (p.sum) store8<F32, VEC>(p.sum, row * p.sum_stride, col, W, y[v]);
+      if (p.sum) store8<F32>(p.sum, row * p.sum_stride, 8 * (v * T + t), W, y[v]);
     }
   }
   if constexpr (NORM != HSTU_ROWS8_AS_IS) {
@@ -180,24 +251,22 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
     for (int v = 0; v < V; ++v) {
       const int col = 8 * (v * T + t);
       float g[8], b[8];
-      load8<F32, VEC>(p.gamma, 0, col, W, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = 0.f;
-      if (p.beta) load8<F32, VEC>(p.beta, 0, col, W, b);
+      values_of<F32>(gamma[v], g);
+      values_of<F32>(beta[v], b);
       // (past the width: gamma and beta are zeros there, and a mean or rstd that is not finite stays out)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
 #pragma clang fp contract(off)      // (every step rounded, as it is in separate operations: half as many codes differ from theirs, 5e-7 of them)
         const float z = (y[v][i] - mean) * rstd * g[i];
-        y[v][i] = col + i < W ? z + b[i] : 0.f;
+        y[v][i] = col + i < W ? (p.beta ? z + b[i] : z) : 0.f;
       }
     }
   }
-  if (p.gate) {
+  if (MORE && p.gate) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float u[8];
-      load8<F32, VEC>(p.gate, row * p.gate_stride, 8 * (v * T + t), W, u);
+      values_of<F32>(gate[v], u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[v][i] *= u[i];
     }
@@ -247,7 +316,7 @@ struct ReadParams {
 };
 
 // a piece of 8 values a thread
-template <bool F32, bool VEC>
+template <bool F32>
 __global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = at / p.pieces;
@@ -262,20 +331,39 @@ __global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = y[i / 2][i % 2] * power;
-  store8<F32, VEC>(p.out, row * p.out_stride, 8 * piece, p.width, f);
+  store8<F32>(p.out, row * p.out_stride, 8 * piece, p.width, f);
 }
 
-template <bool F32, bool VEC, int NORM>
+template <bool F32, int NORM, bool MORE, int FIT>
 void launch_norm(const Params& p, hipStream_t st) {
-#define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, VEC, NORM, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
-  if (p.width <= 128) ROWS8_LAUNCH(16, 1);
-  else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
-  else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
-  else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
-  else if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
-  else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
-  else ROWS8_LAUNCH(1024, 4);
+#define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, NORM, MORE, FIT, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
+  if constexpr (FIT == FIT_PART) {
+    ROWS8_LAUNCH(16, 1);
+    return;
+  } else {
+    if (p.width <= 128) ROWS8_LAUNCH(16, 1);
+    else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
+    else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
+    else if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
+    else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+    else ROWS8_LAUNCH(1024, 4);
+  }
 #undef ROWS8_LAUNCH
+}
+
+template <bool F32, int NORM, bool MORE>
+void launch_norm(const Params& p, hipStream_t st) {
+  if (p.width < 8) launch_norm<F32, NORM, MORE, FIT_PART>(p, st);
+  else if (p.width % 8 == 0) launch_norm<F32, NORM, MORE, FIT_EVEN>(p, st);
+  else launch_norm<F32, NORM, MORE, FIT_REST>(p, st);
+}
+
+template <bool F32, int NORM>
+void launch_norm(const Params& p, hipStream_t st) {
+  if constexpr (NORM != HSTU_ROWS8_AS_IS) {
+    if (p.add || p.gate) { launch_norm<F32, NORM, true>(p, st); return; }
+  }
+  launch_norm<F32, NORM, false>(p, st);
 }
 
 int norm_rows(const HstuRows8NormArgs* a, void* stream) {
@@ -287,6 +375,7 @@ int norm_rows(const HstuRows8NormArgs* a, void* stream) {
   if (a->dtype != HSTU_ROWS8_BF16 && a->dtype != HSTU_ROWS8_FP32) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "dtype %d", a->dtype);
   if (a->norm < HSTU_ROWS8_AS_IS || a->norm > HSTU_ROWS8_RMS) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "norm %d", a->norm);
   if (a->sum && !a->add) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a sum needs something to add");
+  if (a->norm == HSTU_ROWS8_AS_IS && (a->add || a->gate)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "rows as they are have nothing added and no gate");
   if (a->rows.rows == 0) return HSTU_ROWS8_OK;
   if (!a->x) return rows8_fail(HSTU_ROWS8_ERR_NULL, "x is null");
   if (a->norm != HSTU_ROWS8_AS_IS && !a->gamma) return rows8_fail(HSTU_ROWS8_ERR_NULL, "gamma is null");
@@ -294,29 +383,21 @@ int norm_rows(const HstuRows8NormArgs* a, void* stream) {
   const int64_t threads = a->rows.width <= 2048 ? 64 : a->rows.width <= 8192 ? 256 : 1024;
   if (a->rows.rows > ROWS8_THREADS / threads - 16) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)a->rows.rows, a->rows.width);
   const bool f32 = a->dtype == HSTU_ROWS8_FP32;
-  const int unit = f32 ? 4 : 8;
-  bool vec = a->rows.width % 8 == 0;
-  auto rows_of = [&](const void* t, int64_t stride) {
-    if (t && ((uintptr_t)t & (f32 ? 3u : 1u))) return false;
-    vec = vec && (!t || (rows8_aligned16(t) && (stride % unit == 0 || a->rows.rows == 1)));
-    return true;
-  };
-  if (!rows_of(a->x, a->x_stride) || !rows_of(a->add, a->add_stride) || !rows_of(a->gate, a->gate_stride) || !rows_of(a->sum, a->sum_stride) ||
-      !rows_of(a->gamma, 0) || !rows_of(a->beta, 0)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a pointer is not aligned to its type");
+  for (const void* t : {a->x, a->add, a->gate, (const void*)a->sum, a->gamma, a->beta})
+    if ((uintptr_t)t & (f32 ? 3u : 1u)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a pointer is not aligned to its type");
   Params p;
   p.x = a->x; p.add = a->add; p.gate = a->gate; p.gamma = a->gamma; p.beta = a->beta; p.sum = a->sum;
   p.codes = (uint8_t*)a->rows.codes; p.exponents = (uint8_t*)a->rows.exponents;
   p.x_stride = a->x_stride; p.add_stride = a->add_stride; p.gate_stride = a->gate_stride; p.sum_stride = a->sum_stride;
   p.rows = a->rows.rows; p.width = a->rows.width; p.eps = a->eps;
   hipStream_t st = (hipStream_t)stream;
-#define ROWS8_NORM(F32, VEC)                                                                  \
-  do {                                                                                        \
-    if (a->norm == HSTU_ROWS8_LAYER) launch_norm<F32, VEC, HSTU_ROWS8_LAYER>(p, st);          \
-    else if (a->norm == HSTU_ROWS8_RMS) launch_norm<F32, VEC, HSTU_ROWS8_RMS>(p, st);         \
-    else launch_norm<F32, VEC, HSTU_ROWS8_AS_IS>(p, st);                                      \
+#define ROWS8_NORM(F32)                                                                  \
+  do {                                                                                   \
+    if (a->norm == HSTU_ROWS8_LAYER) launch_norm<F32, HSTU_ROWS8_LAYER>(p, st);          \
+    else if (a->norm == HSTU_ROWS8_RMS) launch_norm<F32, HSTU_ROWS8_RMS>(p, st);         \
+    else launch_norm<F32, HSTU_ROWS8_AS_IS>(p, st);                                      \
   } while (0)
-  if (f32) { if (vec) ROWS8_NORM(true, true); else ROWS8_NORM(true, false); }
-  else { if (vec) ROWS8_NORM(false, true); else ROWS8_NORM(false, false); }
+  if (f32) ROWS8_NORM(true); else ROWS8_NORM(false);
 #undef ROWS8_NORM
   return rows8_launched("hstu_rows8_norm");
 }
@@ -338,11 +419,10 @@ int read_rows(const HstuRows8ReadArgs* a, void* stream) {
   p.pieces = rows8_blocks(p.width) * (BLOCK / 8);
   const int64_t all = p.rows * p.pieces;
   if (all > ROWS8_THREADS - 256) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)p.rows, p.width);
-  const bool vec = p.width % 8 == 0 && rows8_aligned16(a->out) && (p.out_stride % (f32 ? 4 : 8) == 0 || p.rows == 1);
   const uint32_t grid = (uint32_t)((all + 255) / 256);
   hipStream_t st = (hipStream_t)stream;
-  if (f32) { if (vec) hstu_rows8_read_kernel<true, true><<<grid, 256, 0, st>>>(p); else hstu_rows8_read_kernel<true, false><<<grid, 256, 0, st>>>(p); }
-  else { if (vec) hstu_rows8_read_kernel<false, true><<<grid, 256, 0, st>>>(p); else hstu_rows8_read_kernel<false, false><<<grid, 256, 0, st>>>(p); }
+  if (f32) hstu_rows8_read_kernel<true><<<grid, 256, 0, st>>>(p);
+  else hstu_rows8_read_kernel<false><<<grid, 256, 0, st>>>(p);
   return rows8_launched("hstu_rows8_read");
 }
 

@@ -64,7 +64,7 @@ def _refused(fn, args, status, word):
 
 
 @pytest.mark.parametrize("change,status,word", ROWS + [
-    (dict(x=None), -1, "x is null"), (dict(gamma=None), -1, "gamma"), (dict(norm=3), -4, "norm"), (dict(sum=0x5000), -4, "sum"), (dict(x=0x3001), -4, "aligned"),
+    (dict(x=None), -1, "x is null"), (dict(gamma=None), -1, "gamma"), (dict(norm=3), -4, "norm"), (dict(sum=0x5000), -4, "sum"), (dict(norm=0, gate=0x5000), -4, "no gate"), (dict(norm=0, add=0x5000), -4, "nothing added"), (dict(x=0x3001), -4, "aligned"),
     (dict(beta=0x4001), -4, "aligned"), (dict(rows=1 << 30), -4, "too many")])
 def test_norm_refused(change, status, word):
   _refused(_lib_rows8.load().hstu_rows8_norm, _norm_args(**change), status, word)
