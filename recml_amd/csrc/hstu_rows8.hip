@@ -4,7 +4,10 @@
 //   hstu_rows8_read   codes and exponents -> rows
 //
 // Both are passes over memory: a row is read once, stays in registers as fp32 through the sum, the statistics (the mean, then the squares
-// about it), the gate and the blocks' maxima, and leaves as one byte a value.
+// about it), the gate and the blocks' maxima, and leaves as one byte a value.  131072 x 512 in bf16 as they are 34 us (5.9 TB/s), with a norm
+// 48, added to others 81 (5.8 TB/s), with a gate 58; 16398 x 1024 with norm and gate 14; 65536 x 1024 in fp32 with a norm 57; a million of
+// 64 45: half of what it writes there are the zeros behind each row.  One row is a chain of latencies, 2 us.  A norm alone in bf16 is
+// bounded by its vector instructions, all else by memory (a large copy runs at 5.0 TB/s); read back, 131072 x 512 take 31 us (6.6 TB/s).
 
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
@@ -66,6 +69,8 @@ struct Eight {
 enum { FIT_EVEN, FIT_REST, FIT_PART };
 
 // Eight values from column `col` on; past the width zeros.  No branch: a piece that is not whole is the row's last eight values, moved down.
+// (Through the caches: past them rows of 268 MB are quicker, 65536 x 2048 as they are 71 -> 63 us, and those of 34 MB slower, 10.0 -> 11.4, as three
+// operands are, 161 -> 172 and 20 -> 23.)
 template <bool F32, int FIT>
 __device__ __forceinline__ Eight<F32> load8(const void* base, int64_t at, int col, int width) {
   constexpr int N = F32 ? 8 : 4;                   // words
@@ -163,14 +168,18 @@ __device__ __forceinline__ uint32_t max_neighbour(uint32_t v) {
   const uint32_t o = of_neighbour<CTRL>(v);
   return o > v ? o : v;
 }
-__device__ __forceinline__ uint32_t max16(uint32_t v) {
-  return max_neighbour<0x140>(max_neighbour<0x141>(max_neighbour<0x4E>(max_neighbour<0xB1>(v))));
+// the largest of a block's 16 threads (of 8 where a row has no more)
+template <int T>
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+  v = max_neighbour<0x141>(max_neighbour<0x4E>(max_neighbour<0xB1>(v)));
+  return T >= 16 ? max_neighbour<0x140>(v) : v;
 }
 
 // the sum over a row's T threads, the same bits in each of them
 template <int T>
 __device__ __forceinline__ float row_sum(float v, float* parts) {
-  v = add_neighbour<0x140>(add_neighbour<0x141>(add_neighbour<0x4E>(add_neighbour<0xB1>(v))));
+  v = add_neighbour<0x141>(add_neighbour<0x4E>(add_neighbour<0xB1>(v)));
+  if constexpr (T >= 16) v = add_neighbour<0x140>(v);
   if constexpr (T >= 32) v += __shfl_xor(v, 16, 64);
   if constexpr (T >= 64) v += __shfl_xor(v, 32, 64);
   if constexpr (T > 64) {
@@ -186,7 +195,7 @@ __device__ __forceinline__ float row_sum(float v, float* parts) {
 
 constexpr int threads_of(int t) { return t < 256 ? 256 : t; }
 
-// T threads a row, V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
+// T threads a row (8 of 64 values up to a workgroup), V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
 // Everything that a row needs is asked for at once: gamma, beta and gate behind the statistics would be a second latency.  MORE: there is
 // something to add or a gate; what is not there (nor beta) is read from x (gamma) once more and left out, so that no branch parts the loads.
 template <bool F32, int NORM, bool MORE, int FIT, int T, int V>
@@ -238,27 +247,35 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
         for (int i = 0; i < 8; ++i) s[i & 1] += y[v][i];
       mean = row_sum<T>(s[0] + s[1], parts) / count;
     }
+    // (past the width: values are zeros, and so are their differences; gamma and beta are zeros too)
     float ss[2] = {0.f, 0.f};
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = 8 * (v * T + t) + i < W ? y[v][i] - mean : 0.f;
-        ss[i & 1] = __builtin_fmaf(d, d, ss[i & 1]);
-      }
-    const float rstd = __builtin_amdgcn_rsqf(row_sum<T>(ss[0] + ss[1], parts) / count + p.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int col = 8 * (v * T + t);
-      float g[8], b[8];
-      values_of<F32>(gamma[v], g);
-      values_of<F32>(beta[v], b);
-      // (past the width: gamma and beta are zeros there, and a mean or rstd that is not finite stays out)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        y[v][i] -= col + (FIT == FIT_EVEN ? 0 : i) < W ? mean : 0.f;
+        ss[i & 1] = __builtin_fmaf(y[v][i], y[v][i], ss[i & 1]);
+      }
+    }
+    const float rstd = __builtin_amdgcn_rsqf(row_sum<T>(ss[0] + ss[1], parts) / count + p.eps);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float g[8];
+      values_of<F32>(gamma[v], g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[v][i] = y[v][i] * rstd * g[i];
+    }
+    if (p.beta) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float b[8];
+        values_of<F32>(beta[v], b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
 #pragma clang fp contract(off)      // (every step rounded, as it is in separate operations: half as many codes differ from theirs, 5e-7 of them)
-        const float z = (y[v][i] - mean) * rstd * g[i];
-        y[v][i] = col + i < W ? (p.beta ? z + b[i] : z) : 0.f;
+          y[v][i] = y[v][i] + b[i];
+        }
       }
     }
   }
@@ -280,7 +297,7 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
       const uint32_t m = __builtin_bit_cast(uint32_t, y[v][i]) & 0x7fffffffu;
       top = m > top ? m : top;
     }
-    top = max16(top);
+    top = block_max<T>(top);
     // floor(log2 top) less the largest code's 8, one more where top is past 464 = 1.8125 * 2^8 powers
     int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x680000u ? 1 : 0);
     e = e < 1 ? 1 : e > 246 ? 246 : e;              // (top = 0 too)
@@ -296,7 +313,9 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
       c = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
       code.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], c, true);
     }
-    if (block < blocks) *(uint2*)(p.codes + row * ((int64_t)blocks * BLOCK) + 8 * piece) = bad ? uint2{0u, 0u} : code;
+    uint8_t* const to = p.codes + row * ((int64_t)blocks * BLOCK) + 8 * piece;
+    if (block < blocks) *(uint2*)to = bad ? uint2{0u, 0u} : code;
+    if constexpr (T == 8) *(uint2*)(to + 64) = uint2{0u, 0u};
     if (t % 16 == 0 && block < (blocks + 3) / 4 * 4)
       p.exponents[((int64_t)(block / 4) * p.rows + row) * 4 + block % 4] = block >= blocks ? (uint8_t)1 : bad ? (uint8_t)255 : (uint8_t)e;
     // (groups whose last blocks no thread has)
@@ -338,10 +357,11 @@ template <bool F32, int NORM, bool MORE, int FIT>
 void launch_norm(const Params& p, hipStream_t st) {
 #define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, NORM, MORE, FIT, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
   if constexpr (FIT == FIT_PART) {
-    ROWS8_LAUNCH(16, 1);
-    return;
+    ROWS8_LAUNCH(8, 1);
   } else {
-    if (p.width <= 128) ROWS8_LAUNCH(16, 1);
+    if (p.width <= 64) ROWS8_LAUNCH(8, 1);
+    else if (p.width <= 128) ROWS8_LAUNCH(16, 1);
+    else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
     else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
     else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
     else if (p.width <= 2048) ROWS8_LAUNCH(64, 4);

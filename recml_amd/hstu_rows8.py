@@ -92,10 +92,9 @@ class Rows8:
     self._put(codes, exponents, width)
 
   def _put(self, codes, exponents, width):
-    put = object.__setattr__
-    put(self, "codes", codes)
-    put(self, "exponents", exponents)
-    put(self, "width", width)
+    _set_codes(self, codes)
+    _set_exponents(self, exponents)
+    _set_width(self, width)
     return self
 
   def __setattr__(self, name, value):
@@ -143,6 +142,9 @@ class Rows8:
 
   def _fill(self, r):
     r.codes, r.exponents, r.rows, r.width = self.codes.data_ptr(), self.exponents.data_ptr(), self.rows, self.width
+
+
+_set_codes, _set_exponents, _set_width = (getattr(Rows8, name).__set__ for name in Rows8.__slots__)      # (past __setattr__)
 
 
 def _flat(t):
