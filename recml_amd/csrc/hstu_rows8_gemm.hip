@@ -118,10 +118,10 @@ __device__ __forceinline__ bf16x8 values8(const intx8& codes, int q, float power
   return __builtin_bit_cast(bf16x8, all);
 }
 
-// LDS of a stage, and of a workgroup (the epilogue's blocks take the stages' place).
+// LDS of a stage of one set of waves, and of a workgroup (what the epilogue and the sum over the sets exchange takes the stages' place).
 constexpr int stage_bytes(int tm, int tn) { return (tm + tn) * (BLOCK + 4); }
-constexpr int lds_bytes(int mb, int nb, int wm, int wn, int stages) {
-  const int ring = stages * stage_bytes(32 * mb * wm, 32 * nb * wn), out = wm * wn * 32 * (32 * nb * 4 + 16);
+constexpr int lds_bytes(int mb, int nb, int wm, int wn, int stages, int ks) {
+  const int ring = stages * ks * stage_bytes(32 * mb * wm, 32 * nb * wn), out = wm * wn * (32 * (32 * nb * 4 + 16) + (ks - 1) * nb * mb * 4096);
   return ring > out ? ring : out;
 }
 
@@ -234,11 +234,13 @@ __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&a
 // lane then holds four consecutive columns of one output row.
 //   A row's 128 bytes lie in LDS as eight 16-byte chunks, chunk c of row r at c ^ (r / 2 % 8): 16 rows reach all 64 banks.  Which
 // contraction elements a lane holds does not matter as long as both operands' lanes hold the same ones.
+//   KS > 1: as many sets of waves, each with the blocks of its turn; their sums are added in LDS in the sets' order.
 //   For results in bf16 the tiles are of 128 x 128 and less (hstu_rows8_turns_kernel has the larger ones).
-template <int MB, int NB, int WM, int WN, int STAGES, bool F32>
-__global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const GemmParams g) {
+template <int MB, int NB, int WM, int WN, int STAGES, int KS, bool F32>
+__global__ __launch_bounds__(64 * WM * WN * KS) void hstu_rows8_gemm_kernel(const GemmParams g) {
   constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN, WAVES = WM * WN;
-  constexpr int X_BYTES = TM * BLOCK, CODES = (TM + TN) * BLOCK, STAGE = stage_bytes(TM, TN);
+  constexpr int OUT_BYTES = 32 * (32 * NB * 4 + 16);            // of a wave, in tile_out
+  constexpr int X_BYTES = TM * BLOCK, CODES = (TM + TN) * BLOCK, PART = stage_bytes(TM, TN), STAGE = KS * PART;
   constexpr int LX = TM / 8 / WAVES, LW = TN / 8 / WAVES, LE = (TM + TN) / 64, LEW = (LE + WAVES - 1) / WAVES;      // direct loads of 8 rows; of 64 rows' exponents
   static_assert(LX * 8 * WAVES == TM && LW * 8 * WAVES == TN && TM % 64 == 0 && TN % 64 == 0, "whole loads a wave");
   constexpr int NLOAD = LX + LW + LEW;
@@ -246,12 +248,12 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const uint32_t smem_lds = __builtin_amdgcn_groupstaticsize();
   const int tid = threadIdx.x, lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int all_w = __builtin_amdgcn_readfirstlane(tid >> 6), ks = all_w / WAVES, w = all_w % WAVES;      // KS sets of waves, a block each
   const int l32 = lane & 31, hh = lane >> 5;
 
   int rt, ct;
   if (!tile_of(g, &rt, &ct)) return;
-  const int m0 = rt * TM, n0 = ct * TN, nt = g.blocks;
+  const int m0 = rt * TM, n0 = ct * TN, nt = (g.blocks + KS - 1) / KS;
 
   // ---- what each lane loads: piece i of an operand is 8 rows, lane l of it the 16 bytes at row l / 8, place l % 8.  Rows past an operand's
   // end are its last one (what they give is not stored).
@@ -283,22 +285,18 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   }
   const uint8_t* x_base = scalar_ptr(g.x + (int64_t)m0 * pitch);
   const uint8_t* w_base = scalar_ptr(g.w + (int64_t)n0 * pitch);
-  int loaded = 0;                                               // stages asked for
-  auto issue_one = [&](int st, int i) __attribute__((always_inline)) {
-    const uint32_t base = smem_lds + (uint32_t)st * STAGE;
-    if (i < LX) lds_dma16(x_base, xo[i < LX ? i : 0], base + 1024u * (w * LX + i));
-    else if (i < LX + LW) lds_dma16(w_base, wo[i < LX ? 0 : i < LX + LW ? i - LX : 0], base + X_BYTES + 1024u * (w * LW + i - LX));
-    else {
-      constexpr int FROM = LX + LW;
-      lds_dma4(e_base[i < FROM ? 0 : i - FROM], eo[i < FROM ? 0 : i - FROM], base + e_to[i < FROM ? 0 : i - FROM]);
-    }
-    if (i == NLOAD - 1) {       // on to the next block; every four blocks to the next group of exponents
-      x_base += BLOCK;
-      w_base += BLOCK;
-      if ((++loaded & 3) == 0)
+  int block = ks;                                               // of the next stage to load (past the last one that is loaded again, and not used)
+  auto issue = [&](int st) __attribute__((always_inline)) {
+    const uint32_t base = smem_lds + (uint32_t)(st * STAGE + ks * PART);
+    const int at = block < g.blocks ? block : g.blocks - 1;
+    const uint8_t *const x_from = x_base + at * BLOCK, *const w_from = w_base + at * BLOCK;
 #pragma unroll
-        for (int e = 0; e < LEW; ++e) e_base[e] += e_step[e];
-    }
+    for (int i = 0; i < LX; ++i) lds_dma16(x_from, xo[i], base + 1024u * (w * LX + i));
+#pragma unroll
+    for (int i = 0; i < LW; ++i) lds_dma16(w_from, wo[i], base + X_BYTES + 1024u * (w * LW + i));
+#pragma unroll
+    for (int i = 0; i < LEW; ++i) lds_dma4(e_base[i] + (at >> 2) * e_step[i], eo[i], base + e_to[i]);
+    block += KS;
   };
 
   // ---- fragments: lane (row l32 of a block of 32, half hh) holds two chunks of each half of the row's 128 bytes
@@ -309,7 +307,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
 #pragma unroll
     for (int h = 0; h < 2; ++h) fo[s][h] = (uint32_t)(l32 * BLOCK + 16 * ((4 * s + 2 * hh + h) ^ ((l32 >> 1) & 7)));
   auto frag = [&](int st, int row0, int s) __attribute__((always_inline)) {
-    const uint8_t* const at = smem + st * STAGE + row0 * BLOCK;
+    const uint8_t* const at = smem + st * STAGE + ks * PART + row0 * BLOCK;
     struct { uint4v a, b; } both = {*(const uint4v*)(at + fo[s][0]), *(const uint4v*)(at + fo[s][1])};
     return __builtin_bit_cast(intx8, both);
   };
@@ -317,7 +315,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   auto x_frag = [&](int st, int b, int s) __attribute__((always_inline)) { return frag(st, 32 * (wm * MB + b), s); };
   int xs[MB], ws[NB];
   auto scales = [&](int st, int t) __attribute__((always_inline)) {
-    const uint8_t* const at = smem + st * STAGE + CODES + 4 * l32 + (t & 3);
+    const uint8_t* const at = smem + st * STAGE + ks * PART + CODES + 4 * l32 + ((t * KS + ks) & 3);
 #pragma unroll
     for (int a = 0; a < NB; ++a) ws[a] = at[4 * (TM + 32 * (wn * NB + a))];
 #pragma unroll
@@ -334,9 +332,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
 
 #pragma unroll
   for (int t = 0; t < STAGES; ++t)
-    if (t < nt)
-#pragma unroll
-      for (int i = 0; i < NLOAD; ++i) issue_one(t, i);
+    if (t < nt) issue(t);
   // (stages younger than the one waited for: as many as the ring has, or fewer near the end, where the wait is for all)
   if (nt >= STAGES) ROWS8_WAIT_VMCNT((STAGES - 1) * NLOAD);
   else ROWS8_WAIT_VMCNT(0);
@@ -344,6 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
   asm volatile("" ::: "memory");
   int st = 0;
   for (int t = 0; t < nt; ++t) {
+    if (KS == 1 || t * KS + ks < g.blocks) {
     scales(st, t);
     float wp[NB], xp[MB];
     if constexpr (F32) {
@@ -379,19 +376,46 @@ __global__ __launch_bounds__(64 * WM * WN) void hstu_rows8_gemm_kernel(const Gem
           for (int a = 0; a < NB; ++a) acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[a], xf[b], acc[a][b], 0, 0, 0, ws[a], 0, xs[b]);
       }
     }
+    }
     // everyone's last read of this stage is done, and the next stage's loads are here
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (t + STAGES <= nt) ROWS8_WAIT_VMCNT((STAGES - 2) * NLOAD);
     else ROWS8_WAIT_VMCNT(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (t + STAGES < nt)
-#pragma unroll
-      for (int i = 0; i < NLOAD; ++i) issue_one(st, i);
+    if (t + STAGES < nt) issue(st);
     st = st + 1 >= STAGES ? 0 : st + 1;
   }
 
-  tile_out<MB, NB, F32>(g, acc, smem + w * (32 * (32 * NB * 4 + 16)), m0 + 32 * MB * wm, n0 + 32 * NB * wn);
+  if constexpr (KS > 1) {
+    // the sets' sums, added in their order
+    floatx4* const sums = (floatx4*)(smem + WAVES * OUT_BYTES);
+    if (ks > 0) {
+#pragma unroll
+      for (int a = 0; a < NB; ++a)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            sums[((((ks - 1) * WAVES + w) * NB + a) * MB + b) * 256 + 64 * q + lane] =
+                floatx4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
+    }
+    __syncthreads();
+    if (ks > 0) return;
+#pragma unroll
+    for (int i = 0; i < KS - 1; ++i)
+#pragma unroll
+      for (int a = 0; a < NB; ++a)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const floatx4 v = sums[(((i * WAVES + w) * NB + a) * MB + b) * 256 + 64 * q + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[a][b][4 * q + e] += v[e];
+          }
+  }
+  tile_out<MB, NB, F32>(g, acc, smem + w * OUT_BYTES, m0 + 32 * MB * wm, n0 + 32 * NB * wn);
 }
 
 // The same product where there is work for tiles of 256 x 256 and a contraction to stream.  Eight waves of 128 x 64 in two halves, one wave of
@@ -863,18 +887,19 @@ int allow_lds(const void* fn, int bytes, int* granted) {
   return HSTU_ROWS8_OK;
 }
 
-template <int MB, int NB, int WM, int WN, int STAGES, bool F32>
+template <int MB, int NB, int WM, int WN, int STAGES, int KS, bool F32>
 int launch_tiles(GemmParams g, hipStream_t st) {
-  constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN, LDS = lds_bytes(MB, NB, WM, WN, STAGES);
+  constexpr int TM = 32 * MB * WM, TN = 32 * NB * WN, LDS = lds_bytes(MB, NB, WM, WN, STAGES, KS);
+  static_assert(LDS <= 160 << 10, "LDS");
   static int granted[64];
   const int64_t rt = ((int64_t)g.rows + TM - 1) / TM, ct = ((int64_t)g.cols + TN - 1) / TN;
-  if (rt * ct > 0x7fffffffll / 16 || (rt * ct + 7) / 8 * 8 * 64 * WM * WN > ROWS8_THREADS)
+  if (rt * ct > 0x7fffffffll / 16 || (rt * ct + 7) / 8 * 8 * 64 * WM * WN * KS > ROWS8_THREADS)
     return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%d x %d outputs are too many for one call", g.rows, g.cols);
   g.row_tiles = (int32_t)rt;
   g.col_tiles = (int32_t)ct;
-  const void* const fn = (const void*)hstu_rows8_gemm_kernel<MB, NB, WM, WN, STAGES, F32>;
+  const void* const fn = (const void*)hstu_rows8_gemm_kernel<MB, NB, WM, WN, STAGES, KS, F32>;
   if (const int rc = allow_lds(fn, LDS, granted)) return rc;
-  hstu_rows8_gemm_kernel<MB, NB, WM, WN, STAGES, F32><<<(uint32_t)((rt * ct + 7) / 8 * 8), 64 * WM * WN, LDS, st>>>(g);
+  hstu_rows8_gemm_kernel<MB, NB, WM, WN, STAGES, KS, F32><<<(uint32_t)((rt * ct + 7) / 8 * 8), 64 * WM * WN * KS, LDS, st>>>(g);
   return rows8_launched("hstu_rows8_gemm");
 }
 
@@ -945,25 +970,38 @@ int launch(const GemmParams& g, hipStream_t st) {
   if constexpr (!F32) {
     if (rows_take(g)) return g.c ? launch_rows<ROWS_ADD>(g, st) : g.activation ? launch_rows<ROWS_SILU>(g, st) : launch_rows<ROWS_PLAIN>(g, st);
   }
-  // The tile under which the call is shortest: rounds of as many tiles as the chip holds (1, 2 and 4 to a CU), each of them a fixed time and one
-  // for each block of the contraction, in us as 73728 x 512 to 2048 and 16384 x 8192 by 8192 measure them.
-  const float fixed[3] = {F32 ? 13.3f : 9.3f, F32 ? 6.1f : 4.1f, F32 ? 2.9f : 1.8f}, block[3] = {F32 ? 3.0f : 1.46f, F32 ? 1.7f : 0.92f, F32 ? 1.1f : 0.77f};
+  // The tiles under which the call is shortest, by what they were measured to take (us; b: blocks of the contraction, n: tiles to a CU).
+  // Where tiles are one to a CU, sets of waves that share a long contraction out are what hides its latencies: 64 x 8192 to 8192 in tiles of 64
+  // x 64 31 us, with four sets 19; 64 x 4096 to 16384 18 and 15; 400 x 1024 to 4096 6.2 and 9.0; in tiles of 128 x 128 800 x 4096 to 4096
+  // 24 and with two sets 21, 400 x 8192 to 8192 45 and 36.
+  //   64 x 64                 rounds of 4 to a CU, and for each block 0.2 a tile of a CU, or its latency
+  //   64 x 64, four sets      n (3 + 0.21 b)
+  //   128 x 128               3 + 0.64 b alone on a CU, rounds of two (4.1 + 0.92 b) otherwise
+  //   128 x 128, two sets     n (4 + 0.52 b)
+  //   256 x 256               n (9.3 + 1.46 b)
+  const float b = (float)g.blocks;
+  auto per = [&](int64_t t, int64_t chip) {
+    const int64_t tiles = (((int64_t)g.rows + t - 1) / t) * (((int64_t)g.cols + t - 1) / t);
+    return (float)((tiles + chip - 1) / chip);
+  };
+  const float n64 = per(64, 256), n128 = per(128, 256), step64 = F32 ? 0.277f * n64 : 0.2f * n64, latency = F32 ? 0.5f : 0.25f;
+  const float us[5] = {(F32 ? 2.9f : 2.0f) * per(64, 1024) + b * (step64 > latency ? step64 : latency),
+                       n64 * ((F32 ? 3.8f : 3.f) + (F32 ? 0.29f : 0.21f) * b),
+                       n128 <= 1.f ? 3.f + (F32 ? 1.08f : 0.64f) * b : per(128, 512) * ((F32 ? 6.1f : 4.1f) + (F32 ? 1.7f : 0.92f) * b),
+                       n128 * ((F32 ? 6.f : 4.f) + (F32 ? 0.94f : 0.52f) * b),
+                       per(256, 256) * ((F32 ? 13.3f : 9.3f) + (F32 ? 3.0f : 1.46f) * b)};
   int best = 0;
-  float least = 0.f;
-  for (int i = 0; i < 3; ++i) {
-    const int64_t t = 256 >> i, tiles = (((int64_t)g.rows + t - 1) / t) * (((int64_t)g.cols + t - 1) / t), chip = 256 << i;
-    const float us = (float)((tiles + chip - 1) / chip) * (fixed[i] + block[i] * (float)g.blocks);
-    if (i == 0 || us < least) { best = i; least = us; }
+  for (int i = 1; i < 5; ++i)
+    if (us[i] < us[best]) best = i;
+  switch (best) {
+    case 0: return launch_tiles<1, 1, 2, 2, 2, 1, F32>(g, st);
+    case 1: return launch_tiles<1, 1, 2, 2, 2, 4, F32>(g, st);
+    case 2: return launch_tiles<2, 2, 2, 2, 2, 1, F32>(g, st);
+    case 3: return launch_tiles<2, 2, 2, 2, 2, 2, F32>(g, st);
+    default:
+      if constexpr (F32) return launch_tiles<4, 2, 2, 4, 2, 1, true>(g, st);
+      else return launch_turns(g, st);
   }
-  if (best == 0) {
-    if constexpr (F32) return launch_tiles<4, 2, 2, 4, 2, true>(g, st);
-    else return launch_turns(g, st);
-  }
-  if (best == 1) return launch_tiles<2, 2, 2, 2, 2, F32>(g, st);
-  // Four stages instead of two halve the workgroups of a CU: that pays where long rows come from past the L2s (64 x 8192 to 8192 20 us
-  // against 30, 200 x 4096 to 4096 12.7 and 12.2, 64 x 512 to 100000 14.6 and 12.6).
-  const bool far = g.blocks >= 16 && ((int64_t)g.rows + g.cols) * g.blocks * BLOCK > 32 << 20;
-  return far ? launch_tiles<1, 1, 2, 2, 4, F32>(g, st) : launch_tiles<1, 1, 2, 2, 2, F32>(g, st);
 }
 
 int gemm(const HstuRows8GemmArgs* a, void* stream) {

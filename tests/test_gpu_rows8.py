@@ -147,7 +147,7 @@ def test_norm_of_what_has_none(gpu):
 
 
 PRODUCTS = [(1, 1, 1), (1, 128, 64), (2, 129, 7), (31, 64, 33), (32, 128, 32), (33, 200, 31), (5, 300, 77), (64, 128, 65), (65, 513, 64), (100, 512, 300), (128, 1000, 256), (129, 640, 513),
-            (300, 384, 130), (17, 2000, 1000), (257, 100, 257), (1, 4100, 48), (70, 8192, 40)]
+            (300, 384, 130), (17, 2000, 1000), (257, 100, 257), (1, 4100, 48), (70, 8192, 40), (129, 2600, 513)]
 
 
 def _check_product(got, x, w, bias, residual, activation, dtype):
@@ -170,7 +170,7 @@ def test_product(gpu, rows, depth, cols, dtype):
 
 
 LARGE = [(700, 512, 2048), (2100, 256, 1030), (9000, 200, 520), (64, 512, 9000), (16, 1024, 5000), (3000, 1024, 4096),
-         (4000, 1500, 4000), (4000, 650, 4090)]
+         (4000, 1500, 4000), (4000, 650, 4090), (700, 4200, 3700), (200, 4000, 4100)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -203,7 +203,7 @@ def test_many_outputs_of_short_contractions(gpu, depth, how):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("rows,depth,cols", [(1, 128, 24), (20, 300, 40), (50, 300, 72), (300, 200, 136), (2000, 200, 1032), (7000, 200, 2120), (2779, 500, 4800)])
+@pytest.mark.parametrize("rows,depth,cols", [(1, 128, 24), (20, 300, 40), (50, 300, 72), (300, 200, 136), (2000, 200, 1032), (7000, 200, 2120), (2779, 500, 4800), (130, 2600, 520), (700, 4200, 3704)])
 def test_leaves_what_is_not_its_own(gpu, rows, depth, cols, dtype):
   """Rows with a stride of their own in the middle of a buffer: what stands between, before and behind them stays."""
   x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
