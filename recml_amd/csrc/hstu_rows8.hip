@@ -3,11 +3,12 @@
 //   hstu_rows8_norm   rows, normed or as they are -> codes and block exponents
 //   hstu_rows8_read   codes and exponents -> rows
 //
-// Both are passes over memory: a row is read once, stays in registers as fp32 through the sum, the statistics (the mean, then the squares
-// about it), the gate and the blocks' maxima, and leaves as one byte a value.  131072 x 512 in bf16 as they are 34 us (5.9 TB/s), with a norm
-// 48, added to others 81 (5.8 TB/s), with a gate 58; 16398 x 1024 with norm and gate 14; 65536 x 1024 in fp32 with a norm 57; a million of
-// 64 45: half of what it writes there are the zeros behind each row.  One row is a chain of latencies, 2 us.  A norm alone in bf16 is
-// bounded by its vector instructions, all else by memory (a large copy runs at 5.0 TB/s); read back, 131072 x 512 take 31 us (6.6 TB/s).
+// Both are passes over memory: a row is read once, stays in registers through the sum, the statistics (the mean, then the squares about it),
+// the gate and the blocks' maxima, and leaves as one byte a value.  131072 x 512 in bf16 as they are 34 us (5.9 TB/s), with a norm 48, added to
+// others 81 (5.8 TB/s), with a gate 58; 16398 x 1024 with norm and gate 14; a million of 64 45: half of what it writes there are the zeros
+// behind each row.  In fp32 65536 x 1024 as they are 59 us (5.7 TB/s), with a norm 69, with a gate 105 (5.8 TB/s).  One row is a chain of
+// latencies, 2 us.  A norm alone is bounded by its vector instructions, all else by memory (a large copy runs at 5.0 TB/s); read back,
+// 131072 x 512 take 31 us (6.6 TB/s).
 
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
@@ -164,6 +165,11 @@ __device__ __forceinline__ uint32_t of_neighbour(uint32_t v) { return (uint32_t)
 template <int CTRL>
 __device__ __forceinline__ float add_neighbour(float v) { return v + __builtin_bit_cast(float, of_neighbour<CTRL>(__builtin_bit_cast(uint32_t, v))); }
 template <int CTRL>
+__device__ __forceinline__ double add_neighbour(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  return v + __builtin_bit_cast(double, (uint64_t)of_neighbour<CTRL>((uint32_t)(w >> 32)) << 32 | of_neighbour<CTRL>((uint32_t)w));
+}
+template <int CTRL>
 __device__ __forceinline__ uint32_t max_neighbour(uint32_t v) {
   const uint32_t o = of_neighbour<CTRL>(v);
   return o > v ? o : v;
@@ -176,8 +182,8 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
 }
 
 // the sum over a row's T threads, the same bits in each of them
-template <int T>
-__device__ __forceinline__ float row_sum(float v, float* parts) {
+template <int T, class Y>
+__device__ __forceinline__ Y row_sum(Y v, Y* parts) {
   v = add_neighbour<0x141>(add_neighbour<0x4E>(add_neighbour<0xB1>(v)));
   if constexpr (T >= 16) v = add_neighbour<0x140>(v);
   if constexpr (T >= 32) v += __shfl_xor(v, 16, 64);
@@ -185,7 +191,7 @@ __device__ __forceinline__ float row_sum(float v, float* parts) {
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0.f;
+    v = 0;
 #pragma unroll
     for (int w = 0; w < T / 64; ++w) v += parts[w];
     __syncthreads();
@@ -193,35 +199,59 @@ __device__ __forceinline__ float row_sum(float v, float* parts) {
   return v;
 }
 
+// What a row's values are until they become codes.  Rows in 32 bits take 64: a value next to a border between two codes takes the one that it has by
+// the definition, where in fp32 4e-7 of them take the other, a whole 2^-3 away, and a block's steps in a row come out 1e-4 off instead of 3e-8.
+// A norm alone pays for it, 65536 x 1024 69 us for 58, 16384 x 999 25 for 17; with a gate 105 for 107.  (Rows in bf16 are no nearer to what they
+// stand for than 2^-9; theirs is fp32, in which 5e-7 of the codes are the neighbour.)
+template <bool F32> struct ValueOf { typedef float type; };
+template <> struct ValueOf<true> { typedef double type; };
+
+// As fp32, of a value in 64 bits its first 20 with what comes behind them in the last one (set where any of it is), so that the rounding
+// to a code of 4, and the comparison with a border, are those of the value.
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)w;
+  return (float)__builtin_bit_cast(double, (uint64_t)((uint32_t)(w >> 32) | (lo < 1u ? lo : 1u)) << 32);
+}
+__device__ __forceinline__ float inverse_root(float v) { return __builtin_amdgcn_rsqf(v); }
+// (squares past fp32 are infinite ones for rows of either type)
+__device__ __forceinline__ double inverse_root(double v) { return v > 0x1.fffffep127 ? 0. : 1. / sqrt(v); }
+
 constexpr int threads_of(int t) { return t < 256 ? 256 : t; }
 
 // T threads a row (8 of 64 values up to a workgroup), V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
-// Everything that a row needs is asked for at once: gamma, beta and gate behind the statistics would be a second latency.  MORE: there is
+// Everything that a row needs is asked for at once: gamma, beta and gate behind the statistics would be a second latency (but for the widest rows
+// in 32 bits, which have no registers for it: 2048 x 32768 with a gate 139 us for 310).  MORE: there is
 // something to add or a gate; what is not there (nor beta) is read from x (gamma) once more and left out, so that no branch parts the loads.
 template <bool F32, int NORM, bool MORE, int FIT, int T, int V>
 __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Params p) {
-  __shared__ float parts[T > 64 ? T / 64 : 1];
+  using Y = typename ValueOf<F32>::type;
+  __shared__ Y parts[T > 64 ? T / 64 : 1];
   const int t = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * (threads_of(T) / T) + threadIdx.x / T;
   if (row >= p.rows) return;                       // (T > 64: a row is the whole workgroup)
   const int W = p.width, blocks = rows8_blocks(W);
+  constexpr bool LATE = F32 && V > 2;               // (registers for what follows the statistics only then)
   Eight<F32> x[V], added[V], gate[V], gamma[V], beta[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
+  auto affine = [&](int v) __attribute__((always_inline)) {
     const int col = 8 * (v * T + t);
-    x[v] = load8<F32, FIT>(p.x, row * p.x_stride, col, W);
-    if constexpr (MORE) {
-      added[v] = load8<F32, FIT>(p.add ? p.add : p.x, row * (p.add ? p.add_stride : p.x_stride), col, W);
-      gate[v] = load8<F32, FIT>(p.gate ? p.gate : p.x, row * (p.gate ? p.gate_stride : p.x_stride), col, W);
-    }
+    if constexpr (MORE) gate[v] = load8<F32, FIT>(p.gate ? p.gate : p.x, row * (p.gate ? p.gate_stride : p.x_stride), col, W);
     if constexpr (NORM != HSTU_ROWS8_AS_IS) {
       gamma[v] = load8<F32, FIT>(p.gamma, 0, col, W);
       beta[v] = load8<F32, FIT>(p.beta ? p.beta : p.gamma, 0, col, W);
     }
-  }
-  float y[V][8];
+  };
 #pragma unroll
-  for (int v = 0; v < V; ++v) values_of<F32>(x[v], y[v]);
+  for (int v = 0; v < V; ++v) {
+    const int col = 8 * (v * T + t);
+    x[v] = load8<F32, FIT>(p.x, row * p.x_stride, col, W);
+    if constexpr (MORE) added[v] = load8<F32, FIT>(p.add ? p.add : p.x, row * (p.add ? p.add_stride : p.x_stride), col, W);
+    if constexpr (!LATE) affine(v);
+  }
+  float f[V][8];
+#pragma unroll
+  for (int v = 0; v < V; ++v) values_of<F32>(x[v], f[v]);
   if (MORE && p.add) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -229,72 +259,76 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
       values_of<F32>(added[v], a);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[v][i] += a[i];
-        if constexpr (!F32) y[v][i] = (float)(bf16_t)y[v][i];
+        f[v][i] += a[i];
+        if constexpr (!F32) f[v][i] = (float)(bf16_t)f[v][i];
       }
-      if (p.sum) store8<F32>(p.sum, row * p.sum_stride, 8 * (v * T + t), W, y[v]);
+      if (p.sum) store8<F32>(p.sum, row * p.sum_stride, 8 * (v * T + t), W, f[v]);
     }
   }
+  Y mean = 0, rstd = 1;
+  // (past the width: values are zeros, and so are their differences; gamma and beta are zeros too)
+  auto difference = [&](int v, int i) __attribute__((always_inline)) {
+    if constexpr (NORM == HSTU_ROWS8_LAYER) return (Y)f[v][i] - (8 * (v * T + t) + (FIT == FIT_EVEN ? 0 : i) < W ? mean : (Y)0);
+    else return (Y)f[v][i];
+  };
   if constexpr (NORM != HSTU_ROWS8_AS_IS) {
     // (divided, not multiplied by 1 / W: the mean of equal values is that value, and their differences from it are zeros)
-    const float count = (float)W;
-    float mean = 0.f;
+    const Y count = (Y)W;
     if constexpr (NORM == HSTU_ROWS8_LAYER) {
-      float s[2] = {0.f, 0.f};
+      Y s[2] = {0, 0};
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i & 1] += y[v][i];
-      mean = row_sum<T>(s[0] + s[1], parts) / count;
+        for (int i = 0; i < 8; ++i) s[i & 1] += f[v][i];
+      mean = row_sum<T, Y>(s[0] + s[1], parts) / count;
     }
-    // (past the width: values are zeros, and so are their differences; gamma and beta are zeros too)
-    float ss[2] = {0.f, 0.f};
+    Y ss[2] = {0, 0};
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int col = 8 * (v * T + t);
+    for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        y[v][i] -= col + (FIT == FIT_EVEN ? 0 : i) < W ? mean : 0.f;
-        ss[i & 1] = __builtin_fmaf(y[v][i], y[v][i], ss[i & 1]);
+        const Y d = difference(v, i);
+        ss[i & 1] = fma(d, d, ss[i & 1]);
       }
-    }
-    const float rstd = __builtin_amdgcn_rsqf(row_sum<T>(ss[0] + ss[1], parts) / count + p.eps);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float g[8];
-      values_of<F32>(gamma[v], g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[v][i] = y[v][i] * rstd * g[i];
-    }
-    if (p.beta) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float b[8];
-        values_of<F32>(beta[v], b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-#pragma clang fp contract(off)      // (every step rounded, as it is in separate operations: half as many codes differ from theirs, 5e-7 of them)
-          y[v][i] = y[v][i] + b[i];
-        }
-      }
-    }
-  }
-  if (MORE && p.gate) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float u[8];
-      values_of<F32>(gate[v], u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[v][i] *= u[i];
-    }
+    rstd = inverse_root(row_sum<T, Y>(ss[0] + ss[1], parts) / count + (Y)p.eps);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
+    if constexpr (LATE) affine(v);
+    if constexpr (LATE) {                            // (the values stay in 32 bits: their differences are taken again)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(f[v][i]));
+    }
+    Y y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = difference(v, i);
+    if constexpr (NORM != HSTU_ROWS8_AS_IS) {
+      float g[8];
+      values_of<F32>(gamma[v], g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = F32 ? y[i] * (rstd * g[i]) : y[i] * rstd * g[i];
+      if (p.beta) {
+        values_of<F32>(beta[v], g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma clang fp contract(off)      // (every step rounded, as it is in separate operations: half as many codes differ from theirs, 5e-7 of them)
+          y[i] = y[i] + g[i];
+        }
+      }
+    }
+    if (MORE && p.gate) {
+      float u[8];
+      values_of<F32>(gate[v], u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= u[i];
+    }
     const int piece = v * T + t, block = piece / 16;
     uint32_t top = 0;
+    float z[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t m = __builtin_bit_cast(uint32_t, y[v][i]) & 0x7fffffffu;
+      z[i] = as_float(y[i]);
+      const uint32_t m = __builtin_bit_cast(uint32_t, z[i]) & 0x7fffffffu;
       top = m > top ? m : top;
     }
     top = block_max<T>(top);
@@ -304,15 +338,12 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
     const bool bad = top >= 0x7f800000u;
     const float inverse = power_of(254 - (uint32_t)e);
     uint2 code;
-    {
-      float z[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = __builtin_amdgcn_fmed3f(y[v][i] * inverse, -448.f, 448.f);
-      int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-      code.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
-      c = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
-      code.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], c, true);
-    }
+    for (int i = 0; i < 8; ++i) z[i] = __builtin_amdgcn_fmed3f(z[i] * inverse, -448.f, 448.f);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+    code.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(z[4], z[5], 0, false);
+    code.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], c, true);
     uint8_t* const to = p.codes + row * ((int64_t)blocks * BLOCK) + 8 * piece;
     if (block < blocks) *(uint2*)to = bad ? uint2{0u, 0u} : code;
     if constexpr (T == 8) *(uint2*)(to + 64) = uint2{0u, 0u};
@@ -364,9 +395,16 @@ void launch_norm(const Params& p, hipStream_t st) {
     else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
     else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
     else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
-    else if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
-    else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
-    else ROWS8_LAUNCH(1024, 4);
+    else if constexpr (F32) {                      // (values in 64 bits leave registers for two pieces)
+      if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
+      else if (p.width <= 4096) ROWS8_LAUNCH(256, 2);
+      else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+      else ROWS8_LAUNCH(1024, 4);
+    } else {
+      if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
+      else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+      else ROWS8_LAUNCH(1024, 4);
+    }
   }
 #undef ROWS8_LAUNCH
 }
