@@ -132,6 +132,18 @@ def test_norm_of_slices(gpu, dtype):
     R.check_stored(got, *R.norm(s.reshape(-1, 96), gamma, beta, 1e-6, u.reshape(-1, 96), "layer"))
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,width", [(4000, 40), (700, 999), (300, 1384), (120, 4097), (40, 16000)])
+def test_codes_of_rows_in_32_bits(gpu, rows, width, kind):
+  """Their values are taken in 64 bits, so that the roundings which norm() counts are 2^29 times smaller (twice that with its own)."""
+  g = _gen(rows + width)
+  x, gate = torch.randn((rows, width), generator=g) * 2 + 0.5, torch.randn((rows, width), generator=g)
+  gamma, beta = torch.randn(width, generator=g) + 1.0, torch.randn(width, generator=g) * 0.2 if kind == "layer" else None
+  got = recml_amd.norm_rows8(x.to(gpu), gamma.to(gpu), None if beta is None else beta.to(gpu), 2.0**-20, rms=kind == "rms", gate=gate.to(gpu))
+  y, off = R.norm(x, gamma, beta, 2.0**-20, gate, kind)
+  R.check_stored(got, y, off * 2.0**-28)
+
+
 def test_norm_of_what_has_none(gpu):
   """Rows of one value, constant rows, rows with a NaN or an infinity, and sums past fp32."""
   x = torch.zeros((6, 200))
