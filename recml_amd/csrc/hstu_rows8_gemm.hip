@@ -140,7 +140,7 @@ __device__ __forceinline__ bool tile_of(const GemmParams& g, int* rt, int* ct) {
 
 // A wave's sums on their way out: blocks of 32 rows x 32 NB columns from (m0, n0) on, through the wave's own LDS (fp32, rows 16 bytes apart
 // from a multiple of 128), then pieces of 8 columns of a row per lane; where rows are not whole vectors, one column per lane (1237 x 1001 to
-// 777 in fp32 12.9 us with pieces of single values, 9.5 so).
+// 777 in fp32 with a residual 14 us with pieces of single values, 11 so; 776 columns 9.0).
 template <int MB, int NB, bool F32>
 __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&acc)[NB][MB], uint8_t* stage, int m0, int n0) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
@@ -159,20 +159,33 @@ __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&a
     const int col = lane % W, n = n0 + col;
     const bool in = n < g.cols;
     const float bias = g.bias && in ? value_of<F32>(g.bias, n) : 0.f;
+    constexpr int PIECE = 16 / ROWS;                   // instructions at a time: what is added to is asked for by all of them first
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
       put(b);
-#pragma unroll 8
-      for (int i = 0; i < 32 / ROWS; ++i) {
-        const int row = ROWS * i + lane / W, m = m0 + 32 * b + row;
-        if (!in || m >= g.rows) continue;
-        float y = *(const float*)(stage + row * PITCH + 4 * col);
-        if (g.c) y += value_of<F32>(g.c, (int64_t)m * g.c_stride + n);
-        y += bias;
-        if (g.activation) y = silu(y);
-        const int64_t to = (int64_t)m * g.out_stride + n;
-        if constexpr (F32) ((float*)g.out)[to] = y;
-        else ((bf16_t*)g.out)[to] = (bf16_t)y;
+#pragma unroll
+      for (int i0 = 0; i0 < 32 / ROWS; i0 += PIECE) {
+        float cv[PIECE];
+        const int mb = m0 + 32 * b + ROWS * i0 + lane / W;
+        if (g.c) {
+#pragma unroll
+          for (int i = 0; i < PIECE; ++i) {
+            const int m = mb + ROWS * i < g.rows ? mb + ROWS * i : g.rows - 1;
+            cv[i] = value_of<F32>(g.c, (int64_t)m * g.c_stride + (in ? n : g.cols - 1));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECE; ++i) {
+          const int m = mb + ROWS * i;
+          if (!in || m >= g.rows) continue;
+          float y = *(const float*)(stage + (ROWS * (i0 + i) + lane / W) * PITCH + 4 * col);
+          if (g.c) y += cv[i];
+          y += bias;
+          if (g.activation) y = silu(y);
+          const int64_t to = (int64_t)m * g.out_stride + n;
+          if constexpr (F32) ((float*)g.out)[to] = y;
+          else ((bf16_t*)g.out)[to] = (bf16_t)y;
+        }
       }
       __builtin_amdgcn_wave_barrier();
     }
