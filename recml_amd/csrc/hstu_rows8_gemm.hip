@@ -962,10 +962,11 @@ int launch_rows(const GemmParams& g, hipStream_t st) {
 
 // Whether the weight goes by rows kept in registers: bf16 results of contractions of up to 1024, whole pieces of 64 columns, at least three
 // pieces for each of the 256 workgroups (two: 4000 x 512 to 2048 12 us either way, 8000 x 512 to 2048, four of them, 16 against 19 in
-// tiles), and a quarter of the last rows' tile wasted at most.  What it does behind the product is one of three.
+// tiles) or, where something is added, five (16398 x 1024 to 1024, four of them, 37 and in tiles 33; 32768 x 768 to 768, six, 33 and 38), and a quarter of
+// the last rows' tile wasted at most.  What it does behind the product is one of three.
 bool rows_take(const GemmParams& g) {
   const int64_t tiles = ((int64_t)g.rows + 255) / 256, pieces = tiles * (g.cols / 64);
-  return g.blocks <= 8 && g.cols % 64 == 0 && g.vec && !g.bias && !(g.c && g.activation) && pieces >= 768 && 4 * (int64_t)g.rows >= 3 * 256 * tiles &&
+  return g.blocks <= 8 && g.cols % 64 == 0 && g.vec && !g.bias && !(g.c && g.activation) && pieces >= (g.c ? 1280 : 768) && 4 * (int64_t)g.rows >= 3 * 256 * tiles &&
          g.out_stride < 1 << 21 && g.c_stride < 1 << 21 && g.cols < 1 << 29;
 }
 
@@ -989,7 +990,7 @@ int launch(const GemmParams& g, hipStream_t st) {
   // 24 and with two sets 21, 400 x 8192 to 8192 45 and 36.
   //   64 x 64                 rounds of 4 to a CU, and for each block 0.2 a tile of a CU, or its latency
   //   64 x 64, four sets      n (3 + 0.21 b)
-  //   128 x 128               3 + 0.64 b alone on a CU, rounds of two (4.1 + 0.92 b) otherwise
+  //   128 x 128               2.5 + 0.64 b alone on a CU, rounds of two (3.7 + 0.9 b) otherwise
   //   128 x 128, two sets     n (4 + 0.52 b)
   //   256 x 256               n (9.3 + 1.46 b)
   const float b = (float)g.blocks;
@@ -1000,7 +1001,7 @@ int launch(const GemmParams& g, hipStream_t st) {
   const float n64 = per(64, 256), n128 = per(128, 256), step64 = F32 ? 0.277f * n64 : 0.2f * n64, latency = F32 ? 0.5f : 0.25f;
   const float us[5] = {(F32 ? 2.9f : 2.0f) * per(64, 1024) + b * (step64 > latency ? step64 : latency),
                        n64 * ((F32 ? 3.8f : 3.f) + (F32 ? 0.29f : 0.21f) * b),
-                       n128 <= 1.f ? 3.f + (F32 ? 1.08f : 0.64f) * b : per(128, 512) * ((F32 ? 6.1f : 4.1f) + (F32 ? 1.7f : 0.92f) * b),
+                       n128 <= 1.f ? (F32 ? 3.f : 2.5f) + (F32 ? 1.08f : 0.64f) * b : per(128, 512) * ((F32 ? 6.1f : 3.7f) + (F32 ? 1.7f : 0.9f) * b),
                        n128 * ((F32 ? 6.f : 4.f) + (F32 ? 0.94f : 0.52f) * b),
                        per(256, 256) * ((F32 ? 13.3f : 9.3f) + (F32 ? 3.0f : 1.46f) * b)};
   int best = 0;
@@ -1009,7 +1010,11 @@ int launch(const GemmParams& g, hipStream_t st) {
   switch (best) {
     case 0: return launch_tiles<1, 1, 2, 2, 2, 1, F32>(g, st);
     case 1: return launch_tiles<1, 1, 2, 2, 2, 4, F32>(g, st);
-    case 2: return launch_tiles<2, 2, 2, 2, 2, 1, F32>(g, st);
+    case 2:
+      // (eight waves of 32 x 64 rather than four of 64 x 64: 16398 x 1024 to 1024 with a residual 33 us for 37, 3000 x 1024 to 4096 19 for 22, 2000 x 512 to
+      // 2048 6.8 for 7.4, 6000 x 4096 to 4096 97 for 94; in fp32, where a wave turns its codes into values, 184 for 191 the other way)
+      if constexpr (F32) return launch_tiles<2, 2, 2, 2, 2, 1, true>(g, st);
+      else return launch_tiles<1, 2, 4, 2, 2, 1, false>(g, st);
     case 3: return launch_tiles<2, 2, 2, 2, 2, 2, F32>(g, st);
     default:
       if constexpr (F32) return launch_tiles<4, 2, 2, 4, 2, 1, true>(g, st);

@@ -214,6 +214,18 @@ def test_many_outputs_of_short_contractions(gpu, depth, how):
     assert torch.equal(got, recml_amd.gemm_rows8(x, w, torch.zeros(cols, dtype=BF16, device=gpu), how == "silu"))
 
 
+@pytest.mark.parametrize("depth", [128, 200, 384, 512, 600, 768, 800, 1000])
+def test_many_sums_of_short_contractions(gpu, depth):
+  """As above where something is added, in as many outputs as that takes."""
+  rows, cols = 256 * 17 - 37, 64 * 77
+  x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
+  c = torch.randn((rows, cols + 8), generator=_gen(depth)).to(BF16).to(gpu)[:, :cols]
+  got = recml_amd.gemm_rows8(x, w, residual=c)
+  y, before, sizes = R.product(R.values(x.codes, x.exponents, depth).to(gpu), R.values(w.codes, w.exponents, depth).to(gpu), None, c, False)
+  assert float(((got.double() - y).abs() - R.product_off(y, before, sizes, depth, BF16, False)).max()) <= 0
+  assert torch.equal(got, recml_amd.gemm_rows8(x, w, residual=c))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("rows,depth,cols", [(1, 128, 24), (20, 300, 40), (50, 300, 72), (300, 200, 136), (2000, 200, 1032), (7000, 200, 2120), (2779, 500, 4800), (130, 2600, 520), (700, 4200, 3704)])
 def test_leaves_what_is_not_its_own(gpu, rows, depth, cols, dtype):
