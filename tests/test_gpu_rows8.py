@@ -93,6 +93,7 @@ def test_layouts(gpu, dtype):
 
 NORMS = [(1, 1), (5, 3), (3, 8), (7, 64), (4, 100), (130, 128), (3, 129), (9, 250), (6, 512), (3, 520), (5, 777), (2, 1000), (3, 1024), (2, 1500), (2, 2048), (2, 3001),
          (2, 8192), (2, 10000)]
+NORMS += [(33, 40), (17, 41), (9, 136), (9, 256), (4, 1001), (3, 2047), (3, 4096), (3, 4095), (2, 8191), (2, 16384), (2, 32767), (2, 32768)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -182,7 +183,7 @@ def test_product(gpu, rows, depth, cols, dtype):
 
 
 LARGE = [(700, 512, 2048), (2100, 256, 1030), (9000, 200, 520), (64, 512, 9000), (16, 1024, 5000), (3000, 1024, 4096),
-         (4000, 1500, 4000), (4000, 650, 4090), (700, 4200, 3700), (200, 4000, 4100)]
+         (4000, 1500, 4000), (4000, 650, 4090), (700, 4200, 3700), (200, 4000, 4100), (1000, 4200, 4000)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
