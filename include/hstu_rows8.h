@@ -53,10 +53,9 @@ typedef struct HstuRows8 {
  *   HSTU_ROWS8_LAYER  y = (s - mean) * rstd * gamma + beta   mean and (biased) variance of the row, rstd = 1 / sqrt(variance + eps)
  *   HSTU_ROWS8_RMS    y = s * rstd * gamma + beta            rstd = 1 / sqrt(mean of s^2 + eps)
  *   HSTU_ROWS8_AS_IS  y = x, with nothing added and no gate
- * rows = (gate *) y in 8 bits.  Statistics and products in fp32, one rounding to the codes.  x, add, gate, sum: [rows, width] of `dtype`
- * with row strides in elements (any alignment of the type); add and
- * gate may be null, sum with add; sum may be x or add, otherwise no output may overlap an input.  gamma [width] of `dtype` (a norm needs
- * it), beta likewise or null. */
+ * rows = (gate *) y in 8 bits.  Statistics and products in fp32, or in 64 bits for rows in fp32, and one rounding to the codes.  x, add, gate,
+ * sum: [rows, width] of `dtype` with row strides in elements (any alignment of the type); add and gate may be null, sum with add; sum may be
+ * x or add (with its stride), otherwise no output may overlap an input.  gamma [width] of `dtype` (a norm needs it), beta likewise or null. */
 typedef struct HstuRows8NormArgs {
   uint32_t struct_size;   /* sizeof(HstuRows8NormArgs) */
   uint32_t version;       /* HSTU_ROWS8_ABI_VERSION    */
@@ -89,9 +88,9 @@ int hstu_rows8_read(const HstuRows8ReadArgs* args, void* stream);
 
 /* out[m, n] = act(sum_k x[m, k] w[n, k] + c[m, n] + bias[n]), x and w the values that their rows stand for, of one width; sums in fp32,
  * one rounding to `dtype`.  For bf16 results each product is cut to 2^-13 of the largest of its eight neighbours along k before it is
- * added (what the matrix instructions on codes do); for fp32 results every product is exact.  out and c: [x.rows, w.rows] of `dtype` with row strides in elements, bias [w.rows]; c and bias may be
- * null; c may be out.  Any alignment of the type; pointers and strides of whole 16 bytes, and as many columns, run faster.  activation: 1 =
- * silu, 0 = none. */
+ * added (what the matrix instructions on codes do); for fp32 results every product is exact.  out and c: [x.rows, w.rows] of `dtype` with row
+ * strides in elements, bias [w.rows]; c and bias may be null; c may be out (with its stride).  Any alignment of the type; pointers and
+ * strides of whole 16 bytes, and as many columns, run faster.  activation: 1 = silu, 0 = none. */
 typedef struct HstuRows8GemmArgs {
   uint32_t struct_size;   /* sizeof(HstuRows8GemmArgs) */
   uint32_t version;       /* HSTU_ROWS8_ABI_VERSION    */

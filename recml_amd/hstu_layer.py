@@ -203,7 +203,8 @@ class HSTUBlock(torch.nn.Module):
   def quantize(self) -> None:
     """Keeps the projections' and the output product's weights in 8 bits (hstu_rows8.Rows8): every call of the block then runs its norms,
     products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
-    a change to them quantize() has to be called again (a call notices and raises).  `dequantize` goes back."""
+    a change to them quantize() has to be called again (a call notices and raises; not what is written past autograd, through .data, nor
+    parametrized weights).  `dequantize` goes back."""
     with torch.no_grad():
       w, b = self._uqkv_weights()
       out = self.output_kernel.reshape(-1, self.hidden_dim)

@@ -247,6 +247,61 @@ def test_leaves_what_is_not_its_own(gpu, rows, depth, cols, dtype):
   assert torch.equal(body[:, :cols], recml_amd.gemm_rows8(x, w, dtype=dtype))
 
 
+def _arguments(kind, dtype):
+  a = kind()
+  a.struct_size, a.version, a.dtype = C.sizeof(a), _lib_rows8.ABI_VERSION, _lib_rows8.FP32 if dtype == F32 else _lib_rows8.BF16
+  return a, C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,depth,cols", [(8, 512, 64), (100, 300, 77), (64, 4096, 520), (257, 640, 1000), (256 * 17 - 37, 384, 64 * 77), (4096, 1500, 4096), (1000, 4200, 1000)])
+def test_product_added_in_place(gpu, rows, depth, cols, dtype):
+  x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
+  out = torch.randn((rows, cols), generator=_gen(rows), dtype=F32).to(dtype).to(gpu)
+  want = recml_amd.gemm_rows8(x, w, residual=out, dtype=dtype)
+  a, stream = _arguments(_lib_rows8.HstuRows8GemmArgs, dtype)
+  x._fill(a.x)
+  w._fill(a.w)
+  a.out = a.c = out.data_ptr()
+  a.out_stride = a.c_stride = cols
+  assert _lib_rows8.load().hstu_rows8_gemm(C.byref(a), stream) == 0
+  assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("width", [3, 64, 999, 2048, 5000, 16001])
+@pytest.mark.parametrize("onto", ["x", "add"])
+def test_norm_of_a_sum_in_place(gpu, width, onto, dtype):
+  g = _gen(width)
+  new = lambda *shape: torch.randn(shape, generator=g).to(dtype).to(gpu)
+  x, add, gate, gamma = new(40, width), new(40, width), new(40, width), new(width)
+  want, total = recml_amd.norm_rows8(x, gamma, gate=gate, add=add)
+  got = recml_amd.Rows8._empty(40, width, x.device)
+  a, stream = _arguments(_lib_rows8.HstuRows8NormArgs, dtype)
+  got._fill(a.rows)
+  a.norm, a.eps = _lib_rows8.LAYER, 1e-6
+  a.x, a.add, a.gate, a.gamma = x.data_ptr(), add.data_ptr(), gate.data_ptr(), gamma.data_ptr()
+  a.x_stride = a.add_stride = a.gate_stride = a.sum_stride = width
+  put = x if onto == "x" else add
+  a.sum = put.data_ptr()
+  assert _lib_rows8.load().hstu_rows8_norm(C.byref(a), stream) == 0
+  assert torch.equal(put, total) and torch.equal(got.codes, want.codes) and torch.equal(got.exponents, want.exponents)
+
+
+def test_first_calls_in_a_capture(gpu):
+  """A graph that no eager call of these sizes came before, replayed between eager work."""
+  g = _gen(21)
+  x, gamma = torch.randn((130, 4300), generator=g).to(BF16).to(gpu), torch.ones(4300, dtype=BF16, device=gpu)
+  w = recml_amd.quantize_rows(torch.randn((1030, 4300), generator=g).to(gpu))
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    kept = recml_amd.gemm_rows8(recml_amd.norm_rows8(x, gamma), w)
+  for i in range(3):
+    x.copy_(torch.randn((130, 4300), generator=g))
+    graph.replay()
+    assert torch.equal(kept, recml_amd.gemm_rows8(recml_amd.norm_rows8(x, gamma), w)), i
+
+
 def test_sums_in_fp32(gpu):
   """An fp32 result has fp32's precision: independent roundings of partial sums, each at most half a step of the sum of the magnitudes, add up to
   sqrt(depth) of that in the mean square."""
