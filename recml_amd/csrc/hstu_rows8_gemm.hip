@@ -989,7 +989,8 @@ int launch(const GemmParams& g, hipStream_t st) {
   // x 64 31 us, with four sets 19; 64 x 4096 to 16384 18 and 15; 400 x 1024 to 4096 6.2 and 9.0; in tiles of 128 x 128 800 x 4096 to 4096
   // 24 and with two sets 21, 400 x 8192 to 8192 45 and 36.
   //   64 x 64                 rounds of 4 to a CU, and for each block 0.2 a tile of a CU, or its latency
-  //   64 x 64, four sets      n (3 + 0.21 b)
+  //   64 x 64, four sets      n (3 + 0.21 b), less what operands that come from memory cost tiles that wait for them more often (64 x 1024 to 4096 among
+  //                           a block's other steps 6.4 us without sets, 5.6 with; called over and over 4.6 and 4.7)
   //   128 x 128               2.5 + 0.64 b alone on a CU, rounds of two (3.7 + 0.9 b) otherwise
   //   128 x 128, two sets     n (4 + 0.52 b)
   //   256 x 256               n (9.3 + 1.46 b)
@@ -1000,7 +1001,7 @@ int launch(const GemmParams& g, hipStream_t st) {
   };
   const float n64 = per(64, 256), n128 = per(128, 256), step64 = F32 ? 0.277f * n64 : 0.2f * n64, latency = F32 ? 0.5f : 0.25f;
   const float us[5] = {(F32 ? 2.9f : 2.0f) * per(64, 1024) + b * (step64 > latency ? step64 : latency),
-                       n64 * ((F32 ? 3.8f : 3.f) + (F32 ? 0.29f : 0.21f) * b),
+                       n64 * ((F32 ? 3.8f : 3.f) + (F32 ? 0.29f : 0.21f) * b) - 0.8f,
                        n128 <= 1.f ? (F32 ? 3.f : 2.5f) + (F32 ? 1.08f : 0.64f) * b : per(128, 512) * ((F32 ? 6.1f : 3.7f) + (F32 ? 1.7f : 0.9f) * b),
                        n128 * ((F32 ? 6.f : 4.f) + (F32 ? 0.94f : 0.52f) * b),
                        per(256, 256) * ((F32 ? 13.3f : 9.3f) + (F32 ? 3.0f : 1.46f) * b)};
