@@ -200,7 +200,7 @@ __device__ __forceinline__ Y row_sum(Y v, Y* parts) {
 }
 
 // What a row's values are until they become codes.  Rows in 32 bits take 64: a value next to a border between two codes takes the one that it has by
-// the definition, where in fp32 4e-7 of them take the other, a whole 2^-3 away, and a block's steps in a row come out 1e-4 off instead of 3e-8.
+// the definition, where in fp32 5e-7 of them take the other, a whole 2^-3 away, and a block's steps in a row come out 1e-4 off instead of 3e-8.
 // A norm alone pays for it, 65536 x 1024 69 us for 58, 16384 x 999 25 for 17; with a gate 105 for 107.  (Rows in bf16 are no nearer to what they
 // stand for than 2^-9; theirs is fp32, in which 5e-7 of the codes are the neighbour.)
 template <bool F32> struct ValueOf { typedef float type; };

@@ -200,7 +200,7 @@ def quantize_rows(x) -> Rows8:
   """Rows in 8 bits: x [..., W], float32 or bfloat16 (a copy is made where the last axis is not contiguous or the others do not flatten to
   one row stride), as they are.  The leading axes become one.  A weight [K, N] is quantised as quantize_rows(w.t()).
 
-  Every value is off by at most 2^-4 of itself, or half the smallest step of its block of 128 (2^-18 of the block's largest value); a
+  Every value is off by at most 2^-4 of itself, or half the smallest step of its block of 128 (2^-17 of the block's largest value at most); a
   block that holds a value which is not finite stands for NaN."""
   return _norm("quantize_rows", x, None, None, 0.0, None, None, _lib_rows8.AS_IS)[0]
 
