@@ -35,7 +35,7 @@ struct GemmParams {
   int32_t rows, cols;                // of the output: rows of x, rows of w
   int32_t blocks;                    // of 128 along the contraction
   int32_t row_tiles, col_tiles;
-  int32_t activation, vec;           // vec: out, c and bias are whole vectors of 8 everywhere
+  int32_t activation, vec;           // vec: out and c are whole vectors of 16 bytes everywhere
 };
 
 #define ROWS8_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt((((n) & 15) | ((((n) >> 4) & 3) << 14)) | 0x0F70)
@@ -65,39 +65,42 @@ __device__ __forceinline__ float value_of(const void* base, int64_t at) {
   return F32 ? ((const float*)base)[at] : (float)((const bf16_t*)base)[at];
 }
 
-// Eight values of the output's type, side by side on a 16-byte boundary.
+// Eight values of the output's type side by side, at any place that the type may have: the wide accesses of this chip need no more.
+typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t words2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float floats4 __attribute__((ext_vector_type(4), aligned(4)));
 template <bool F32>
 __device__ __forceinline__ void row_load8(const void* base, int64_t at, float (&f)[8]) {
   if constexpr (F32) {
-    const floatx4* const from = (const floatx4*)((const float*)base + at);
-    const floatx4 lo = from[0], hi = from[1];
+    const floats4* const from = (const floats4*)((const float*)base + at);
+    const floatx4 lo = (floatx4)from[0], hi = (floatx4)from[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
   } else {
-    unpack8(*(const uint4v*)((const bf16_t*)base + at), f);
+    unpack8((uint4v)*(const words4*)((const bf16_t*)base + at), f);
   }
 }
 template <bool F32>
 __device__ __forceinline__ void row_store8(void* base, int64_t at, const float (&f)[8]) {
   if constexpr (F32) {
-    floatx4* const to = (floatx4*)((float*)base + at);
-    to[0] = floatx4{f[0], f[1], f[2], f[3]};
-    to[1] = floatx4{f[4], f[5], f[6], f[7]};
+    floats4* const to = (floats4*)((float*)base + at);
+    to[0] = floats4{f[0], f[1], f[2], f[3]};
+    to[1] = floats4{f[4], f[5], f[6], f[7]};
   } else {
-    *(uint4v*)((bf16_t*)base + at) = pack8(f);      // (past the L2s, as the bf16 products store large outputs, it is no faster)
+    *(words4*)((bf16_t*)base + at) = pack8(f);      // (past the L2s, as the bf16 products store large outputs, it is no faster)
   }
 }
 
 // Four values of a row added, from column `at` on; none past `cols`.
 template <bool F32>
-__device__ __forceinline__ void add4(const void* base, int64_t row, int at, int cols, bool vec, floatx4& y) {
-  if (vec) {
+__device__ __forceinline__ void add4(const void* base, int64_t row, int at, int cols, floatx4& y) {
+  if (at + 4 <= cols) {
     if constexpr (F32) {
-      const floatx4 v = *(const floatx4*)((const float*)base + row + at);
+      const floatx4 v = (floatx4)*(const floats4*)((const float*)base + row + at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] += v[i];
     } else {
-      const uint2 v = *(const uint2*)((const bf16_t*)base + row + at);
+      const words2 v = *(const words2*)((const bf16_t*)base + row + at);
       y[0] += __builtin_bit_cast(float, v.x << 16);
       y[1] += __builtin_bit_cast(float, v.x & 0xffff0000u);
       y[2] += __builtin_bit_cast(float, v.y << 16);
@@ -139,8 +142,8 @@ __device__ __forceinline__ bool tile_of(const GemmParams& g, int* rt, int* ct) {
 }
 
 // A wave's sums on their way out: blocks of 32 rows x 32 NB columns from (m0, n0) on, through the wave's own LDS (fp32, rows 16 bytes apart
-// from a multiple of 128), then pieces of 8 columns of a row per lane; where rows are not whole vectors, one column per lane (1237 x 1001 to
-// 777 in fp32 with a residual 14 us with pieces of single values, 11 so; 776 columns 9.0).
+// from a multiple of 128), then pieces of 8 columns of a row per lane, wherever rows begin and end: 911 x 1218 to 11469 23 us, to 11472 23, by single
+// values 32; 1237 x 1001 to 777 in fp32 with a residual 9.1, to 776 9.0, by single values 11.
 template <int MB, int NB, bool F32>
 __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&acc)[NB][MB], uint8_t* stage, int m0, int n0) {
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
@@ -154,38 +157,25 @@ __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&a
             floatx4{acc[a][b][4 * q4], acc[a][b][4 * q4 + 1], acc[a][b][4 * q4 + 2], acc[a][b][4 * q4 + 3]};
     __builtin_amdgcn_wave_barrier();
   };
-  if (!g.vec) {
-    constexpr int ROWS = 64 / W;                       // of an instruction
-    const int col = lane % W, n = n0 + col;
+  if (n0 + 8 > g.cols) {                               // fewer columns than a piece: one a lane, 8 rows an instruction
+    const int col = lane % 8, n = n0 + col;
     const bool in = n < g.cols;
     const float bias = g.bias && in ? value_of<F32>(g.bias, n) : 0.f;
-    constexpr int PIECE = 16 / ROWS;                   // instructions at a time: what is added to is asked for by all of them first
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
       put(b);
+      const int mb = m0 + 32 * b + lane / 8;
+      float cv[4];
 #pragma unroll
-      for (int i0 = 0; i0 < 32 / ROWS; i0 += PIECE) {
-        float cv[PIECE];
-        const int mb = m0 + 32 * b + ROWS * i0 + lane / W;
-        if (g.c) {
+      for (int i = 0; i < 4; ++i) cv[i] = g.c && in && mb + 8 * i < g.rows ? value_of<F32>(g.c, (int64_t)(mb + 8 * i) * g.c_stride + n) : 0.f;
 #pragma unroll
-          for (int i = 0; i < PIECE; ++i) {
-            const int m = mb + ROWS * i < g.rows ? mb + ROWS * i : g.rows - 1;
-            cv[i] = value_of<F32>(g.c, (int64_t)m * g.c_stride + (in ? n : g.cols - 1));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < PIECE; ++i) {
-          const int m = mb + ROWS * i;
-          if (!in || m >= g.rows) continue;
-          float y = *(const float*)(stage + (ROWS * (i0 + i) + lane / W) * PITCH + 4 * col);
-          if (g.c) y += cv[i];
-          y += bias;
-          if (g.activation) y = silu(y);
-          const int64_t to = (int64_t)m * g.out_stride + n;
-          if constexpr (F32) ((float*)g.out)[to] = y;
-          else ((bf16_t*)g.out)[to] = (bf16_t)y;
-        }
+      for (int i = 0; i < 4; ++i) {
+        if (!in || mb + 8 * i >= g.rows) continue;
+        float y = *(const float*)(stage + (8 * i + lane / 8) * PITCH + 4 * col) + cv[i] + bias;
+        if (g.activation) y = silu(y);
+        const int64_t to = (int64_t)(mb + 8 * i) * g.out_stride + n;
+        if constexpr (F32) ((float*)g.out)[to] = y;
+        else ((bf16_t*)g.out)[to] = (bf16_t)y;
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -193,24 +183,32 @@ __device__ __forceinline__ void tile_out(const GemmParams& g, const floatx16 (&a
   }
   constexpr int LPR = W / 8, RPI = 64 / LPR, PIECES = 32 / RPI;        // lanes per row, rows per instruction
   const int rr = lane / LPR, cc = lane - rr * LPR;
-  const int n = n0 + 8 * cc;
+  // a row's last piece, if it is not whole, is its last eight columns (some written twice, with the same values)
+  const bool part = n0 + W > g.cols && g.cols % 8;
+  const bool has = n0 + 8 * cc < g.cols;
+  const int n = n0 + 8 * cc < g.cols - 8 ? n0 + 8 * cc : has ? g.cols - 8 : n0 + 8 * cc, col = n - n0;
   float bias[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) bias[i] = 0.f;
-  if (g.bias && n < g.cols) row_load8<F32>(g.bias, n, bias);
+  if (g.bias && has) row_load8<F32>(g.bias, n, bias);
 #pragma unroll
   for (int b = 0; b < MB; ++b) {
     put(b);
     float y[PIECES][8];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const uint8_t* at = stage + (RPI * i + rr) * PITCH + 32 * cc;
+      const uint8_t* at = stage + (RPI * i + rr) * PITCH + 4 * col;
+      if (part) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[i][e] = ((const float*)at)[e];
+        continue;
+      }
       const floatx4 lo = *(const floatx4*)at, hi = *(const floatx4*)(at + 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { y[i][e] = lo[e]; y[i][4 + e] = hi[e]; }
     }
     const int mb = m0 + 32 * b + rr;      // the lane's row of piece 0
-    auto inside = [&](int i) __attribute__((always_inline)) { return mb + RPI * i < g.rows && n < g.cols; };
+    auto inside = [&](int i) __attribute__((always_inline)) { return has && mb + RPI * i < g.rows; };
     if (g.c) {
       float cv[PIECES][8];
 #pragma unroll
@@ -869,15 +867,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void hstu_rows8_few_kernel(const Ge
     // the lane's four columns of row 16 t + l16
     const int row = 16 * t + l16, at = n0 + 4 * q;
     if (row >= g.rows || at >= g.cols) continue;
-    if (g.c) add4<F32>(g.c, (int64_t)row * g.c_stride, at, g.cols, g.vec, y);
-    if (g.bias) add4<F32>(g.bias, 0, at, g.cols, g.vec, y);
+    if (g.c) add4<F32>(g.c, (int64_t)row * g.c_stride, at, g.cols, y);
+    if (g.bias) add4<F32>(g.bias, 0, at, g.cols, y);
     if (g.activation) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = silu(y[e]);
     }
-    if (g.vec) {
-      if constexpr (F32) *(floatx4*)((float*)g.out + (int64_t)row * g.out_stride + at) = y;
-      else *(uint2*)((bf16_t*)g.out + (int64_t)row * g.out_stride + at) = uint2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+    if (at + 4 <= g.cols) {
+      if constexpr (F32) *(floats4*)((float*)g.out + (int64_t)row * g.out_stride + at) = y;
+      else *(words2*)((bf16_t*)g.out + (int64_t)row * g.out_stride + at) = words2{pack2(y[0], y[1]), pack2(y[2], y[3])};
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
