@@ -989,20 +989,22 @@ int launch(const GemmParams& g, hipStream_t st) {
   //   64 x 64                 rounds of 4 to a CU, and for each block 0.2 a tile of a CU, or its latency
   //   64 x 64, four sets      n (3 + 0.21 b), less what operands that come from memory cost tiles that wait for them more often (64 x 1024 to 4096 among
   //                           a block's other steps 6.4 us without sets, 5.6 with; called over and over 4.6 and 4.7)
-  //   128 x 128               2.5 + 0.64 b alone on a CU, rounds of two (3.7 + 0.9 b) otherwise
+  //   128 x 128               rounds of two to a CU 4.2 + 0.9 b, of one 2.5 + 0.64 b
   //   128 x 128, two sets     n (4 + 0.52 b)
-  //   256 x 256               n (9.3 + 1.46 b)
+  //   256 x 256               9.3 + 1.46 b for a chip full of them, which its power sets; where the last round is not full, the clock is higher
+  //                           (6000 x 4096 to 4096, a round and a half, 94 us; 16384 x 1024 to 1024, one, 22, and with 14 rows more 45)
   const float b = (float)g.blocks;
-  auto per = [&](int64_t t, int64_t chip) {
-    const int64_t tiles = (((int64_t)g.rows + t - 1) / t) * (((int64_t)g.cols + t - 1) / t);
-    return (float)((tiles + chip - 1) / chip);
-  };
-  const float n64 = per(64, 256), n128 = per(128, 256), step64 = F32 ? 0.277f * n64 : 0.2f * n64, latency = F32 ? 0.5f : 0.25f;
+  auto tiles = [&](int64_t t) { return (((int64_t)g.rows + t - 1) / t) * (((int64_t)g.cols + t - 1) / t); };
+  auto per = [&](int64_t t, int64_t chip) { return (float)((tiles(t) + chip - 1) / chip); };
+  const float n64 = per(64, 256), n128 = per(128, 256), n256 = per(256, 256), step64 = F32 ? 0.277f * n64 : 0.2f * n64, latency = F32 ? 0.5f : 0.25f;
+  const float one = F32 ? 3.f + 1.08f * b : 2.5f + 0.64f * b, two = F32 ? 6.1f + 1.7f * b : 4.2f + 0.9f * b;
+  const int64_t rest = tiles(128) % 512;
+  const float steps256 = F32 ? 3.0f * b * n256 : 1.46f * b * (float)tiles(256) / 256.f, least256 = F32 ? 0.f : 1.15f * b * n256;
   const float us[5] = {(F32 ? 2.9f : 2.0f) * per(64, 1024) + b * (step64 > latency ? step64 : latency),
                        n64 * ((F32 ? 3.8f : 3.f) + (F32 ? 0.29f : 0.21f) * b) - 0.8f,
-                       n128 <= 1.f ? (F32 ? 3.f : 2.5f) + (F32 ? 1.08f : 0.64f) * b : per(128, 512) * ((F32 ? 6.1f : 3.7f) + (F32 ? 1.7f : 0.9f) * b),
+                       (float)(tiles(128) / 512) * two + (rest > 256 ? two : rest ? one : 0.f),
                        n128 * ((F32 ? 6.f : 4.f) + (F32 ? 0.94f : 0.52f) * b),
-                       per(256, 256) * ((F32 ? 13.3f : 9.3f) + (F32 ? 3.0f : 1.46f) * b)};
+                       n256 * (F32 ? 13.3f : 9.3f) + (steps256 > least256 ? steps256 : least256)};
   int best = 0;
   for (int i = 1; i < 5; ++i)
     if (us[i] < us[best]) best = i;
