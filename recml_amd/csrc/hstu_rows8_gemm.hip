@@ -590,14 +590,14 @@ __device__ __forceinline__ void each(F&& f) { each_of(std::make_integer_sequence
 // 4096 109 and 78; added to other rows, 73728 x 512 to 512 48 and 40; 73728 x 256 to 1024 56 and 41, x 64 to 256 16 and 13.  SiLU's two
 // quarter-rate instructions a value are as much work as the products are.  Two blocks of 32 rows a wave halve the reads of LDS and are no
 // faster (97 and 77).
-enum { ROWS_PLAIN, ROWS_SILU, ROWS_ADD };
+enum { ROWS_PLAIN = 0, ROWS_SILU = 1, ROWS_ADD = 2 };            // (bits)
 template <int KB, int OUT>
 __global__ __launch_bounds__(512, 2) void hstu_rows8_rows_kernel(const GemmParams g) {
   constexpr int NS = 2 * KB, AHEAD = 1, STAGES = 3, GROUPS = (KB + 3) / 4, PITCH = KB * BLOCK;
   constexpr int CODES = 32 * PITCH, STAGE = CODES + 256;
   constexpr int LP = (4 * KB + 7) / 8, NLOAD = LP + 1;              // direct loads of 1 KB per wave and stage, and of exponents
   constexpr int STORES = 4;
-  constexpr bool ADD = OUT == ROWS_ADD;
+  constexpr bool ADD = OUT & ROWS_ADD;
   static_assert(KB <= 8 && NS % (AHEAD + 1) == 0 && STAGES == 3, "fragments keep their registers from step to step");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const uint32_t smem_lds = __builtin_amdgcn_groupstaticsize();
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(512, 2) void hstu_rows8_rows_kernel(const GemmParam
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[i] = acc[par][4 * q4 + i];
-    if constexpr (OUT == ROWS_SILU) {
+    if constexpr (OUT & ROWS_SILU) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = silu(z[i]);
     }
@@ -958,13 +958,14 @@ int launch_rows(const GemmParams& g, hipStream_t st) {
   }
 }
 
-// Whether the weight goes by rows kept in registers: bf16 results of contractions of up to 1024, whole pieces of 64 columns, at least three
+// Whether the weight goes by rows kept in registers: bf16 results of contractions of up to 1024, whole pieces of 64 columns on whole vectors (else its
+// stores, which go past the caches, are 280 us for 104 at 73728 x 512 to 2047, and through them no quicker than tiles), at least three
 // pieces for each of the 256 workgroups (two: 4000 x 512 to 2048 12 us either way, 8000 x 512 to 2048, four of them, 16 against 19 in
-// tiles) or, where something is added, five (16398 x 1024 to 1024, four of them, 37 and in tiles 33; 32768 x 768 to 768, six, 33 and 38), and a quarter of
-// the last rows' tile wasted at most.  What it does behind the product is one of three.
+// tiles) or, where rows are added, five (16398 x 1024 to 1024, four of them, 37 and in tiles 33; 32768 x 768 to 768, six, 33 and 38), and a quarter
+// of the last rows' tile wasted at most.  Of rows to be added and a bias it takes one (a bias as rows without a stride).
 bool rows_take(const GemmParams& g) {
   const int64_t tiles = ((int64_t)g.rows + 255) / 256, pieces = tiles * (g.cols / 64);
-  return g.blocks <= 8 && g.cols % 64 == 0 && g.vec && !g.bias && !(g.c && g.activation) && pieces >= (g.c ? 1280 : 768) && 4 * (int64_t)g.rows >= 3 * 256 * tiles &&
+  return g.blocks <= 8 && g.cols % 64 == 0 && g.vec && !(g.c && g.bias) && pieces >= (g.c ? 1280 : 768) && 4 * (int64_t)g.rows >= 3 * 256 * tiles &&
          g.out_stride < 1 << 21 && g.c_stride < 1 << 21 && g.cols < 1 << 29;
 }
 
@@ -980,7 +981,15 @@ template <bool F32>
 int launch(const GemmParams& g, hipStream_t st) {
   if (const int few = few_take(g)) return few == 1 ? launch_few<1, F32>(g, st) : launch_few<2, F32>(g, st);
   if constexpr (!F32) {
-    if (rows_take(g)) return g.c ? launch_rows<ROWS_ADD>(g, st) : g.activation ? launch_rows<ROWS_SILU>(g, st) : launch_rows<ROWS_PLAIN>(g, st);
+    if (rows_take(g)) {
+      GemmParams r = g;
+      if (g.bias) {
+        r.c = g.bias;
+        r.c_stride = 0;
+      }
+      return r.c ? (g.activation ? launch_rows<ROWS_ADD | ROWS_SILU>(r, st) : launch_rows<ROWS_ADD>(r, st))
+                 : (g.activation ? launch_rows<ROWS_SILU>(r, st) : launch_rows<ROWS_PLAIN>(r, st));
+    }
   }
   // The tiles under which the call is shortest, by what they were measured to take (us; b: blocks of the contraction, n: tiles to a CU).
   // Where tiles are one to a CU, sets of waves that share a long contraction out are what hides its latencies: 64 x 8192 to 8192 in tiles of 64
@@ -1047,7 +1056,7 @@ int gemm(const HstuRows8GemmArgs* a, void* stream) {
   g.out_stride = a->out_stride; g.c_stride = a->c_stride;
   g.rows = (int32_t)a->x.rows; g.cols = (int32_t)a->w.rows; g.blocks = rows8_blocks(a->x.width);
   g.activation = a->activation;
-  g.vec = g.cols % 8 == 0 && rows8_aligned16(a->out) && a->out_stride % unit == 0 && rows8_aligned16(a->bias) &&
+  g.vec = g.cols % 8 == 0 && rows8_aligned16(a->out) && a->out_stride % unit == 0 &&
           (!a->c || (rows8_aligned16(a->c) && a->c_stride % unit == 0));
   return f32 ? launch<true>(g, (hipStream_t)stream) : launch<false>(g, (hipStream_t)stream);
 }

@@ -227,6 +227,20 @@ def test_many_sums_of_short_contractions(gpu, depth):
   assert torch.equal(got, recml_amd.gemm_rows8(x, w, residual=c))
 
 
+@pytest.mark.parametrize("how", ["bias", "bias silu", "added silu", "added bias"])
+@pytest.mark.parametrize("depth", [128, 200, 384, 512, 600, 768, 800, 1000])
+def test_many_outputs_of_short_contractions_with_a_bias(gpu, depth, how):
+  """A bias that starts between two 16-byte pieces among them."""
+  rows, cols = 256 * 17 - 37, 64 * 77
+  x, w = (recml_amd.quantize_rows(_rows(n, depth, F32, n, 0.5).to(gpu)) for n in (rows, cols))
+  b = torch.randn(cols + 1, generator=_gen(depth)).to(BF16).to(gpu)[1:] if "bias" in how else None
+  c = torch.randn((rows, cols), generator=_gen(depth + 1)).to(BF16).to(gpu) if "added" in how else None
+  got = recml_amd.gemm_rows8(x, w, b, "silu" in how, residual=c)
+  y, before, sizes = R.product(R.values(x.codes, x.exponents, depth).to(gpu), R.values(w.codes, w.exponents, depth).to(gpu), b, c, "silu" in how)
+  assert float(((got.double() - y).abs() - R.product_off(y, before, sizes, depth, BF16, "silu" in how)).max()) <= 0
+  assert torch.equal(got, recml_amd.gemm_rows8(x, w, b, "silu" in how, residual=c))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("rows,depth,cols", [(1, 128, 24), (20, 300, 40), (50, 300, 72), (300, 200, 136), (2000, 200, 1032), (7000, 200, 2120), (2779, 500, 4800), (130, 2600, 520), (700, 4200, 3704)])
 def test_leaves_what_is_not_its_own(gpu, rows, depth, cols, dtype):
