@@ -174,17 +174,22 @@ __device__ __forceinline__ uint32_t max_neighbour(uint32_t v) {
   const uint32_t o = of_neighbour<CTRL>(v);
   return o > v ? o : v;
 }
-// the largest of a block's 16 threads (of 8 where a row has no more)
+// the largest of a block's 16 threads (of fewer where a row has no more)
 template <int T>
 __device__ __forceinline__ uint32_t block_max(uint32_t v) {
-  v = max_neighbour<0x141>(max_neighbour<0x4E>(max_neighbour<0xB1>(v)));
-  return T >= 16 ? max_neighbour<0x140>(v) : v;
+  v = max_neighbour<0xB1>(v);
+  if constexpr (T >= 4) v = max_neighbour<0x4E>(v);
+  if constexpr (T >= 8) v = max_neighbour<0x141>(v);
+  if constexpr (T >= 16) v = max_neighbour<0x140>(v);
+  return v;
 }
 
 // the sum over a row's T threads, the same bits in each of them
 template <int T, class Y>
 __device__ __forceinline__ Y row_sum(Y v, Y* parts) {
-  v = add_neighbour<0x141>(add_neighbour<0x4E>(add_neighbour<0xB1>(v)));
+  v = add_neighbour<0xB1>(v);
+  if constexpr (T >= 4) v = add_neighbour<0x4E>(v);
+  if constexpr (T >= 8) v = add_neighbour<0x141>(v);
   if constexpr (T >= 16) v = add_neighbour<0x140>(v);
   if constexpr (T >= 32) v += __shfl_xor(v, 16, 64);
   if constexpr (T >= 64) v += __shfl_xor(v, 32, 64);
@@ -220,7 +225,7 @@ __device__ __forceinline__ double inverse_root(double v) { return v > 0x1.fffffe
 
 constexpr int threads_of(int t) { return t < 256 ? 256 : t; }
 
-// T threads a row (8 of 64 values up to a workgroup), V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
+// T threads a row (2 of 16 values up to a workgroup), V pieces of 8 values each: piece v of thread t holds the values from 8 (v T + t) on, so a block's are 16 neighbours.
 // Everything that a row needs is asked for at once: gamma, beta and gate behind the statistics would be a second latency (but for the widest rows
 // in 32 bits, which have no registers for it: 2048 x 32768 with a gate 139 us for 310).  MORE: there is
 // something to add or a gate; what is not there (nor beta) is read from x (gamma) once more and left out, so that no branch parts the loads.
@@ -346,7 +351,8 @@ __global__ __launch_bounds__(threads_of(T)) void hstu_rows8_norm_kernel(const Pa
     code.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[6], z[7], c, true);
     uint8_t* const to = p.codes + row * ((int64_t)blocks * BLOCK) + 8 * piece;
     if (block < blocks) *(uint2*)to = bad ? uint2{0u, 0u} : code;
-    if constexpr (T == 8) *(uint2*)(to + 64) = uint2{0u, 0u};
+#pragma unroll
+    for (int i = T; i < 16; i += T) *(uint2*)(to + 8 * i) = uint2{0u, 0u};
     if (t % 16 == 0 && block < (blocks + 3) / 4 * 4)
       p.exponents[((int64_t)(block / 4) * p.rows + row) * 4 + block % 4] = block >= blocks ? (uint8_t)1 : bad ? (uint8_t)255 : (uint8_t)e;
     // (groups whose last blocks no thread has)
@@ -362,17 +368,17 @@ struct ReadParams {
   void* out;
   int64_t out_stride, rows;
   int32_t width;
-  int32_t pieces;          // of 8 values, in a row's codes
+  int32_t pieces;          // of 8 values, in a row
 };
 
 // a piece of 8 values a thread
 template <bool F32>
 __global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = at / p.pieces;
-  const int piece = (int)(at - row * p.pieces);
-  if (row >= p.rows || 8 * piece >= p.width) return;
-  const uint2 w = *(const uint2*)(p.codes + at * 8);
+  const uint32_t at = blockIdx.x * 256u + threadIdx.x, of = at / (uint32_t)p.pieces;      // (a launch has fewer than 2^32 threads)
+  const int64_t row = of;
+  const int piece = (int)(at - of * (uint32_t)p.pieces);
+  if (row >= p.rows) return;
+  const uint2 w = *(const uint2*)(p.codes + row * ((int64_t)rows8_blocks(p.width) * BLOCK) + 8 * piece);
   const int block = piece / 16;
   const uint32_t e = p.exponents[((int64_t)(block / 4) * p.rows + row) * 4 + block % 4];
   const float power = e == 255u ? __builtin_nanf("") : power_of(e);
@@ -386,11 +392,15 @@ __global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p
 
 template <bool F32, int NORM, bool MORE, int FIT>
 void launch_norm(const Params& p, hipStream_t st) {
+  // (479394 x 9, normed, 45 us by eight threads a row, 31 by two; 302579 x 21 with a gate 24 and, by four, 18; as they are, where the zeros behind the values are most of the work, 250075 x 9 11 and 15)
+  constexpr int FEW = NORM == HSTU_ROWS8_AS_IS ? 8 : 2, SOME = NORM == HSTU_ROWS8_AS_IS ? 8 : 4;
 #define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, NORM, MORE, FIT, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
   if constexpr (FIT == FIT_PART) {
-    ROWS8_LAUNCH(8, 1);
+    ROWS8_LAUNCH(FEW, 1);
   } else {
-    if (p.width <= 64) ROWS8_LAUNCH(8, 1);
+    if (p.width <= 8 * FEW) ROWS8_LAUNCH(FEW, 1);
+    else if (p.width <= 8 * SOME) ROWS8_LAUNCH(SOME, 1);
+    else if (p.width <= 64) ROWS8_LAUNCH(8, 1);
     else if (p.width <= 128) ROWS8_LAUNCH(16, 1);
     else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
     else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
@@ -474,7 +484,7 @@ int read_rows(const HstuRows8ReadArgs* a, void* stream) {
   ReadParams p;
   p.codes = (const uint8_t*)a->rows.codes; p.exponents = (const uint8_t*)a->rows.exponents;
   p.out = a->out; p.out_stride = a->out_stride; p.rows = a->rows.rows; p.width = a->rows.width;
-  p.pieces = rows8_blocks(p.width) * (BLOCK / 8);
+  p.pieces = (p.width + 7) / 8;
   const int64_t all = p.rows * p.pieces;
   if (all > ROWS8_THREADS - 256) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)p.rows, p.width);
   const uint32_t grid = (uint32_t)((all + 255) / 256);

@@ -93,7 +93,7 @@ def test_layouts(gpu, dtype):
 
 NORMS = [(1, 1), (5, 3), (3, 8), (7, 64), (4, 100), (130, 128), (3, 129), (9, 250), (6, 512), (3, 520), (5, 777), (2, 1000), (3, 1024), (2, 1500), (2, 2048), (2, 3001),
          (2, 8192), (2, 10000)]
-NORMS += [(33, 40), (17, 41), (9, 136), (9, 256), (4, 1001), (3, 2047), (3, 4096), (3, 4095), (2, 8191), (2, 16384), (2, 32767), (2, 32768)]
+NORMS += [(33, 40), (17, 41), (9, 136), (9, 256), (4, 1001), (3, 2047), (3, 4096), (3, 4095), (2, 8191), (2, 16384), (2, 32767), (2, 32768), (130, 5), (300, 9), (129, 16), (70, 17), (65, 31), (66, 32)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
