@@ -136,14 +136,25 @@ def _glorot_uniform(shape, fan_in, fan_out, generator, dtype, device):
   return w.to(device=device, dtype=dtype)
 
 
-def _versions(tensors):
-  """Which tensors they are, and how often they were written to (so that a copy of them knows whether it still is one)."""
-  return tuple((t, 0 if t.is_inference() else t._version) for t in tensors if t is not None)
+class _MadeOf:
+  """The parameters that weights in 8 bits were made of, and how often they had been written to, so that a call knows whether they still are
+  what it reads.  A copied parameter counts its writes anew: a copy of this one (copy.deepcopy, pickle) refers to the copied parameters and
+  starts from their counts, if the original was up to date, and is never up to date if it was not."""
 
+  __slots__ = ("tensors", "versions")
 
-def _unchanged(kept, tensors) -> bool:
-  now = _versions(tensors)
-  return len(now) == len(kept) and all(a is b and m == n for (a, m), (b, n) in zip(kept, now))
+  def __init__(self, tensors, whole=True):
+    self.tensors = tuple(tensors)
+    self.versions = self._now() if whole else None
+
+  def _now(self):
+    return tuple(0 if t.is_inference() else t._version for t in self.tensors)
+
+  def up_to_date(self, tensors) -> bool:
+    return len(tensors) == len(self.tensors) and all(a is b for a, b in zip(self.tensors, tensors)) and self._now() == self.versions
+
+  def __reduce__(self):
+    return _MadeOf, (self.tensors, self.up_to_date(self.tensors))
 
 
 class HSTUBlock(torch.nn.Module):
@@ -204,12 +215,13 @@ class HSTUBlock(torch.nn.Module):
     """Keeps the projections' and the output product's weights in 8 bits (hstu_rows8.Rows8): every call of the block then runs its norms,
     products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
     a change to them quantize() has to be called again (a call notices and raises; not what is written past autograd, through .data, nor
-    parametrized weights).  `dequantize` goes back."""
+    parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits too and notices changes to its own
+    parameters.  `dequantize` goes back."""
     with torch.no_grad():
       w, b = self._uqkv_weights()
       out = self.output_kernel.reshape(-1, self.hidden_dim)
       kept = hstu_rows8.quantize_rows(w.t()), b, hstu_rows8.quantize_rows(out.t())
-    self._rows8 = (*kept, _versions(self._quantized_weights()))
+    self._rows8 = (*kept, _MadeOf(self._quantized_weights()))
 
   def dequantize(self) -> None:
     """Back to the parameters' own type."""
@@ -225,7 +237,7 @@ class HSTUBlock(torch.nn.Module):
     """Whether a call of a block with weights in 8 bits can be one; raises if not."""
     if self._wants_grad(*inputs):
       raise ValueError("a block with its weights in 8 bits has no gradient: call it under torch.no_grad(), or dequantize() it first")
-    if not _unchanged(self._rows8[3], self._quantized_weights()):
+    if not self._rows8[3].up_to_date(self._quantized_weights()):
       raise ValueError("the block's weights have changed since quantize(): call it again")
 
   def _dropout_kw(self, dropout_seed=None) -> dict:
@@ -527,7 +539,7 @@ class HSTU(torch.nn.Module):
     self._head8 = None
     if head:
       with torch.no_grad():
-        self._head8 = hstu_rows8.quantize_rows(self.reverse_embedding.t()), _versions([self.reverse_embedding])
+        self._head8 = hstu_rows8.quantize_rows(self.reverse_embedding.t()), _MadeOf([self.reverse_embedding])
 
   def dequantize(self) -> None:
     """Back to the parameters' own type."""
@@ -613,7 +625,7 @@ class HSTU(torch.nn.Module):
   def _head(self, x):
     if self._head8 is not None:
       w, made_of = self._head8
-      if not _unchanged(made_of, [self.reverse_embedding]):
+      if not made_of.up_to_date([self.reverse_embedding]):
         raise ValueError("the head's weight has changed since quantize(): call it again")
       if _differentiates(x, self.reverse_embedding):
         raise ValueError("a head with its weight in 8 bits has no gradient: call it under torch.no_grad(), or dequantize() the model first")

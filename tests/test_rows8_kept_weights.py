@@ -1,0 +1,120 @@
+"""Weights kept in 8 bits know whether they still are the parameters': written to, replaced, copied, saved and loaded.  (No GPU: what stands for
+the rows in 8 bits here is a copy of the weight, and no block is run.)"""
+
+import copy
+import io
+
+import pytest
+import torch
+
+import recml_amd
+from recml_amd import hstu_rows8
+
+
+@pytest.fixture
+def stand_ins(monkeypatch):
+  monkeypatch.setattr(hstu_rows8, "quantize_rows", lambda x: x.clone())
+  monkeypatch.setattr(hstu_rows8, "gemm_rows8", lambda x, w, *args, **kw: x @ w.t())
+  monkeypatch.setattr(torch.Tensor, "rows", property(lambda t: t.shape[0]), raising=False)
+
+
+def _model(seed, dtype=torch.float32):
+  return recml_amd.HSTU(vocab_size=11, max_positions=8, model_dim=8, num_heads=2, num_layers=2, dtype=dtype, seed=seed).eval()
+
+
+def _saved(model):
+  file = io.BytesIO()
+  torch.save(model, file)
+  file.seek(0)
+  return torch.load(file, weights_only=False)
+
+
+COPIES = {"deepcopy": copy.deepcopy, "saved and loaded": _saved}
+
+
+def _runs(model):
+  """Asks the blocks and the head as their calls do."""
+  for block in model.decoder_blocks:
+    block._check_rows8()
+  if model._head8 is not None:
+    x = torch.ones((2, model.model_dim), dtype=model.reverse_embedding.dtype)
+    assert torch.equal(model._head(x), x @ model.reverse_embedding)
+
+
+def _refused(model):
+  for block in model.decoder_blocks:
+    with pytest.raises(ValueError, match="changed since quantize"):
+      block._check_rows8()
+  if model._head8 is not None:
+    with pytest.raises(ValueError, match="head's weight has changed"):
+      model._head(torch.ones((2, model.model_dim), dtype=model.reverse_embedding.dtype))
+
+
+@pytest.mark.parametrize("how", sorted(COPIES))
+@pytest.mark.parametrize("loads", [0, 1, 2])
+def test_a_copy_is_as_good_as_what_it_is_of(stand_ins, loads, how):
+  model = _model(1)
+  for i in range(loads):
+    model.load_state_dict(_model(2 + i).state_dict())
+  model.quantize(head=True)
+  again = COPIES[how](model)
+  _runs(again)
+  assert torch.equal(again.decoder_blocks[1]._rows8[0], model.decoder_blocks[1]._rows8[0])
+  _runs(COPIES[how](again))
+  _runs(model)
+
+
+@pytest.mark.parametrize("how", sorted(COPIES))
+@pytest.mark.parametrize("before", [0, 1, 2])
+@pytest.mark.parametrize("after", [1, 2])
+def test_a_copy_notices_what_is_written_to_it(stand_ins, before, after, how):
+  """However many times it was written to before it was copied."""
+  model = _model(1)
+  for i in range(before):
+    model.load_state_dict(_model(2 + i).state_dict())
+  model.quantize(head=True)
+  again = COPIES[how](model)
+  for i in range(after):
+    again.load_state_dict(_model(7 + i).state_dict())
+  _refused(again)
+  _runs(model)
+  again.quantize(head=True)
+  _runs(again)
+
+
+@pytest.mark.parametrize("how", sorted(COPIES))
+def test_a_copy_of_what_has_changed_is_refused_too(stand_ins, how):
+  model = _model(1)
+  model.quantize(head=True)
+  model.load_state_dict(_model(2).state_dict())
+  _refused(model)
+  again = COPIES[how](model)
+  _refused(again)
+  _refused(COPIES[how](again))
+  again.load_state_dict(_model(3).state_dict())
+  _refused(again)
+  again.quantize(head=True)
+  _runs(again)
+
+
+@pytest.mark.parametrize("how", sorted(COPIES))
+def test_a_copy_of_what_was_replaced_is_refused_too(stand_ins, how):
+  model = _model(1)
+  model.quantize(head=True)
+  for block in model.decoder_blocks:
+    block.q_kernel = torch.nn.Parameter(block.q_kernel.detach().clone(), requires_grad=False)
+  model.reverse_embedding = torch.nn.Parameter(model.reverse_embedding.detach().clone(), requires_grad=False)
+  _refused(model)
+  _refused(COPIES[how](model))
+
+
+def test_a_shallow_copy_sees_the_same_parameters(stand_ins):
+  block = _model(1).decoder_blocks[0]
+  block.quantize()
+  again = copy.copy(block)
+  again._check_rows8()
+  with torch.no_grad():
+    block.u_kernel.mul_(2.0)
+  for b in (block, again):
+    with pytest.raises(ValueError, match="changed since quantize"):
+      b._check_rows8()
