@@ -139,22 +139,35 @@ def _glorot_uniform(shape, fan_in, fan_out, generator, dtype, device):
 class _MadeOf:
   """The parameters that weights in 8 bits were made of, and how often they had been written to, so that a call knows whether they still are
   what it reads.  A copied parameter counts its writes anew: a copy of this one (copy.deepcopy, pickle) refers to the copied parameters and
-  starts from their counts, if the original was up to date, and is never up to date if it was not."""
+  starts from their counts, if the original was up to date, and is never up to date if it was not, or if the copies count nothing."""
 
   __slots__ = ("tensors", "versions")
 
   def __init__(self, tensors, whole=True):
     self.tensors = tuple(tensors)
-    self.versions = self._now() if whole else None
+    self.versions = self._now() if whole and self.counted(tensors) else None
+
+  @staticmethod
+  def counted(tensors) -> bool:
+    """Whether writes to them are counted: those of tensors made under torch.inference_mode() are not."""
+    return not any(t.is_inference() for t in tensors)
 
   def _now(self):
-    return tuple(0 if t.is_inference() else t._version for t in self.tensors)
+    return tuple(t._version for t in self.tensors)
 
   def up_to_date(self, tensors) -> bool:
-    return len(tensors) == len(self.tensors) and all(a is b for a, b in zip(self.tensors, tensors)) and self._now() == self.versions
+    return (self.versions is not None and len(tensors) == len(self.tensors) and all(a is b for a, b in zip(self.tensors, tensors))
+            and self._now() == self.versions)
 
   def __reduce__(self):
     return _MadeOf, (self.tensors, self.up_to_date(self.tensors))
+
+
+def _check_counted(weights):
+  """Raises where a later change to the weights could not be noticed."""
+  if not _MadeOf.counted(weights):
+    raise ValueError("weights made under torch.inference_mode() do not tell when they are written to: make the model, or load its weights, outside "
+                     "of it before quantize()")
 
 
 class HSTUBlock(torch.nn.Module):
@@ -216,7 +229,8 @@ class HSTUBlock(torch.nn.Module):
     products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
     a change to them quantize() has to be called again (a call notices and raises; not what is written past autograd, through .data, nor
     parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits too and notices changes to its own
-    parameters.  `dequantize` goes back."""
+    parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused.  `dequantize` goes back."""
+    _check_counted(self._quantized_weights())
     with torch.no_grad():
       w, b = self._uqkv_weights()
       out = self.output_kernel.reshape(-1, self.hidden_dim)
@@ -534,6 +548,10 @@ class HSTU(torch.nn.Module):
     products on them, in inference only, on a GPU.  The parameters stay as they are; call it again after a change to them."""
     if head and self.reverse_embedding is None:
       raise ValueError("the model has no output head")
+    for block in self.decoder_blocks:
+      _check_counted(block._quantized_weights())
+    if head:
+      _check_counted([self.reverse_embedding])
     for block in self.decoder_blocks:
       block.quantize()
     self._head8 = None

@@ -118,3 +118,40 @@ def test_a_shallow_copy_sees_the_same_parameters(stand_ins):
   for b in (block, again):
     with pytest.raises(ValueError, match="changed since quantize"):
       b._check_rows8()
+
+
+def test_parameters_that_do_not_count_their_writes_are_refused(stand_ins):
+  """Those made under inference mode."""
+  with torch.inference_mode():
+    model = _model(1)
+  with pytest.raises(ValueError, match="inference_mode"):
+    model.quantize()
+  with pytest.raises(ValueError, match="inference_mode"):
+    model.decoder_blocks[0].quantize()
+  assert all(block._rows8 is None for block in model.decoder_blocks)
+  model = _model(1)
+  model.reverse_embedding = None
+  with torch.inference_mode():
+    model.reverse_embedding = torch.nn.Parameter(torch.ones((8, 11)), requires_grad=False)
+  with pytest.raises(ValueError, match="inference_mode"):
+    model.quantize(head=True)
+  assert all(block._rows8 is None for block in model.decoder_blocks)      # (before any work)
+
+
+@pytest.mark.parametrize("how", sorted(COPIES))
+def test_copies_made_under_inference_mode_are_refused(stand_ins, how):
+  model = _model(1)
+  model.quantize(head=True)
+  with torch.inference_mode():
+    again = COPIES[how](model)
+  if any(p.is_inference() for p in again.parameters()):
+    _refused(again)
+
+
+def test_what_is_written_under_inference_mode_is_noticed(stand_ins):
+  model = _model(1)
+  with torch.inference_mode():
+    model.quantize(head=True)
+    _runs(model)
+    model.load_state_dict(_model(2).state_dict())
+    _refused(model)
