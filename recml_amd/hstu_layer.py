@@ -137,14 +137,16 @@ def _glorot_uniform(shape, fan_in, fan_out, generator, dtype, device):
 
 
 class _MadeOf:
-  """The parameters that weights in 8 bits were made of, and how often they had been written to, so that a call knows whether they still are
-  what it reads.  A copied parameter counts its writes anew: a copy of this one (copy.deepcopy, pickle) refers to the copied parameters and
+  """The parameters that weights in 8 bits were made of, where they lay and how often they had been written to, so that a call knows whether they
+  still are what it reads (a conversion or a move puts other memory under the same parameter, and is no write to it; the memory is held, so that none
+  that comes later can lie there).  A copied parameter counts its writes anew: a copy of this one (copy.deepcopy, pickle) refers to the copied parameters and
   starts from their counts, if the original was up to date, and is never up to date if it was not, or if the copies count nothing."""
 
-  __slots__ = ("tensors", "versions")
+  __slots__ = ("tensors", "memory", "versions")
 
   def __init__(self, tensors, whole=True):
     self.tensors = tuple(tensors)
+    self.memory = tuple(t.detach() for t in self.tensors)
     self.versions = self._now() if whole and self.counted(tensors) else None
 
   @staticmethod
@@ -153,7 +155,7 @@ class _MadeOf:
     return not any(t.is_inference() for t in tensors)
 
   def _now(self):
-    return tuple(t._version for t in self.tensors)
+    return tuple((t._version, t.data_ptr(), t.dtype) for t in self.tensors)
 
   def up_to_date(self, tensors) -> bool:
     return (self.versions is not None and len(tensors) == len(self.tensors) and all(a is b for a, b in zip(self.tensors, tensors))
@@ -227,9 +229,10 @@ class HSTUBlock(torch.nn.Module):
   def quantize(self) -> None:
     """Keeps the projections' and the output product's weights in 8 bits (hstu_rows8.Rows8): every call of the block then runs its norms,
     products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
-    a change to them quantize() has to be called again (a call notices and raises; not what is written past autograd, through .data, nor
-    parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits too and notices changes to its own
-    parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused.  `dequantize` goes back."""
+    a change to them quantize() has to be called again (a call notices and raises, after a conversion or a move of the model too; not what is
+    written past autograd, into .data, nor parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits
+    too and notices changes to its own parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused.
+    `dequantize` goes back."""
     _check_counted(self._quantized_weights())
     with torch.no_grad():
       w, b = self._uqkv_weights()

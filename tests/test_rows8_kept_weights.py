@@ -155,3 +155,27 @@ def test_what_is_written_under_inference_mode_is_noticed(stand_ins):
     _runs(model)
     model.load_state_dict(_model(2).state_dict())
     _refused(model)
+
+
+def test_parameters_whose_memory_was_replaced_are_noticed(stand_ins):
+  """Converted to another type or put elsewhere: the parameter stays, and its count too."""
+  model = _model(1)
+  model.quantize(head=True)
+  model.to(torch.float32).to("cpu").eval().requires_grad_(False)
+  _runs(model)
+  model.to(torch.bfloat16)
+  _refused(model)
+  model.quantize(head=True)
+  _runs(model)
+  for p in model.parameters():
+    p.data = p.data.clone()
+  _refused(model)
+
+
+def test_there_and_back_is_noticed(stand_ins):
+  """Values that were rounded on the way may come to lie where the old ones lay."""
+  for _ in range(20):
+    model = _model(1)
+    model.quantize(head=True)
+    model.to(torch.bfloat16).to(torch.float32)
+    _refused(model)
