@@ -161,6 +161,12 @@ class _MadeOf:
     return (self.versions is not None and len(tensors) == len(self.tensors) and all(a is b for a, b in zip(self.tensors, tensors))
             and self._now() == self.versions)
 
+  def spend(self) -> bool:
+    """Whether what was made may be written over: once, by whoever asks first (a shallow copy of a block has it too).  From then on this is
+    never up to date."""
+    mine, self.versions = self.versions is not None, None
+    return mine
+
   def __reduce__(self):
     return _MadeOf, (self.tensors, self.up_to_date(self.tensors))
 
@@ -232,16 +238,19 @@ class HSTUBlock(torch.nn.Module):
     a change to them quantize() has to be called again (a call notices and raises, after a conversion or a move of the model too; not what is
     written past autograd, into .data, nor parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits
     too and notices changes to its own parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused.
-    `dequantize` goes back."""
+    Called again, it writes the codes in their old place, if the weights are as large and on that device as before: captured calls replay
+    with the new ones (a replay asks nothing; until then it has the old).  `dequantize` goes back, and captured calls must not be replayed
+    any more."""
     _check_counted(self._quantized_weights())
     with torch.no_grad():
       w, b = self._uqkv_weights()
       out = self.output_kernel.reshape(-1, self.hidden_dim)
-      kept = hstu_rows8.quantize_rows(w.t()), b, hstu_rows8.quantize_rows(out.t())
+      old = self._rows8[:3] if self._rows8 is not None and self._rows8[3].spend() else (None, None, None)
+      kept = hstu_rows8.renew_rows(w.t(), old[0]), hstu_rows8.renew(b, old[1]), hstu_rows8.renew_rows(out.t(), old[2])
     self._rows8 = (*kept, _MadeOf(self._quantized_weights()))
 
   def dequantize(self) -> None:
-    """Back to the parameters' own type."""
+    """Back to the parameters' own type.  Frees the codes: calls that were captured with them must not be replayed."""
     self._rows8 = None
 
   def _quantized_weights(self):
@@ -548,7 +557,8 @@ class HSTU(torch.nn.Module):
 
   def quantize(self, *, head: bool = False) -> None:
     """Keeps the blocks' weights in 8 bits (HSTUBlock.quantize), and with `head` the head's: forward, prefill and extend then run their
-    products on them, in inference only, on a GPU.  The parameters stay as they are; call it again after a change to them."""
+    products on them, in inference only, on a GPU.  The parameters stay as they are; call it again after a change to them, with the same `head`
+    if captured calls are to go on (without it the head's codes are freed, as all are by `dequantize`)."""
     if head and self.reverse_embedding is None:
       raise ValueError("the model has no output head")
     for block in self.decoder_blocks:
@@ -557,13 +567,14 @@ class HSTU(torch.nn.Module):
       _check_counted([self.reverse_embedding])
     for block in self.decoder_blocks:
       block.quantize()
-    self._head8 = None
+    old, self._head8 = self._head8, None
     if head:
       with torch.no_grad():
-        self._head8 = hstu_rows8.quantize_rows(self.reverse_embedding.t()), _MadeOf([self.reverse_embedding])
+        kept = hstu_rows8.renew_rows(self.reverse_embedding.t(), old[0] if old is not None and old[1].spend() else None)
+      self._head8 = kept, _MadeOf([self.reverse_embedding])
 
   def dequantize(self) -> None:
-    """Back to the parameters' own type."""
+    """Back to the parameters' own type (HSTUBlock.dequantize)."""
     for block in self.decoder_blocks:
       block.dequantize()
     self._head8 = None

@@ -205,6 +205,25 @@ def quantize_rows(x) -> Rows8:
   return _norm("quantize_rows", x, None, None, 0.0, None, None, _lib_rows8.AS_IS)[0]
 
 
+def renew_rows(x, rows) -> Rows8:
+  """quantize_rows(x) of a matrix in the place of `rows`, so that what reads them there (a captured graph) reads the new ones; new rows where
+  `rows` are None, or others in number, width or device."""
+  fresh = quantize_rows(x)
+  if not isinstance(rows, Rows8) or (rows.rows, rows.width, rows.device) != (fresh.rows, fresh.width, fresh.device):
+    return fresh
+  renew(fresh.exponents, rows.exponents)
+  renew(fresh.codes, rows.codes)
+  return rows
+
+
+def renew(fresh, kept):
+  """`fresh` in the place of `kept`, or as it is where that has no such place."""
+  if fresh is None or kept is None or (fresh.shape, fresh.dtype, fresh.device) != (kept.shape, kept.dtype, kept.device):
+    return fresh
+  with torch.inference_mode():                     # (`kept` may have been made there)
+    return kept.copy_(fresh)
+
+
 def norm_rows8(x, gamma, beta=None, eps: float = 1e-6, *, gate=None, add=None, rms: bool = False):
   """A norm of rows over their last axis, in 8 bits: gate * layer_norm(x + add), the statistics in fp32, one rounding.
 
