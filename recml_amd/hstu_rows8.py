@@ -101,7 +101,7 @@ class Rows8:
     raise AttributeError("Rows8 are what they were made of: make new ones")
 
   def __reduce__(self):
-    return Rows8, (self.codes, self.exponents, self.width)
+    return _loaded, (self.codes, self.exponents, self.width)
 
   def __repr__(self):
     return f"Rows8({self.rows} rows of {self.width} on {self.codes.device})"
@@ -131,6 +131,7 @@ class Rows8:
     got = _native.read_rows8(self.codes, self.exponents, self.width, dtype)
     if got is not None:
       return got
+    _check_gpu("codes", self.codes)
     if dtype not in _DTYPES:
       raise ValueError(f"dtype must be torch.bfloat16 or torch.float32, got {dtype}")
     out = torch.empty((self.rows, self.width), dtype=dtype, device=self.device)
@@ -142,6 +143,12 @@ class Rows8:
 
   def _fill(self, r):
     r.codes, r.exponents, r.rows, r.width = self.codes.data_ptr(), self.exponents.data_ptr(), self.rows, self.width
+
+
+def _loaded(codes, exponents, width):
+  """Rows8 that were copied or saved.  On a GPU they are checked as new ones are; elsewhere (a file loaded with map_location="cpu") they are kept,
+  and refused where something is asked of them."""
+  return Rows8(codes, exponents, width) if codes.is_cuda else Rows8._of(codes, exponents, width)
 
 
 _set_codes, _set_exponents, _set_width = (getattr(Rows8, name).__set__ for name in Rows8.__slots__)      # (past __setattr__)
@@ -252,6 +259,7 @@ def gemm_rows8(x, w, bias=None, activation: bool = False, *, residual=None, dtyp
   for name, t in (("x", x), ("w", w)):
     if not isinstance(t, Rows8):
       raise TypeError(f"{name} must be Rows8, got {type(t).__name__}")
+    _check_gpu(f"{name}.codes", t.codes)
   if x.width != w.width or x.device != w.device:
     raise ValueError(f"x [M, K] and w [N, K] on one device expected, got rows of {x.width} on {x.device} and of {w.width} on {w.device}")
   if dtype not in _DTYPES:
