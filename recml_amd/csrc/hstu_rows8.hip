@@ -390,48 +390,62 @@ __global__ __launch_bounds__(256) void hstu_rows8_read_kernel(const ReadParams p
   store8<F32>(p.out, row * p.out_stride, 8 * piece, p.width, f);
 }
 
+template <bool F32, int NORM, bool MORE, int FIT, int T, int V>
+int launch_norm(const Params& p, hipStream_t st) {
+  constexpr int THREADS = threads_of(T), ROWS = THREADS / T;      // of a workgroup
+  const int64_t groups = (p.rows + ROWS - 1) / ROWS;
+  if (groups > ROWS8_THREADS / THREADS) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)p.rows, p.width);
+  hstu_rows8_norm_kernel<F32, NORM, MORE, FIT, T, V><<<(uint32_t)groups, THREADS, 0, st>>>(p);
+  return rows8_launched("hstu_rows8_norm");
+}
+
 template <bool F32, int NORM, bool MORE, int FIT>
-void launch_norm(const Params& p, hipStream_t st) {
+int launch_norm(const Params& p, hipStream_t st) {
   // (479394 x 9, normed, 45 us by eight threads a row, 31 by two; 302579 x 21 with a gate 24 and, by four, 18; as they are, where the zeros behind the values are most of the work, 250075 x 9 11 and 15)
   constexpr int FEW = NORM == HSTU_ROWS8_AS_IS ? 8 : 2, SOME = NORM == HSTU_ROWS8_AS_IS ? 8 : 4;
-#define ROWS8_LAUNCH(T, V) hstu_rows8_norm_kernel<F32, NORM, MORE, FIT, T, V><<<(uint32_t)((p.rows + threads_of(T) / T - 1) / (threads_of(T) / T)), threads_of(T), 0, st>>>(p)
+#define ROWS8_LAUNCH(T, V) return launch_norm<F32, NORM, MORE, FIT, T, V>(p, st)
   if constexpr (FIT == FIT_PART) {
     ROWS8_LAUNCH(FEW, 1);
   } else {
     if (p.width <= 8 * FEW) ROWS8_LAUNCH(FEW, 1);
-    else if (p.width <= 8 * SOME) ROWS8_LAUNCH(SOME, 1);
-    else if (p.width <= 64) ROWS8_LAUNCH(8, 1);
-    else if (p.width <= 128) ROWS8_LAUNCH(16, 1);
-    else if (p.width <= 256) ROWS8_LAUNCH(32, 1);
-    else if (p.width <= 512) ROWS8_LAUNCH(64, 1);
-    else if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
-    else if constexpr (F32) {                      // (values in 64 bits leave registers for two pieces)
+    if (p.width <= 8 * SOME) ROWS8_LAUNCH(SOME, 1);
+    if (p.width <= 64) ROWS8_LAUNCH(8, 1);
+    if (p.width <= 128) ROWS8_LAUNCH(16, 1);
+    if (p.width <= 256) ROWS8_LAUNCH(32, 1);
+    if (p.width <= 512) ROWS8_LAUNCH(64, 1);
+    if (p.width <= 1024) ROWS8_LAUNCH(64, 2);
+    if constexpr (F32) {                           // (values in 64 bits leave registers for two pieces)
       if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
-      else if (p.width <= 4096) ROWS8_LAUNCH(256, 2);
-      else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
-      else ROWS8_LAUNCH(1024, 4);
+      if (p.width <= 4096) ROWS8_LAUNCH(256, 2);
+      if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+      ROWS8_LAUNCH(1024, 4);
     } else {
       if (p.width <= 2048) ROWS8_LAUNCH(64, 4);
-      else if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
-      else ROWS8_LAUNCH(1024, 4);
+      if (p.width <= 8192) ROWS8_LAUNCH(256, 4);
+      ROWS8_LAUNCH(1024, 4);
     }
   }
 #undef ROWS8_LAUNCH
 }
 
 template <bool F32, int NORM, bool MORE>
-void launch_norm(const Params& p, hipStream_t st) {
-  if (p.width < 8) launch_norm<F32, NORM, MORE, FIT_PART>(p, st);
-  else if (p.width % 8 == 0) launch_norm<F32, NORM, MORE, FIT_EVEN>(p, st);
-  else launch_norm<F32, NORM, MORE, FIT_REST>(p, st);
+int launch_norm(const Params& p, hipStream_t st) {
+  if (p.width < 8) return launch_norm<F32, NORM, MORE, FIT_PART>(p, st);
+  return p.width % 8 == 0 ? launch_norm<F32, NORM, MORE, FIT_EVEN>(p, st) : launch_norm<F32, NORM, MORE, FIT_REST>(p, st);
 }
 
 template <bool F32, int NORM>
-void launch_norm(const Params& p, hipStream_t st) {
+int launch_norm(const Params& p, hipStream_t st) {
   if constexpr (NORM != HSTU_ROWS8_AS_IS) {
-    if (p.add || p.gate) { launch_norm<F32, NORM, true>(p, st); return; }
+    if (p.add || p.gate) return launch_norm<F32, NORM, true>(p, st);
   }
-  launch_norm<F32, NORM, false>(p, st);
+  return launch_norm<F32, NORM, false>(p, st);
+}
+
+template <bool F32>
+int launch_norm(const Params& p, int norm, hipStream_t st) {
+  if (norm == HSTU_ROWS8_LAYER) return launch_norm<F32, HSTU_ROWS8_LAYER>(p, st);
+  return norm == HSTU_ROWS8_RMS ? launch_norm<F32, HSTU_ROWS8_RMS>(p, st) : launch_norm<F32, HSTU_ROWS8_AS_IS>(p, st);
 }
 
 int norm_rows(const HstuRows8NormArgs* a, void* stream) {
@@ -447,9 +461,6 @@ int norm_rows(const HstuRows8NormArgs* a, void* stream) {
   if (a->rows.rows == 0) return HSTU_ROWS8_OK;
   if (!a->x) return rows8_fail(HSTU_ROWS8_ERR_NULL, "x is null");
   if (a->norm != HSTU_ROWS8_AS_IS && !a->gamma) return rows8_fail(HSTU_ROWS8_ERR_NULL, "gamma is null");
-  // (a workgroup a row at most)
-  const int64_t threads = a->rows.width <= 2048 ? 64 : a->rows.width <= 8192 ? 256 : 1024;
-  if (a->rows.rows > ROWS8_THREADS / threads - 16) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%lld rows of %d are too many for one call", (long long)a->rows.rows, a->rows.width);
   const bool f32 = a->dtype == HSTU_ROWS8_FP32;
   for (const void* t : {a->x, a->add, a->gate, (const void*)a->sum, a->gamma, a->beta})
     if ((uintptr_t)t & (f32 ? 3u : 1u)) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "a pointer is not aligned to its type");
@@ -459,15 +470,7 @@ int norm_rows(const HstuRows8NormArgs* a, void* stream) {
   p.x_stride = a->x_stride; p.add_stride = a->add_stride; p.gate_stride = a->gate_stride; p.sum_stride = a->sum_stride;
   p.rows = a->rows.rows; p.width = a->rows.width; p.eps = a->eps;
   hipStream_t st = (hipStream_t)stream;
-#define ROWS8_NORM(F32)                                                                  \
-  do {                                                                                   \
-    if (a->norm == HSTU_ROWS8_LAYER) launch_norm<F32, HSTU_ROWS8_LAYER>(p, st);          \
-    else if (a->norm == HSTU_ROWS8_RMS) launch_norm<F32, HSTU_ROWS8_RMS>(p, st);         \
-    else launch_norm<F32, HSTU_ROWS8_AS_IS>(p, st);                                      \
-  } while (0)
-  if (f32) ROWS8_NORM(true); else ROWS8_NORM(false);
-#undef ROWS8_NORM
-  return rows8_launched("hstu_rows8_norm");
+  return f32 ? launch_norm<true>(p, a->norm, st) : launch_norm<false>(p, a->norm, st);
 }
 
 int read_rows(const HstuRows8ReadArgs* a, void* stream) {
