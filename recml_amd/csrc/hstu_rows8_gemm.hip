@@ -929,7 +929,9 @@ int launch_turns(GemmParams g, hipStream_t st) {
 template <int MT, bool F32>
 int launch_few(const GemmParams& g, hipStream_t st) {
   const int waves = g.blocks < FEW_WAVES ? g.blocks : FEW_WAVES;
-  hstu_rows8_few_kernel<MT, F32><<<(uint32_t)((g.cols + 15) / 16), 64 * waves, 0, st>>>(g);
+  const int64_t groups = ((int64_t)g.cols + 15) / 16;
+  if (groups * 64 * waves > ROWS8_THREADS) return rows8_fail(HSTU_ROWS8_ERR_SHAPE, "%d x %d outputs are too many for one call", g.rows, g.cols);
+  hstu_rows8_few_kernel<MT, F32><<<(uint32_t)groups, 64 * waves, 0, st>>>(g);
   return rows8_launched("hstu_rows8_gemm");
 }
 

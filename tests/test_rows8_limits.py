@@ -21,3 +21,17 @@ def test_norm_of_too_many_rows(rows, width, norm):
   lib = _lib_rows8.load()
   assert lib.hstu_rows8_norm(C.byref(a), None) == -4
   assert "too many" in lib.hstu_rows8_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype", [_lib_rows8.BF16, _lib_rows8.FP32])
+@pytest.mark.parametrize("rows", [1, 16])
+def test_product_of_few_rows_with_too_many_columns(rows, dtype):
+  """Sixteen columns a workgroup of 512 threads."""
+  a = _lib_rows8.HstuRows8GemmArgs()
+  a.struct_size, a.version = C.sizeof(a), _lib_rows8.ABI_VERSION
+  _rows(a.x, rows, 2048)
+  _rows(a.w, (1 << 27) + 16, 2048)
+  a.out, a.out_stride, a.dtype = 0x3000, a.w.rows, dtype
+  lib = _lib_rows8.load()
+  assert lib.hstu_rows8_gemm(C.byref(a), None) == -4
+  assert "too many" in lib.hstu_rows8_last_error().decode()
