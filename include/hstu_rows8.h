@@ -53,7 +53,9 @@ typedef struct HstuRows8 {
  *   HSTU_ROWS8_LAYER  y = (s - mean) * rstd * gamma + beta   mean and (biased) variance of the row, rstd = 1 / sqrt(variance + eps)
  *   HSTU_ROWS8_RMS    y = s * rstd * gamma + beta            rstd = 1 / sqrt(mean of s^2 + eps)
  *   HSTU_ROWS8_AS_IS  y = x, with nothing added and no gate
- * rows = (gate *) y in 8 bits.  Statistics and products in fp32, or in 64 bits for rows in fp32, and one rounding to the codes.  x, add, gate,
+ * rows = (gate *) y in 8 bits.  Statistics and products in fp32, or in 64 bits for rows in fp32, and one rounding to the codes.  A sum of squares
+ * past fp32's largest (for rows in fp32: a mean of squares) counts as infinite: rstd = 0.  Rows in bf16 whose variance (mean of s^2) + eps lies
+ * below 2^-126 have no rstd and stand for NaN: only an eps that small lets them.  x, add, gate,
  * sum: [rows, width] of `dtype` with row strides in elements (any alignment of the type); add and gate may be null, sum with add; sum may be
  * x or add (with its stride), otherwise no output may overlap an input.  gamma [width] of `dtype` (a norm needs it), beta likewise or null. */
 typedef struct HstuRows8NormArgs {

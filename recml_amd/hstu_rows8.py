@@ -232,7 +232,8 @@ def renew(fresh, kept):
 
 
 def norm_rows8(x, gamma, beta=None, eps: float = 1e-6, *, gate=None, add=None, rms: bool = False):
-  """A norm of rows over their last axis, in 8 bits: gate * layer_norm(x + add), the statistics in fp32, one rounding.
+  """A norm of rows over their last axis, in 8 bits: gate * layer_norm(x + add), statistics and products in fp32, or in 64 bits for float32 rows, one
+  rounding.  (A row whose sum of squares, for float32 their mean, is past fp32's largest comes back as zeros, times gamma, plus beta.)
 
   Args:
     x: [..., W], float32 or bfloat16 (a copy is made where the last axis is not contiguous or the others do not flatten to one row

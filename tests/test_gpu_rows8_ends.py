@@ -53,3 +53,26 @@ def test_small_rows_times_large_ones(gpu, rows, depth, cols, dtype):
   if dtype == F32:
     off = off + 2.0**-134 * b.abs().sum(1)[None, :]
   assert float(((recml_amd.gemm_rows8(x, w, dtype=dtype).cpu().double() - y).abs() - off).max()) <= 0
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("dtype,last", [(BF16, 59), (F32, 63)])
+def test_the_largest_rows_that_have_a_norm(gpu, dtype, last, rms):
+  """256 values of 2^p of both signs, whose norm is their sign: the sum of their squares has to lie within fp32 for rows in bf16, its mean for
+  rows in fp32; past that it counts as infinite and the row as zeros."""
+  signs = torch.where(torch.randperm(256, generator=torch.Generator().manual_seed(1)) < 128, 1.0, -1.0)
+  gamma = torch.ones(256, dtype=dtype, device=gpu)
+  for p in (last, last + 1, 100):
+    x = (signs * 2.0**p).to(dtype)[None].to(gpu)
+    want = signs if p == last else torch.zeros(256)
+    assert torch.equal(recml_amd.norm_rows8(x, gamma, rms=rms).values(F32)[0].cpu(), want), p
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("dtype,first", [(BF16, -63), (F32, -126)])
+def test_the_smallest_rows_that_have_a_norm_without_eps(gpu, dtype, first, rms):
+  """The mean of their squares has to be a normal number of the type that statistics are in: fp32 for rows in bf16, 64 bits for rows in fp32."""
+  signs = torch.where(torch.randperm(256, generator=torch.Generator().manual_seed(1)) < 128, 1.0, -1.0)
+  gamma = torch.ones(256, dtype=dtype, device=gpu)
+  x = (signs * 2.0**first).to(dtype)[None].to(gpu)
+  assert torch.equal(recml_amd.norm_rows8(x, gamma, eps=0.0, rms=rms).values(F32)[0].cpu(), signs)
