@@ -171,6 +171,26 @@ class _MadeOf:
     return _MadeOf, (self.tensors, self.up_to_date(self.tensors))
 
 
+_QUANTIZED = "u_kernel", "q_kernel", "k_kernel", "v_kernel", "output_kernel"
+_QUANTIZED_WITH_BIAS = (*_QUANTIZED, "u_bias", "q_bias", "k_bias", "v_bias")
+_HEAD = ("reverse_embedding",)
+
+
+def _sources(module, names):
+  """The parameters of these names, and in the place of one with a parametrization what that keeps."""
+  P, found = module._parameters, []
+  for n in names:
+    if n in P:
+      found.append(P[n])
+    elif n in module.__dict__:
+      raise ValueError(f"{n} is a tensor that a hook makes anew before a forward (a pruning mask, say), not a parameter or a parametrized one: make "
+                       "it permanent before quantize()")
+    else:
+      made = module.parametrizations[n]
+      found += [*made.parameters(), *made.buffers()]
+  return found
+
+
 def _check_counted(weights):
   """Raises where a later change to the weights could not be noticed."""
   if not _MadeOf.counted(weights):
@@ -236,8 +256,9 @@ class HSTUBlock(torch.nn.Module):
     """Keeps the projections' and the output product's weights in 8 bits (hstu_rows8.Rows8): every call of the block then runs its norms,
     products and gate on rows in 8 bits, in inference only, on a GPU.  The parameters stay as they are and are what state_dict has; after
     a change to them quantize() has to be called again (a call notices and raises, after a conversion or a move of the model too; not what is
-    written past autograd, into .data, nor parametrized weights).  A copy of the block, or the block saved and loaded, has its weights in 8 bits
-    too and notices changes to its own parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused.
+    written past autograd, into .data).  A copy of the block, or the block saved and loaded, has its weights in 8 bits
+    too and notices changes to its own parameters.  Parameters made under torch.inference_mode(), which do not tell of writes, are refused,
+    and so are weights that hooks make anew (pruning masks: make them permanent first).
     Called again, it writes the codes in their old place, if the weights are as large and on that device as before: captured calls replay
     with the new ones (a replay asks nothing; until then it has the old).  `dequantize` goes back, and captured calls must not be replayed
     any more.
@@ -258,10 +279,8 @@ class HSTUBlock(torch.nn.Module):
     self._rows8 = None
 
   def _quantized_weights(self):
-    """The parameters that quantize copied (not those that something else, a parametrization say, makes anew for each call)."""
-    P = self._parameters
-    names = [f"{n}_{kind}" for kind in (("kernel", "bias") if self.use_bias else ("kernel",)) for n in ("u", "q", "k", "v")] + ["output_kernel"]
-    return [P[n] for n in names if n in P]
+    """What the weights that quantize copied are made of."""
+    return _sources(self, _QUANTIZED_WITH_BIAS if self.use_bias else _QUANTIZED)
 
   def _check_rows8(self, *inputs):
     """Whether a call of a block with weights in 8 bits can be one; raises if not."""
@@ -568,14 +587,14 @@ class HSTU(torch.nn.Module):
     for block in self.decoder_blocks:
       _check_counted(block._quantized_weights())
     if head:
-      _check_counted([self.reverse_embedding])
+      _check_counted(_sources(self, _HEAD))
     for block in self.decoder_blocks:
       block.quantize()
     old, self._head8 = self._head8, None
     if head:
       with torch.no_grad():
         kept = hstu_rows8.renew_rows(self.reverse_embedding.t(), old[0] if old is not None and old[1].spend() else None)
-      self._head8 = kept, _MadeOf([self.reverse_embedding])
+      self._head8 = kept, _MadeOf(_sources(self, _HEAD))
 
   def dequantize(self) -> None:
     """Back to the parameters' own type (HSTUBlock.dequantize)."""
@@ -661,7 +680,7 @@ class HSTU(torch.nn.Module):
   def _head(self, x):
     if self._head8 is not None:
       w, made_of = self._head8
-      if not made_of.up_to_date([self.reverse_embedding]):
+      if not made_of.up_to_date(_sources(self, _HEAD)):
         raise ValueError("the head's weight has changed since quantize(): call it again")
       if _differentiates(x, self.reverse_embedding):
         raise ValueError("a head with its weight in 8 bits has no gradient: call it under torch.no_grad(), or dequantize() the model first")

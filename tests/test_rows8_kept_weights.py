@@ -6,6 +6,7 @@ import io
 
 import pytest
 import torch
+from torch.nn.utils import parametrize, prune
 
 import recml_amd
 from recml_amd import hstu_rows8
@@ -179,3 +180,75 @@ def test_there_and_back_is_noticed(stand_ins):
     model.quantize(head=True)
     model.to(torch.bfloat16).to(torch.float32)
     _refused(model)
+
+
+class _Scaled(torch.nn.Module):
+  def __init__(self):
+    super().__init__()
+    self.scale = torch.nn.Parameter(torch.tensor(2.0), requires_grad=False)
+
+  def forward(self, w):
+    return w * self.scale
+
+
+def test_what_parametrized_weights_are_made_of_is_noticed(stand_ins):
+  """The tensor that is kept, and what its parametrization keeps."""
+  block = _model(1).decoder_blocks[0]
+  parametrize.register_parametrization(block, "u_kernel", _Scaled())
+  made = block.parametrizations.u_kernel
+  for change in (lambda: made.original.mul_(2.0), lambda: made[0].scale.add_(1.0), lambda: block.k_kernel.zero_()):
+    block.quantize()
+    assert torch.equal(block._rows8[0][: block.hidden_dim], (made.original * made[0].scale).reshape(block.hidden_dim, -1).t())
+    block._check_rows8()
+    again = copy.deepcopy(block)
+    again._check_rows8()
+    with torch.no_grad():
+      change()
+    with pytest.raises(ValueError, match="changed since quantize"):
+      block._check_rows8()
+    again._check_rows8()
+
+
+def test_what_a_parametrized_head_is_made_of_is_noticed(stand_ins):
+  model = _model(1)
+  parametrize.register_parametrization(model, "reverse_embedding", _Scaled())
+  model.quantize(head=True)
+  _runs(model)
+  with torch.no_grad():
+    model.item_embedding.add_(1.0)
+  _runs(model)
+  with torch.no_grad():
+    model.parametrizations.reverse_embedding.original.mul_(2.0)
+  with pytest.raises(ValueError, match="head's weight has changed"):
+    model._head(torch.ones((2, 8)))
+  model.quantize(head=True)
+  _runs(model)
+
+
+def test_weights_that_a_hook_makes_are_refused(stand_ins):
+  """A pruned weight is made again by the next forward only: what stands there may be old."""
+  block = _model(1).decoder_blocks[0]
+  prune.l1_unstructured(block, "output_kernel", amount=0.5)
+  with pytest.raises(ValueError, match="output_kernel is a tensor that a hook makes"):
+    block.quantize()
+  prune.remove(block, "output_kernel")
+  block.quantize()
+  block._check_rows8()
+  assert torch.equal(block._rows8[2], block.output_kernel.reshape(8, 8).t()) and int((block.output_kernel == 0).sum()) == 32
+  prune.l1_unstructured(block, "u_kernel", amount=0.5)
+  with pytest.raises(ValueError, match="u_kernel is a tensor that a hook makes"):
+    block._check_rows8()
+
+
+def test_what_is_not_quantised_may_change(stand_ins):
+  """Norms and the output's bias are read as they are."""
+  block = recml_amd.HSTUBlock(8, 2, use_bias=True)
+  block.quantize()
+  with torch.no_grad():
+    for p in (block.input_ln_gamma, block.input_ln_beta, block.attn_ln_gamma, block.attn_ln_beta, block.output_bias):
+      p.add_(1.0)
+  block._check_rows8()
+  with torch.no_grad():
+    block.v_bias.add_(1.0)
+  with pytest.raises(ValueError, match="changed since quantize"):
+    block._check_rows8()
