@@ -270,8 +270,9 @@ class HSTUBlock(torch.nn.Module):
     with torch.no_grad():
       w, b = self._uqkv_weights()
       out = self.output_kernel.reshape(-1, self.hidden_dim)
-      old = self._rows8[:3] if self._rows8 is not None and self._rows8[3].spend() else (None, None, None)
-      kept = hstu_rows8.renew_rows(w.t(), old[0]), hstu_rows8.renew(b, old[1]), hstu_rows8.renew_rows(out.t(), old[2])
+      kept = hstu_rows8.quantize_rows(w.t()), b, hstu_rows8.quantize_rows(out.t())
+      if self._rows8 is not None and self._rows8[3].spend():
+        kept = tuple(map(hstu_rows8.renew, self._rows8, kept))
     self._rows8 = (*kept, _MadeOf(self._quantized_weights()))
 
   def dequantize(self) -> None:
@@ -590,11 +591,14 @@ class HSTU(torch.nn.Module):
       _check_counted(_sources(self, _HEAD))
     for block in self.decoder_blocks:
       block.quantize()
-    old, self._head8 = self._head8, None
-    if head:
-      with torch.no_grad():
-        kept = hstu_rows8.renew_rows(self.reverse_embedding.t(), old[0] if old is not None and old[1].spend() else None)
-      self._head8 = kept, _MadeOf(_sources(self, _HEAD))
+    if not head:
+      self._head8 = None
+      return
+    with torch.no_grad():
+      kept = hstu_rows8.quantize_rows(self.reverse_embedding.t())
+      if self._head8 is not None and self._head8[1].spend():
+        kept = hstu_rows8.renew(self._head8[0], kept)
+    self._head8 = kept, _MadeOf(_sources(self, _HEAD))
 
   def dequantize(self) -> None:
     """Back to the parameters' own type (HSTUBlock.dequantize)."""

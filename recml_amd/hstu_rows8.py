@@ -212,20 +212,16 @@ def quantize_rows(x) -> Rows8:
   return _norm("quantize_rows", x, None, None, 0.0, None, None, _lib_rows8.AS_IS)[0]
 
 
-def renew_rows(x, rows) -> Rows8:
-  """quantize_rows(x) of a matrix in the place of `rows`, so that what reads them there (a captured graph) reads the new ones; new rows where
-  `rows` are None, or others in number, width or device."""
-  fresh = quantize_rows(x)
-  if not isinstance(rows, Rows8) or (rows.rows, rows.width, rows.device) != (fresh.rows, fresh.width, fresh.device):
-    return fresh
-  renew(fresh.exponents, rows.exponents)
-  renew(fresh.codes, rows.codes)
-  return rows
-
-
-def renew(fresh, kept):
-  """`fresh` in the place of `kept`, or as it is where that has no such place."""
-  if fresh is None or kept is None or (fresh.shape, fresh.dtype, fresh.device) != (kept.shape, kept.dtype, kept.device):
+def renew(kept, fresh):
+  """`fresh` (Rows8, a tensor or None) in the place of `kept`, so that what reads it there (a captured graph) reads the new one; or as it is, where
+  that is of another kind or size, or elsewhere."""
+  if isinstance(fresh, Rows8):
+    if not isinstance(kept, Rows8) or (kept.rows, kept.width, kept.device) != (fresh.rows, fresh.width, fresh.device):
+      return fresh
+    renew(kept.codes, fresh.codes)
+    renew(kept.exponents, fresh.exponents)
+    return kept
+  if fresh is None or kept is None or (kept.shape, kept.dtype, kept.device) != (fresh.shape, fresh.dtype, fresh.device):
     return fresh
   with torch.inference_mode():                     # (`kept` may have been made there)
     return kept.copy_(fresh)

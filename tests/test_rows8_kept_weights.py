@@ -252,3 +252,27 @@ def test_what_is_not_quantised_may_change(stand_ins):
     block.v_bias.add_(1.0)
   with pytest.raises(ValueError, match="changed since quantize"):
     block._check_rows8()
+
+
+def test_a_call_that_fails_leaves_what_was_there(stand_ins, monkeypatch):
+  """No memory, say: the codes stay where they lay, and are written by the next call."""
+  model = _model(1)
+  model.quantize(head=True)
+  kept = [t.data_ptr() for block in model.decoder_blocks for t in (block._rows8[0], block._rows8[2])] + [model._head8[0].data_ptr()]
+  model.load_state_dict(_model(2).state_dict())
+  with monkeypatch.context() as m:
+    calls = []
+
+    def fails(x):
+      calls.append(x)
+      if len(calls) == 2:
+        raise torch.OutOfMemoryError("none left")
+      return x.clone()
+
+    m.setattr(hstu_rows8, "quantize_rows", fails)
+    with pytest.raises(torch.OutOfMemoryError):
+      model.quantize(head=True)
+  _refused(model)
+  model.quantize(head=True)
+  _runs(model)
+  assert kept == [t.data_ptr() for block in model.decoder_blocks for t in (block._rows8[0], block._rows8[2])] + [model._head8[0].data_ptr()]
