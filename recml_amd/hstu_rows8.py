@@ -70,7 +70,7 @@ class Rows8:
   """Rows in 8 bits.
 
   codes: uint8 [rows, 128 ceil(width / 128)], e4m3, zeros past the width; exponents: uint8 [ceil(width / 512), rows, 4], the biased powers of
-  two of four blocks of 128 side by side (255: the block stands for NaN).  Both contiguous, on one device.  Format:
+  two (1 to 246) of four blocks of 128 side by side (255: the block stands for NaN).  Both contiguous, on one device.  Format:
   include/hstu_rows8.h.  A weight [K, N] is kept as its N output columns: quantize_rows(w.t())."""
 
   __slots__ = ("codes", "exponents", "width")
